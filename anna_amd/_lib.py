@@ -203,6 +203,46 @@ PROTOTYPES.update({
     "anna_mi_lm_head_int4_topk": [_P, _I, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _I, _P, _I64, _I64, _I64, _I64,
                                   _I64, _I64, _P, _P, _P, _P],
 })
+
+
+class PagedDesc(ctypes.Structure):
+    """anna_mi_paged_desc."""
+
+    _fields_ = [
+        ("dtype", _I), ("num_layers", _I64), ("num_pages", _I64), ("kv_heads", _I64), ("q_heads", _I64),
+        ("head_dim", _I64), ("max_sequences", _I64), ("max_pages", _I64), ("pool", _P), ("table", _P),
+    ]
+
+
+class PagedSpan(ctypes.Structure):
+    """anna_mi_paged_span."""
+
+    _fields_ = [
+        ("sequences", _I64), ("tokens", _I64), ("words", _I64), ("partial_rows", _I64), ("split_items", _I64),
+        ("split_units", _I64), ("split_rows", _I64), ("touch_items", _I64), ("split_capacity", _I64),
+        ("unit_capacity", _I64), ("touch_capacity", _I64), ("tile_items", _I64), ("tile_capacity", _I64),
+        ("few_rows", _I64), ("buf", _P), ("partial_stats", _P), ("partial_values", _P),
+    ]
+
+
+_SPAN = ctypes.POINTER(PagedSpan)
+PROTOTYPES.update({
+    "anna_mi_paged_create": [ctypes.POINTER(PagedDesc), ctypes.POINTER(_P)],
+    "anna_mi_paged_destroy": [_P],
+    "anna_mi_paged_add": [_P, _I64, _P],
+    "anna_mi_paged_fork": [_P, _I64, _P, _P, _P],
+    "anna_mi_paged_extend": [_P, _I64, _P, _P, _P, _P],
+    "anna_mi_paged_truncate": [_P, ctypes.c_int32, _I64, _P],
+    "anna_mi_paged_free": [_P, _I64, _P, _P],
+    "anna_mi_paged_compact": [_P, ctypes.POINTER(_I64), _P],
+    "anna_mi_paged_resize": [_P, _I64, _P, _P],
+    "anna_mi_paged_lengths": [_P, _I64, _P, _P, ctypes.POINTER(_I64)],
+    "anna_mi_paged_span_plan": [_P, _I64, _P, _P, _P, _SPAN],
+    "anna_mi_paged_span_fill": [_P, _I64, _P, _P, _P, _SPAN, _P],
+    "anna_mi_paged_store": [_P, _I64, _SPAN, _P, _I64, _I64, _P, _I64, _I64, _I, _P],
+    "anna_mi_paged_read": [_P, _I64, _SPAN, _P, _P, _I, _P],
+    "anna_mi_paged_attend": [_P, _I64, _SPAN, _P, _I64, _I64, _P, _I64, _I64, _P, _F, _I, _P],
+})
 # entry points that do not return a status code
 RAW_PROTOTYPES: dict[str, tuple] = {
     "anna_mi_sizeof_moe_mlp_args": (_I64, []),
@@ -218,6 +258,8 @@ RAW_PROTOTYPES: dict[str, tuple] = {
     "anna_mi_lm_head_int4_topk_workspace": (_I64, [_I64, _I64]),
     "anna_mi_sizeof_tq_rows_append_args": (_I64, []),
     "anna_mi_sizeof_tq_store_args": (_I64, []),
+    "anna_mi_sizeof_paged_desc": (_I64, []),
+    "anna_mi_sizeof_paged_span": (_I64, []),
     "anna_mi_tq_decode_workgroups": (_I64, [_I64, _I64, _P, _I64]),
 }
 

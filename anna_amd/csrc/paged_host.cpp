@@ -1,0 +1,582 @@
+// The paged 4-bit cache's host side: which pages are whose, and the plans of its launches.
+//
+// The free pages are a stack, so that a sequence that ends gives its pages to the next one; a page
+// carries the number of sequences that hold it and is copied when one of several holders writes
+// into it.  Every call checks all its arguments before it changes anything.
+#include <limits.h>
+
+#include <algorithm>
+#include <mutex>
+#include <new>
+#include <vector>
+
+#include "paged.hpp"
+
+using namespace anna;
+using namespace anna::paged;
+
+struct anna_mi_paged {
+  std::mutex lock;
+  anna_mi_paged_desc d;
+  std::vector<int32_t> table;   // [max_sequences][max_pages]
+  std::vector<int64_t> length;  // -1: not in use
+  std::vector<int32_t> refs;    // of every page
+  std::vector<int32_t> free_pages, free_seqs;
+  std::vector<uint8_t> seen;  // by sequence, zero between calls
+
+  int32_t* row(int64_t seq) { return table.data() + seq * d.max_pages; }
+  int64_t pages(int64_t seq) const { return (length[seq] + PAGE - 1) / PAGE; }
+  int64_t page_size() const { return d.kv_heads * page_bytes(d.head_dim); }
+};
+
+namespace {
+
+// Workgroups that an attention launch is split into at most, over all KV heads (and the tiles themselves).
+constexpr int64_t SPLIT_TARGET = 1024, TILE_TARGET = 512;
+
+int hip_ok(hipError_t e, const char* what) { return e == hipSuccess ? ANNA_MI_OK : fail_hip(e, what); }
+
+// Batches words of the three kinds into as few launches as they need.
+struct Updates {
+  Update u;
+  hipStream_t stream;
+  int rc = ANNA_MI_OK;
+  std::vector<int32_t> records, entries, copies;
+  Updates(anna_mi_paged* h, void* s) : stream(as_stream(s)) {
+    memset(&u, 0, sizeof(u));
+    u.table = h->d.table;
+    u.width = h->d.max_pages;
+  }
+  void entry(int64_t index, int32_t page) { entries.insert(entries.end(), {(int32_t)index, page}); }
+  void copy(int32_t row, int32_t source, int64_t pages) { copies.insert(copies.end(), {row, source, (int32_t)pages}); }
+  int launch() {
+    constexpr int R = sizeof(Record) / 4;
+    size_t r = 0, e = 0, c = 0;
+    while (r < records.size() || e < entries.size() || c < copies.size()) {
+      int n = 0;
+      auto take = [&](const std::vector<int32_t>& v, size_t& at, int step) {
+        const int k = (int)std::min<size_t>((v.size() - at) / step, (UPDATE_WORDS - n) / step);
+        if (k > 0) memcpy(u.words + n, v.data() + at, 4 * (size_t)k * step);
+        n += k * step;
+        at += (size_t)k * step;
+        return k;
+      };
+      u.records = take(records, r, R);
+      u.entries = take(entries, e, 2);
+      u.copies = take(copies, c, 3);
+      const int rc = launch_update(u, stream);
+      if (rc != ANNA_MI_OK) return rc;
+    }
+    return ANNA_MI_OK;
+  }
+};
+
+// pairs: (source, page), ...
+int copy_pages(const anna_mi_paged* h, const void* from, int64_t from_pages, void* to, int64_t to_pages,
+               const std::vector<int32_t>& pairs, hipStream_t stream) {
+  Copy c;
+  c.from = (const uint8_t*)from;
+  c.to = (uint8_t*)to;
+  c.page = h->page_size();
+  c.from_layer = from_pages * c.page;
+  c.to_layer = to_pages * c.page;
+  for (size_t at = 0; at < pairs.size(); at += UPDATE_WORDS) {
+    c.pairs = (int32_t)std::min<size_t>(UPDATE_WORDS, pairs.size() - at) / 2;
+    memcpy(c.words, pairs.data() + at, 8 * (size_t)c.pairs);
+    const int rc = launch_copy(c, h->d.num_layers, stream);
+    if (rc != ANNA_MI_OK) return rc;
+  }
+  return ANNA_MI_OK;
+}
+
+// Sequences in use, each at most once.
+int check_seqs(anna_mi_paged* h, int64_t n, const int32_t* seqs) {
+  int64_t k = 0;
+  int rc = ANNA_MI_OK;
+  for (; k < n; k++) {
+    const int64_t s = seqs[k];
+    if (s < 0 || s >= h->d.max_sequences || h->length[s] < 0) {
+      set_error("sequence %lld is not in use", (long long)s);
+      rc = ANNA_MI_EINVAL;
+      break;
+    }
+    if (h->seen[s]) {
+      set_error("sequence %lld appears twice", (long long)s);
+      rc = ANNA_MI_EINVAL;
+      break;
+    }
+    h->seen[s] = 1;
+  }
+  for (int64_t i = 0; i < k; i++) h->seen[seqs[i]] = 0;
+  return rc;
+}
+
+// Gives back what sequence s holds from its page `from` on; the pages that nobody holds any more go to `freed`.
+void drop_pages(anna_mi_paged* h, int64_t s, int64_t from, std::vector<int32_t>& freed) {
+  int32_t* row = h->row(s);
+  for (int64_t c = from; c < h->pages(s); c++) {
+    if (--h->refs[row[c]] == 0) freed.push_back(row[c]);
+    row[c] = 0;
+  }
+}
+
+// On the stack so that they are taken again in the order in which they were freed.
+void give_back(anna_mi_paged* h, const std::vector<int32_t>& freed) {
+  h->free_pages.insert(h->free_pages.end(), freed.rbegin(), freed.rend());
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// The layout of a span: its tiles, and the sizes that follow from them.
+struct Plan {
+  std::vector<Record> records;
+  int64_t few_rows = 16, split_items = 0, tile_items = 0, units = 0, unit_rows = 0, touches = 0, tokens = 0;
+  int64_t split_bound = 0, touch_bound = 0, partial_rows = 0, partial_bound = 0;
+};
+
+int make_plan(anna_mi_paged* h, int64_t n, const int32_t* seqs, const int64_t* starts, const int64_t* counts, Plan& p) {
+  ANNA_CHECK(n >= 0 && (n == 0 || (seqs && starts && counts)), "span: null arrays");
+  int rc = check_seqs(h, n, seqs);
+  if (rc != ANNA_MI_OK) return rc;
+  const int64_t G = h->d.q_heads / h->d.kv_heads, H = h->d.kv_heads;
+  const int64_t most = 4096 / h->d.head_dim;  // rows of a split tile whose sums stay in registers
+  for (int64_t i = 0; i < n; i++) {
+    ANNA_CHECK(starts[i] >= 0 && counts[i] >= 0 && starts[i] <= h->length[seqs[i]] && counts[i] <= h->length[seqs[i]] - starts[i],
+               "span: tokens %lld .. %lld of sequence %d, which holds %lld", (long long)starts[i],
+               (long long)(starts[i] + counts[i]), (int)seqs[i], (long long)h->length[seqs[i]]);
+    p.tokens += counts[i];
+    const int64_t rows = counts[i] * G;
+    p.few_rows = std::max(p.few_rows, std::min(most, rows > 32 ? (int64_t)64 : rows > 16 ? (int64_t)32 : (int64_t)16));
+  }
+  ANNA_CHECK(p.tokens * G <= INT_MAX / 2, "span: too many tokens");
+  // a record for each tile, then the items that share its pages
+  int64_t offset = 0, total = 0;
+  for (int64_t i = 0; i < n; i++) {
+    const int64_t rows = counts[i] * G, R = p.few_rows;
+    const int64_t tiles = std::max<int64_t>(1, ceil_div(rows, R));
+    for (int64_t t = 0; t < tiles; t++) {
+      Record r = {};
+      r.index = (int32_t)i, r.row = seqs[i], r.start = (int32_t)starts[i], r.count = (int32_t)counts[i];
+      r.offset = (int32_t)offset, r.tile = (int32_t)t;
+      r.pages = rows ? (int32_t)((starts[i] + (std::min(rows, (t + 1) * R) - 1) / G) / PAGE + 1) : 0;
+      r.touch0 = (int32_t)p.touches;
+      total += r.pages;
+      p.records.push_back(r);
+    }
+    if (counts[i] > 0) p.touches += (starts[i] + counts[i] - 1) / PAGE - starts[i] / PAGE + 1;
+    if (counts[i] > 0) p.touch_bound += (counts[i] + PAGE - 2) / PAGE + 1;
+    offset += counts[i];
+  }
+  const int64_t target = std::max<int64_t>(1, SPLIT_TARGET / H), per = std::max<int64_t>(1, ceil_div(total, target));
+  int64_t most_rows = 0;
+  for (Record& r : p.records) {
+    const int64_t rows = std::min<int64_t>(p.few_rows, r.count * G - r.tile * p.few_rows);
+    r.item0 = (int32_t)p.split_items;
+    r.splits = (int32_t)ceil_div(r.pages, per);
+    r.part = -1;
+    r.unit = -1;
+    if (r.splits > 1) {
+      r.part = (int32_t)p.partial_rows, r.unit = (int32_t)p.units++;
+      p.partial_rows += r.splits * rows;
+      p.unit_rows = std::max(p.unit_rows, rows);
+    }
+    most_rows = std::max(most_rows, rows);
+    p.split_items += r.splits;
+  }
+  p.split_bound = total ? (int64_t)p.records.size() + target : 0;
+  p.partial_bound = std::min(p.split_bound, 2 * target) * most_rows;  // a tile that is split has more than `per` pages
+  ANNA_CHECK(p.partial_bound <= INT_MAX && p.split_bound <= INT_MAX / 64 && H * p.split_bound <= INT_MAX, "span: too many tokens");
+  return ANNA_MI_OK;
+}
+
+template <class F> int guarded(anna_mi_paged* h, const char* what, F f) {
+  ANNA_CHECK(h, "%s: null handle", what);
+  try {
+    std::lock_guard<std::mutex> g(h->lock);
+    return f();
+  } catch (const std::exception& e) {
+    set_error("%s: %s", what, e.what());
+    return ANNA_MI_EINVAL;
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t anna_mi_sizeof_paged_desc(void) { return sizeof(anna_mi_paged_desc); }
+int64_t anna_mi_sizeof_paged_span(void) { return sizeof(anna_mi_paged_span); }
+
+int anna_mi_paged_create(const anna_mi_paged_desc* desc, anna_mi_paged** handle) {
+  ANNA_CHECK(desc && handle, "paged_create: null argument");
+  const anna_mi_paged_desc& d = *desc;
+  ANNA_CHECK(d.dtype == ANNA_MI_BF16 || d.dtype == ANNA_MI_F16, "paged_create: dtype must be bf16 or fp16");
+  ANNA_CHECK(d.head_dim == 64 || d.head_dim == 128 || d.head_dim == 256, "paged_create: head_dim must be 64, 128 or 256, got %lld",
+             (long long)d.head_dim);
+  ANNA_CHECK(d.kv_heads > 0 && d.kv_heads <= 1024 && d.q_heads > 0 && d.q_heads <= 65536 && d.q_heads % d.kv_heads == 0,
+             "paged_create: q_heads must be a multiple of kv_heads");
+  ANNA_CHECK(d.num_layers > 0 && d.num_layers <= 65535 && d.num_pages > 0 && d.num_pages < INT_MAX, "paged_create: bad num_layers or num_pages");
+  ANNA_CHECK(d.max_sequences > 0 && d.max_pages > 0 && d.max_sequences <= INT_MAX / d.max_pages && d.max_pages <= INT_MAX / (2 * PAGE),
+             "paged_create: bad max_sequences or max_pages");
+  ANNA_CHECK(d.pool && d.table, "paged_create: null pool or table");
+  ANNA_CHECK((uintptr_t)d.pool % 16 == 0, "paged_create: the pool must be 16-byte aligned");
+  try {
+    auto* h = new anna_mi_paged;
+    *handle = h;
+    h->d = d;
+    h->table.assign(d.max_sequences * d.max_pages, 0);
+    h->length.assign(d.max_sequences, -1);
+    h->seen.assign(d.max_sequences, 0);
+    h->refs.assign(d.num_pages, 0);
+    for (int64_t i = d.num_pages - 1; i >= 0; i--) h->free_pages.push_back((int32_t)i);
+    for (int64_t i = d.max_sequences - 1; i >= 0; i--) h->free_seqs.push_back((int32_t)i);
+  } catch (const std::exception& e) {
+    set_error("paged_create: %s", e.what());
+    return ANNA_MI_EINVAL;
+  }
+  return ANNA_MI_OK;
+}
+
+int anna_mi_paged_destroy(anna_mi_paged* handle) {
+  delete handle;
+  return ANNA_MI_OK;
+}
+
+int anna_mi_paged_add(anna_mi_paged* h, int64_t n, int32_t* seqs) {
+  return guarded(h, "paged_add", [&]() -> int {
+    ANNA_CHECK(n >= 0 && (n == 0 || seqs), "paged_add: bad arguments");
+    ANNA_CHECK(n <= (int64_t)h->free_seqs.size(), "paged_add: %lld sequences asked, %lld of %lld are free", (long long)n,
+               (long long)h->free_seqs.size(), (long long)h->d.max_sequences);
+    for (int64_t i = 0; i < n; i++) {
+      seqs[i] = h->free_seqs.back();
+      h->free_seqs.pop_back();
+      h->length[seqs[i]] = 0;
+    }
+    return ANNA_MI_OK;
+  });
+}
+
+int anna_mi_paged_fork(anna_mi_paged* h, int64_t n, const int32_t* parents, int32_t* children, void* stream) {
+  return guarded(h, "paged_fork", [&]() -> int {
+    ANNA_CHECK(n >= 0 && (n == 0 || (parents && children)), "paged_fork: bad arguments");
+    for (int64_t i = 0; i < n; i++)
+      ANNA_CHECK(parents[i] >= 0 && parents[i] < h->d.max_sequences && h->length[parents[i]] >= 0,
+                 "paged_fork: sequence %d is not in use", (int)parents[i]);
+    ANNA_CHECK(n <= (int64_t)h->free_seqs.size(), "paged_fork: %lld sequences asked, %lld of %lld are free", (long long)n,
+               (long long)h->free_seqs.size(), (long long)h->d.max_sequences);
+    Updates up(h, stream);
+    up.copies.reserve(3 * n);
+    for (int64_t i = 0; i < n; i++) {
+      const int32_t c = h->free_seqs.back(), p = parents[i];
+      h->free_seqs.pop_back();
+      children[i] = c;
+      h->length[c] = h->length[p];
+      const int64_t pages = h->pages(p);
+      memcpy(h->row(c), h->row(p), 4 * pages);
+      for (int64_t k = 0; k < pages; k++) h->refs[h->row(c)[k]]++;
+      if (pages > 0) up.copy(c, p, pages);
+    }
+    return up.launch();
+  });
+}
+
+int anna_mi_paged_extend(anna_mi_paged* h, int64_t n, const int32_t* seqs, const int64_t* counts, int64_t* starts, void* stream) {
+  return guarded(h, "paged_extend", [&]() -> int {
+    ANNA_CHECK(n >= 0 && (n == 0 || (seqs && counts)), "paged_extend: bad arguments");
+    int rc = check_seqs(h, n, seqs);
+    if (rc != ANNA_MI_OK) return rc;
+    // pages to take: those that are new, and a copy of a last page for all its holders but the last
+    std::vector<int32_t> shared;  // last pages whose holders here each counted as one that leaves
+    int64_t need = 0;
+    for (int64_t i = 0; i < n; i++) {
+      const int64_t old = h->length[seqs[i]];
+      ANNA_CHECK(counts[i] >= 0, "paged_extend: count %lld", (long long)counts[i]);
+      ANNA_CHECK(counts[i] <= h->d.max_pages * PAGE - old, "paged_extend: sequence %d would hold %lld tokens, at most %lld fit",
+                 (int)seqs[i], (long long)(old + counts[i]), (long long)(h->d.max_pages * PAGE));
+      need += ceil_div(old + counts[i], PAGE) - ceil_div(old, PAGE);
+      if (counts[i] > 0 && old % PAGE != 0) {
+        const int32_t last = h->row(seqs[i])[old / PAGE];
+        if (h->refs[last] > 1) shared.push_back(last);
+      }
+    }
+    if (!shared.empty()) {
+      std::sort(shared.begin(), shared.end());
+      for (size_t k = 0; k < shared.size();) {
+        size_t e = k;
+        while (e < shared.size() && shared[e] == shared[k]) e++;
+        need += std::min<int64_t>(e - k, h->refs[shared[k]] - 1);
+        k = e;
+      }
+    }
+    ANNA_CHECK(need <= (int64_t)h->free_pages.size(), "paged_extend: %lld pages needed, %lld of %lld are free", (long long)need,
+               (long long)h->free_pages.size(), (long long)h->d.num_pages);
+    Updates up(h, stream);
+    std::vector<int32_t> pairs;
+    up.entries.reserve(2 * need);
+    pairs.reserve(2 * shared.size());
+    auto take = [&](int64_t seq, int64_t c) {
+      const int32_t page = h->free_pages.back();
+      h->free_pages.pop_back();
+      h->refs[page] = 1;
+      h->row(seq)[c] = page;
+      up.entry(seq * h->d.max_pages + c, page);
+      return page;
+    };
+    for (int64_t i = 0; i < n; i++) {
+      const int64_t s = seqs[i], old = h->length[s];
+      if (starts) starts[i] = old;
+      if (counts[i] == 0) continue;
+      if (old % PAGE != 0) {
+        const int32_t last = h->row(s)[old / PAGE];
+        if (h->refs[last] > 1) {
+          h->refs[last]--;
+          const int32_t page = take(s, old / PAGE);
+          pairs.insert(pairs.end(), {last, page});
+        }
+      }
+      for (int64_t c = ceil_div(old, PAGE); c < ceil_div(old + counts[i], PAGE); c++) take(s, c);
+      h->length[s] = old + counts[i];
+    }
+    rc = copy_pages(h, h->d.pool, h->d.num_pages, h->d.pool, h->d.num_pages, pairs, as_stream(stream));
+    return rc != ANNA_MI_OK ? rc : up.launch();
+  });
+}
+
+int anna_mi_paged_truncate(anna_mi_paged* h, int32_t seq, int64_t length, void* stream) {
+  return guarded(h, "paged_truncate", [&]() -> int {
+    int rc = check_seqs(h, 1, &seq);
+    if (rc != ANNA_MI_OK) return rc;
+    ANNA_CHECK(length >= 0 && length <= h->length[seq], "paged_truncate: length %lld of a sequence of %lld", (long long)length,
+               (long long)h->length[seq]);
+    std::vector<int32_t> freed;
+    const int64_t keep = ceil_div(length, PAGE);
+    Updates up(h, stream);
+    if (keep < h->pages(seq)) up.copy(seq, -1, keep);
+    drop_pages(h, seq, keep, freed);
+    give_back(h, freed);
+    h->length[seq] = length;
+    return up.launch();
+  });
+}
+
+int anna_mi_paged_free(anna_mi_paged* h, int64_t n, const int32_t* seqs, void* stream) {
+  return guarded(h, "paged_free", [&]() -> int {
+    ANNA_CHECK(n >= 0 && (n == 0 || seqs), "paged_free: bad arguments");
+    int rc = check_seqs(h, n, seqs);
+    if (rc != ANNA_MI_OK) return rc;
+    Updates up(h, stream);
+    std::vector<int32_t> freed;
+    for (int64_t i = 0; i < n; i++) {
+      if (h->length[seqs[i]] > 0) up.copy(seqs[i], -1, 0);
+      drop_pages(h, seqs[i], 0, freed);
+      h->length[seqs[i]] = -1;
+    }
+    give_back(h, freed);
+    for (int64_t i = n - 1; i >= 0; i--) h->free_seqs.push_back(seqs[i]);
+    return up.launch();
+  });
+}
+
+int anna_mi_paged_compact(anna_mi_paged* h, int64_t* live, void* stream) {
+  return guarded(h, "paged_compact", [&]() -> int {
+    const int64_t n = h->d.num_pages - (int64_t)h->free_pages.size();
+    // pages behind the first n move into the holes before them: sources and targets are disjoint
+    std::vector<int32_t> to(h->d.num_pages, -1), pairs;
+    int64_t hole = 0;
+    for (int64_t p = n; p < h->d.num_pages; p++) {
+      if (h->refs[p] == 0) continue;
+      while (h->refs[hole] != 0) hole++;
+      pairs.insert(pairs.end(), {(int32_t)p, (int32_t)hole});
+      to[p] = (int32_t)hole++;
+    }
+    Updates up(h, stream);
+    for (int64_t s = 0; s < h->d.max_sequences; s++)
+      for (int64_t c = 0; h->length[s] > 0 && c < h->pages(s); c++) {
+        int32_t& page = h->row(s)[c];
+        if (to[page] < 0) continue;
+        page = to[page];
+        up.entry(s * h->d.max_pages + c, page);
+      }
+    for (size_t k = 0; k < pairs.size(); k += 2) std::swap(h->refs[pairs[k]], h->refs[pairs[k + 1]]);
+    h->free_pages.clear();
+    for (int64_t p = h->d.num_pages - 1; p >= n; p--) h->free_pages.push_back((int32_t)p);
+    if (live) *live = n;
+    const int rc = copy_pages(h, h->d.pool, h->d.num_pages, h->d.pool, h->d.num_pages, pairs, as_stream(stream));
+    return rc != ANNA_MI_OK ? rc : up.launch();
+  });
+}
+
+int anna_mi_paged_resize(anna_mi_paged* h, int64_t num_pages, void* pool, void* stream) {
+  return guarded(h, "paged_resize", [&]() -> int {
+    const int64_t n = h->d.num_pages - (int64_t)h->free_pages.size();
+    ANNA_CHECK(num_pages >= n && num_pages > 0 && num_pages < INT_MAX, "paged_resize: %lld pages, %lld are in use", (long long)num_pages,
+               (long long)n);
+    ANNA_CHECK(pool && (uintptr_t)pool % 16 == 0 && pool != h->d.pool, "paged_resize: needs another, 16-byte aligned pool");
+    std::vector<int32_t> to(h->d.num_pages, -1), pairs, refs(num_pages, 0);
+    pairs.reserve(2 * num_pages);
+    int32_t next = 0;
+    Updates up(h, stream);
+    for (int64_t s = 0; s < h->d.max_sequences; s++)
+      for (int64_t c = 0; h->length[s] > 0 && c < h->pages(s); c++) {
+        int32_t& page = h->row(s)[c];
+        if (to[page] < 0) {
+          to[page] = next;
+          refs[next] = h->refs[page];
+          pairs.insert(pairs.end(), {page, next++});
+        }
+        if (page != to[page]) up.entry(s * h->d.max_pages + c, to[page]);
+        page = to[page];
+      }
+    for (int64_t p = next; p < num_pages; p++) pairs.insert(pairs.end(), {-1, (int32_t)p});
+    const void* old = h->d.pool;
+    const int64_t old_pages = h->d.num_pages;
+    h->refs.swap(refs);
+    h->free_pages.clear();
+    for (int64_t p = num_pages - 1; p >= next; p--) h->free_pages.push_back((int32_t)p);
+    h->d.pool = pool;
+    h->d.num_pages = num_pages;
+    const int rc = copy_pages(h, old, old_pages, pool, num_pages, pairs, as_stream(stream));
+    return rc != ANNA_MI_OK ? rc : up.launch();
+  });
+}
+
+int anna_mi_paged_lengths(anna_mi_paged* h, int64_t n, const int32_t* seqs, int64_t* lengths, int64_t* live_pages) {
+  return guarded(h, "paged_lengths", [&]() -> int {
+    ANNA_CHECK(n >= 0 && (n == 0 || (seqs && lengths)), "paged_lengths: bad arguments");
+    for (int64_t i = 0; i < n; i++)
+      lengths[i] = seqs[i] >= 0 && seqs[i] < h->d.max_sequences ? h->length[seqs[i]] : -1;
+    if (live_pages) *live_pages = h->d.num_pages - (int64_t)h->free_pages.size();
+    return ANNA_MI_OK;
+  });
+}
+
+int anna_mi_paged_span_plan(anna_mi_paged* h, int64_t n, const int32_t* seqs, const int64_t* starts, const int64_t* counts,
+                            anna_mi_paged_span* span) {
+  return guarded(h, "paged_span_plan", [&]() -> int {
+    ANNA_CHECK(span, "paged_span_plan: null span");
+    Plan p;
+    const int rc = make_plan(h, n, seqs, starts, counts, p);
+    if (rc != ANNA_MI_OK) return rc;
+    memset(span, 0, sizeof(*span));
+    span->sequences = n;
+    span->tokens = p.tokens;
+    span->few_rows = p.few_rows;
+    span->split_capacity = p.split_bound;
+    span->unit_capacity = (int64_t)p.records.size();
+    span->touch_capacity = p.touch_bound;
+    span->tile_capacity = p.tile_items;
+    span->partial_rows = p.partial_bound;
+    span->words = sections(*span).words;
+    return ANNA_MI_OK;
+  });
+}
+
+int anna_mi_paged_span_fill(anna_mi_paged* h, int64_t n, const int32_t* seqs, const int64_t* starts, const int64_t* counts,
+                            anna_mi_paged_span* span, void* stream) {
+  return guarded(h, "paged_span_fill", [&]() -> int {
+    ANNA_CHECK(span && span->buf && (uintptr_t)span->buf % 16 == 0, "paged_span_fill: null or unaligned buffer");
+    Plan p;
+    const int rc = make_plan(h, n, seqs, starts, counts, p);
+    if (rc != ANNA_MI_OK) return rc;
+    ANNA_CHECK(n == span->sequences && p.tokens == span->tokens && p.few_rows == span->few_rows && p.split_items <= span->split_capacity &&
+                   p.tile_items <= span->tile_capacity && (int64_t)p.records.size() <= span->unit_capacity &&
+                   p.touches <= span->touch_capacity && p.partial_rows <= span->partial_rows && sections(*span).words <= span->words,
+               "span: these tokens do not fit the span that is filled");
+    ANNA_CHECK(p.partial_rows == 0 || (span->partial_stats && span->partial_values), "paged_span_fill: null partials");
+    span->split_items = p.split_items;
+    span->tile_items = p.tile_items;
+    span->split_units = p.units;
+    span->split_rows = p.unit_rows;
+    span->touch_items = p.touches;
+    Updates up(h, stream);
+    const Sections at = sections(*span);
+    Update& u = up.u;
+    u.buf = span->buf;
+    u.header[0] = (int32_t)p.split_items, u.header[1] = (int32_t)p.tile_items, u.header[2] = (int32_t)p.units;
+    u.header[3] = (int32_t)p.touches;
+    u.rows_at = at.rows, u.split_at = at.split, u.tile_at = at.tile, u.units_at = at.units, u.touch_at = at.touch;
+    u.group = (int32_t)(h->d.q_heads / h->d.kv_heads);
+    u.split_rows = (int32_t)p.few_rows;
+    u.tile_rows = tile_rows(h->d.head_dim);
+    up.records.resize(p.records.size() * (sizeof(Record) / 4));
+    if (!p.records.empty()) memcpy(up.records.data(), p.records.data(), p.records.size() * sizeof(Record));
+    return up.launch();
+  });
+}
+
+namespace {
+int check_layer(anna_mi_paged* h, int64_t layer, const anna_mi_paged_span* span, const char* what) {
+  ANNA_CHECK(span && span->buf, "%s: null span", what);
+  ANNA_CHECK(layer >= 0 && layer < h->d.num_layers, "%s: layer %lld of %lld", what, (long long)layer, (long long)h->d.num_layers);
+  return ANNA_MI_OK;
+}
+uint8_t* layer_pool(anna_mi_paged* h, int64_t layer) {
+  return (uint8_t*)h->d.pool + layer * h->d.num_pages * h->page_size();
+}
+bool aligned(const void* p, int64_t token, int64_t head) { return (uintptr_t)p % 16 == 0 && token % 8 == 0 && head % 8 == 0; }
+}  // namespace
+
+int anna_mi_paged_store(anna_mi_paged* h, int64_t layer, const anna_mi_paged_span* span, const void* keys, int64_t key_stride_token,
+                        int64_t key_stride_head, const void* values, int64_t value_stride_token, int64_t value_stride_head,
+                        int capacity_grid, void* stream) {
+  return guarded(h, "paged_store", [&]() -> int {
+    const int rc = check_layer(h, layer, span, "paged_store");
+    if (rc != ANNA_MI_OK || span->tokens == 0) return rc;
+    ANNA_CHECK(keys && values, "paged_store: null keys or values");
+    ANNA_CHECK(aligned(keys, key_stride_token, key_stride_head) && aligned(values, value_stride_token, value_stride_head),
+               "paged_store: keys and values need rows of 16-byte alignment");
+    return launch_store(h->d.dtype, h->d.head_dim, layer_pool(h, layer), h->d.table, h->d.max_pages, span->buf,
+                        (const Touch*)(span->buf + sections(*span).touch),
+                        capacity_grid ? span->touch_capacity : span->touch_items, h->d.kv_heads, keys, key_stride_token,
+                        key_stride_head, values, value_stride_token, value_stride_head, as_stream(stream));
+  });
+}
+
+int anna_mi_paged_read(anna_mi_paged* h, int64_t layer, const anna_mi_paged_span* span, void* keys, void* values, int capacity_grid,
+                       void* stream) {
+  return guarded(h, "paged_read", [&]() -> int {
+    const int rc = check_layer(h, layer, span, "paged_read");
+    if (rc != ANNA_MI_OK || span->tokens == 0) return rc;
+    ANNA_CHECK(keys && values && (uintptr_t)keys % 16 == 0 && (uintptr_t)values % 16 == 0, "paged_read: null or unaligned output");
+    return launch_read(h->d.dtype, h->d.head_dim, layer_pool(h, layer), h->d.table, h->d.max_pages, span->buf,
+                       (const Touch*)(span->buf + sections(*span).touch),
+                       capacity_grid ? span->touch_capacity : span->touch_items, h->d.kv_heads, keys, values,
+                       as_stream(stream));
+  });
+}
+
+int anna_mi_paged_attend(anna_mi_paged* h, int64_t layer, const anna_mi_paged_span* span, const void* query,
+                         int64_t query_stride_token, int64_t query_stride_head, const void* gate, int64_t gate_stride_token,
+                         int64_t gate_stride_head, void* out, float scaling, int capacity_grid, void* stream) {
+  return guarded(h, "paged_attend", [&]() -> int {
+    const int rc = check_layer(h, layer, span, "paged_attend");
+    if (rc != ANNA_MI_OK || span->tokens == 0) return rc;
+    ANNA_CHECK(query && out && (uintptr_t)out % 16 == 0, "paged_attend: null query or output, or an unaligned output");
+    ANNA_CHECK(aligned(query, query_stride_token, query_stride_head) &&
+                   (!gate || aligned(gate, gate_stride_token, gate_stride_head)),
+               "paged_attend: query and gate need rows of 16-byte alignment");
+    ANNA_CHECK(scaling > 0 && scaling < 1.0e30f, "paged_attend: scaling must be positive and finite");
+    const Sections at = sections(*span);
+    Attend a;
+    a.pool = layer_pool(h, layer);
+    a.table = h->d.table;
+    a.width = h->d.max_pages;
+    a.header = span->buf;
+    a.split = (const Item*)(span->buf + at.split);
+    a.tile = (const Item*)(span->buf + at.tile);
+    a.units = (const Unit*)(span->buf + at.units);
+    a.query = query, a.q_token = query_stride_token, a.q_head = query_stride_head;
+    a.gate = gate, a.g_token = gate_stride_token, a.g_head = gate_stride_head;
+    a.out = out;
+    a.stats = span->partial_stats, a.values = span->partial_values;
+    a.scale = scaling * 1.44269504088896340736f;
+    a.kv_heads = (int32_t)h->d.kv_heads;
+    a.group = (int32_t)(h->d.q_heads / h->d.kv_heads);
+    const bool all = capacity_grid != 0;
+    return launch_attend(h->d.dtype, h->d.head_dim, a, all ? span->split_capacity : span->split_items, span->few_rows,
+                         all ? span->tile_capacity : span->tile_items, all ? span->unit_capacity : span->split_units,
+                         all ? span->few_rows : span->split_rows, as_stream(stream));
+  });
+}
+
+}  // extern "C"

@@ -669,6 +669,98 @@ int anna_mi_moe_prefill(const anna_mi_moe_prefill_args* args, void* stream);
 int64_t anna_mi_sizeof_moe_prefill_args(void);
 int anna_mi_moe_grouped_int4_mlp(const anna_mi_moe_mlp_args* args, void* stream);
 
+/* ------------------------------------------------------------- paged 4-bit KV cache
+ * A pool of pages shared by all sequences, with copy on write (no counterpart in the reference,
+ * whose rows own their storage: turboquant.py:1027-1140).  A page holds 64 tokens of every KV head of
+ * a layer; the same page number is used in every layer.
+ *
+ * Values are held in groups of 64 (of one token and head) as 4-bit codes:
+ *   scale = bf16(max((max - min) / 15, max|x| / 120)), 0 below 2^-100;   zero = rint(min / scale)
+ *   code = clamp(rint(x / scale) - zero, 0, 15);                         x' = (code + zero) * scale
+ * A token whose keys or values of a head hold a NaN or an infinity is kept as NaN keys and zero
+ * values: queries that see it answer NaN, no other query is touched.
+ *
+ * Page of one KV head, 72 * head_dim bytes (head_dim = 64, 128 or 256; NG = head_dim / 64):
+ *   key codes    [64 tokens][4 quarters][head_dim/32] words: word (q, s) of a token holds dims
+ *                32 s + 8 q + e, e = 0..7, at bits 4 * ((e % 2) * 4 + e / 2)
+ *   value codes  [2 halves of 32 tokens][NG][64 lanes][4] words: word w of lane (q = lane / 16,
+ *                r = lane % 16) of group g holds dim 64 g + 16 w + r of the tokens 4 q + e (e < 4)
+ *                and 16 + 4 q + e - 4 (e >= 4), at the same bits
+ *   key scales   bf16 [16][NG][4] (token 4 i + j of group g at [i][g][j])
+ *   key offsets  bf16 [64][NG], the whole number zero - 128
+ *   value scales, value offsets   bf16 [16][NG][4] each
+ * Values' scales and offsets are finite wherever the pool was zeroed first and written by these
+ * calls, also behind the last token.
+ *
+ * The handle counts pages, references and lengths on the host (its calls lock it); the pool, the
+ * page table and the spans' buffers are the caller's device memory.  Calls that share a handle
+ * must not overlap on the GPU. */
+typedef struct anna_mi_paged anna_mi_paged;
+
+typedef struct {
+  int dtype; /* of the dense keys, values, queries and outputs: bf16 or fp16 */
+  int64_t num_layers, num_pages, kv_heads, q_heads, head_dim, max_sequences, max_pages;
+  void* pool;     /* [num_layers][num_pages][kv_heads][72 * head_dim] bytes, zeroed */
+  int32_t* table; /* [max_sequences][max_pages], zeroed; entries past a sequence's pages stay 0 */
+} anna_mi_paged_desc;
+
+/* Tokens start .. start + count - 1 of some sequences, and how attention over them is laid out. */
+typedef struct {
+  int64_t sequences, tokens;
+  int64_t words, partial_rows; /* what the caller allocates: int32 words of buf, rows of the partials */
+  int64_t split_items, split_units, split_rows, touch_items; /* sizes of this fill */
+  int64_t split_capacity, unit_capacity, touch_capacity;     /* and of the buffer's sections */
+  int64_t tile_items, tile_capacity;
+  int64_t few_rows; /* query rows of a tile of the split form: 16, 32 or 64 */
+  int32_t* buf;
+  float* partial_stats;  /* [partial_rows][kv_heads][2] */
+  float* partial_values; /* [partial_rows][kv_heads][head_dim] */
+} anna_mi_paged_span;
+
+int anna_mi_paged_create(const anna_mi_paged_desc* desc, anna_mi_paged** handle);
+int anna_mi_paged_destroy(anna_mi_paged* handle);
+/* n new, empty sequences / n sequences that share all pages of their parents (parents may repeat) */
+int anna_mi_paged_add(anna_mi_paged* handle, int64_t n, int32_t* seqs);
+int anna_mi_paged_fork(anna_mi_paged* handle, int64_t n, const int32_t* parents, int32_t* children, void* stream);
+/* Lengthens sequences by counts (0 allowed), whose old lengths go to starts (may be NULL).  A partly
+ * filled last page that others share is copied first, in every layer. */
+int anna_mi_paged_extend(anna_mi_paged* handle, int64_t n, const int32_t* seqs, const int64_t* counts,
+                         int64_t* starts, void* stream);
+int anna_mi_paged_truncate(anna_mi_paged* handle, int32_t seq, int64_t length, void* stream);
+int anna_mi_paged_free(anna_mi_paged* handle, int64_t n, const int32_t* seqs, void* stream);
+/* Moves the pages in use to the pool's front, in place; *live is their number. */
+int anna_mi_paged_compact(anna_mi_paged* handle, int64_t* live, void* stream);
+/* The pages in use, in the sequences' order, at the front of another pool of num_pages pages, whose
+ * other pages are zeroed; the caller may free the old pool once the stream has passed. */
+int anna_mi_paged_resize(anna_mi_paged* handle, int64_t num_pages, void* pool, void* stream);
+/* lengths[i] of seqs[i], -1 for one not in use; pages in use; seqs may be NULL with n = 0 */
+int anna_mi_paged_lengths(anna_mi_paged* handle, int64_t n, const int32_t* seqs, int64_t* lengths, int64_t* live_pages);
+
+/* Sizes of a span (its capacities too); then, with buf and the partials allocated, its fill.  A fill
+ * of the same sequences count and counts fits the buffer of an earlier one (its capacities). */
+int anna_mi_paged_span_plan(anna_mi_paged* handle, int64_t n, const int32_t* seqs, const int64_t* starts,
+                            const int64_t* counts, anna_mi_paged_span* span);
+int anna_mi_paged_span_fill(anna_mi_paged* handle, int64_t n, const int32_t* seqs, const int64_t* starts,
+                            const int64_t* counts, anna_mi_paged_span* span, void* stream);
+
+/* capacity_grid != 0 in the calls below: launches for every fill that fits the span's buffer (a
+ * captured graph), not for the last one.
+ *
+ * keys/values [tokens][kv_heads][head_dim] of a span into its pages of a layer, and back */
+int anna_mi_paged_store(anna_mi_paged* handle, int64_t layer, const anna_mi_paged_span* span, const void* keys,
+                        int64_t key_stride_token, int64_t key_stride_head, const void* values,
+                        int64_t value_stride_token, int64_t value_stride_head, int capacity_grid, void* stream);
+int anna_mi_paged_read(anna_mi_paged* handle, int64_t layer, const anna_mi_paged_span* span, void* keys, void* values,
+                       int capacity_grid, void* stream);
+/* out [tokens][q_heads][head_dim] = softmax(scaling q k^T) v over the tokens up to and with each
+ * query's own, times sigmoid(gate) when given. */
+int anna_mi_paged_attend(anna_mi_paged* handle, int64_t layer, const anna_mi_paged_span* span, const void* query,
+                         int64_t query_stride_token, int64_t query_stride_head, const void* gate,
+                         int64_t gate_stride_token, int64_t gate_stride_head, void* out, float scaling,
+                         int capacity_grid, void* stream);
+int64_t anna_mi_sizeof_paged_desc(void);
+int64_t anna_mi_sizeof_paged_span(void);
+
 #ifdef __cplusplus
 }
 #endif
