@@ -9,6 +9,9 @@ namespace paged {
 
 constexpr int PAGE = 64;   // tokens of a page
 constexpr int GROUP = 64;  // values with one scale and zero
+// What codes carry when they enter a matrix instruction, and offsets are without: 16 + code is exact in bf16's
+// eight bits by bit operations alone, and the smallest such number keeps the sums that cancel small.
+constexpr int CODE_BASE = 16;
 
 // Byte offsets in a page of one KV head of head_dim D.
 constexpr int64_t page_bytes(int64_t D) { return 72 * D; }
@@ -53,6 +56,7 @@ inline Sections sections(const anna_mi_paged_span& s) {
 // One tile of one sequence, from which its items, its unit and (tile 0) its touches are written.
 struct Record {
   int32_t index, row, start, count, offset, tile, item0, pages, splits, part, unit, touch0;
+  int32_t tiled;  // 1: of the tile form
 };
 
 // The words of an update travel in the kernel's arguments (at most 4 KB of them): no staging memory whose
@@ -95,9 +99,10 @@ struct Attend {
   float scale;  // scaling * log2(e)
   int32_t kv_heads, group;
 };
-int tile_rows(int64_t head_dim);  // query rows of a tile of the tile form
-int launch_attend(int dtype, int64_t head_dim, const Attend& a, int64_t split_items, int64_t few_rows, int64_t tile_items,
-                  int64_t units, int64_t unit_rows, hipStream_t stream);
+struct Grid {
+  int64_t split_items, few_rows, tile_items, tile_rows, units, unit_rows;
+};
+int launch_attend(int dtype, int64_t head_dim, const Attend& a, const Grid& g, hipStream_t stream);
 int launch_store(int dtype, int64_t head_dim, uint8_t* pool, const int32_t* table, int64_t width,
                  const int32_t* header, const Touch* touch, int64_t touches, int64_t kv_heads, const void* keys, int64_t k_token, int64_t k_head, const void* values,
                  int64_t v_token, int64_t v_head, hipStream_t stream);

@@ -32,7 +32,7 @@ struct anna_mi_paged {
 namespace {
 
 // Workgroups that an attention launch is split into at most, over all KV heads (and the tiles themselves).
-constexpr int64_t SPLIT_TARGET = 1024, TILE_TARGET = 512;
+constexpr int64_t SPLIT_TARGET = 1024, TILE_TARGET = 512, TILE_FILL = 256, TILE_PAGES = 8;
 
 int hip_ok(hipError_t e, const char* what) { return e == hipSuccess ? ANNA_MI_OK : fail_hip(e, what); }
 
@@ -127,11 +127,13 @@ void give_back(anna_mi_paged* h, const std::vector<int32_t>& freed) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// The layout of a span: its tiles, and the sizes that follow from them.
+// The layout of a span: its tiles, and the sizes that follow from them.  What a buffer has room for (the
+// bounds) depends on the counts alone, so that a span can be filled again as its sequences grow.
 struct Plan {
   std::vector<Record> records;
-  int64_t few_rows = 16, split_items = 0, tile_items = 0, units = 0, unit_rows = 0, touches = 0, tokens = 0;
-  int64_t split_bound = 0, touch_bound = 0, partial_rows = 0, partial_bound = 0;
+  int64_t few_rows = 16, tile_rows = 128, units = 0, unit_rows = 0, touches = 0, tokens = 0;
+  int64_t items[2] = {0, 0}, bound[2] = {0, 0};  // of the split form, of the tile form
+  int64_t touch_bound = 0, partial_rows = 0, partial_bound = 0;
 };
 
 int make_plan(anna_mi_paged* h, int64_t n, const int32_t* seqs, const int64_t* starts, const int64_t* counts, Plan& p) {
@@ -140,39 +142,54 @@ int make_plan(anna_mi_paged* h, int64_t n, const int32_t* seqs, const int64_t* s
   if (rc != ANNA_MI_OK) return rc;
   const int64_t G = h->d.q_heads / h->d.kv_heads, H = h->d.kv_heads;
   const int64_t most = 4096 / h->d.head_dim;  // rows of a split tile whose sums stay in registers
+  int64_t large = 0;                          // tiles of 256 rows
   for (int64_t i = 0; i < n; i++) {
     ANNA_CHECK(starts[i] >= 0 && counts[i] >= 0 && starts[i] <= h->length[seqs[i]] && counts[i] <= h->length[seqs[i]] - starts[i],
                "span: tokens %lld .. %lld of sequence %d, which holds %lld", (long long)starts[i],
                (long long)(starts[i] + counts[i]), (int)seqs[i], (long long)h->length[seqs[i]]);
     p.tokens += counts[i];
     const int64_t rows = counts[i] * G;
-    p.few_rows = std::max(p.few_rows, std::min(most, rows > 32 ? (int64_t)64 : rows > 16 ? (int64_t)32 : (int64_t)16));
+    if (rows > most) large += ceil_div(rows, 256);
+    else p.few_rows = std::max<int64_t>(p.few_rows, rows > 32 ? 64 : rows > 16 ? 32 : 16);
   }
   ANNA_CHECK(p.tokens * G <= INT_MAX / 2, "span: too many tokens");
-  // a record for each tile, then the items that share its pages
-  int64_t offset = 0, total = 0;
+  // a wave takes 32 rows: workgroups of 8 share a page's conversion among twice as many rows as those of
+  // 4, which there are twice as many of
+  if (large * H >= TILE_FILL) p.tile_rows = 256;
+  int64_t offset = 0, total[2] = {0, 0}, tiles[2] = {0, 0}, rows_of[2] = {0, 0};
   for (int64_t i = 0; i < n; i++) {
-    const int64_t rows = counts[i] * G, R = p.few_rows;
-    const int64_t tiles = std::max<int64_t>(1, ceil_div(rows, R));
-    for (int64_t t = 0; t < tiles; t++) {
+    const int64_t rows = counts[i] * G, f = rows > most, R = f ? p.tile_rows : p.few_rows;
+    for (int64_t t = 0; t < std::max<int64_t>(1, ceil_div(rows, R)); t++) {
       Record r = {};
       r.index = (int32_t)i, r.row = seqs[i], r.start = (int32_t)starts[i], r.count = (int32_t)counts[i];
-      r.offset = (int32_t)offset, r.tile = (int32_t)t;
+      r.offset = (int32_t)offset, r.tile = (int32_t)t, r.tiled = (int32_t)f;
       r.pages = rows ? (int32_t)((starts[i] + (std::min(rows, (t + 1) * R) - 1) / G) / PAGE + 1) : 0;
       r.touch0 = (int32_t)p.touches;
-      total += r.pages;
+      total[f] += r.pages;
+      tiles[f]++;
+      rows_of[f] = std::max(rows_of[f], std::min(rows, R));
       p.records.push_back(r);
     }
     if (counts[i] > 0) p.touches += (starts[i] + counts[i] - 1) / PAGE - starts[i] / PAGE + 1;
     if (counts[i] > 0) p.touch_bound += (counts[i] + PAGE - 2) / PAGE + 1;
     offset += counts[i];
   }
-  const int64_t target = std::max<int64_t>(1, SPLIT_TARGET / H), per = std::max<int64_t>(1, ceil_div(total, target));
-  int64_t most_rows = 0;
+  // Tiles of the tile form in falling order of their pages, so that the long ones start first.
+  if (tiles[1] > 1)
+    std::stable_sort(p.records.begin(), p.records.end(), [](const Record& a, const Record& b) {
+      return a.tiled != b.tiled ? a.tiled < b.tiled : a.tiled && a.pages > b.pages;
+    });
+  // How many pages an item takes: the split form's are shared out to SPLIT_TARGET workgroups, the tile form's
+  // only while there are too few tiles for the chip, and not below TILE_PAGES, as an item's partial result
+  // is written and read again.
+  const int64_t target[2] = {std::max<int64_t>(1, SPLIT_TARGET / H), std::max<int64_t>(1, TILE_TARGET / H)};
+  const int64_t per[2] = {std::max<int64_t>(1, ceil_div(total[0], target[0])),
+                          tiles[1] >= target[1] ? INT_MAX : std::max<int64_t>(TILE_PAGES, ceil_div(total[1], target[1]))};
   for (Record& r : p.records) {
-    const int64_t rows = std::min<int64_t>(p.few_rows, r.count * G - r.tile * p.few_rows);
-    r.item0 = (int32_t)p.split_items;
-    r.splits = (int32_t)ceil_div(r.pages, per);
+    const int f = r.tiled;
+    const int64_t R = f ? p.tile_rows : p.few_rows, rows = std::min<int64_t>(R, r.count * G - r.tile * R);
+    r.item0 = (int32_t)p.items[f];
+    r.splits = (int32_t)(f ? std::max<int64_t>(1, (r.pages + per[1] / 2) / per[1]) : ceil_div(r.pages, per[0]));
     r.part = -1;
     r.unit = -1;
     if (r.splits > 1) {
@@ -180,12 +197,16 @@ int make_plan(anna_mi_paged* h, int64_t n, const int32_t* seqs, const int64_t* s
       p.partial_rows += r.splits * rows;
       p.unit_rows = std::max(p.unit_rows, rows);
     }
-    most_rows = std::max(most_rows, rows);
-    p.split_items += r.splits;
+    p.items[f] += r.splits;
   }
-  p.split_bound = total ? (int64_t)p.records.size() + target : 0;
-  p.partial_bound = std::min(p.split_bound, 2 * target) * most_rows;  // a tile that is split has more than `per` pages
-  ANNA_CHECK(p.partial_bound <= INT_MAX && p.split_bound <= INT_MAX / 64 && H * p.split_bound <= INT_MAX, "span: too many tokens");
+  // a tile that is split has more than `per` pages, so the items of such tiles are at most 2 * target
+  for (int f = 0; f < 2; f++)
+    if (rows_of[f] > 0) {
+      const bool splits = f == 0 || tiles[1] < target[1];
+      p.bound[f] = tiles[f] + (splits ? target[f] : 0);
+      if (splits) p.partial_bound += std::min(p.bound[f], 2 * target[f]) * rows_of[f];
+    }
+  ANNA_CHECK(p.partial_bound <= INT_MAX && H * (p.bound[0] + p.bound[1]) <= INT_MAX / 64, "span: too many tokens");
   return ANNA_MI_OK;
 }
 
@@ -461,10 +482,11 @@ int anna_mi_paged_span_plan(anna_mi_paged* h, int64_t n, const int32_t* seqs, co
     span->sequences = n;
     span->tokens = p.tokens;
     span->few_rows = p.few_rows;
-    span->split_capacity = p.split_bound;
+    span->tile_rows = p.tile_rows;
+    span->split_capacity = p.bound[0];
     span->unit_capacity = (int64_t)p.records.size();
     span->touch_capacity = p.touch_bound;
-    span->tile_capacity = p.tile_items;
+    span->tile_capacity = p.bound[1];
     span->partial_rows = p.partial_bound;
     span->words = sections(*span).words;
     return ANNA_MI_OK;
@@ -478,13 +500,13 @@ int anna_mi_paged_span_fill(anna_mi_paged* h, int64_t n, const int32_t* seqs, co
     Plan p;
     const int rc = make_plan(h, n, seqs, starts, counts, p);
     if (rc != ANNA_MI_OK) return rc;
-    ANNA_CHECK(n == span->sequences && p.tokens == span->tokens && p.few_rows == span->few_rows && p.split_items <= span->split_capacity &&
-                   p.tile_items <= span->tile_capacity && (int64_t)p.records.size() <= span->unit_capacity &&
+    ANNA_CHECK(n == span->sequences && p.tokens == span->tokens && p.few_rows == span->few_rows && p.tile_rows == span->tile_rows &&
+                   p.items[0] <= span->split_capacity && p.items[1] <= span->tile_capacity && (int64_t)p.records.size() <= span->unit_capacity &&
                    p.touches <= span->touch_capacity && p.partial_rows <= span->partial_rows && sections(*span).words <= span->words,
                "span: these tokens do not fit the span that is filled");
     ANNA_CHECK(p.partial_rows == 0 || (span->partial_stats && span->partial_values), "paged_span_fill: null partials");
-    span->split_items = p.split_items;
-    span->tile_items = p.tile_items;
+    span->split_items = p.items[0];
+    span->tile_items = p.items[1];
     span->split_units = p.units;
     span->split_rows = p.unit_rows;
     span->touch_items = p.touches;
@@ -492,12 +514,12 @@ int anna_mi_paged_span_fill(anna_mi_paged* h, int64_t n, const int32_t* seqs, co
     const Sections at = sections(*span);
     Update& u = up.u;
     u.buf = span->buf;
-    u.header[0] = (int32_t)p.split_items, u.header[1] = (int32_t)p.tile_items, u.header[2] = (int32_t)p.units;
+    u.header[0] = (int32_t)p.items[0], u.header[1] = (int32_t)p.items[1], u.header[2] = (int32_t)p.units;
     u.header[3] = (int32_t)p.touches;
     u.rows_at = at.rows, u.split_at = at.split, u.tile_at = at.tile, u.units_at = at.units, u.touch_at = at.touch;
     u.group = (int32_t)(h->d.q_heads / h->d.kv_heads);
     u.split_rows = (int32_t)p.few_rows;
-    u.tile_rows = tile_rows(h->d.head_dim);
+    u.tile_rows = (int32_t)p.tile_rows;
     up.records.resize(p.records.size() * (sizeof(Record) / 4));
     if (!p.records.empty()) memcpy(up.records.data(), p.records.data(), p.records.size() * sizeof(Record));
     return up.launch();
@@ -572,10 +594,12 @@ int anna_mi_paged_attend(anna_mi_paged* h, int64_t layer, const anna_mi_paged_sp
     a.scale = scaling * 1.44269504088896340736f;
     a.kv_heads = (int32_t)h->d.kv_heads;
     a.group = (int32_t)(h->d.q_heads / h->d.kv_heads);
-    const bool all = capacity_grid != 0;
-    return launch_attend(h->d.dtype, h->d.head_dim, a, all ? span->split_capacity : span->split_items, span->few_rows,
-                         all ? span->tile_capacity : span->tile_items, all ? span->unit_capacity : span->split_units,
-                         all ? span->few_rows : span->split_rows, as_stream(stream));
+    Grid g = {span->split_items, span->few_rows, span->tile_items, span->tile_rows, span->split_units, span->split_rows};
+    if (capacity_grid) {
+      g.split_items = span->split_capacity, g.tile_items = span->tile_capacity, g.units = span->unit_capacity;
+      g.unit_rows = span->tile_capacity > 0 ? span->tile_rows : span->few_rows;
+    }
+    return launch_attend(h->d.dtype, h->d.head_dim, a, g, as_stream(stream));
   });
 }
 

@@ -15,7 +15,7 @@ __global__ __launch_bounds__(256) void paged_update_kernel(const Update u) {
   if (blk < u.records) {
     const Record r = reinterpret_cast<const Record*>(words)[blk];
     if (blk == 0 && tid < 4) u.buf[tid] = u.header[tid];
-    const int rows = min(u.split_rows, r.count * u.group - r.tile * u.split_rows);
+    const int R = r.tiled ? u.tile_rows : u.split_rows, rows = min(R, r.count * u.group - r.tile * R);
     if (r.tile == 0) {
       if (tid == 0) u.buf[u.rows_at + r.index] = r.row;
       const int first = r.start / PAGE, pages = r.count > 0 ? (r.start + r.count - 1) / PAGE - first + 1 : 0;
@@ -25,14 +25,14 @@ __global__ __launch_bounds__(256) void paged_update_kernel(const Update u) {
         touch[k] = Touch{r.row, p, t0 - p * PAGE, t1 - p * PAGE, r.offset + t0 - r.start, {0, 0, 0}};
       }
     }
-    Item* items = reinterpret_cast<Item*>(u.buf + u.split_at) + r.item0;
+    Item* items = reinterpret_cast<Item*>(u.buf + (r.tiled ? u.tile_at : u.split_at)) + r.item0;
     for (int k = tid; k < r.splits; k += 256) {
       const int p0 = (int)((int64_t)r.pages * k / r.splits), p1 = (int)((int64_t)r.pages * (k + 1) / r.splits);
       items[k] = Item{r.row, r.start, r.count, r.offset, p0, p1, r.part < 0 ? -1 : r.part + k * rows, r.tile};
     }
     if (r.unit >= 0 && tid == 0)
       reinterpret_cast<Unit*>(u.buf + u.units_at)[r.unit] =
-          Unit{r.offset, r.tile * u.split_rows, rows, r.part, r.splits, {0, 0, 0}};
+          Unit{r.offset, r.tile * R, rows, r.part, r.splits, {0, 0, 0}};
     return;
   }
   blk -= u.records;
@@ -179,9 +179,9 @@ __global__ __launch_bounds__(256) void paged_store_kernel(uint8_t* __restrict__ 
     if (c % 8 == 0) {
       const int at = ((token / 4) * NG + g) * 4 + token % 4;
       ((uint16_t*)(page + K_SCALES * D))[at] = k.scale;
-      ((uint16_t*)(page + K_OFFSETS * D))[token * NG + g] = f32_to_bf16_bits((float)(k.zero - 128));
+      ((uint16_t*)(page + K_OFFSETS * D))[token * NG + g] = f32_to_bf16_bits((float)(k.zero - CODE_BASE));
       ((uint16_t*)(page + V_SCALES * D))[at] = v.scale;
-      ((uint16_t*)(page + V_OFFSETS * D))[at] = f32_to_bf16_bits((float)(v.zero - 128));
+      ((uint16_t*)(page + V_OFFSETS * D))[at] = f32_to_bf16_bits((float)(v.zero - CODE_BASE));
     }
   }
   __syncthreads();
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(256) void paged_store_kernel(uint8_t* __restrict__ 
 
 // 8 codes (bytes) of a group to values of the dense type: exact in fp32, then rounded once.
 template <int DT> __device__ __forceinline__ u32x4 expand(uint32_t lo, uint32_t hi, uint16_t scale, uint16_t offset) {
-  const float s = bf16_bits_to_f32(scale), z = bf16_bits_to_f32(offset) + 128.0f;
+  const float s = bf16_bits_to_f32(scale), z = bf16_bits_to_f32(offset) + (float)CODE_BASE;
   u32x4 out;
 #pragma unroll
   for (int k = 0; k < 4; k++) {

@@ -687,7 +687,7 @@ int anna_mi_moe_grouped_int4_mlp(const anna_mi_moe_mlp_args* args, void* stream)
  *                r = lane % 16) of group g holds dim 64 g + 16 w + r of the tokens 4 q + e (e < 4)
  *                and 16 + 4 q + e - 4 (e >= 4), at the same bits
  *   key scales   bf16 [16][NG][4] (token 4 i + j of group g at [i][g][j])
- *   key offsets  bf16 [64][NG], the whole number zero - 128
+ *   key offsets  bf16 [64][NG], the whole number zero - 16
  *   value scales, value offsets   bf16 [16][NG][4] each
  * Values' scales and offsets are finite wherever the pool was zeroed first and written by these
  * calls, also behind the last token.
@@ -711,7 +711,7 @@ typedef struct {
   int64_t split_items, split_units, split_rows, touch_items; /* sizes of this fill */
   int64_t split_capacity, unit_capacity, touch_capacity;     /* and of the buffer's sections */
   int64_t tile_items, tile_capacity;
-  int64_t few_rows; /* query rows of a tile of the split form: 16, 32 or 64 */
+  int64_t few_rows, tile_rows; /* query rows of a tile: of the split form 16, 32 or 64, of the tile form 128 or 256 */
   int32_t* buf;
   float* partial_stats;  /* [partial_rows][kv_heads][2] */
   float* partial_values; /* [partial_rows][kv_heads][head_dim] */
