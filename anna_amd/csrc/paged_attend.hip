@@ -339,46 +339,48 @@ template <int D> __device__ __forceinline__ void load_values(Share<D>& s, const 
   }
 }
 
-// To LDS; true if a scale is beyond what fp16 holds.
-template <int D, bool F16> __device__ __forceinline__ bool put_keys(const Share<D>& s, u32x4* lds, int quarter, int lane) {
-  constexpr int NG = D / GROUP, KW = D / 32;
-  const int q = lane / 16, r = lane % 16, row = 16 * (r / 8) + 8 * (quarter & 1) + r % 8;
+// Whether fp16 holds the operands that these scales make.
+template <int D> __device__ __forceinline__ bool keys_wide(const Share<D>& s) {
   bool wide = false;
 #pragma unroll
-  for (int g = 0; g < NG; g++) {
-    const float scale = bf16_bits_to_f32(s.ks[g]), offset = bf16_bits_to_f32(s.ko[g]);
-    wide |= scale > K_SCALE_MOST;
-    const f16x2 s2 = {(_Float16)scale, (_Float16)scale}, o2 = {(_Float16)offset, (_Float16)offset};
+  for (int g = 0; g < D / GROUP; g++) wide |= bf16_bits_to_f32(s.ks[g]) > K_SCALE_MOST;
+  return wide;
+}
+template <int D> __device__ __forceinline__ bool values_wide(const Share<D>& s) {
+  const uint32_t sw[4] = {s.vs[0].x, s.vs[0].y, s.vs[1].x, s.vs[1].y};
+  bool wide = false;
 #pragma unroll
-    for (int k = 2 * g; k < 2 * g + 2; k++)
-      lds[((quarter / 2) * 2 * KW + 2 * k + q / 2) * 64 + (q & 1) * 32 + row] =
-          F16 ? dense_f16(s.kw[k], &o2, &s2, 0) : dense_bf16(s.kw[k], &offset, &scale, 0);
+  for (int k = 0; k < 4; k++) {
+    const float x = bf16_lo(sw[k]), y = bf16_hi(sw[k]);
+    wide |= fmaxf(x, y) > V_SCALE_MOST || (x < V_SCALE_LEAST && x > 0.0f) || (y < V_SCALE_LEAST && y > 0.0f);
   }
   return wide;
 }
-template <int D, bool F16> __device__ __forceinline__ bool put_values(const Share<D>& s, u32x4* lds, int unit, int lane) {
+
+// Word k of a thread's keys / values to LDS.
+template <int D, bool F16> __device__ __forceinline__ void put_key(const Share<D>& s, u32x4* lds, int quarter, int k, int lane) {
+  constexpr int KW = D / 32;
+  const int q = lane / 16, r = lane % 16, row = 16 * (r / 8) + 8 * (quarter & 1) + r % 8;
+  const float scale = bf16_bits_to_f32(s.ks[k / 2]), offset = bf16_bits_to_f32(s.ko[k / 2]);
+  const f16x2 s2 = {(_Float16)scale, (_Float16)scale}, o2 = {(_Float16)offset, (_Float16)offset};
+  lds[((quarter / 2) * 2 * KW + 2 * k + q / 2) * 64 + (q & 1) * 32 + row] =
+      F16 ? dense_f16(s.kw[k], &o2, &s2, 0) : dense_bf16(s.kw[k], &offset, &scale, 0);
+}
+template <int D, bool F16> __device__ __forceinline__ void put_value(const Share<D>& s, u32x4* lds, int unit, int w, int lane) {
   constexpr int NG = D / GROUP;
   const int half = unit / NG, g = unit % NG, q = lane / 16, r = lane % 16;
   const uint32_t sw[4] = {s.vs[0].x, s.vs[0].y, s.vs[1].x, s.vs[1].y}, ow[4] = {s.vo[0].x, s.vo[0].y, s.vo[1].x, s.vo[1].y};
-  bool wide = false;
   float scale[8], offset[8];
   f16x2 s2[4], o2[4];
 #pragma unroll
   for (int k = 0; k < 4; k++) {
     scale[2 * k] = bf16_lo(sw[k]), scale[2 * k + 1] = bf16_hi(sw[k]);
     offset[2 * k] = bf16_lo(ow[k]), offset[2 * k + 1] = bf16_hi(ow[k]);
-    s2[k] = f16x2{(_Float16)scale[2 * k], (_Float16)scale[2 * k + 1]};
-    o2[k] = f16x2{(_Float16)offset[2 * k], (_Float16)offset[2 * k + 1]};
+    s2[k] = f16_pair(sw[k]);
+    o2[k] = f16_pair(ow[k]);
   }
-  if (F16) {
-#pragma unroll
-    for (int k = 0; k < 8; k++) wide |= scale[k] > V_SCALE_MOST || (scale[k] < V_SCALE_LEAST && scale[k] > 0.0f);
-  }
-#pragma unroll
-  for (int w = 0; w < 4; w++)
-    lds[((half * (D / 32) + 2 * g + w / 2) * 2 + q / 2) * 64 + (q & 1) * 32 + (w & 1) * 16 + r] =
-        F16 ? dense_f16(s.vw[w], o2, s2, 1) : dense_bf16(s.vw[w], offset, scale, 1);
-  return wide;
+  lds[((half * (D / 32) + 2 * g + w / 2) * 2 + q / 2) * 64 + (q & 1) * 32 + (w & 1) * 16 + r] =
+      F16 ? dense_f16(s.vw[w], o2, s2, 1) : dense_bf16(s.vw[w], offset, scale, 1);
 }
 
 // LDS of a buffer: keys then values, 128 * D bytes each.
@@ -391,19 +393,34 @@ template <int D> struct Rows {
 };
 
 // One page in LDS for a wave's rows.  limit: tokens of the page that the lane's query sees; cut: whether any lane's
-// is below PAGE.
-template <int D, bool F16, class Q>
-__device__ __forceinline__ void take_page(Rows<D>& w, const u32x4* lds, Q query, int limit, bool cut, float scale, int lane) {
+// is below PAGE.  Fragments are read one step ahead of the matrix instructions that take them, and the order of the
+// steps is pinned: left to itself the compiler reads all of them first and spills.  side(k) is work for the vector
+// unit that runs beneath step k's matrix instructions.
+#define PIN() __builtin_amdgcn_sched_barrier(0)
+template <int D, bool F16, class Q, class S>
+__device__ __forceinline__ void take_page(Rows<D>& w, const u32x4* lds, Q query, int limit, bool cut, float scale, int lane, S side) {
   constexpr int KSTEPS = D / 16, DTILES = D / 32;
   const int hl = lane / 32;
   const u32x4* values = lds + 8 * D;
   f32x16 z[2];
 #pragma unroll
-  for (int half = 0; half < 2; half++) {
+  for (int half = 0; half < 2; half++)
 #pragma unroll
     for (int j = 0; j < 16; j++) z[half][j] = 0;
+  u32x4 f[2][2];
 #pragma unroll
-    for (int s = 0; s < KSTEPS; s++) z[half] = mfma32<F16>(lds[(half * KSTEPS + s) * 64 + lane], query(s), z[half]);
+  for (int half = 0; half < 2; half++) f[0][half] = lds[half * KSTEPS * 64 + lane];
+#pragma unroll
+  for (int s = 0; s < KSTEPS; s++) {
+    if (s + 1 < KSTEPS) {
+#pragma unroll
+      for (int half = 0; half < 2; half++) f[(s + 1) & 1][half] = lds[(half * KSTEPS + s + 1) * 64 + lane];
+    }
+    const u32x4 q = query(s);
+#pragma unroll
+    for (int half = 0; half < 2; half++) z[half] = mfma32<F16>(f[s & 1][half], q, z[half]);
+    side(s);
+    PIN();
   }
   if (cut) {
 #pragma unroll
@@ -443,17 +460,35 @@ __device__ __forceinline__ void take_page(Rows<D>& w, const u32x4* lds, Q query,
       } else p[k][e] = pack_bf16(x, y);
     }
   w.l += sum;
+  PIN();
+  // steps of two dim tiles
+  constexpr int STEPS = 4 * DTILES / 2;
+  auto fragment = [&](int step, int u) {
+    const int k = step / (DTILES / 2), d = 2 * (step % (DTILES / 2)) + u;
+    return values[(((k / 2) * DTILES + d) * 2 + (k & 1)) * 64 + lane];
+  };
 #pragma unroll
-  for (int k = 0; k < 4; k++)
+  for (int u = 0; u < 2; u++) f[0][u] = fragment(0, u);
 #pragma unroll
-    for (int d = 0; d < DTILES; d++) w.acc[d] = mfma32<F16>(values[(((k / 2) * DTILES + d) * 2 + (k & 1)) * 64 + lane], p[k], w.acc[d]);
+  for (int step = 0; step < STEPS; step++) {
+    if (step + 1 < STEPS) {
+#pragma unroll
+      for (int u = 0; u < 2; u++) f[(step + 1) & 1][u] = fragment(step + 1, u);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const int d = 2 * (step % (DTILES / 2)) + u;
+      w.acc[d] = mfma32<F16>(f[step & 1][u], p[step / (DTILES / 2)], w.acc[d]);
+    }
+    PIN();
+  }
 }
 
-template <int DT, int D, int NW, int BUFFERS>
+template <int DT, int D, int NW>
 __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
   constexpr int NG = D / GROUP, KSTEPS = D / 16, UNITS = 2 * NG;
-  constexpr int KEYS = (4 + NW - 1) / NW, VALUES = (UNITS + NW - 1) / NW, SHARES = KEYS > VALUES ? KEYS : VALUES;
-  __shared__ __align__(16) u32x4 lds[BUFFERS * buffer_words<D>()];
+  constexpr int KEYS = 1, VALUES = (UNITS + NW - 1) / NW, SHARES = VALUES;
+  __shared__ __align__(16) u32x4 lds[2 * buffer_words<D>()];
   __shared__ int wide[4];  // by page % 4: a scale is beyond what fp16 holds
   const int H = a.kv_heads, G = a.group;
   const int h = blockIdx.x % H, index = blockIdx.x / H;
@@ -516,17 +551,28 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
       if (unit < UNITS) load_values(share[k], page, unit, lane);
     }
   };
-  auto put = [&](u32x4* to, int slot) {
+  auto check = [&](int slot) {
     bool beyond = false;
 #pragma unroll
     for (int k = 0; k < KEYS; k++)
-      if (wave + k * NW < 4) beyond |= put_keys<D, true>(share[k], to, wave + k * NW, lane);
+      if (wave + k * NW < 4) beyond |= keys_wide(share[k]);
 #pragma unroll
-    for (int k = 0; k < VALUES; k++) {
-      const int unit = NW - 1 - wave + k * NW;
-      if (unit < UNITS) beyond |= put_values<D, true>(share[k], to + 8 * D, unit, lane);
-    }
+    for (int k = 0; k < VALUES; k++)
+      if (NW - 1 - wave + k * NW < UNITS) beyond |= values_wide(share[k]);
     if (beyond) wide[slot] = 1;
+  };
+  // word k of this thread's keys and of its values (with 8 waves a wave has only one of the two)
+  constexpr int WORDS = NW == 8 ? (D / 32 > 4 ? D / 32 : 4) : D / 32 + 4 * VALUES;
+  auto put_word = [&](u32x4* to, int k) {
+    if (NW == 8) {
+      if (wave < 4) {
+        if (k < D / 32) put_key<D, true>(share[0], to, wave, k, lane);
+      } else if (k < 4 && NW - 1 - wave < UNITS) put_value<D, true>(share[0], to + 8 * D, NW - 1 - wave, k, lane);
+    } else if (k < D / 32) put_key<D, true>(share[0], to, wave, k, lane);
+    else {
+      const int n = (k - D / 32) / 4, unit = NW - 1 - wave + n * NW;
+      if (unit < UNITS) put_value<D, true>(share[n], to + 8 * D, unit, (k - D / 32) % 4, lane);
+    }
   };
   // LDS only: loads of the next page stay in flight
   auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
@@ -536,42 +582,51 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
   const int sees = valid ? it.start + t + 1 : 0;
 
   load(page_of(it.page0));
-  if (BUFFERS == 2) {
-    put(lds, it.page0 & 3);
-    if (it.page0 + 1 < it.page1) load(page_of(it.page0 + 1));
-    barrier();
-  }
+  check(it.page0 & 3);
+#pragma unroll
+  for (int k = 0; k < WORDS; k++) put_word(lds, k);
+  if (it.page0 + 1 < it.page1) load(page_of(it.page0 + 1));
+  barrier();
   for (int p = it.page0; p < it.page1; p++) {
-    const int turn = BUFFERS == 2 ? (p - it.page0) & 1 : 0;
-    u32x4* now = lds + turn * buffer_words<D>();
+    const int turn = (p - it.page0) & 1;
+    u32x4 *now = lds + turn * buffer_words<D>(), *then = lds + (turn ^ 1) * buffer_words<D>();
+    const bool more = p + 1 < it.page1, slow = all_wide || wide[p & 3] != 0;
     if (threadIdx.x == 0) wide[(p + 2) & 3] = 0;
-    if (BUFFERS == 2) {
-      if (p + 1 < it.page1) put(lds + (turn ^ 1) * buffer_words<D>(), (p + 1) & 3);
-      if (p + 2 < it.page1) load(page_of(p + 2));
-    } else {
-      put(now, p & 3);
-      if (p + 1 < it.page1) load(page_of(p + 1));
-      barrier();
-    }
-    const bool slow = all_wide || wide[p & 3] != 0;
+    if (more) check((p + 1) & 3);
     const int limit = sees - p * PAGE;
-    if (!slow) {
-      if (p * PAGE < last) take_page<D, true>(w, now, fast_query, limit, p * PAGE + PAGE > first, a.scale, lane);
+    constexpr int PER = (WORDS + KSTEPS - 1) / KSTEPS;
+    auto side = [&](int s) {
+      if (more) {
+#pragma unroll
+        for (int k = s * PER; k < (s + 1) * PER; k++)
+          if (k < WORDS) put_word(then, k);
+      }
+    };
+    const bool mine = p * PAGE < last;
+    if (mine && !slow) {
+      take_page<D, true>(w, now, fast_query, limit, p * PAGE + PAGE > first, a.scale, lane, side);
     } else {
+#pragma unroll
+      for (int s = 0; s < KSTEPS; s++) side(s);
+    }
+    if (p + 2 < it.page1) load(page_of(p + 2));
+    if (slow) {
       // the page again, as bf16
       barrier();
       const uint8_t* page = page_of(p);
       Share<D> again;
       for (int k = wave; k < 4; k += NW) {
         load_keys(again, page, k, lane);
-        put_keys<D, false>(again, now, k, lane);
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) put_key<D, false>(again, now, k, i, lane);
       }
       for (int k = wave; k < UNITS; k += NW) {
         load_values(again, page, k, lane);
-        put_values<D, false>(again, now + 8 * D, k, lane);
+#pragma unroll
+        for (int i = 0; i < 4; i++) put_value<D, false>(again, now + 8 * D, k, i, lane);
       }
       barrier();
-      if (p * PAGE < last) take_page<D, false>(w, now, slow_query, limit, p * PAGE + PAGE > first, a.scale, lane);
+      if (mine) take_page<D, false>(w, now, slow_query, limit, p * PAGE + PAGE > first, a.scale, lane, [](int) {});
     }
     barrier();
   }
@@ -640,8 +695,8 @@ template <int DT, int D> int launch(const Attend& a, const Grid& g, hipStream_t 
     }
   }
   if (tile > 0) {
-    if (g.tile_rows == 256) paged_tile_kernel<DT, D, 8, 2><<<tile, 512, 0, stream>>>(a);
-    else paged_tile_kernel<DT, D, 4, D == 256 ? 1 : 2><<<tile, 256, 0, stream>>>(a);
+    if (g.tile_rows == 128) paged_tile_kernel<DT, D, 4><<<tile, 256, 0, stream>>>(a);
+    else if constexpr (D <= 128) paged_tile_kernel<DT, D, 8><<<tile, 512, 0, stream>>>(a);
   }
   if (g.units > 0) paged_merge_kernel<DT, D><<<dim3((unsigned)(g.units * a.kv_heads), (unsigned)g.unit_rows), 256, 0, stream>>>(a);
   ANNA_LAUNCH_CHECK("paged attend");

@@ -32,7 +32,7 @@ struct anna_mi_paged {
 namespace {
 
 // Workgroups that an attention launch is split into at most, over all KV heads (and the tiles themselves).
-constexpr int64_t SPLIT_TARGET = 1024, TILE_TARGET = 512, TILE_FILL = 256, TILE_PAGES = 8;
+constexpr int64_t SPLIT_TARGET = 1024, TILE_TARGET = 512, TILE_FILL = 256, TILE_PAGES = 8, TILE_LEAST = 64;
 
 int hip_ok(hipError_t e, const char* what) { return e == hipSuccess ? ANNA_MI_OK : fail_hip(e, what); }
 
@@ -149,16 +149,16 @@ int make_plan(anna_mi_paged* h, int64_t n, const int32_t* seqs, const int64_t* s
                (long long)(starts[i] + counts[i]), (int)seqs[i], (long long)h->length[seqs[i]]);
     p.tokens += counts[i];
     const int64_t rows = counts[i] * G;
-    if (rows > most) large += ceil_div(rows, 256);
-    else p.few_rows = std::max<int64_t>(p.few_rows, rows > 32 ? 64 : rows > 16 ? 32 : 16);
+    if (rows > TILE_LEAST) large += ceil_div(rows, 256);
+    else p.few_rows = std::max(p.few_rows, std::min<int64_t>(most, rows > 32 ? 64 : rows > 16 ? 32 : 16));
   }
   ANNA_CHECK(p.tokens * G <= INT_MAX / 2, "span: too many tokens");
   // a wave takes 32 rows: workgroups of 8 share a page's conversion among twice as many rows as those of
   // 4, which there are twice as many of
-  if (large * H >= TILE_FILL) p.tile_rows = 256;
+  if (large * H >= TILE_FILL && h->d.head_dim < 256) p.tile_rows = 256;
   int64_t offset = 0, total[2] = {0, 0}, tiles[2] = {0, 0}, rows_of[2] = {0, 0};
   for (int64_t i = 0; i < n; i++) {
-    const int64_t rows = counts[i] * G, f = rows > most, R = f ? p.tile_rows : p.few_rows;
+    const int64_t rows = counts[i] * G, f = rows > TILE_LEAST, R = f ? p.tile_rows : p.few_rows;
     for (int64_t t = 0; t < std::max<int64_t>(1, ceil_div(rows, R)); t++) {
       Record r = {};
       r.index = (int32_t)i, r.row = seqs[i], r.start = (int32_t)starts[i], r.count = (int32_t)counts[i];
