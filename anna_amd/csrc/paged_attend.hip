@@ -5,7 +5,7 @@
 //
 // Split form.  A workgroup takes the query rows of one KV head (R = 16, 32 or 64 rows: tokens times
 // query heads of that KV head) and some of the sequence's pages; each of its four waves takes every
-// fourth page with an online softmax of its own, and the waves' results are joined at the end.
+// fourth step (a page, or half of one) with an online softmax of its own, and the waves' results are joined at the end.
 // Codes go to the matrix cores as whole numbers: 16 + code has the bits 0x4180 | code << 3 in bf16
 // (in fp16 0x4C00 | code << 6), so 8 codes cost 8 instructions and no conversion.  With
 // o = zero - 16 (the cache's offsets, exact in bf16)
@@ -18,6 +18,8 @@
 //   tokens of its query.  O^T = V^T P^T: the lane's eight tokens of two such tiles are its eight k of
 //   the second product, so P never leaves the lane; the value codes are stored in that order.
 // For fp16 activations ps is split into two bf16 terms: one alone is coarser than the output's type.
+#include <type_traits>
+
 #include "paged.hpp"
 
 namespace anna {
@@ -36,36 +38,44 @@ template <int DT> __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 
   else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
+// The mask of codes16 in a vector register of its own: with it there, a mask and a merge are one instruction
+// (v_and_or_b32 takes one operand that is no vector register).
+template <int DT> __device__ __forceinline__ uint32_t code_mask() {
+  uint32_t mask = DT == ANNA_MI_BF16 ? 0x00780078u : 0x03C003C0u;
+  asm volatile("" : "+v"(mask));
+  return mask;
+}
 // 16 + code of the 8 codes of a word, as operand elements of the type.
-template <int DT> __device__ __forceinline__ u32x4 codes16(uint32_t w) {
+template <int DT> __device__ __forceinline__ u32x4 codes16(uint32_t w, uint32_t mask) {
   if constexpr (DT == ANNA_MI_BF16)
-    return u32x4{((w << 3) & 0x00780078u) | 0x41804180u, ((w >> 1) & 0x00780078u) | 0x41804180u,
-                 ((w >> 5) & 0x00780078u) | 0x41804180u, ((w >> 9) & 0x00780078u) | 0x41804180u};
+    return u32x4{((w << 3) & mask) | 0x41804180u, ((w >> 1) & mask) | 0x41804180u, ((w >> 5) & mask) | 0x41804180u,
+                 ((w >> 9) & mask) | 0x41804180u};
   else
-    return u32x4{((w << 6) & 0x03C003C0u) | 0x4C004C00u, ((w << 2) & 0x03C003C0u) | 0x4C004C00u,
-                 ((w >> 2) & 0x03C003C0u) | 0x4C004C00u, ((w >> 6) & 0x03C003C0u) | 0x4C004C00u};
+    return u32x4{((w << 6) & mask) | 0x4C004C00u, ((w << 2) & mask) | 0x4C004C00u, ((w >> 2) & mask) | 0x4C004C00u,
+                 ((w >> 6) & mask) | 0x4C004C00u};
 }
 
 __device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-  return f32_to_bf16_bits(a) | (uint32_t)f32_to_bf16_bits(b) << 16;
+  const bf16x2 v = {(__bf16)a, (__bf16)b};
+  return __builtin_bit_cast(uint32_t, v);
 }
 
 // 2^x of the difference to a running maximum that may still be -inf.
 __device__ __forceinline__ float weight(float m, float top) { return m == NEG ? 0.0f : __builtin_amdgcn_exp2f(m - top); }
 
-template <int DT> __device__ __forceinline__ float gated(float v, const void* gate, int64_t at) {
-  const float g = Elem<DT>::to_f32(((const uint16_t*)gate)[at]);
-  return v / (1.0f + __expf(-g));
-}
+__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __expf(-x)); }
 
 // Four neighbouring values of an output row, gated.
 template <int DT>
 __device__ __forceinline__ void write_out(const Attend& a, int D, int64_t token, int head, int d, f32x4 v, int64_t heads) {
   if (a.gate) {
+    const u16x4 g = *(const u16x4*)((const uint16_t*)a.gate + token * a.g_token + head * a.g_head + d);
 #pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = gated<DT>(v[i], a.gate, token * a.g_token + head * a.g_head + d + i);
+    for (int i = 0; i < 4; i++) v[i] *= sigmoid(Elem<DT>::to_f32(g[i]));
   }
   u16x4 o;
 #pragma unroll
@@ -73,26 +83,85 @@ __device__ __forceinline__ void write_out(const Attend& a, int D, int64_t token,
   *(u16x4*)((uint16_t*)a.out + (token * heads + head) * D + d) = o;
 }
 
+// Tokens of a wave's step: a page, or half of one where a page's registers would leave no room for a second wave.
+template <int D, int NQ> constexpr int step_tokens() { return D == 256 || NQ > 1 ? 32 : 64; }
+
+// What a wave holds of a step's tokens in registers.  Lane offsets are unsigned 32-bit numbers, so that the page's
+// address stays in scalar registers.
+template <int D, int T> struct StepKeys {
+  static constexpr int TT = T / 16, NG = D / GROUP, KS = D / 32;
+  uint32_t code[TT][KS];
+  uint16_t offset[TT][NG];
+  uint2 scale[TT][NG];
+  __device__ __forceinline__ void load(const uint8_t* page, int half, uint32_t lane) {
+    const uint32_t q = lane / 16, r = lane % 16;
+    const uint32_t at_code = r * (D / 2) + q * (D / 8), at_scale = K_SCALES * D + q * NG * 8, at_offset = K_OFFSETS * D + r * NG * 2;
+#pragma unroll
+    for (int t = 0; t < TT; t++) {
+      const uint8_t *code_row = page + (2 * half + t) * 8 * D, *scale_row = page + (2 * half + t) * 32 * NG;
+      __builtin_memcpy(code[t], __builtin_assume_aligned(code_row + at_code, D / 8 < 16 ? D / 8 : 16), D / 8);
+      __builtin_memcpy(scale[t], __builtin_assume_aligned(scale_row + at_scale, NG > 1 ? 16 : 8), NG * 8);
+      __builtin_memcpy(offset[t], __builtin_assume_aligned(scale_row + at_offset, NG * 2), NG * 2);
+    }
+  }
+};
+template <int D, int T> struct StepValues {
+  static constexpr int HALVES = T / 32, NG = D / GROUP;
+  u32x4 code[HALVES][NG];
+  uint2 scale[HALVES][2][NG], offset[HALVES][2][NG];
+  __device__ __forceinline__ void load(const uint8_t* page, int half, uint32_t lane) {
+    const uint32_t q = lane / 16;
+    const uint32_t at_code = V_CODES * D + lane * 16, at_scale = V_SCALES * D + q * NG * 8, at_offset = V_OFFSETS * D + q * NG * 8;
+#pragma unroll
+    for (int t = 0; t < HALVES; t++) {
+      const uint8_t *code_row = page + (half + t) * 16 * D, *scale_row = page + (half + t) * 64 * NG;
+#pragma unroll
+      for (int g = 0; g < NG; g++) code[t][g] = *(const u32x4*)(code_row + g * 1024 + at_code);
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        __builtin_memcpy(scale[t][u], __builtin_assume_aligned(scale_row + u * 32 * NG + at_scale, NG > 1 ? 16 : 8), NG * 8);
+        __builtin_memcpy(offset[t][u], __builtin_assume_aligned(scale_row + u * 32 * NG + at_offset, NG > 1 ? 16 : 8), NG * 8);
+      }
+    }
+  }
+};
+
+#define PIN() __builtin_amdgcn_sched_barrier(0)
+
 // NQ: 16-row column tiles of queries.
 template <int DT, int D, int NQ>
-__global__ __launch_bounds__(256) void paged_split_kernel(const Attend a) {
-  constexpr int NG = D / GROUP, KS = D / 32, DTILES = D / 16, R = 16 * NQ;
+__global__ __launch_bounds__(256, NQ * D <= 256 ? 2 : 1) void paged_split_kernel(const Attend a) {
+  constexpr int NG = D / GROUP, KS = D / 32, DTILES = D / 16, R = 16 * NQ, T = step_tokens<D, NQ>(), TT = T / 16, STEPS = PAGE / T;
   constexpr bool TWO = DT == ANNA_MI_F16;  // ps as two bf16 terms
   __shared__ __align__(16) float joined[4][16][D + 4];
   __shared__ float wave_m[4][16], wave_l[4][16];
 
   const int H = a.kv_heads, G = a.group;
   const int h = blockIdx.x % H, index = blockIdx.x / H;
-  if (index >= a.header[0]) return;
   const Item it = a.split[index];
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, q = lane / 16, r = lane % 16;
+  if (index >= a.header[0]) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, q = lane / 16, r = lane % 16;
   const int rows = it.count * G;
   const int32_t* table = a.table + it.row * a.width;
+  auto page_at = [&](int32_t page) { return a.pool + ((int64_t)page * H + h) * page_bytes(D); };
+
+  // Steps wave, wave + 4, ...  A step's keys are asked for as soon as the last step's are used up, its values
+  // likewise: the loads have the other half of the step to arrive in, and need no second set of registers.
+  int step = it.page0 * STEPS + wave;
+  const int end = it.page1 * STEPS;
+  StepKeys<D, T> k;
+  StepValues<D, T> v;
+  if (step < end) {
+    const uint8_t* page = page_at(table[step / STEPS]);
+    k.load(page, step % STEPS, lane);
+    v.load(page, step % STEPS, lane);
+  }
+  int32_t next = step + 4 < end ? table[(step + 4) / STEPS] : 0;
 
   // queries: column r of tile n is row it.tile * R + 16 n + r
   u32x4 qf[NQ][KS];
-  u32x4 qsum[NQ][NG];  // the groups' sums as three bf16 terms in k = 0, 1, 2 of the first quarter
-  int limit[NQ];       // tokens that the query sees
+  uint2 qsum[NQ][NG];  // the groups' sums as three bf16 terms, in k = 0, 1, 2 of the first quarter
+  int limit[NQ];             // tokens that the query sees
 #pragma unroll
   for (int n = 0; n < NQ; n++) {
     const int row = it.tile * R + 16 * n + r, t = row / G, head = h * G + row % G;
@@ -101,6 +170,10 @@ __global__ __launch_bounds__(256) void paged_split_kernel(const Attend a) {
     const uint16_t* p = (const uint16_t*)a.query + (int64_t)(it.offset + t) * a.q_token + head * a.q_head + q * 8;
 #pragma unroll
     for (int s = 0; s < KS; s++) qf[n][s] = valid ? *(const u32x4*)(p + 32 * s) : u32x4{0, 0, 0, 0};
+  }
+  PIN();
+#pragma unroll
+  for (int n = 0; n < NQ; n++)
 #pragma unroll
     for (int g = 0; g < NG; g++) {
       float sum = 0;
@@ -112,9 +185,8 @@ __global__ __launch_bounds__(256) void paged_split_kernel(const Attend a) {
       sum += lane_xor16(sum);
       sum += lane_xor32(sum);
       const float hi = bf16_bits_to_f32(f32_to_bf16_bits(sum)), mid = bf16_bits_to_f32(f32_to_bf16_bits(sum - hi));
-      qsum[n][g] = q == 0 ? u32x4{pack_bf16(hi, mid), pack_bf16(sum - hi - mid, 0.0f), 0, 0} : u32x4{0, 0, 0, 0};
+      qsum[n][g] = q == 0 ? uint2{pack_bf16(hi, mid), pack_bf16(sum - hi - mid, 0.0f)} : uint2{0, 0};
     }
-  }
 
   f32x4 acc[NQ][DTILES], off[NQ][NG];
   float m[NQ], l[NQ];
@@ -127,49 +199,53 @@ __global__ __launch_bounds__(256) void paged_split_kernel(const Attend a) {
     for (int g = 0; g < NG; g++) off[n][g] = f32x4{0, 0, 0, 0};
   }
 
-  for (int p = it.page0 + wave; p < it.page1; p += 4) {
-    const uint8_t* page = a.pool + ((int64_t)table[p] * H + h) * page_bytes(D);
-    f32x4 z[NQ][4];
+  const uint32_t vmask = code_mask<ANNA_MI_BF16>(), kmask = DT == ANNA_MI_BF16 ? vmask : code_mask<DT>();
+  for (; step < end; step += 4) {
+    f32x4 z[NQ][TT];
 #pragma unroll
-    for (int tl = 0; tl < 4; tl++) {
-      const uint8_t* kc = page + (tl * 16 + r) * (D / 2) + q * (D / 8);
-      uint32_t w[KS];
-      __builtin_memcpy(w, __builtin_assume_aligned(kc, D / 8 < 16 ? D / 8 : 16), 4 * KS);
-      const uint16_t* ko = (const uint16_t*)(page + K_OFFSETS * D) + (tl * 16 + r) * NG;
-      const uint2* ks = (const uint2*)(page + K_SCALES * D) + (tl * 4 + q) * NG;
+    for (int t = 0; t < TT; t++) {
 #pragma unroll
       for (int g = 0; g < NG; g++) {
-        const uint32_t o = ko[g] * 0x10001u;
-        const uint2 s = ks[g];
-        const u32x4 a0 = codes16<DT>(w[2 * g]), a1 = codes16<DT>(w[2 * g + 1]);
+        const uint32_t o = k.offset[t][g] * 0x10001u;
+        const uint2 s = k.scale[t][g];
+        const u32x4 a0 = codes16<DT>(k.code[t][2 * g], kmask), a1 = codes16<DT>(k.code[t][2 * g + 1], kmask);
 #pragma unroll
         for (int n = 0; n < NQ; n++) {
-          f32x4 c = mfma_bf16(u32x4{o, o, 0, 0}, qsum[n][g], f32x4{0, 0, 0, 0});
+          f32x4 c = mfma_bf16(u32x4{o, o, 0, 0}, u32x4{qsum[n][g].x, qsum[n][g].y, 0, 0}, f32x4{0, 0, 0, 0});
           c = mfma<DT>(a0, qf[n][2 * g], c);
           c = mfma<DT>(a1, qf[n][2 * g + 1], c);
-          if (g == 0) z[n][tl] = f32x4{0, 0, 0, 0};
-          z[n][tl][0] += bf16_lo(s.x) * c[0];
-          z[n][tl][1] += bf16_hi(s.x) * c[1];
-          z[n][tl][2] += bf16_lo(s.y) * c[2];
-          z[n][tl][3] += bf16_hi(s.y) * c[3];
+          if (g == 0) z[n][t] = f32x4{bf16_lo(s.x) * c[0], bf16_hi(s.x) * c[1], bf16_lo(s.y) * c[2], bf16_hi(s.y) * c[3]};
+          else {
+            z[n][t][0] += bf16_lo(s.x) * c[0];
+            z[n][t][1] += bf16_hi(s.x) * c[1];
+            z[n][t][2] += bf16_lo(s.y) * c[2];
+            z[n][t][3] += bf16_hi(s.y) * c[3];
+          }
         }
       }
     }
-    // online softmax: a lane holds tokens 16 tl + 4 q + i of the query in its column
+    PIN();
+    const uint8_t* page = page_at(next);
+    if (step + 4 < end) k.load(page, (step + 4) % STEPS, lane);
+    if (step + 8 < end) next = table[(step + 8) / STEPS];
+    PIN();
+    // online softmax: a lane holds tokens 16 t + 4 q + i of the query in its column
+    const int first = step * T;
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
-      if (p * PAGE + PAGE > it.start) {  // only pages with tokens of the span hold any that are not seen
+      if (first + T > it.start) {  // only steps with tokens of the span hold any that are not seen
+        asm volatile("");          // a branch, not a select for every score of every step
 #pragma unroll
-        for (int tl = 0; tl < 4; tl++)
+        for (int t = 0; t < TT; t++)
 #pragma unroll
           for (int i = 0; i < 4; i++)
-            if (p * PAGE + tl * 16 + 4 * q + i >= limit[n]) z[n][tl][i] = NEG;
+            if (first + t * 16 + 4 * q + i >= limit[n]) z[n][t][i] = NEG;
       }
       float top = NEG;
 #pragma unroll
-      for (int tl = 0; tl < 4; tl++)
+      for (int t = 0; t < TT; t++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) top = fmaxf(top, z[n][tl][i]);
+        for (int i = 0; i < 4; i++) top = fmaxf(top, z[n][t][i]);
       top *= a.scale;
       top = fmaxf(top, lane_xor16(top));
       top = fmaxf(top, lane_xor32(top));
@@ -186,47 +262,47 @@ __global__ __launch_bounds__(256) void paged_split_kernel(const Attend a) {
       }
       float sum = 0;
 #pragma unroll
-      for (int tl = 0; tl < 4; tl++)
+      for (int t = 0; t < TT; t++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          z[n][tl][i] = __builtin_amdgcn_exp2f(fmaf(z[n][tl][i], a.scale, -base));
-          sum += z[n][tl][i];
+          z[n][t][i] = __builtin_amdgcn_exp2f(fmaf(z[n][t][i], a.scale, -base));
+          sum += z[n][t][i];
         }
       l[n] += sum;
     }
 #pragma unroll
-    for (int half = 0; half < 2; half++)
+    for (int half = 0; half < T / 32; half++)
 #pragma unroll
       for (int g = 0; g < NG; g++) {
-        const int t0 = (half * 8 + q) * NG + g, t1 = (half * 8 + 4 + q) * NG + g;
-        const uint2 s0 = ((const uint2*)(page + V_SCALES * D))[t0], s1 = ((const uint2*)(page + V_SCALES * D))[t1];
-        const uint2 o0 = ((const uint2*)(page + V_OFFSETS * D))[t0], o1 = ((const uint2*)(page + V_OFFSETS * D))[t1];
-        const u32x4 w = ((const u32x4*)(page + V_CODES * D))[(half * NG + g) * 64 + lane];
+        const uint2 s0 = v.scale[half][0][g], s1 = v.scale[half][1][g], o0 = v.offset[half][0][g], o1 = v.offset[half][1][g];
         u32x4 ps[NQ], rest[NQ];
 #pragma unroll
         for (int n = 0; n < NQ; n++) {
           const f32x4 x = z[n][2 * half], y = z[n][2 * half + 1];
-          const float v[8] = {x[0] * bf16_lo(s0.x), x[1] * bf16_hi(s0.x), x[2] * bf16_lo(s0.y), x[3] * bf16_hi(s0.y),
+          const float u[8] = {x[0] * bf16_lo(s0.x), x[1] * bf16_hi(s0.x), x[2] * bf16_lo(s0.y), x[3] * bf16_hi(s0.y),
                               y[0] * bf16_lo(s1.x), y[1] * bf16_hi(s1.x), y[2] * bf16_lo(s1.y), y[3] * bf16_hi(s1.y)};
 #pragma unroll
-          for (int k = 0; k < 4; k++) {
-            ps[n][k] = pack_bf16(v[2 * k], v[2 * k + 1]);
-            if (TWO) rest[n][k] = pack_bf16(v[2 * k] - bf16_lo(ps[n][k]), v[2 * k + 1] - bf16_hi(ps[n][k]));
+          for (int e = 0; e < 4; e++) {
+            ps[n][e] = pack_bf16(u[2 * e], u[2 * e + 1]);
+            if (TWO) rest[n][e] = pack_bf16(u[2 * e] - bf16_lo(ps[n][e]), u[2 * e + 1] - bf16_hi(ps[n][e]));
           }
           const u32x4 o = {o0.x, o0.y, o1.x, o1.y};
           off[n][g] = mfma_bf16(o, ps[n], off[n][g]);
           if (TWO) off[n][g] = mfma_bf16(o, rest[n], off[n][g]);
         }
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const u32x4 av = codes16<ANNA_MI_BF16>(w[k]);
+        for (int e = 0; e < 4; e++) {
+          const u32x4 av = codes16<ANNA_MI_BF16>(v.code[half][g][e], vmask);
 #pragma unroll
           for (int n = 0; n < NQ; n++) {
-            acc[n][4 * g + k] = mfma_bf16(av, ps[n], acc[n][4 * g + k]);
-            if (TWO) acc[n][4 * g + k] = mfma_bf16(av, rest[n], acc[n][4 * g + k]);
+            acc[n][4 * g + e] = mfma_bf16(av, ps[n], acc[n][4 * g + e]);
+            if (TWO) acc[n][4 * g + e] = mfma_bf16(av, rest[n], acc[n][4 * g + e]);
           }
         }
       }
+    PIN();
+    if (step + 4 < end) v.load(page, (step + 4) % STEPS, lane);
+    PIN();
   }
 
   // the waves' results joined, one column tile at a time
@@ -271,117 +347,127 @@ __global__ __launch_bounds__(256) void paged_split_kernel(const Attend a) {
 //
 // The operands are fp16 for both types: (code + zero) * scale rounded to 11 bits, probabilities (times 2^8, so
 // that small ones stay above fp16's subnormals) too, which keeps the result within a tenth of the output's
-// own rounding.  fp16 holds only so much: a page with scales beyond the limits below, and every page of
-// queries above them, is taken in bf16 instead, at bf16's precision.
+// own rounding.  fp16 holds only so much: from the first page on with scales beyond the limits below, and for
+// queries above them from the first page on, an item goes on in bf16 instead, at bf16's precision.
 constexpr float K_SCALE_MOST = 16.0f;                // |k| < 2^11: with |q| <= 2^11 subnormal roundings stay below 2^-14
 constexpr float V_SCALE_MOST = 256.0f;               // |v| < 2^15
 constexpr float V_SCALE_LEAST = 3.814697265625e-6f;  // 2^-18: subnormal roundings stay below a 2^-7th of a code's step
 constexpr float Q_MOST = 2048.0f;
-constexpr float P_SHIFT = 8.0f;
+constexpr float P_SHIFT = 8.0f, P_SLACK = 4.0f;
 
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-
-// (code + zero) * scale of a word's 8 codes; offset and scale of each pair of codes.
-__device__ __forceinline__ u32x4 dense_f16(uint32_t w, const f16x2* offset, const f16x2* scale, int step) {
-  const u32x4 c = codes16<ANNA_MI_F16>(w);
-  u32x4 o;
-#pragma unroll
-  for (int k = 0; k < 4; k++)
-    o[k] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(f16x2, (uint32_t)c[k]) + offset[k * step]) * scale[k * step]);
-  return o;
-}
-__device__ __forceinline__ u32x4 dense_bf16(uint32_t w, const float* offset, const float* scale, int step) {
-  const u32x4 c = codes16<ANNA_MI_BF16>(w);
-  u32x4 o;
-#pragma unroll
-  for (int k = 0; k < 4; k++)
-    o[k] = pack_bf16((bf16_lo(c[k]) + offset[2 * k * step]) * scale[2 * k * step],
-                     (bf16_hi(c[k]) + offset[(2 * k + 1) * step]) * scale[(2 * k + 1) * step]);
-  return o;
-}
 __device__ __forceinline__ f16x2 f16_pair(uint32_t v) { return f16x2{(_Float16)bf16_lo(v), (_Float16)bf16_hi(v)}; }
+// (code + zero) * scale of a pair: the sum is exact, the product rounded once.
+__device__ __forceinline__ uint32_t scaled(uint32_t code16, uint32_t offset, uint32_t scale) {
+  return __builtin_bit_cast(uint32_t, (__builtin_bit_cast(f16x2, code16) + __builtin_bit_cast(f16x2, offset)) * __builtin_bit_cast(f16x2, scale));
+}
 
 template <bool F16> __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
   if constexpr (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// What a thread holds of a page until it goes to LDS: its share of the codes with their scales and offsets.
-// Keys by 16-token quarters of a page, values by 16-byte words of a (half, group): UNITS of each a page.
-template <int D> struct Share {
+// What a thread holds of a page until it goes to LDS: the codes of a token's keys (by 16-token quarters of a page)
+// and of 16-byte words of values (by halves and groups: UNITS of them a page), with their scales and offsets as
+// loaded, and as the pairs that the conversion takes (in the same registers, once the loads are in).
+template <int D> struct KeyShare {
   static constexpr int NG = D / GROUP, KW = D / 32;
-  uint32_t kw[KW];
-  uint16_t ks[NG], ko[NG];
-  u32x4 vw;
-  uint2 vs[2], vo[2];
+  uint32_t code[KW];
+  uint32_t scale[NG], offset[NG];
+  __device__ __forceinline__ void load(const uint8_t* page, int quarter, uint32_t lane) {
+    const uint32_t q = lane / 16, r = lane % 16;
+    __builtin_memcpy(code, __builtin_assume_aligned(page + quarter * 8 * D + (r * (D / 2) + q * (D / 8)), D / 8 < 16 ? D / 8 : 16), D / 8);
+    const uint8_t* row = page + quarter * 32 * NG;
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+      scale[g] = *(const uint16_t*)(row + (K_SCALES * D + ((r / 4) * NG * 4 + r % 4) * 2) + g * 8);
+      offset[g] = *(const uint16_t*)(row + (K_OFFSETS * D + r * NG * 2) + g * 2);
+    }
+  }
+  __device__ __forceinline__ bool wide() const {  // beyond what fp16 holds
+    bool any = false;
+#pragma unroll
+    for (int g = 0; g < NG; g++) any |= bf16_lo(scale[g]) > K_SCALE_MOST;
+    return any;
+  }
+  __device__ __forceinline__ void convert() {
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+      scale[g] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)bf16_lo(scale[g]), (_Float16)bf16_lo(scale[g])});
+      offset[g] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)bf16_lo(offset[g]), (_Float16)bf16_lo(offset[g])});
+    }
+  }
+  // Where word 0 goes (the dims 8 q + e of a token); word k (the dims 32 k further) 2 k fragments behind it.  Rows in LDS
+  // are permuted as said above.
+  static __device__ __forceinline__ int at(int quarter, int lane) {
+    const int q = lane / 16, r = lane % 16, row = 16 * (r / 8) + 8 * (quarter & 1) + r % 8;
+    return ((quarter / 2) * 2 * KW + q / 2) * 64 + (q & 1) * 32 + row;
+  }
+  __device__ __forceinline__ void put_f16(u32x4* to, int k, uint32_t mask) const {
+    u32x4 c = codes16<ANNA_MI_F16>(code[k], mask);
+#pragma unroll
+    for (int i = 0; i < 4; i++) c[i] = scaled(c[i], offset[k / 2], scale[k / 2]);
+    to[128 * k] = c;
+  }
+  __device__ __forceinline__ void put_bf16(u32x4* to, int k) const {
+    const u32x4 c = codes16<ANNA_MI_BF16>(code[k], 0x00780078u);
+    const float s = bf16_lo(scale[k / 2]), o = bf16_lo(offset[k / 2]);
+    u32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = pack_bf16((bf16_lo(c[i]) + o) * s, (bf16_hi(c[i]) + o) * s);
+    to[128 * k] = v;
+  }
 };
-
-template <int D> __device__ __forceinline__ void load_keys(Share<D>& s, const uint8_t* page, int quarter, int lane) {
-  constexpr int NG = D / GROUP;
-  const int q = lane / 16, r = lane % 16, token = quarter * 16 + r;
-  __builtin_memcpy(s.kw, __builtin_assume_aligned(page + token * (D / 2) + q * (D / 8), D / 8 < 16 ? D / 8 : 16), D / 8);
+template <int D> struct ValueShare {
+  static constexpr int NG = D / GROUP;
+  u32x4 code;
+  uint32_t scale[4], offset[4];  // of the tokens' pairs
+  __device__ __forceinline__ void load(const uint8_t* page, int unit, uint32_t lane) {
+    const uint32_t q = lane / 16, half = unit / NG, g = unit % NG;
+    code = *(const u32x4*)(page + unit * 1024 + (V_CODES * D + lane * 16));
+    const uint8_t* row = page + half * 64 * NG + g * 8;
 #pragma unroll
-  for (int g = 0; g < NG; g++) {
-    s.ks[g] = ((const uint16_t*)(page + K_SCALES * D))[((token / 4) * NG + g) * 4 + token % 4];
-    s.ko[g] = ((const uint16_t*)(page + K_OFFSETS * D))[token * NG + g];
+    for (int u = 0; u < 2; u++) {
+      const uint2 s = *(const uint2*)(row + u * 32 * NG + (V_SCALES * D + q * NG * 8));
+      const uint2 o = *(const uint2*)(row + u * 32 * NG + (V_OFFSETS * D + q * NG * 8));
+      scale[2 * u] = s.x, scale[2 * u + 1] = s.y, offset[2 * u] = o.x, offset[2 * u + 1] = o.y;
+    }
   }
-}
-template <int D> __device__ __forceinline__ void load_values(Share<D>& s, const uint8_t* page, int unit, int lane) {
-  constexpr int NG = D / GROUP;
-  const int half = unit / NG, g = unit % NG, q = lane / 16;
-  s.vw = ((const u32x4*)(page + V_CODES * D))[unit * 64 + lane];
+  __device__ __forceinline__ bool wide() const {
+    bool any = false;
 #pragma unroll
-  for (int u = 0; u < 2; u++) {
-    const int at = (half * 8 + 4 * u + q) * NG + g;
-    s.vs[u] = ((const uint2*)(page + V_SCALES * D))[at];
-    s.vo[u] = ((const uint2*)(page + V_OFFSETS * D))[at];
+    for (int k = 0; k < 4; k++) {
+      const float x = bf16_lo(scale[k]), y = bf16_hi(scale[k]);
+      any |= fmaxf(x, y) > V_SCALE_MOST || (x < V_SCALE_LEAST && x > 0.0f) || (y < V_SCALE_LEAST && y > 0.0f);
+    }
+    return any;
   }
-}
-
-// Whether fp16 holds the operands that these scales make.
-template <int D> __device__ __forceinline__ bool keys_wide(const Share<D>& s) {
-  bool wide = false;
+  __device__ __forceinline__ void convert() {
 #pragma unroll
-  for (int g = 0; g < D / GROUP; g++) wide |= bf16_bits_to_f32(s.ks[g]) > K_SCALE_MOST;
-  return wide;
-}
-template <int D> __device__ __forceinline__ bool values_wide(const Share<D>& s) {
-  const uint32_t sw[4] = {s.vs[0].x, s.vs[0].y, s.vs[1].x, s.vs[1].y};
-  bool wide = false;
-#pragma unroll
-  for (int k = 0; k < 4; k++) {
-    const float x = bf16_lo(sw[k]), y = bf16_hi(sw[k]);
-    wide |= fmaxf(x, y) > V_SCALE_MOST || (x < V_SCALE_LEAST && x > 0.0f) || (y < V_SCALE_LEAST && y > 0.0f);
+    for (int k = 0; k < 4; k++) {
+      scale[k] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)bf16_lo(scale[k]), (_Float16)bf16_hi(scale[k])});
+      offset[k] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)bf16_lo(offset[k]), (_Float16)bf16_hi(offset[k])});
+    }
   }
-  return wide;
-}
-
-// Word k of a thread's keys / values to LDS.
-template <int D, bool F16> __device__ __forceinline__ void put_key(const Share<D>& s, u32x4* lds, int quarter, int k, int lane) {
-  constexpr int KW = D / 32;
-  const int q = lane / 16, r = lane % 16, row = 16 * (r / 8) + 8 * (quarter & 1) + r % 8;
-  const float scale = bf16_bits_to_f32(s.ks[k / 2]), offset = bf16_bits_to_f32(s.ko[k / 2]);
-  const f16x2 s2 = {(_Float16)scale, (_Float16)scale}, o2 = {(_Float16)offset, (_Float16)offset};
-  lds[((quarter / 2) * 2 * KW + 2 * k + q / 2) * 64 + (q & 1) * 32 + row] =
-      F16 ? dense_f16(s.kw[k], &o2, &s2, 0) : dense_bf16(s.kw[k], &offset, &scale, 0);
-}
-template <int D, bool F16> __device__ __forceinline__ void put_value(const Share<D>& s, u32x4* lds, int unit, int w, int lane) {
-  constexpr int NG = D / GROUP;
-  const int half = unit / NG, g = unit % NG, q = lane / 16, r = lane % 16;
-  const uint32_t sw[4] = {s.vs[0].x, s.vs[0].y, s.vs[1].x, s.vs[1].y}, ow[4] = {s.vo[0].x, s.vo[0].y, s.vo[1].x, s.vo[1].y};
-  float scale[8], offset[8];
-  f16x2 s2[4], o2[4];
-#pragma unroll
-  for (int k = 0; k < 4; k++) {
-    scale[2 * k] = bf16_lo(sw[k]), scale[2 * k + 1] = bf16_hi(sw[k]);
-    offset[2 * k] = bf16_lo(ow[k]), offset[2 * k + 1] = bf16_hi(ow[k]);
-    s2[k] = f16_pair(sw[k]);
-    o2[k] = f16_pair(ow[k]);
+  // Where word 0 goes (dim r of the group); word w (the dims 16 w further) 16 rows or a dim tile behind it.
+  static __device__ __forceinline__ int at(int unit, int lane) {
+    const int half = unit / NG, g = unit % NG, q = lane / 16, r = lane % 16;
+    return 8 * D + ((half * (D / 32) + 2 * g) * 2 + q / 2) * 64 + (q & 1) * 32 + r;
   }
-  lds[((half * (D / 32) + 2 * g + w / 2) * 2 + q / 2) * 64 + (q & 1) * 32 + (w & 1) * 16 + r] =
-      F16 ? dense_f16(s.vw[w], o2, s2, 1) : dense_bf16(s.vw[w], offset, scale, 1);
-}
+  __device__ __forceinline__ void put_f16(u32x4* to, int w, uint32_t mask) const {
+    u32x4 c = codes16<ANNA_MI_F16>(code[w], mask);
+#pragma unroll
+    for (int i = 0; i < 4; i++) c[i] = scaled(c[i], offset[i], scale[i]);
+    to[128 * (w / 2) + 16 * (w & 1)] = c;
+  }
+  __device__ __forceinline__ void put_bf16(u32x4* to, int w) const {
+    const u32x4 c = codes16<ANNA_MI_BF16>(code[w], 0x00780078u);
+    u32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      v[i] = pack_bf16((bf16_lo(c[i]) + bf16_lo(offset[i])) * bf16_lo(scale[i]), (bf16_hi(c[i]) + bf16_hi(offset[i])) * bf16_hi(scale[i]));
+    to[128 * (w / 2) + 16 * (w & 1)] = v;
+  }
+};
 
 // LDS of a buffer: keys then values, 128 * D bytes each.
 template <int D> constexpr int buffer_words() { return 2 * 128 * D / 16; }
@@ -392,14 +478,53 @@ template <int D> struct Rows {
   float m, l;
 };
 
+// The running maximum of a lane's query with the scores `top` added, less P_SHIFT: P_SHIFT above it the
+// probabilities would be 2^P_SHIFT.  It moves only when it has to, by more than P_SLACK, which leaves them within
+// fp16 and spares nearly all rescaling.  Returns the factor of everything summed so far.
+template <int D> __device__ __forceinline__ bool new_top(Rows<D>& w, float top, float scale, float& factor) {
+  top = fmaxf(top, lane_xor32(top));
+  top = fmaf(top, scale, -P_SHIFT);
+  const bool moves = top > w.m + P_SLACK;
+  factor = 1.0f;
+  if (!__any(moves)) return false;
+  if (moves) {
+    factor = weight(w.m, top);
+    w.m = top;
+  }
+  return true;
+}
+__device__ __forceinline__ float top_of(const f32x16& z) {
+  float top = NEG;
+#pragma unroll
+  for (int j = 0; j < 16; j++) top = fmaxf(top, z[j]);
+  return top;
+}
+// Token of a half page that row j of a lane's scores stands for.
+__device__ __forceinline__ int token_of(int j, int hl) { return 16 * ((j >> 2) & 1) + 8 * (j >> 3) + 4 * hl + (j & 3); }
+__device__ __forceinline__ void hide_from(f32x16& z, int half, int hl, int limit) {
+#pragma unroll
+  for (int j = 0; j < 16; j++)
+    if (32 * half + token_of(j, hl) >= limit) z[j] = NEG;
+}
+// Two neighbouring probabilities of a lane, as a pair of the operand type.
+template <bool F16> __device__ __forceinline__ uint32_t probability(const f32x16& z, int j, float scale, float base, float& sum) {
+  const float x = __builtin_amdgcn_exp2f(fmaf(z[j], scale, -base)), y = __builtin_amdgcn_exp2f(fmaf(z[j + 1], scale, -base));
+  sum += x + y;
+  if (!F16) return pack_bf16(x, y);
+  return __builtin_bit_cast(uint32_t, f16x2{(_Float16)x, (_Float16)y});
+}
+
 // One page in LDS for a wave's rows.  limit: tokens of the page that the lane's query sees; cut: whether any lane's
-// is below PAGE.  Fragments are read one step ahead of the matrix instructions that take them, and the order of the
-// steps is pinned: left to itself the compiler reads all of them first and spills.  side(k) is work for the vector
-// unit that runs beneath step k's matrix instructions.
-#define PIN() __builtin_amdgcn_sched_barrier(0)
-template <int D, bool F16, class Q, class S>
-__device__ __forceinline__ void take_page(Rows<D>& w, const u32x4* lds, Q query, int limit, bool cut, float scale, int lane, S side) {
+// is below PAGE.  The two halves of the page go through one behind the other, so that the vector unit's softmax of
+// one runs beneath the matrix instructions of the other, and the next page's conversion beneath the rest:
+//   scores 0, first(k) | scores 1, softmax 0 | values 0, softmax 1 | values 1, second(k)
+// Every step is a pair of matrix instructions, a pair of fragments AHEAD steps ahead, and a share of the vector
+// work; the order is pinned, as the compiler left to itself reads all fragments first and spills.
+template <int D, bool F16, int AHEAD, class Q, class A, class B>
+__device__ __forceinline__ void take_page(Rows<D>& w, const u32x4* lds, Q query, int limit, bool cut, float scale, int lane, A first,
+                                          B second) {
   constexpr int KSTEPS = D / 16, DTILES = D / 32;
+  constexpr int KHALF = KSTEPS / 2, VHALF = DTILES, VSTEPS = 2 * DTILES, RING = AHEAD + 1;
   const int hl = lane / 32;
   const u32x4* values = lds + 8 * D;
   f32x16 z[2];
@@ -407,131 +532,155 @@ __device__ __forceinline__ void take_page(Rows<D>& w, const u32x4* lds, Q query,
   for (int half = 0; half < 2; half++)
 #pragma unroll
     for (int j = 0; j < 16; j++) z[half][j] = 0;
-  u32x4 f[2][2];
-#pragma unroll
-  for (int half = 0; half < 2; half++) f[0][half] = lds[half * KSTEPS * 64 + lane];
-#pragma unroll
-  for (int s = 0; s < KSTEPS; s++) {
-    if (s + 1 < KSTEPS) {
-#pragma unroll
-      for (int half = 0; half < 2; half++) f[(s + 1) & 1][half] = lds[(half * KSTEPS + s + 1) * 64 + lane];
-    }
-    const u32x4 q = query(s);
-#pragma unroll
-    for (int half = 0; half < 2; half++) z[half] = mfma32<F16>(f[s & 1][half], q, z[half]);
-    side(s);
-    PIN();
-  }
-  if (cut) {
-#pragma unroll
-    for (int half = 0; half < 2; half++)
-#pragma unroll
-      for (int j = 0; j < 16; j++)
-        if (32 * half + 16 * ((j >> 2) & 1) + 8 * (j >> 3) + 4 * hl + (j & 3) >= limit) z[half][j] = NEG;
-  }
-  float top = NEG;
-#pragma unroll
-  for (int half = 0; half < 2; half++)
-#pragma unroll
-    for (int j = 0; j < 16; j++) top = fmaxf(top, z[half][j]);
-  top = fmaxf(top, lane_xor32(top));
-  // the maximum less P_SHIFT, so that probabilities reach 2^P_SHIFT
-  top = fmaxf(fmaf(top, scale, -P_SHIFT), w.m);
-  const float base = top == NEG ? 0.0f : top;
-  if (__any(top > w.m)) {
-    const float f = weight(w.m, base);
-    w.l *= f;
-#pragma unroll
-    for (int d = 0; d < DTILES; d++) w.acc[d] *= f;
-    w.m = top;
-  }
-  float sum = 0;
-  u32x4 p[4];
-#pragma unroll
-  for (int k = 0; k < 4; k++)
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const float x = __builtin_amdgcn_exp2f(fmaf(z[k / 2][8 * (k & 1) + 2 * e], scale, -base));
-      const float y = __builtin_amdgcn_exp2f(fmaf(z[k / 2][8 * (k & 1) + 2 * e + 1], scale, -base));
-      sum += x + y;
-      if (F16) {
-        const f16x2 h = {(_Float16)x, (_Float16)y};
-        p[k][e] = __builtin_bit_cast(uint32_t, h);
-      } else p[k][e] = pack_bf16(x, y);
-    }
-  w.l += sum;
-  PIN();
-  // steps of two dim tiles
-  constexpr int STEPS = 4 * DTILES / 2;
-  auto fragment = [&](int step, int u) {
-    const int k = step / (DTILES / 2), d = 2 * (step % (DTILES / 2)) + u;
-    return values[(((k / 2) * DTILES + d) * 2 + (k & 1)) * 64 + lane];
-  };
-#pragma unroll
-  for (int u = 0; u < 2; u++) f[0][u] = fragment(0, u);
-#pragma unroll
-  for (int step = 0; step < STEPS; step++) {
-    if (step + 1 < STEPS) {
-#pragma unroll
-      for (int u = 0; u < 2; u++) f[(step + 1) & 1][u] = fragment(step + 1, u);
-    }
+  u32x4 f[RING][2], p[4];
+  float sum = 0, base = 0, factor[2];
+  bool moved[2];
+  // step i of the scores: two k steps of half i / KHALF; of the values: two dim tiles of 16 tokens
+  auto read = [&](int i) {
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-      const int d = 2 * (step % (DTILES / 2)) + u;
-      w.acc[d] = mfma32<F16>(f[step & 1][u], p[step / (DTILES / 2)], w.acc[d]);
+      if (i < KSTEPS) f[i % RING][u] = lds[(i / KHALF * KSTEPS + 2 * (i % KHALF) + u) * 64 + lane];
+      else if (i < KSTEPS + VSTEPS) {
+        const int k = (i - KSTEPS) / (DTILES / 2), d = 2 * ((i - KSTEPS) % (DTILES / 2)) + u;
+        f[i % RING][u] = values[(((k / 2) * DTILES + d) * 2 + (k & 1)) * 64 + lane];
+      }
+    }
+  };
+  auto reference = [&](int half) {
+    if (cut) {
+      asm volatile("");  // a branch, not a select for every score of every page
+      hide_from(z[half], half, hl, limit);
+    }
+    moved[half] = new_top(w, top_of(z[half]), scale, factor[half]);
+    base = w.m == NEG ? 0.0f : w.m;
+  };
+  auto rescale = [&](int half) {
+    if (moved[half]) {
+#pragma unroll
+      for (int d = 0; d < DTILES; d++) w.acc[d] *= factor[half];
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++) read(i);
+#pragma unroll
+  for (int i = 0; i < KSTEPS; i++) {
+    if (i == KHALF) {
+      first(KHALF);
+      PIN();
+      reference(0);
+      w.l *= factor[0];
+      rescale(0);
+      PIN();
+    }
+    read(i + AHEAD);
+#pragma unroll
+    for (int u = 0; u < 2; u++) z[i / KHALF] = mfma32<F16>(f[i % RING][u], query(2 * (i % KHALF) + u), z[i / KHALF]);
+    if (i < KHALF) first(i);
+    else {
+      constexpr int PAIRS = (8 + KHALF - 1) / KHALF;  // of probabilities a step
+#pragma unroll
+      for (int k = (i - KHALF) * PAIRS; k < (i - KHALF + 1) * PAIRS; k++)
+        if (k < 8) p[k / 4][k % 4] = probability<F16>(z[0], 2 * k, scale, base, sum);
     }
     PIN();
   }
+  reference(1);
+  PIN();
+  const float sum0 = sum;
+  sum = 0;
+#pragma unroll
+  for (int i = 0; i < VSTEPS; i++) {
+    if (i == VHALF) {
+      w.l = (w.l + sum0) * factor[1] + sum;
+      rescale(1);
+      PIN();
+    }
+    read(KSTEPS + i + AHEAD);
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const int d = 2 * (i % (DTILES / 2)) + u;
+      w.acc[d] = mfma32<F16>(f[(KSTEPS + i) % RING][u], p[i / (DTILES / 2)], w.acc[d]);
+    }
+    if (i < VHALF) {
+      constexpr int PAIRS = (8 + VHALF - 1) / VHALF;
+#pragma unroll
+      for (int k = i * PAIRS; k < (i + 1) * PAIRS; k++)
+        if (k < 8) p[2 + k / 4][k % 4] = probability<F16>(z[1], 2 * k, scale, base, sum);
+    } else second(i - VHALF);
+    PIN();
+  }
+  second(VHALF);
 }
 
 template <int DT, int D, int NW>
 __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
-  constexpr int NG = D / GROUP, KSTEPS = D / 16, UNITS = 2 * NG;
-  constexpr int KEYS = 1, VALUES = (UNITS + NW - 1) / NW, SHARES = VALUES;
+  constexpr int NG = D / GROUP, KSTEPS = D / 16, KW = D / 32, UNITS = 2 * NG;
+  // Waves 0 to 3 turn keys, the last ones values: with 8 waves a wave has one of the two, with 4 all have both.
+  constexpr int VALUES = (UNITS + NW - 1) / NW, AHEAD = NW == 4 ? 2 : 1;
   __shared__ __align__(16) u32x4 lds[2 * buffer_words<D>()];
   __shared__ int wide[4];  // by page % 4: a scale is beyond what fp16 holds
   const int H = a.kv_heads, G = a.group;
   const int h = blockIdx.x % H, index = blockIdx.x / H;
-  if (index >= a.header[1]) return;
   const Item it = a.tile[index];
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, hl = lane / 32;
+  if (index >= a.header[1]) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, hl = lane / 32;
   const int rows = it.count * G, row0 = it.tile * 32 * NW + 32 * wave, row = row0 + lane % 32, t = row / G;
   const bool valid = row < rows;
   const int32_t* table = a.table + it.row * a.width;
   const int head = h * G + row % G;
+  auto page_at = [&](int32_t page) { return a.pool + ((int64_t)page * H + h) * page_bytes(D); };
+
+  union Held {  // with 8 waves one of the two
+    KeyShare<D> keys;
+    ValueShare<D> values;
+  };
+  struct Both {
+    KeyShare<D> keys;
+    ValueShare<D> values[VALUES];
+  };
+  std::conditional_t<NW == 8, Held, Both> held;
+  KeyShare<D>& keys = held.keys;
+  ValueShare<D>* values;
+  if constexpr (NW == 8) values = &held.values;
+  else values = held.values;
+  const bool has_keys = NW == 4 || wave < 4;
+  auto unit_of = [&](int n) { return NW - 1 - wave + n * NW; };
+  auto has_unit = [&](int n) { return (n + 1) * NW <= UNITS || unit_of(n) < UNITS; };
+  auto load_keys = [&](int32_t id) {
+    if (has_keys) keys.load(page_at(id), wave, lane);
+  };
+  auto load_values = [&](int32_t id) {
+#pragma unroll
+    for (int n = 0; n < VALUES; n++)
+      if (has_unit(n)) values[n].load(page_at(id), unit_of(n), lane);
+  };
+  auto page_id = [&](int p) { return table[min(p, it.page1 - 1)]; };
+  int32_t next = page_id(it.page0);
+  load_keys(next);
+  load_values(next);
+  next = page_id(it.page0 + 1);
+
   const uint16_t* source = (const uint16_t*)a.query + (int64_t)(it.offset + t) * a.q_token + head * a.q_head + hl * 8;
   auto raw_query = [&](int s) { return valid ? *(const u32x4*)(source + 16 * s) : u32x4{0, 0, 0, 0}; };
-  auto page_of = [&](int p) { return a.pool + ((int64_t)table[p] * H + h) * page_bytes(D); };
-
-  if (threadIdx.x < 4) wide[threadIdx.x] = 0;
   u32x4 qf[KSTEPS];
+#pragma unroll
+  for (int s = 0; s < KSTEPS; s++) qf[s] = raw_query(s);
+  if (threadIdx.x < 4) wide[threadIdx.x] = 0;
   bool large = false;
   auto too_large = [](float x) { return fabsf(x) > Q_MOST && fabsf(x) < INFINITY; };  // others spoil their own row alone
 #pragma unroll
-  for (int s = 0; s < KSTEPS; s++) {
-    qf[s] = raw_query(s);
-    if (DT == ANNA_MI_BF16) {
+  for (int s = 0; s < KSTEPS; s++)
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
+    for (int k = 0; k < 4; k++) {
+      if (DT == ANNA_MI_BF16) {
         large |= too_large(bf16_lo(qf[s][k])) || too_large(bf16_hi(qf[s][k]));
         qf[s][k] = __builtin_bit_cast(uint32_t, f16_pair(qf[s][k]));
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; k++)
+      } else {
         large |= too_large(f16_bits_to_f32((uint16_t)qf[s][k])) || too_large(f16_bits_to_f32((uint16_t)(qf[s][k] >> 16)));
+      }
     }
-  }
   const bool all_wide = __syncthreads_or(large) != 0;
-  auto fast_query = [&](int s) { return qf[s]; };
-  auto slow_query = [&](int s) {
-    u32x4 v = raw_query(s);
-    if (DT == ANNA_MI_F16) {
-#pragma unroll
-      for (int k = 0; k < 4; k++) v[k] = pack_bf16(f16_bits_to_f32((uint16_t)v[k]), f16_bits_to_f32((uint16_t)(v[k] >> 16)));
-    }
-    return v;
-  };
+  auto query = [&](int s) { return qf[s]; };
 
   Rows<D> w;
   w.m = NEG, w.l = 0;
@@ -540,141 +689,220 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
 #pragma unroll
     for (int j = 0; j < 16; j++) w.acc[d][j] = 0;
 
-  Share<D> share[SHARES];
-  auto load = [&](const uint8_t* page) {
-#pragma unroll
-    for (int k = 0; k < KEYS; k++)
-      if (wave + k * NW < 4) load_keys(share[k], page, wave + k * NW, lane);
-#pragma unroll
-    for (int k = 0; k < VALUES; k++) {
-      const int unit = NW - 1 - wave + k * NW;  // from the last wave on: with 8 waves, other waves than the keys'
-      if (unit < UNITS) load_values(share[k], page, unit, lane);
-    }
+  // The loads are in: a flag if the page is none for fp16, and the scales as fp16.
+  auto convert_keys = [&](int slot) {
+    if (!has_keys) return;
+    if (keys.wide()) wide[slot] = 1;
+    keys.convert();
   };
-  auto check = [&](int slot) {
+  auto convert_values = [&](int slot) {
     bool beyond = false;
 #pragma unroll
-    for (int k = 0; k < KEYS; k++)
-      if (wave + k * NW < 4) beyond |= keys_wide(share[k]);
-#pragma unroll
-    for (int k = 0; k < VALUES; k++)
-      if (NW - 1 - wave + k * NW < UNITS) beyond |= values_wide(share[k]);
+    for (int n = 0; n < VALUES; n++)
+      if (has_unit(n)) {
+        beyond |= values[n].wide();
+        values[n].convert();
+      }
     if (beyond) wide[slot] = 1;
   };
-  // word k of this thread's keys and of its values (with 8 waves a wave has only one of the two)
-  constexpr int WORDS = NW == 8 ? (D / 32 > 4 ? D / 32 : 4) : D / 32 + 4 * VALUES;
-  auto put_word = [&](u32x4* to, int k) {
-    if (NW == 8) {
-      if (wave < 4) {
-        if (k < D / 32) put_key<D, true>(share[0], to, wave, k, lane);
-      } else if (k < 4 && NW - 1 - wave < UNITS) put_value<D, true>(share[0], to + 8 * D, NW - 1 - wave, k, lane);
-    } else if (k < D / 32) put_key<D, true>(share[0], to, wave, k, lane);
-    else {
-      const int n = (k - D / 32) / 4, unit = NW - 1 - wave + n * NW;
-      if (unit < UNITS) put_value<D, true>(share[n], to + 8 * D, unit, (k - D / 32) % 4, lane);
-    }
+  const uint32_t mask = code_mask<ANNA_MI_F16>();
+  const int key_at = KeyShare<D>::at(wave & 3, lane);
+  int value_at[VALUES];
+#pragma unroll
+  for (int n = 0; n < VALUES; n++) value_at[n] = ValueShare<D>::at(has_unit(n) ? unit_of(n) : 0, lane);
+  auto put_key = [&](u32x4* to, int k) {
+    if (has_keys) keys.put_f16(to + key_at, k, mask);
+  };
+  auto put_value = [&](u32x4* to, int k) {
+    if (has_unit(k / 4)) values[k / 4].put_f16(to + value_at[k / 4], k % 4, mask);
   };
   // LDS only: loads of the next page stay in flight
   auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
-  const int first = it.start + row0 / G + 1;                            // tokens that the wave's first row sees
+  const int seen_by_all = it.start + row0 / G + 1;                                 // tokens that the wave's first row sees
   const int last = row0 < rows ? it.start + min(row0 + 31, rows - 1) / G + 1 : 0;  // and its last
   const int sees = valid ? it.start + t + 1 : 0;
 
-  load(page_of(it.page0));
-  check(it.page0 & 3);
+  convert_keys(it.page0 & 3);
+  convert_values(it.page0 & 3);
 #pragma unroll
-  for (int k = 0; k < WORDS; k++) put_word(lds, k);
-  if (it.page0 + 1 < it.page1) load(page_of(it.page0 + 1));
+  for (int k = 0; k < KW; k++) put_key(lds, k);
+#pragma unroll
+  for (int k = 0; k < 4 * VALUES; k++) put_value(lds, k);
+  load_keys(next);
+  load_values(next);
+  next = page_id(it.page0 + 2);
   barrier();
-  for (int p = it.page0; p < it.page1; p++) {
+  int p = it.page0;
+  for (; p < it.page1 && !all_wide && __builtin_amdgcn_readfirstlane(wide[p & 3]) == 0; p++) {
     const int turn = (p - it.page0) & 1;
     u32x4 *now = lds + turn * buffer_words<D>(), *then = lds + (turn ^ 1) * buffer_words<D>();
-    const bool more = p + 1 < it.page1, slow = all_wide || wide[p & 3] != 0;
     if (threadIdx.x == 0) wide[(p + 2) & 3] = 0;
-    if (more) check((p + 1) & 3);
-    const int limit = sees - p * PAGE;
-    constexpr int PER = (WORDS + KSTEPS - 1) / KSTEPS;
-    auto side = [&](int s) {
-      if (more) {
+    // The next page's values are converted in the first quarter of this one, its keys in the last; the loads of the
+    // page after it follow each, and have a page's time to arrive.  Behind the last page all this goes on with the last
+    // one, for nobody: a load that is not always there would have the compiler wait for all of them.
+    constexpr int KHALF = KSTEPS / 2, VHALF = D / 32;
+    auto first = [&](int i) {
+      constexpr int PER = (4 * VALUES + KHALF - 1) / KHALF;
+      if (i == 0) convert_values((p + 1) & 3);
 #pragma unroll
-        for (int k = s * PER; k < (s + 1) * PER; k++)
-          if (k < WORDS) put_word(then, k);
+      for (int k = i * PER; k < (i + 1) * PER; k++)
+        if (k < 4 * VALUES) put_value(then, k);
+      if (i == KHALF) load_values(next);
+    };
+    auto second = [&](int i) {
+      constexpr int PER = (KW + VHALF - 1) / VHALF;
+      if (i == 0) convert_keys((p + 1) & 3);
+#pragma unroll
+      for (int k = i * PER; k < (i + 1) * PER; k++)
+        if (k < KW) put_key(then, k);
+      if (i == VHALF) {
+        load_keys(next);
+        next = page_id(p + 3);
       }
     };
-    const bool mine = p * PAGE < last;
-    if (mine && !slow) {
-      take_page<D, true>(w, now, fast_query, limit, p * PAGE + PAGE > first, a.scale, lane, side);
+    if (p * PAGE < last) {
+      take_page<D, true, AHEAD>(w, now, query, sees - p * PAGE, p * PAGE + PAGE > seen_by_all, a.scale, lane, first, second);
     } else {
 #pragma unroll
-      for (int s = 0; s < KSTEPS; s++) side(s);
-    }
-    if (p + 2 < it.page1) load(page_of(p + 2));
-    if (slow) {
-      // the page again, as bf16
-      barrier();
-      const uint8_t* page = page_of(p);
-      Share<D> again;
-      for (int k = wave; k < 4; k += NW) {
-        load_keys(again, page, k, lane);
+      for (int i = 0; i <= KHALF; i++) first(i);
 #pragma unroll
-        for (int i = 0; i < D / 32; i++) put_key<D, false>(again, now, k, i, lane);
-      }
-      for (int k = wave; k < UNITS; k += NW) {
-        load_values(again, page, k, lane);
-#pragma unroll
-        for (int i = 0; i < 4; i++) put_value<D, false>(again, now + 8 * D, k, i, lane);
-      }
-      barrier();
-      if (mine) take_page<D, false>(w, now, slow_query, limit, p * PAGE + PAGE > first, a.scale, lane, [](int) {});
+      for (int i = 0; i <= VHALF; i++) second(i);
     }
     barrier();
   }
+  // From the first page on that fp16 does not hold, in bf16: one buffer, nothing ahead.
+  if (p < it.page1) {
+#pragma unroll
+    for (int s = 0; s < KSTEPS; s++) {
+      qf[s] = raw_query(s);
+      if (DT == ANNA_MI_F16) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) qf[s][k] = pack_bf16(f16_bits_to_f32((uint16_t)qf[s][k]), f16_bits_to_f32((uint16_t)(qf[s][k] >> 16)));
+      }
+    }
+    for (; p < it.page1; p++) {
+      const uint8_t* page = page_at(table[p]);
+      if (NW == 4 || wave < 4) {
+        KeyShare<D> again;
+        again.load(page, wave, lane);
+#pragma unroll
+        for (int i = 0; i < KW; i++) again.put_bf16(lds + key_at, i);
+      }
+      for (int k = NW - 1 - wave; k < UNITS; k += NW) {
+        ValueShare<D> again;
+        again.load(page, k, lane);
+#pragma unroll
+        for (int i = 0; i < 4; i++) again.put_bf16(lds + ValueShare<D>::at(k, lane), i);
+      }
+      barrier();
+      if (p * PAGE < last)
+        take_page<D, false, 1>(w, lds, query, sees - p * PAGE, p * PAGE + PAGE > seen_by_all, a.scale, lane, [](int) {}, [](int) {});
+      barrier();
+    }
+  }
 
-  // a lane holds, of its query, dims 32 d + 8 b + 4 hl + i
+  // A lane holds, of its query, dims 32 d + 8 b + 4 hl + i.  Through LDS, as fp32, to whole rows: lanes that write 8
+// bytes of 32 rows each took 13 us a workgroup (128 rows of head_dim 256, gated), this @@ us.
   const float total = w.l + lane_xor32(w.l);
-  if (!valid) return;
-  const int64_t part = (int64_t)(it.part + 32 * wave + lane % 32) * H + h;
+  if (it.part >= 0) {
+    if (!valid) return;
+    const int64_t part = (int64_t)(it.part + 32 * wave + lane % 32) * H + h;
+#pragma unroll
+    for (int d = 0; d < D / 32; d++)
+#pragma unroll
+      for (int b = 0; b < 4; b++)
+        *(f32x4*)(a.values + part * D + 32 * d + 8 * b + 4 * hl) = f32x4{w.acc[d][4 * b], w.acc[d][4 * b + 1], w.acc[d][4 * b + 2], w.acc[d][4 * b + 3]};
+    if (hl == 0) a.stats[2 * part] = w.m, a.stats[2 * part + 1] = total;
+    return;
+  }
+  constexpr int PART = 4 * D / NW, UNITS4 = PART / 4;  // dims of a pass: what the wave's share of LDS holds for 32 rows
+  f32x4* mine = (f32x4*)lds + wave * 32 * UNITS4;
   const float inv = 1.0f / total;
 #pragma unroll
-  for (int d = 0; d < D / 32; d++)
+  for (int pass = 0; pass < D / PART; pass++) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last pass is read
 #pragma unroll
-    for (int b = 0; b < 4; b++) {
-      const int dim = 32 * d + 8 * b + 4 * hl;
-      const f32x4 v = {w.acc[d][4 * b], w.acc[d][4 * b + 1], w.acc[d][4 * b + 2], w.acc[d][4 * b + 3]};
-      if (it.part < 0) write_out<DT>(a, D, it.offset + t, head, dim, v * inv, (int64_t)H * G);
-      else *(f32x4*)(a.values + part * D + dim) = v;
+    for (int d = 0; d < PART / 32; d++)
+#pragma unroll
+      for (int b = 0; b < 4; b++) {
+        const f32x16& x = w.acc[pass * (PART / 32) + d];
+        const int unit = 8 * d + 2 * b + hl;
+        mine[(lane % 32) * UNITS4 + (unit ^ (lane & 15))] = f32x4{x[4 * b], x[4 * b + 1], x[4 * b + 2], x[4 * b + 3]} * inv;
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    constexpr int LANES = PART / 8;  // of a row, eight dims each
+#pragma unroll
+    for (int i = 0; i < 32 * LANES / 64; i++) {
+      const int r = i * (64 / LANES) + lane / LANES, c = lane % LANES;
+      const f32x4 x = mine[r * UNITS4 + ((2 * c) ^ (r & 15))], y = mine[r * UNITS4 + ((2 * c + 1) ^ (r & 15))];
+      const int out_row = row0 + r;
+      if (out_row >= rows) continue;
+      const int64_t token = it.offset + out_row / G;
+      const int out_head = h * G + out_row % G, dim = pass * PART + 8 * c;
+      float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+      if (a.gate) {
+        const u32x4 g = *(const u32x4*)((const uint16_t*)a.gate + token * a.g_token + out_head * a.g_head + dim);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          v[2 * k] *= sigmoid(Elem<DT>::to_f32((uint16_t)g[k]));
+          v[2 * k + 1] *= sigmoid(Elem<DT>::to_f32((uint16_t)(g[k] >> 16)));
+        }
+      }
+      u32x4 o;
+#pragma unroll
+      for (int k = 0; k < 4; k++) o[k] = Elem<DT>::cvt(v[2 * k]) | (uint32_t)Elem<DT>::cvt(v[2 * k + 1]) << 16;
+      *(u32x4*)((uint16_t*)a.out + (token * H * G + out_head) * D + dim) = o;
     }
-  if (it.part >= 0 && hl == 0) a.stats[2 * part] = w.m, a.stats[2 * part + 1] = total;
+  }
 }
 
-// Joins the items of a tile: one workgroup a query row, its four waves each every fourth item.
+// Joins the items of a tile: one workgroup a query row, its teams of D / 4 lanes each every TEAMS-th item, AHEAD of
+// them in flight.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const Attend a) {
-  constexpr int LANES = D / 4, TEAMS = 256 / LANES;
+  constexpr int LANES = D / 4, TEAMS = 256 / LANES, AHEAD = 4;
   __shared__ __align__(16) float joined[TEAMS][D];
   __shared__ float team_m[TEAMS], team_l[TEAMS];
   const int H = a.kv_heads, G = a.group, h = blockIdx.x % H, index = blockIdx.x / H;
-  if (index >= a.header[2]) return;
   const Unit u = a.units[index];
+  if (index >= a.header[2]) return;
   const int row = blockIdx.y;
   if (row >= u.rows) return;
   const int team = threadIdx.x / LANES, d = threadIdx.x % LANES * 4;
   float top = NEG, total = 0;
   f32x4 v = {0, 0, 0, 0};
-  for (int k = team; k < u.splits; k += TEAMS) {
-    const int64_t part = (int64_t)(u.part + k * u.rows + row) * H + h;
-    const float m = a.stats[2 * part], l = a.stats[2 * part + 1];
-    const f32x4 x = *(const f32x4*)(a.values + part * D + d);
-    const float next = fmaxf(top, m), f0 = weight(top, next), f1 = weight(m, next);
-    total = total * f0 + l * f1;
-    v = v * f0 + x * f1;
+  for (int k0 = team; k0 < u.splits; k0 += TEAMS * AHEAD) {
+    float m[AHEAD], l[AHEAD];
+    f32x4 x[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; k++) {
+      m[k] = NEG, l[k] = 0, x[k] = f32x4{0, 0, 0, 0};
+      if (k0 + k * TEAMS < u.splits) {
+        const int64_t part = (int64_t)(u.part + (k0 + k * TEAMS) * u.rows + row) * H + h;
+        m[k] = a.stats[2 * part], l[k] = a.stats[2 * part + 1];
+        x[k] = *(const f32x4*)(a.values + part * D + d);
+      }
+    }
+    float next = top;
+#pragma unroll
+    for (int k = 0; k < AHEAD; k++) next = fmaxf(next, m[k]);
+    float f = weight(top, next);
+    total *= f;
+    v *= f;
+#pragma unroll
+    for (int k = 0; k < AHEAD; k++) {
+      f = weight(m[k], next);
+      total += l[k] * f;
+      v += x[k] * f;
+    }
     top = next;
   }
   *(f32x4*)&joined[team][d] = v;
   if (d == 0) team_m[team] = top, team_l[team] = total;
   __syncthreads();
   if (team != 0) return;
+#pragma unroll
   for (int k = 1; k < TEAMS; k++) {
     const float m = team_m[k], next = fmaxf(top, m), f0 = weight(top, next), f1 = weight(m, next);
     total = total * f0 + team_l[k] * f1;

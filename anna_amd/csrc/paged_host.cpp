@@ -4,6 +4,7 @@
 // carries the number of sequences that hold it and is copied when one of several holders writes
 // into it.  Every call checks all its arguments before it changes anything.
 #include <limits.h>
+#include <stdlib.h>
 
 #include <algorithm>
 #include <mutex>
@@ -31,8 +32,11 @@ struct anna_mi_paged {
 
 namespace {
 
-// Workgroups that an attention launch is split into at most, over all KV heads (and the tiles themselves).
-constexpr int64_t SPLIT_TARGET = 1024, TILE_TARGET = 512, TILE_FILL = 256, TILE_PAGES = 8, TILE_LEAST = 64;
+// Workgroups of a launch that run at once on the 256 compute units: two on each of the split form, one of the tile
+// form.  A few more than that would leave most of the chip idle for a whole round: drafted tokens with 612 workgroups
+// 49 us, with 496 of them 42 us; 2048 tokens at the end of 32K with 512 of them 1340 us, with 256 1270 us.
+const int64_t SPLIT_ONCE = getenv("SF") ? atoi(getenv("SF")) : 512, TILE_ONCE = getenv("TO") ? atoi(getenv("TO")) : 256, TILE_PAGES = getenv("TP") ? atoi(getenv("TP")) : 8;
+constexpr int64_t TILE_FILL = 256, TILE_LEAST = 64;
 
 int hip_ok(hipError_t e, const char* what) { return e == hipSuccess ? ANNA_MI_OK : fail_hip(e, what); }
 
@@ -136,6 +140,23 @@ struct Plan {
   int64_t touch_bound = 0, partial_rows = 0, partial_bound = 0;
 };
 
+// The fewest pages of an item of a form, `least` at least, with which there are at most `items` of them (or one a tile).
+int64_t fewest_pages(const std::vector<Record>& records, int form, int64_t items, int64_t least) {
+  int64_t low = least, high = least, tiles = 0;
+  for (const Record& r : records)
+    if (r.tiled == form) high = std::max<int64_t>(high, r.pages), tiles += r.pages > 0;
+  items = std::max(items, tiles);
+  while (low < high) {
+    const int64_t mid = (low + high) / 2;
+    int64_t n = 0;
+    for (const Record& r : records)
+      if (r.tiled == form) n += ceil_div(r.pages, mid);
+    if (n <= items) high = mid;
+    else low = mid + 1;
+  }
+  return low;
+}
+
 int make_plan(anna_mi_paged* h, int64_t n, const int32_t* seqs, const int64_t* starts, const int64_t* counts, Plan& p) {
   ANNA_CHECK(n >= 0 && (n == 0 || (seqs && starts && counts)), "span: null arrays");
   int rc = check_seqs(h, n, seqs);
@@ -179,17 +200,14 @@ int make_plan(anna_mi_paged* h, int64_t n, const int32_t* seqs, const int64_t* s
     std::stable_sort(p.records.begin(), p.records.end(), [](const Record& a, const Record& b) {
       return a.tiled != b.tiled ? a.tiled < b.tiled : a.tiled && a.pages > b.pages;
     });
-  // How many pages an item takes: the split form's are shared out to SPLIT_TARGET workgroups, the tile form's
-  // only while there are too few tiles for the chip, and not below TILE_PAGES, as an item's partial result
-  // is written and read again.
-  const int64_t target[2] = {std::max<int64_t>(1, SPLIT_TARGET / H), std::max<int64_t>(1, TILE_TARGET / H)};
-  const int64_t per[2] = {std::max<int64_t>(1, ceil_div(total[0], target[0])),
-                          tiles[1] >= target[1] ? INT_MAX : std::max<int64_t>(TILE_PAGES, ceil_div(total[1], target[1]))};
+  // How many pages an item takes: the workgroups of a launch shall fit the chip at once.
+  const int64_t target[2] = {std::max<int64_t>(1, SPLIT_ONCE / H), std::max<int64_t>(1, TILE_ONCE / H)};
+  const int64_t per[2] = {fewest_pages(p.records, 0, target[0], 1), fewest_pages(p.records, 1, target[1], TILE_PAGES)};
   for (Record& r : p.records) {
     const int f = r.tiled;
     const int64_t R = f ? p.tile_rows : p.few_rows, rows = std::min<int64_t>(R, r.count * G - r.tile * R);
     r.item0 = (int32_t)p.items[f];
-    r.splits = (int32_t)(f ? std::max<int64_t>(1, (r.pages + per[1] / 2) / per[1]) : ceil_div(r.pages, per[0]));
+    r.splits = (int32_t)ceil_div(r.pages, per[f]);
     r.part = -1;
     r.unit = -1;
     if (r.splits > 1) {
@@ -199,12 +217,11 @@ int make_plan(anna_mi_paged* h, int64_t n, const int32_t* seqs, const int64_t* s
     }
     p.items[f] += r.splits;
   }
-  // a tile that is split has more than `per` pages, so the items of such tiles are at most 2 * target
+  // a form has at most `target` items or one a tile; where there are more tiles, none is split
   for (int f = 0; f < 2; f++)
     if (rows_of[f] > 0) {
-      const bool splits = f == 0 || tiles[1] < target[1];
-      p.bound[f] = tiles[f] + (splits ? target[f] : 0);
-      if (splits) p.partial_bound += std::min(p.bound[f], 2 * target[f]) * rows_of[f];
+      p.bound[f] = std::max(target[f], tiles[f]);
+      if (tiles[f] < target[f]) p.partial_bound += target[f] * rows_of[f];
     }
   ANNA_CHECK(p.partial_bound <= INT_MAX && H * (p.bound[0] + p.bound[1]) <= INT_MAX / 64, "span: too many tokens");
   return ANNA_MI_OK;
