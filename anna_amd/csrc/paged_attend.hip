@@ -433,13 +433,17 @@ template <int D> struct ValueShare {
     }
   }
   __device__ __forceinline__ bool wide() const {
-    bool any = false;
+    // the scales are finite and not negative: their bits are in their order; 0 goes to the end by the 1 taken off
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 most = __builtin_bit_cast(u16x2, scale[0]), least = most - (uint16_t)1;
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const float x = bf16_lo(scale[k]), y = bf16_hi(scale[k]);
-      any |= fmaxf(x, y) > V_SCALE_MOST || (x < V_SCALE_LEAST && x > 0.0f) || (y < V_SCALE_LEAST && y > 0.0f);
+    for (int k = 1; k < 4; k++) {
+      const u16x2 x = __builtin_bit_cast(u16x2, scale[k]);
+      most = __builtin_elementwise_max(most, x);
+      least = __builtin_elementwise_min(least, (u16x2)(x - (uint16_t)1));
     }
-    return any;
+    constexpr uint32_t MOST = __builtin_bit_cast(uint32_t, V_SCALE_MOST) >> 16, LEAST = (__builtin_bit_cast(uint32_t, V_SCALE_LEAST) >> 16) - 1;
+    return (int)(max(most[0], most[1]) > MOST) | (int)(min(least[0], least[1]) < LEAST);
   }
   __device__ __forceinline__ void convert() {
 #pragma unroll
@@ -518,7 +522,7 @@ template <bool F16> __device__ __forceinline__ uint32_t probability(const f32x16
 // is below PAGE.  The two halves of the page go through one behind the other, so that the vector unit's softmax of
 // one runs beneath the matrix instructions of the other, and the next page's conversion beneath the rest:
 //   scores 0, first(k) | scores 1, softmax 0 | values 0, softmax 1 | values 1, second(k)
-// Every step is a pair of matrix instructions, a pair of fragments AHEAD steps ahead, and a share of the vector
+// Every step k is a pair of matrix instructions, a pair of fragments AHEAD steps ahead, and a share of the vector
 // work; the order is pinned, as the compiler left to itself reads all fragments first and spills.
 template <int D, bool F16, int AHEAD, class Q, class A, class B>
 __device__ __forceinline__ void take_page(Rows<D>& w, const u32x4* lds, Q query, int limit, bool cut, float scale, int lane, A first,
@@ -560,6 +564,11 @@ __device__ __forceinline__ void take_page(Rows<D>& w, const u32x4* lds, Q query,
       for (int d = 0; d < DTILES; d++) w.acc[d] *= factor[half];
     }
   };
+  // share i of n of a half's eight pairs of probabilities
+  auto probabilities = [&](int half, int i, int n) {
+#pragma unroll
+    for (int k = 8 * i / n; k < 8 * (i + 1) / n; k++) p[2 * half + k / 4][k % 4] = probability<F16>(z[half], 2 * k, scale, base, sum);
+  };
 #pragma unroll
   for (int i = 0; i < AHEAD; i++) read(i);
 #pragma unroll
@@ -576,12 +585,7 @@ __device__ __forceinline__ void take_page(Rows<D>& w, const u32x4* lds, Q query,
 #pragma unroll
     for (int u = 0; u < 2; u++) z[i / KHALF] = mfma32<F16>(f[i % RING][u], query(2 * (i % KHALF) + u), z[i / KHALF]);
     if (i < KHALF) first(i);
-    else {
-      constexpr int PAIRS = (8 + KHALF - 1) / KHALF;  // of probabilities a step
-#pragma unroll
-      for (int k = (i - KHALF) * PAIRS; k < (i - KHALF + 1) * PAIRS; k++)
-        if (k < 8) p[k / 4][k % 4] = probability<F16>(z[0], 2 * k, scale, base, sum);
-    }
+    else probabilities(0, i - KHALF, KHALF);
     PIN();
   }
   reference(1);
@@ -601,12 +605,8 @@ __device__ __forceinline__ void take_page(Rows<D>& w, const u32x4* lds, Q query,
       const int d = 2 * (i % (DTILES / 2)) + u;
       w.acc[d] = mfma32<F16>(f[(KSTEPS + i) % RING][u], p[i / (DTILES / 2)], w.acc[d]);
     }
-    if (i < VHALF) {
-      constexpr int PAIRS = (8 + VHALF - 1) / VHALF;
-#pragma unroll
-      for (int k = i * PAIRS; k < (i + 1) * PAIRS; k++)
-        if (k < 8) p[2 + k / 4][k % 4] = probability<F16>(z[1], 2 * k, scale, base, sum);
-    } else second(i - VHALF);
+    if (i < VHALF) probabilities(1, i, VHALF);
+    else second(i - VHALF);
     PIN();
   }
   second(VHALF);
@@ -692,7 +692,7 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
   // The loads are in: a flag if the page is none for fp16, and the scales as fp16.
   auto convert_keys = [&](int slot) {
     if (!has_keys) return;
-    if (keys.wide()) wide[slot] = 1;
+    if (__any(keys.wide())) wide[slot] = 1;
     keys.convert();
   };
   auto convert_values = [&](int slot) {
@@ -703,7 +703,7 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
         beyond |= values[n].wide();
         values[n].convert();
       }
-    if (beyond) wide[slot] = 1;
+    if (__any(beyond)) wide[slot] = 1;
   };
   const uint32_t mask = code_mask<ANNA_MI_F16>();
   const int key_at = KeyShare<D>::at(wave & 3, lane);

@@ -4,7 +4,6 @@
 // carries the number of sequences that hold it and is copied when one of several holders writes
 // into it.  Every call checks all its arguments before it changes anything.
 #include <limits.h>
-#include <stdlib.h>
 
 #include <algorithm>
 #include <mutex>
@@ -35,8 +34,10 @@ namespace {
 // Workgroups of a launch that run at once on the 256 compute units: two on each of the split form, one of the tile
 // form.  A few more than that would leave most of the chip idle for a whole round: drafted tokens with 612 workgroups
 // 49 us, with 496 of them 42 us; 2048 tokens at the end of 32K with 512 of them 1340 us, with 256 1270 us.
-const int64_t SPLIT_ONCE = getenv("SF") ? atoi(getenv("SF")) : 512, TILE_ONCE = getenv("TO") ? atoi(getenv("TO")) : 256, TILE_PAGES = getenv("TP") ? atoi(getenv("TP")) : 8;
-constexpr int64_t TILE_FILL = 256, TILE_LEAST = 64;
+constexpr int64_t SPLIT_ONCE = 512, TILE_ONCE = 256;
+// Tiles of 256 rows when they fill the chip; an item of the tile form has TILE_PAGES pages at least, as its partial
+// result is written and read again; up to TILE_LEAST query rows of a KV head are the split form's.
+constexpr int64_t TILE_FILL = 256, TILE_PAGES = 8, TILE_LEAST = 64;
 
 int hip_ok(hipError_t e, const char* what) { return e == hipSuccess ? ANNA_MI_OK : fail_hip(e, what); }
 

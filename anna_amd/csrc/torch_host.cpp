@@ -11,15 +11,19 @@
 // stamp check and its error text stay in one place.  The stream is an argument (the caller's current
 // stream), so no device header is needed.
 #include <pybind11/pybind11.h>
+#include <pybind11/stl.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
 
+#include <cstdint>
 #include <cstdlib>
 #include <optional>
 #include <stdexcept>
 #include <string>
+#include <utility>
+#include <vector>
 
 #include "../../include/anna_mi.h"
 
@@ -44,6 +48,15 @@ struct Library {
   decltype(&anna_mi_moe_combine) moe_combine = nullptr;
   decltype(&anna_mi_moe_prefill_workspace) moe_prefill_workspace = nullptr;
   decltype(&anna_mi_moe_prefill) moe_prefill = nullptr;
+  decltype(&anna_mi_paged_fork) paged_fork = nullptr;
+  decltype(&anna_mi_paged_free) paged_free = nullptr;
+  decltype(&anna_mi_paged_extend) paged_extend = nullptr;
+  decltype(&anna_mi_paged_lengths) paged_lengths = nullptr;
+  decltype(&anna_mi_paged_span_plan) paged_span_plan = nullptr;
+  decltype(&anna_mi_paged_span_fill) paged_span_fill = nullptr;
+  decltype(&anna_mi_paged_store) paged_store = nullptr;
+  decltype(&anna_mi_paged_read) paged_read = nullptr;
+  decltype(&anna_mi_paged_attend) paged_attend = nullptr;
 } lib;
 
 void bind(const py::dict& d) {
@@ -64,6 +77,15 @@ void bind(const py::dict& d) {
   get("anna_mi_moe_combine", lib.moe_combine);
   get("anna_mi_moe_prefill_workspace", lib.moe_prefill_workspace);
   get("anna_mi_moe_prefill", lib.moe_prefill);
+  get("anna_mi_paged_fork", lib.paged_fork);
+  get("anna_mi_paged_free", lib.paged_free);
+  get("anna_mi_paged_extend", lib.paged_extend);
+  get("anna_mi_paged_lengths", lib.paged_lengths);
+  get("anna_mi_paged_span_plan", lib.paged_span_plan);
+  get("anna_mi_paged_span_fill", lib.paged_span_fill);
+  get("anna_mi_paged_store", lib.paged_store);
+  get("anna_mi_paged_read", lib.paged_read);
+  get("anna_mi_paged_attend", lib.paged_attend);
 }
 
 void check(int rc, const char* name) {
@@ -459,6 +481,123 @@ OptTensor moe_block(const Tensor& x, const Tensor& logits, const Tensor& gq, con
   return out;
 }
 
+// ---------------------------------------------------------------- paged cache
+
+anna_mi_paged* paged(uintptr_t handle) { return reinterpret_cast<anna_mi_paged*>(handle); }
+anna_mi_paged_span* span_at(uintptr_t address) { return reinterpret_cast<anna_mi_paged_span*>(address); }
+
+// Whole numbers of a list or tuple, each within [low, high]; nullopt for anything else.
+template <class T> std::optional<std::vector<T>> whole(const py::handle& list, int64_t low, int64_t high) {
+  if (!PyList_CheckExact(list.ptr()) && !PyTuple_CheckExact(list.ptr())) return std::nullopt;
+  PyObject** items = PySequence_Fast_ITEMS(list.ptr());
+  std::vector<T> v(PySequence_Fast_GET_SIZE(list.ptr()));
+  for (size_t i = 0; i < v.size(); i++) {
+    if (!PyLong_CheckExact(items[i])) return std::nullopt;
+    int overflow = 0;
+    const long long x = PyLong_AsLongLongAndOverflow(items[i], &overflow);
+    if (overflow || x < low || x > high) return std::nullopt;
+    v[i] = (T)x;
+  }
+  return v;
+}
+constexpr int64_t I32 = INT32_MAX, I64 = INT64_MAX / 4;
+
+py::object paged_fork(uintptr_t handle, const py::object& parents, uintptr_t stream) {
+  const auto p = whole<int32_t>(parents, 0, I32);
+  if (!p) return py::none();
+  std::vector<int32_t> children(p->size());
+  check(lib.paged_fork(paged(handle), (int64_t)p->size(), p->data(), children.data(), stream_ptr(stream)), "anna_mi_paged_fork");
+  return py::cast(children);
+}
+
+bool paged_free(uintptr_t handle, const py::object& seqs, uintptr_t stream) {
+  const auto s = whole<int32_t>(seqs, 0, I32);
+  if (!s) return false;
+  check(lib.paged_free(paged(handle), (int64_t)s->size(), s->data(), stream_ptr(stream)), "anna_mi_paged_free");
+  return true;
+}
+
+// Fills a span anew, with its buffer and workspace: extend (starts is None) by counts, None for one each, or the
+// tokens that the sequences hold already.  -> (seqs, starts, counts, tensors), or None.
+py::object paged_span(uintptr_t handle, uintptr_t span, const py::object& seqs, const py::object& starts, const py::object& counts,
+                      int64_t max_length, int64_t kv_heads, int64_t head_dim, int64_t device, uintptr_t stream) {
+  const auto s = whole<int32_t>(seqs, 0, I32);
+  if (!s) return py::none();
+  const int64_t n = (int64_t)s->size();
+  std::optional<std::vector<int64_t>> c, at;
+  if (counts.is_none()) c = std::vector<int64_t>(n, 1);
+  else c = whole<int64_t>(counts, 0, I64);
+  if (!c || (int64_t)c->size() != n) return py::none();
+  if (starts.is_none()) {
+    at = std::vector<int64_t>(n);
+    check(lib.paged_lengths(paged(handle), n, s->data(), at->data(), nullptr), "anna_mi_paged_lengths");
+    for (int64_t i = 0; i < n; i++)
+      if ((*at)[i] < 0 || (*c)[i] > max_length - (*at)[i]) return py::none();
+    check(lib.paged_extend(paged(handle), n, s->data(), c->data(), at->data(), stream_ptr(stream)), "anna_mi_paged_extend");
+  } else {
+    at = whole<int64_t>(starts, 0, I64);
+    if (!at || (int64_t)at->size() != n) return py::none();
+  }
+  anna_mi_paged_span* out = span_at(span);
+  check(lib.paged_span_plan(paged(handle), n, s->data(), at->data(), c->data(), out), "anna_mi_paged_span_plan");
+  const auto ints = at::TensorOptions().dtype(at::kInt).device(at::kCUDA, (c10::DeviceIndex)device);
+  std::vector<Tensor> held{at::empty({out->words}, ints)};
+  if (out->partial_rows > 0) {
+    held.push_back(at::empty({out->partial_rows, kv_heads, 2}, ints.dtype(at::kFloat)));
+    held.push_back(at::empty({out->partial_rows, kv_heads, head_dim}, ints.dtype(at::kFloat)));
+    out->partial_stats = (float*)ptr(held[1]);
+    out->partial_values = (float*)ptr(held[2]);
+  }
+  out->buf = (int32_t*)ptr(held[0]);
+  check(lib.paged_span_fill(paged(handle), n, s->data(), at->data(), c->data(), out, stream_ptr(stream)), "anna_mi_paged_span_fill");
+  return py::make_tuple(*s, *at, *c, held);
+}
+
+// Rows [tokens, heads, head_dim] of the cache's type that the kernels read as they are
+bool paged_rows(const Tensor& t, const at::Device& dev, at::ScalarType dt, int64_t tokens, int64_t heads, int64_t head_dim) {
+  return plain(t, dev) && t.scalar_type() == dt && t.dim() == 3 && t.size(0) == tokens && t.size(1) == heads && t.size(2) == head_dim &&
+         t.stride(2) == 1 && (tokens <= 1 || t.stride(0) % 8 == 0) && (heads <= 1 || t.stride(1) % 8 == 0) &&
+         reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+int64_t token_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : 0; }
+int64_t head_stride(const Tensor& t) { return t.size(1) > 1 ? t.stride(1) : 0; }
+
+bool paged_store(uintptr_t handle, int64_t layer, uintptr_t span, const Tensor& keys, const Tensor& values, const Tensor& pool,
+                 at::ScalarType dtype, int64_t head_dim, bool capturing, uintptr_t stream) {
+  const anna_mi_paged_span* s = span_at(span);
+  if (!paged_rows(keys, pool.device(), dtype, s->tokens, pool.size(2), head_dim) ||
+      !paged_rows(values, pool.device(), dtype, s->tokens, pool.size(2), head_dim))
+    return false;
+  check(lib.paged_store(paged(handle), layer, s, ptr(keys), token_stride(keys), head_stride(keys), ptr(values), token_stride(values),
+                        head_stride(values), capturing, stream_ptr(stream)),
+        "anna_mi_paged_store");
+  return true;
+}
+
+std::pair<Tensor, Tensor> paged_read(uintptr_t handle, int64_t layer, uintptr_t span, const Tensor& pool, at::ScalarType dtype,
+                                     int64_t head_dim, bool capturing, uintptr_t stream) {
+  const anna_mi_paged_span* s = span_at(span);
+  Tensor keys = at::empty({s->tokens, pool.size(2), head_dim}, pool.options().dtype(dtype)), values = at::empty_like(keys);
+  check(lib.paged_read(paged(handle), layer, s, ptr(keys), ptr(values), capturing, stream_ptr(stream)), "anna_mi_paged_read");
+  return {keys, values};
+}
+
+OptTensor paged_attend(uintptr_t handle, int64_t layer, uintptr_t span, const Tensor& query, const OptTensor& gate, const OptTensor& out,
+                       const Tensor& pool, at::ScalarType dtype, int64_t q_heads, int64_t head_dim, double scaling, bool capturing,
+                       uintptr_t stream) {
+  const anna_mi_paged_span* s = span_at(span);
+  const at::Device dev = pool.device();
+  if (!paged_rows(query, dev, dtype, s->tokens, q_heads, head_dim) || (gate && !paged_rows(*gate, dev, dtype, s->tokens, q_heads, head_dim)) ||
+      (out && (!paged_rows(*out, dev, dtype, s->tokens, q_heads, head_dim) || !out->is_contiguous())) || !(scaling > 0.0 && scaling < 1e30))
+    return std::nullopt;
+  Tensor o = out ? *out : at::empty({s->tokens, q_heads, head_dim}, query.options().requires_grad(false));
+  check(lib.paged_attend(paged(handle), layer, s, ptr(query), token_stride(query), head_stride(query), ptr(gate),
+                         gate ? token_stride(*gate) : 0, gate ? head_stride(*gate) : 0, ptr(o), (float)scaling, capturing,
+                         stream_ptr(stream)),
+        "anna_mi_paged_attend");
+  return o;
+}
+
 }  // namespace
 
 #ifndef ANNA_MI_SOURCE_HASH
@@ -476,4 +615,10 @@ PYBIND11_MODULE(_torch_host, m) {
   m.def("decode_pool", &decode_pool, no_gil);
   m.def("tq_store", &tq_store, no_gil);
   m.def("moe_block", &moe_block, no_gil);
+  m.def("paged_fork", &paged_fork);
+  m.def("paged_free", &paged_free);
+  m.def("paged_span", &paged_span);
+  m.def("paged_store", &paged_store, no_gil);
+  m.def("paged_read", &paged_read, no_gil);
+  m.def("paged_attend", &paged_attend, no_gil);
 }

@@ -65,6 +65,7 @@ class PagedSpan:
         self.counts: list[int] = []
         self._c = _lib.PagedSpan()
         self._ref = ctypes.byref(self._c)
+        self._address = ctypes.addressof(self._c)
         self._tensors: list[torch.Tensor] = []
         self._streams: set[int] = set()
         self._version = -1
@@ -93,6 +94,20 @@ class PagedSpan:
         cache._call("anna_mi_paged_span_fill", n, seqs, starts, counts, self._ref, cache._stream())
         self.seqs, self.starts, self.counts = list(seqs), list(starts), list(counts)
         self._version = cache._version
+
+    def _fresh(self, seqs, starts, counts) -> bool:
+        """A new span's fill by the host module; False for calls that it leaves to the general way."""
+        cache = self.cache
+        if not cache._here():
+            return False
+        stream = cache._stream()
+        got = _lib.host().paged_span(cache._handle.value, self._address, seqs, starts, counts, cache.max_length,
+                                     cache.kv_heads, cache.head_dim, cache.device.index, stream)
+        if got is None:
+            return False
+        self.seqs, self.starts, self.counts, self._tensors = got
+        self._streams, self._version = {stream}, cache._version
+        return True
 
     @property
     def rows(self) -> torch.Tensor:
@@ -145,11 +160,15 @@ class PagedInt4Cache:
         return torch._C._cuda_getCurrentRawStream(self.device.index)
 
     def _call(self, name: str, *args) -> None:
-        if torch.cuda.current_device() != self.device.index:
+        if self._here():
+            _lib.call(name, self._handle, *args)
+        else:
             with torch.cuda.device(self.device):
                 _lib.call(name, self._handle, *args)
-        else:
-            _lib.call(name, self._handle, *args)
+
+    def _here(self) -> bool:
+        """Whether the cache's device is the current one, which the host module's calls take for granted."""
+        return torch.cuda.current_device() == self.device.index
 
     def _counts(self, what: str) -> None:
         if torch.cuda.is_current_stream_capturing():
@@ -170,6 +189,10 @@ class PagedInt4Cache:
         """A new sequence for every listed one (which may repeat), holding the same tokens in the same pages.
         A page is copied when one of the sequences that share it grows into it."""
         self._counts("fork")
+        if self._here():
+            children = _lib.host().paged_fork(self._handle.value, parents, self._stream())
+            if children is not None:
+                return children
         parents = _ints(parents, ctypes.c_int32)
         children = (ctypes.c_int32 * len(parents))()
         self._call("anna_mi_paged_fork", len(parents), parents, children, self._stream())
@@ -181,6 +204,12 @@ class PagedInt4Cache:
         too few pages.  ``span``: an earlier span of as many sequences with the same counts, which is
         filled again in place (a captured graph holds its addresses)."""
         self._counts("extend")
+        if span is None:
+            span = PagedSpan(self)
+            with self._lock:
+                if span._fresh(seqs, None, counts):
+                    return span
+            span = None
         seqs = _ints(seqs, ctypes.c_int32)
         counts = _ints([1] * len(seqs) if counts is None else counts, ctypes.c_int64)
         if len(counts) != len(seqs):
@@ -200,6 +229,11 @@ class PagedInt4Cache:
     def span(self, seqs, starts, counts, *, span: PagedSpan | None = None) -> PagedSpan:
         """The span of tokens that the sequences hold already: to store them anew, read them, or attend for them."""
         self._counts("span")
+        if span is None:
+            span = PagedSpan(self)
+            if starts is not None and counts is not None and span._fresh(seqs, starts, counts):
+                return span
+            span = None
         seqs, starts, counts = _ints(seqs, ctypes.c_int32), _ints(starts, ctypes.c_int64), _ints(counts, ctypes.c_int64)
         if not len(seqs) == len(starts) == len(counts):
             raise ValueError(f"{len(seqs)} sequences, {len(starts)} starts and {len(counts)} counts")
@@ -226,8 +260,9 @@ class PagedInt4Cache:
     def free(self, seqs) -> None:
         """Ends sequences; pages that no other sequence shares return to the pool."""
         self._counts("free")
-        seqs = _ints(seqs, ctypes.c_int32)
-        self._call("anna_mi_paged_free", len(seqs), seqs, self._stream())
+        if not (self._here() and _lib.host().paged_free(self._handle.value, seqs, self._stream())):
+            seqs = _ints(seqs, ctypes.c_int32)
+            self._call("anna_mi_paged_free", len(seqs), seqs, self._stream())
         self._version += 1
 
     def _lengths(self, seqs):
@@ -313,25 +348,35 @@ class PagedInt4Cache:
 
     def store(self, layer: int, span: PagedSpan, keys: torch.Tensor, values: torch.Tensor) -> None:
         """Quantizes the span's keys and values [tokens, kv_heads, head_dim] into the layer's pages."""
-        stream = self._check("store", layer, span)
+        stream, capturing = self._check("store", layer, span), torch.cuda.is_current_stream_capturing()
+        if self._here() and _lib.host().paged_store(self._handle.value, layer, span._address, keys, values, self.pool, self.dtype,
+                                                    self.head_dim, capturing, stream):
+            return
         keys, values = self._rows("keys", keys, span, self.kv_heads), self._rows("values", values, span, self.kv_heads)
         self._call("anna_mi_paged_store", layer, span._ref, keys.data_ptr(), *self._strides(keys), values.data_ptr(),
-                   *self._strides(values), torch.cuda.is_current_stream_capturing(), stream)
+                   *self._strides(values), capturing, stream)
 
     def read(self, layer: int, span: PagedSpan) -> tuple[torch.Tensor, torch.Tensor]:
         """The span's keys and values as the cache holds them, dense [tokens, kv_heads, head_dim]."""
-        stream = self._check("read", layer, span)
+        stream, capturing = self._check("read", layer, span), torch.cuda.is_current_stream_capturing()
+        if self._here():
+            return _lib.host().paged_read(self._handle.value, layer, span._address, self.pool, self.dtype, self.head_dim,
+                                          capturing, stream)
         keys, values = (torch.empty((span._c.tokens, self.kv_heads, self.head_dim), dtype=self.dtype, device=self.device)
                         for _ in range(2))
-        self._call("anna_mi_paged_read", layer, span._ref, keys.data_ptr(), values.data_ptr(),
-                   torch.cuda.is_current_stream_capturing(), stream)
+        self._call("anna_mi_paged_read", layer, span._ref, keys.data_ptr(), values.data_ptr(), capturing, stream)
         return keys, values
 
     def attend(self, layer: int, span: PagedSpan, query: torch.Tensor, *, scaling: float,
                gate: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """Causal attention for the span's tokens: query [tokens, q_heads, head_dim] over all tokens of its
         sequence up to and with its own -> the same shape.  gate (optional, same shape as query): out *= sigmoid(gate)."""
-        stream = self._check("attend", layer, span)
+        stream, capturing = self._check("attend", layer, span), torch.cuda.is_current_stream_capturing()
+        if self._here():
+            got = _lib.host().paged_attend(self._handle.value, layer, span._address, query, gate, out, self.pool, self.dtype,
+                                           self.q_heads, self.head_dim, scaling, capturing, stream)
+            if got is not None:
+                return got
         if not 0.0 < scaling < 1e30:
             raise ValueError(f"scaling must be positive and finite, got {scaling}")
         query = self._rows("query", query, span, self.q_heads)
@@ -344,5 +389,5 @@ class PagedInt4Cache:
             raise ValueError(f"out must be a contiguous, 16-byte aligned {self.dtype} tensor of the query's shape")
         self._call("anna_mi_paged_attend", layer, span._ref, query.data_ptr(), *self._strides(query),
                    None if gate is None else gate.data_ptr(), *((0, 0) if gate is None else self._strides(gate)),
-                   out.data_ptr(), scaling, torch.cuda.is_current_stream_capturing(), stream)
+                   out.data_ptr(), scaling, capturing, stream)
         return out
