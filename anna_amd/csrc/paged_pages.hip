@@ -96,6 +96,14 @@ __device__ __forceinline__ float group_max(float v) {
   return fmaxf(v, dpp_move<0x141>(v));
 }
 
+// x / y by the (nearly exact) reciprocal of y and one correction: exact where the quotient has few bits, as the halves
+// between two codes or two bf16 scales have, and elsewhere far nearer to it than it is to such a half (x and y have 19
+// bits between them).  Three instructions, where a division takes ten.
+__device__ __forceinline__ float quotient(float x, float y, float reciprocal) {
+  const float q = x * reciprocal;
+  return fmaf(fmaf(-q, y, x), reciprocal, q);
+}
+
 // Codes of this lane's 8 values (one a byte), and the group's scale (bf16 bits) and zero.
 struct Coded {
   uint32_t lo, hi;
@@ -116,21 +124,28 @@ template <int DT> __device__ __forceinline__ Coded quantize(u32x4 raw) {
   high = group_max(high);
   // halves, so that a spread of twice the largest value stays finite; the quotients are correctly
   // rounded, so one that lies between two bf16 values stays there and goes to the even one
-  const float spread = fmaxf((0.5f * high - 0.5f * low) / 7.5f, fmaxf(fabsf(low), fabsf(high)) / 120.0f);
+  const float spread = fmaxf(quotient(0.5f * high - 0.5f * low, 7.5f, 1.0f / 7.5f),
+                             quotient(fmaxf(fabsf(low), fabsf(high)), 120.0f, 1.0f / 120.0f));
   Coded c = {0, 0, 0, 0};
   if (!(spread >= 7.888609052210118e-31f)) return c;  // 2^-100
   c.scale = f32_to_bf16_bits(spread);
-  const float scale = bf16_bits_to_f32(c.scale);
-  const float zero = rintf(low / scale);
+  const float scale = bf16_bits_to_f32(c.scale), inverse = __builtin_amdgcn_rcpf(scale);
+  auto steps = [&](float v) { return rintf(quotient(v, scale, inverse)); };
+  const float zero = steps(low);
   c.zero = (int)zero;
 #pragma unroll
-  for (int k = 0; k < 8; k++) {
-    const float q = fminf(fmaxf(rintf(x[k] / scale) - zero, 0.0f), 15.0f);
-    const uint32_t code = (uint32_t)q;
-    if (k < 4) c.lo |= code << (8 * k);
-    else c.hi |= code << (8 * (k - 4));
+  for (int k = 0; k < 4; k++) {
+    c.lo = __builtin_amdgcn_cvt_pk_u8_f32(__builtin_amdgcn_fmed3f(steps(x[k]) - zero, 0.0f, 15.0f), k, c.lo);
+    c.hi = __builtin_amdgcn_cvt_pk_u8_f32(__builtin_amdgcn_fmed3f(steps(x[4 + k]) - zero, 0.0f, 15.0f), k, c.hi);
   }
   return c;
+}
+
+// Two nibbles a byte: bytes 0 and 2 of x with the next one above each, as 16 bits.
+__device__ __forceinline__ uint32_t nibbles(uint32_t x) { return __builtin_amdgcn_perm(0, x | x >> 4, 0x0C0C0200); }
+// A word of 8 codes, one a byte: code e at bits 4 * ((e % 2) * 4 + e / 2).
+__device__ __forceinline__ uint32_t code_word(uint32_t lo, uint32_t hi) {
+  return nibbles(__builtin_amdgcn_perm(hi, lo, 0x06040200)) | nibbles(__builtin_amdgcn_perm(hi, lo, 0x07050301)) << 16;
 }
 
 template <int DT, int D>
@@ -138,78 +153,82 @@ __global__ __launch_bounds__(256) void paged_store_kernel(uint8_t* __restrict__ 
                                                           const int32_t* __restrict__ header, const Touch* __restrict__ touch,
                                                           int heads, const uint16_t* __restrict__ keys, int64_t k_token, int64_t k_head,
                                                           const uint16_t* __restrict__ values, int64_t v_token, int64_t v_head) {
-  constexpr int NG = D / GROUP, CHUNKS = D / 8, STEPS = PAGE * CHUNKS / 256, PITCH = D + 16;
-  __shared__ __align__(16) uint8_t codes[PAGE * PITCH];  // of the values
+  constexpr int NG = D / GROUP, CHUNKS = D / 8, PITCH = D + 16;
+  __shared__ __align__(16) uint8_t codes[PAGE * PITCH];     // of the values
+  __shared__ __align__(16) uint8_t image[page_bytes(D)];  // of a page that is written whole, in 16-byte words at the end
   __shared__ int bad[PAGE];
   const int tid = threadIdx.x, item = blockIdx.x / heads, h = blockIdx.x % heads;
   if (item >= header[3]) return;
   const Touch t = touch[item];
   uint8_t* page = pool + ((int64_t)table[t.row * width + t.page] * heads + h) * page_bytes(D);
   const int slots = (t.end - t.begin) * CHUNKS;
+  const bool whole = t.end - t.begin == PAGE;
+  auto put = [&](int at, auto value) {
+    if (whole) *(decltype(value)*)(image + at) = value;
+    else *(decltype(value)*)(page + at) = value;
+  };
   if (tid < PAGE) bad[tid] = 0;
-  u32x4 kr[STEPS], vr[STEPS];
-#pragma unroll
-  for (int s = 0; s < STEPS; s++) {
-    const int slot = s * 256 + tid, n = slot / CHUNKS, c = slot % CHUNKS;
-    if (slot < slots) {
-      kr[s] = *(const u32x4*)(keys + (t.token + n) * k_token + h * k_head + c * 8);
-      vr[s] = *(const u32x4*)(values + (t.token + n) * v_token + h * v_head + c * 8);
-    }
-  }
+  const uint16_t *k_from = keys + t.token * k_token + h * k_head, *v_from = values + t.token * v_token + h * v_head;
+  auto key = [&](int slot) { return *(const u32x4*)(k_from + slot / CHUNKS * k_token + slot % CHUNKS * 8); };
+  auto value = [&](int slot) { return *(const u32x4*)(v_from + slot / CHUNKS * v_token + slot % CHUNKS * 8); };
+  // The values go by twice: once for what is not finite, which concerns a token's keys and values, and once, out of
+  // the cache, for their codes.  Only the first of a thread's, all that a single token has, stay in registers.
+  u32x4 k0 = {0, 0, 0, 0}, v0 = {0, 0, 0, 0};
+  if (tid < slots) k0 = key(tid), v0 = value(tid);
   __syncthreads();
-#pragma unroll
-  for (int s = 0; s < STEPS; s++) {
-    const int slot = s * 256 + tid;
-    if (slot < slots && (not_finite<DT>(kr[s]) || not_finite<DT>(vr[s]))) bad[slot / CHUNKS] = 1;
-  }
+  if (tid < slots && (not_finite<DT>(k0) || not_finite<DT>(v0))) bad[tid / CHUNKS] = 1;
+  for (int slot = tid + 256; slot < slots; slot += 256)
+    if (not_finite<DT>(key(slot)) || not_finite<DT>(value(slot))) bad[slot / CHUNKS] = 1;
   __syncthreads();
-#pragma unroll
-  for (int s = 0; s < STEPS; s++) {
-    const int slot = s * 256 + tid;
-    if (slot >= slots) break;  // whole groups of 8 lanes
+  for (int slot = tid; slot < slots; slot += 256) {  // whole groups of 8 lanes
+    const u32x4 kr = slot == tid ? k0 : key(slot), vr = slot == tid ? v0 : value(slot);
     const int n = slot / CHUNKS, c = slot % CHUNKS, token = t.begin + n, g = c / 8;
-    const bool lost = bad[n] != 0;
-    Coded k = quantize<DT>(kr[s]), v = quantize<DT>(vr[s]);
-    if (lost) k = Coded{0, 0, 0x7FC0, 0}, v = Coded{0, 0, 0, 0};
-    uint32_t word = 0;
-#pragma unroll
-    for (int e = 0; e < 8; e++) word |= (((e < 4 ? k.lo : k.hi) >> (8 * (e & 3))) & 15u) << code_shift(e);
-    *(uint32_t*)(page + token * (D / 2) + ((c % 4) * (D / 32) + c / 4) * 4) = word;
+    Coded k = {0, 0, 0x7FC0, 0}, v = {0, 0, 0, 0};
+    if (!bad[n]) {
+      k = quantize<DT>(kr);
+      v = quantize<DT>(vr);
+    }
+    put(token * (D / 2) + ((c % 4) * (D / 32) + c / 4) * 4, code_word(k.lo, k.hi));
     *(uint2*)(codes + token * PITCH + c * 8) = uint2{v.lo, v.hi};
     if (c % 8 == 0) {
-      const int at = ((token / 4) * NG + g) * 4 + token % 4;
-      ((uint16_t*)(page + K_SCALES * D))[at] = k.scale;
-      ((uint16_t*)(page + K_OFFSETS * D))[token * NG + g] = f32_to_bf16_bits((float)(k.zero - CODE_BASE));
-      ((uint16_t*)(page + V_SCALES * D))[at] = v.scale;
-      ((uint16_t*)(page + V_OFFSETS * D))[at] = f32_to_bf16_bits((float)(v.zero - CODE_BASE));
+      const int at = 2 * (((token / 4) * NG + g) * 4 + token % 4);
+      put(K_SCALES * D + at, k.scale);
+      put(K_OFFSETS * D + 2 * (token * NG + g), f32_to_bf16_bits((float)(k.zero - CODE_BASE)));
+      put(V_SCALES * D + at, v.scale);
+      put(V_OFFSETS * D + at, f32_to_bf16_bits((float)(v.zero - CODE_BASE)));
     }
   }
   __syncthreads();
-  // value words: 8 tokens of a dim each; those of which the span holds only some keep the others
+  // Value words: 8 tokens of a dim each; those of which the span holds only some keep the others.  A thread takes four
+  // neighbouring dims: a dword of each token, two tokens to a byte, then the four dims' bytes apart.
   for (int unit = tid; unit < 2 * NG * 64; unit += 256) {
-    const int half = unit / (NG * 64), g = unit / 64 % NG, lane = unit % 64, q = lane / 16, r = lane % 16;
+    const int half = unit / (NG * 64), g = unit / 64 % NG, w = unit / 16 % 4, q = unit / 4 % 4, r = unit % 4 * 4;
+    const int first = half * 32 + 4 * q;
     uint32_t mask = 0;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      const int token = half * 32 + (e < 4 ? 0 : 12) + 4 * q + e;
+      const int token = first + (e < 4 ? e : 12 + e);
       if (token >= t.begin && token < t.end) mask |= 15u << code_shift(e);
     }
     if (mask == 0) continue;
-    u32x4 w = {0, 0, 0, 0};
+    uint32_t v[8], two[4];
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const int token = half * 32 + (e < 4 ? 0 : 12) + 4 * q + e;
+    for (int e = 0; e < 8; e++)
+      v[e] = *(const uint32_t*)(codes + (first + (e < 4 ? e : 12 + e)) * PITCH + 64 * g + 16 * w + r) & 0x0F0F0F0Fu;
+    // nibbles 0 .. 7 of a word are tokens 0, 2, 4, 6, 1, 3, 5, 7
+    two[0] = v[0] | v[2] << 4, two[1] = v[4] | v[6] << 4, two[2] = v[1] | v[3] << 4, two[3] = v[5] | v[7] << 4;
+    const uint32_t ab = __builtin_amdgcn_perm(two[1], two[0], 0x05010400), AB = __builtin_amdgcn_perm(two[1], two[0], 0x07030602);
+    const uint32_t cd = __builtin_amdgcn_perm(two[3], two[2], 0x05010400), CD = __builtin_amdgcn_perm(two[3], two[2], 0x07030602);
+    const uint32_t word[4] = {__builtin_amdgcn_perm(cd, ab, 0x05040100), __builtin_amdgcn_perm(cd, ab, 0x07060302),
+                              __builtin_amdgcn_perm(CD, AB, 0x05040100), __builtin_amdgcn_perm(CD, AB, 0x07060302)};
+    const int at = V_CODES * D + (((half * NG + g) * 64 + q * 16 + r) * 4 + w) * 4;
 #pragma unroll
-      for (int k = 0; k < 4; k++) w[k] |= (codes[token * PITCH + 64 * g + 16 * k + r] & 15u) << code_shift(e);
-    }
-    u32x4* to = (u32x4*)(page + V_CODES * D) + unit;
-    if (mask != 0xFFFFFFFFu) {
-      const u32x4 old = *to;
-#pragma unroll
-      for (int k = 0; k < 4; k++) w[k] = (w[k] & mask) | (old[k] & ~mask);
-    }
-    *to = w;
+    for (int k = 0; k < 4; k++)
+      put(at + 16 * k, mask == 0xFFFFFFFFu ? word[k] : (word[k] & mask) | (*(const uint32_t*)(page + at + 16 * k) & ~mask));
   }
+  if (!whole) return;
+  __syncthreads();
+  for (int at = tid * 16; at < page_bytes(D); at += 256 * 16) *(u32x4*)(page + at) = *(const u32x4*)(image + at);
 }
 
 // 8 codes (bytes) of a group to values of the dense type: exact in fp32, then rounded once.

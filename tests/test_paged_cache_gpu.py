@@ -220,6 +220,54 @@ def test_attend_large_and_small_values(gpu):
                 assert ((err <= tol) | (torch.isnan(err) & torch.isnan(want))).all(), (dtype, factor, n)
 
 
+@pytest.mark.parametrize("D,H,HQ", [(64, 2, 4), (128, 1, 4), (256, 1, 2)])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("what", ["key", "value", "tiny value", "query"])
+def test_tiles_beyond_fp16(gpu, D, H, HQ, dtype, what):
+    """Scales of keys or values, or queries, that leave what fp16 operands hold, from some page on: the tiles' form goes
+    on in bf16 there, to bf16's tolerance."""
+    n, factor = 300, {"key": 2.0 ** 9, "value": 2.0 ** 14 if dtype == BF else 2.0 ** 12, "tiny value": 2.0 ** -22, "query": 2.0 ** 12}[what]
+    cache = make(D=D, H=H, HQ=HQ, dtype=dtype)
+    seqs = cache.add(1)
+    k, v, q = (rows((n, h, D), torch.float32, i) for i, h in ((1, H), (2, H), (3, HQ)))
+    if what == "key":
+        k[150:170] *= factor
+    elif what == "query":
+        q[190:, 0] *= factor
+    else:
+        v[150:170] *= factor
+    # large scores have large errors: keep them apart from the ranges that are tested
+    scaling = D ** -0.5 / (factor if what in ("key", "query") else 1.0)
+    big = torch.finfo(dtype).max
+    k, v, q = (x.clamp(-big, big).to(dtype) for x in (k, v, q))
+    cache.store(0, cache.extend(seqs, [n]), k, v)
+    m = Mirror()
+    m.store(seqs[0], 0, k.cpu(), v.cpu())
+    got = cache.attend(0, cache.span(seqs, [0], [n]), q, scaling=scaling)
+    want, tol = attention(q.cpu(), *m.rows[seqs[0]], 0, scaling, BF)  # bf16's steps
+    want16, tol16 = attention(q.cpu(), *m.rows[seqs[0]], 0, scaling, dtype)
+    err = (got.cpu().double() - want).abs()
+    assert (err <= tol + tol16).all()
+    if what != "query":
+        assert (err[:128] <= tol16[:128]).all()  # the tiles before that are the type's
+
+
+def test_attend_many_query_heads(gpu):
+    """More query heads on a key/value head than a tile of the split form has rows."""
+    cache = make(D=64, H=1, HQ=80)
+    seqs, m = fill(cache, [300, 70])
+    check_attend(cache, m, seqs, [299, 69], [1, 1])
+
+
+def test_attend_many_sequences(gpu):
+    lens = [(37 * i) % 150 + 1 for i in range(300)]
+    cache = make(D=64, H=2, HQ=4, pages=1000, sequences=300, length=200)
+    seqs, m = fill(cache, lens)
+    check_attend(cache, m, seqs, [n - 1 for n in lens], [1] * 300)
+    kids = cache.fork(seqs[:0])
+    assert kids == []
+
+
 @pytest.mark.parametrize("count", [1, 100])
 def test_attend_strided_inputs_and_out(gpu, count):
     cache = make(D=128, HQ=8, H=2)
@@ -487,6 +535,10 @@ def test_refusals_leave_the_cache_as_it_was(gpu):
         (lambda: cache.extend([-1]), RuntimeError, "not in use"),
         (lambda: cache.extend([1 << 40]), ValueError, "range"),
         (lambda: cache.extend([0.5]), TypeError, "integer"),
+        (lambda: cache.extend(seqs, [1, 1 << 62]), RuntimeError, "max_length"),
+        (lambda: cache.extend(seqs, (1, 1 << 70)), ValueError, "range"),
+        (lambda: cache.fork([-1]), RuntimeError, "not in use"),
+        (lambda: cache.free([1 << 40]), ValueError, "range"),
         (lambda: cache.span(seqs, [0, 30], [101, 1]), RuntimeError, "holds"),
         (lambda: cache.span(seqs, [-1, 0], [1, 1]), RuntimeError, "holds"),
         (lambda: cache.span(seqs, [0], [1]), ValueError, "starts"),
@@ -520,6 +572,20 @@ def test_refusals_leave_the_cache_as_it_was(gpu):
     cache.free([seqs[1]])
     with pytest.raises(RuntimeError, match="holds 0 tokens|not in use"):
         cache.read(0, span)
+
+
+def test_sequences_by_other_integers(gpu):
+    """Lists, tuples, arrays and numpy integers name sequences alike; the host module takes plain lists alone."""
+    np = pytest.importorskip("numpy")
+    cache = make(D=64, H=2, HQ=4, length=100)
+    seqs, m = fill(cache, [20, 30])
+    for names in (seqs, tuple(seqs), np.array(seqs), [np.int64(s) for s in seqs], torch.tensor(seqs)):
+        span = cache.extend(names, np.array([1, 2]))
+        assert span.seqs == seqs and span.counts == [1, 2] and span.tokens == 3
+        kids = cache.fork(names)
+        cache.free(np.array(kids))
+        assert list(cache.span(names, [0, 0], (1, 1)).rows.cpu()) == seqs
+    assert cache.lengths(seqs) == [25, 40]
 
 
 def test_empty_spans(gpu):
