@@ -61,7 +61,7 @@ struct Record {
 
 // The words of an update travel in the kernel's arguments (at most 4 KB of them): no staging memory whose
 // life would have to be tied to the stream, and one launch for the few words of a decode step.
-constexpr int UPDATE_WORDS = 960;
+constexpr int UPDATE_WORDS = 952;
 struct Update {
   int32_t* table;
   int64_t width;
@@ -69,9 +69,13 @@ struct Update {
   int32_t header[4];
   int64_t rows_at, split_at, tile_at, units_at, touch_at;
   int32_t group, split_rows, tile_rows;  // query heads of a KV head; rows of the two forms' tiles
-  int32_t records, entries, copies;      // in this order in words
-  int32_t words[UPDATE_WORDS];           // Record; (index, page); (row, source row or -1, pages): the rest of row is zeroed
+  uint8_t* pool;  // for page copies within it: bytes of a layer and of a page of all KV heads, layers
+  int64_t pool_layer, page;
+  int32_t layers;
+  int32_t records, entries, copies, pairs;  // in this order in words
+  int32_t words[UPDATE_WORDS];  // Record; (index, page); (row, source row or -1, pages): the rest of row is zeroed; (page, page)
 };
+static_assert(sizeof(Update) <= 4096, "an update is a kernel argument");
 int launch_update(const Update& u, hipStream_t stream);
 
 struct Copy {
@@ -82,6 +86,7 @@ struct Copy {
   int32_t pairs;
   int32_t words[UPDATE_WORDS];  // (source page or -1 for zeros, page)
 };
+static_assert(sizeof(Copy) <= 4096, "a copy is a kernel argument");
 int launch_copy(const Copy& c, int64_t layers, hipStream_t stream);
 
 struct Attend {

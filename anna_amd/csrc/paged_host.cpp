@@ -4,6 +4,7 @@
 // carries the number of sequences that hold it and is copied when one of several holders writes
 // into it.  Every call checks all its arguments before it changes anything.
 #include <limits.h>
+#include <stddef.h>
 
 #include <algorithm>
 #include <mutex>
@@ -23,6 +24,8 @@ struct anna_mi_paged {
   std::vector<int32_t> refs;    // of every page
   std::vector<int32_t> free_pages, free_seqs;
   std::vector<uint8_t> seen;  // by sequence, zero between calls
+  // of an extend whose launch is left to the span's fill: table entries (index, page) and page copies (source, page)
+  std::vector<int32_t> entries, pairs;
 
   int32_t* row(int64_t seq) { return table.data() + seq * d.max_pages; }
   int64_t pages(int64_t seq) const { return (length[seq] + PAGE - 1) / PAGE; }
@@ -41,23 +44,26 @@ constexpr int64_t TILE_FILL = 256, TILE_PAGES = 8, TILE_LEAST = 64;
 
 int hip_ok(hipError_t e, const char* what) { return e == hipSuccess ? ANNA_MI_OK : fail_hip(e, what); }
 
-// Batches words of the three kinds into as few launches as they need.
+// Batches words of the four kinds into as few launches as they need.
 struct Updates {
   Update u;
   hipStream_t stream;
-  int rc = ANNA_MI_OK;
-  std::vector<int32_t> records, entries, copies;
+  std::vector<int32_t> records, entries, copies, pairs;
   Updates(anna_mi_paged* h, void* s) : stream(as_stream(s)) {
-    memset(&u, 0, sizeof(u));
+    memset(&u, 0, offsetof(Update, words));
     u.table = h->d.table;
     u.width = h->d.max_pages;
+    u.pool = (uint8_t*)h->d.pool;
+    u.page = h->page_size();
+    u.pool_layer = h->d.num_pages * u.page;
+    u.layers = (int32_t)h->d.num_layers;
   }
   void entry(int64_t index, int32_t page) { entries.insert(entries.end(), {(int32_t)index, page}); }
   void copy(int32_t row, int32_t source, int64_t pages) { copies.insert(copies.end(), {row, source, (int32_t)pages}); }
   int launch() {
     constexpr int R = sizeof(Record) / 4;
-    size_t r = 0, e = 0, c = 0;
-    while (r < records.size() || e < entries.size() || c < copies.size()) {
+    size_t r = 0, e = 0, c = 0, p = 0;
+    while (r < records.size() || e < entries.size() || c < copies.size() || p < pairs.size()) {
       int n = 0;
       auto take = [&](const std::vector<int32_t>& v, size_t& at, int step) {
         const int k = (int)std::min<size_t>((v.size() - at) / step, (UPDATE_WORDS - n) / step);
@@ -69,12 +75,22 @@ struct Updates {
       u.records = take(records, r, R);
       u.entries = take(entries, e, 2);
       u.copies = take(copies, c, 3);
+      u.pairs = take(pairs, p, 2);
       const int rc = launch_update(u, stream);
       if (rc != ANNA_MI_OK) return rc;
     }
     return ANNA_MI_OK;
   }
 };
+
+// What an extend left to a span's fill, for any other call that comes first.
+int flush(anna_mi_paged* h, void* stream) {
+  if (h->entries.empty() && h->pairs.empty()) return ANNA_MI_OK;
+  Updates up(h, stream);
+  up.entries.swap(h->entries);
+  up.pairs.swap(h->pairs);
+  return up.launch();
+}
 
 // pairs: (source, page), ...
 int copy_pages(const anna_mi_paged* h, const void* from, int64_t from_pages, void* to, int64_t to_pages,
@@ -303,6 +319,8 @@ int anna_mi_paged_fork(anna_mi_paged* h, int64_t n, const int32_t* parents, int3
                  "paged_fork: sequence %d is not in use", (int)parents[i]);
     ANNA_CHECK(n <= (int64_t)h->free_seqs.size(), "paged_fork: %lld sequences asked, %lld of %lld are free", (long long)n,
                (long long)h->free_seqs.size(), (long long)h->d.max_sequences);
+    const int rc = flush(h, stream);
+    if (rc != ANNA_MI_OK) return rc;
     Updates up(h, stream);
     up.copies.reserve(3 * n);
     for (int64_t i = 0; i < n; i++) {
@@ -323,6 +341,7 @@ int anna_mi_paged_extend(anna_mi_paged* h, int64_t n, const int32_t* seqs, const
   return guarded(h, "paged_extend", [&]() -> int {
     ANNA_CHECK(n >= 0 && (n == 0 || (seqs && counts)), "paged_extend: bad arguments");
     int rc = check_seqs(h, n, seqs);
+    if (rc == ANNA_MI_OK) rc = flush(h, stream);
     if (rc != ANNA_MI_OK) return rc;
     // pages to take: those that are new, and a copy of a last page for all its holders but the last
     std::vector<int32_t> shared;  // last pages whose holders here each counted as one that leaves
@@ -349,16 +368,14 @@ int anna_mi_paged_extend(anna_mi_paged* h, int64_t n, const int32_t* seqs, const
     }
     ANNA_CHECK(need <= (int64_t)h->free_pages.size(), "paged_extend: %lld pages needed, %lld of %lld are free", (long long)need,
                (long long)h->free_pages.size(), (long long)h->d.num_pages);
-    Updates up(h, stream);
-    std::vector<int32_t> pairs;
-    up.entries.reserve(2 * need);
-    pairs.reserve(2 * shared.size());
+    h->entries.reserve(2 * need);
+    h->pairs.reserve(2 * shared.size());
     auto take = [&](int64_t seq, int64_t c) {
       const int32_t page = h->free_pages.back();
       h->free_pages.pop_back();
       h->refs[page] = 1;
       h->row(seq)[c] = page;
-      up.entry(seq * h->d.max_pages + c, page);
+      h->entries.insert(h->entries.end(), {(int32_t)(seq * h->d.max_pages + c), page});
       return page;
     };
     for (int64_t i = 0; i < n; i++) {
@@ -370,14 +387,13 @@ int anna_mi_paged_extend(anna_mi_paged* h, int64_t n, const int32_t* seqs, const
         if (h->refs[last] > 1) {
           h->refs[last]--;
           const int32_t page = take(s, old / PAGE);
-          pairs.insert(pairs.end(), {last, page});
+          h->pairs.insert(h->pairs.end(), {last, page});
         }
       }
       for (int64_t c = ceil_div(old, PAGE); c < ceil_div(old + counts[i], PAGE); c++) take(s, c);
       h->length[s] = old + counts[i];
     }
-    rc = copy_pages(h, h->d.pool, h->d.num_pages, h->d.pool, h->d.num_pages, pairs, as_stream(stream));
-    return rc != ANNA_MI_OK ? rc : up.launch();
+    return ANNA_MI_OK;
   });
 }
 
@@ -387,6 +403,8 @@ int anna_mi_paged_truncate(anna_mi_paged* h, int32_t seq, int64_t length, void* 
     if (rc != ANNA_MI_OK) return rc;
     ANNA_CHECK(length >= 0 && length <= h->length[seq], "paged_truncate: length %lld of a sequence of %lld", (long long)length,
                (long long)h->length[seq]);
+    rc = flush(h, stream);
+    if (rc != ANNA_MI_OK) return rc;
     std::vector<int32_t> freed;
     const int64_t keep = ceil_div(length, PAGE);
     Updates up(h, stream);
@@ -402,6 +420,7 @@ int anna_mi_paged_free(anna_mi_paged* h, int64_t n, const int32_t* seqs, void* s
   return guarded(h, "paged_free", [&]() -> int {
     ANNA_CHECK(n >= 0 && (n == 0 || seqs), "paged_free: bad arguments");
     int rc = check_seqs(h, n, seqs);
+    if (rc == ANNA_MI_OK) rc = flush(h, stream);
     if (rc != ANNA_MI_OK) return rc;
     Updates up(h, stream);
     std::vector<int32_t> freed;
@@ -418,6 +437,8 @@ int anna_mi_paged_free(anna_mi_paged* h, int64_t n, const int32_t* seqs, void* s
 
 int anna_mi_paged_compact(anna_mi_paged* h, int64_t* live, void* stream) {
   return guarded(h, "paged_compact", [&]() -> int {
+    int rc = flush(h, stream);
+    if (rc != ANNA_MI_OK) return rc;
     const int64_t n = h->d.num_pages - (int64_t)h->free_pages.size();
     // pages behind the first n move into the holes before them: sources and targets are disjoint
     std::vector<int32_t> to(h->d.num_pages, -1), pairs;
@@ -440,7 +461,7 @@ int anna_mi_paged_compact(anna_mi_paged* h, int64_t* live, void* stream) {
     h->free_pages.clear();
     for (int64_t p = h->d.num_pages - 1; p >= n; p--) h->free_pages.push_back((int32_t)p);
     if (live) *live = n;
-    const int rc = copy_pages(h, h->d.pool, h->d.num_pages, h->d.pool, h->d.num_pages, pairs, as_stream(stream));
+    rc = copy_pages(h, h->d.pool, h->d.num_pages, h->d.pool, h->d.num_pages, pairs, as_stream(stream));
     return rc != ANNA_MI_OK ? rc : up.launch();
   });
 }
@@ -451,6 +472,8 @@ int anna_mi_paged_resize(anna_mi_paged* h, int64_t num_pages, void* pool, void* 
     ANNA_CHECK(num_pages >= n && num_pages > 0 && num_pages < INT_MAX, "paged_resize: %lld pages, %lld are in use", (long long)num_pages,
                (long long)n);
     ANNA_CHECK(pool && (uintptr_t)pool % 16 == 0 && pool != h->d.pool, "paged_resize: needs another, 16-byte aligned pool");
+    int rc = flush(h, stream);
+    if (rc != ANNA_MI_OK) return rc;
     std::vector<int32_t> to(h->d.num_pages, -1), pairs, refs(num_pages, 0);
     pairs.reserve(2 * num_pages);
     int32_t next = 0;
@@ -474,7 +497,7 @@ int anna_mi_paged_resize(anna_mi_paged* h, int64_t num_pages, void* pool, void* 
     for (int64_t p = num_pages - 1; p >= next; p--) h->free_pages.push_back((int32_t)p);
     h->d.pool = pool;
     h->d.num_pages = num_pages;
-    const int rc = copy_pages(h, old, old_pages, pool, num_pages, pairs, as_stream(stream));
+    rc = copy_pages(h, old, old_pages, pool, num_pages, pairs, as_stream(stream));
     return rc != ANNA_MI_OK ? rc : up.launch();
   });
 }
@@ -540,6 +563,8 @@ int anna_mi_paged_span_fill(anna_mi_paged* h, int64_t n, const int32_t* seqs, co
     u.tile_rows = (int32_t)p.tile_rows;
     up.records.resize(p.records.size() * (sizeof(Record) / 4));
     if (!p.records.empty()) memcpy(up.records.data(), p.records.data(), p.records.size() * sizeof(Record));
+    up.entries.swap(h->entries);
+    up.pairs.swap(h->pairs);
     return up.launch();
   });
 }
@@ -560,7 +585,8 @@ int anna_mi_paged_store(anna_mi_paged* h, int64_t layer, const anna_mi_paged_spa
                         int64_t key_stride_head, const void* values, int64_t value_stride_token, int64_t value_stride_head,
                         int capacity_grid, void* stream) {
   return guarded(h, "paged_store", [&]() -> int {
-    const int rc = check_layer(h, layer, span, "paged_store");
+    int rc = check_layer(h, layer, span, "paged_store");
+    if (rc == ANNA_MI_OK) rc = flush(h, stream);
     if (rc != ANNA_MI_OK || span->tokens == 0) return rc;
     ANNA_CHECK(keys && values, "paged_store: null keys or values");
     ANNA_CHECK(aligned(keys, key_stride_token, key_stride_head) && aligned(values, value_stride_token, value_stride_head),
@@ -575,7 +601,8 @@ int anna_mi_paged_store(anna_mi_paged* h, int64_t layer, const anna_mi_paged_spa
 int anna_mi_paged_read(anna_mi_paged* h, int64_t layer, const anna_mi_paged_span* span, void* keys, void* values, int capacity_grid,
                        void* stream) {
   return guarded(h, "paged_read", [&]() -> int {
-    const int rc = check_layer(h, layer, span, "paged_read");
+    int rc = check_layer(h, layer, span, "paged_read");
+    if (rc == ANNA_MI_OK) rc = flush(h, stream);
     if (rc != ANNA_MI_OK || span->tokens == 0) return rc;
     ANNA_CHECK(keys && values && (uintptr_t)keys % 16 == 0 && (uintptr_t)values % 16 == 0, "paged_read: null or unaligned output");
     return launch_read(h->d.dtype, h->d.head_dim, layer_pool(h, layer), h->d.table, h->d.max_pages, span->buf,
@@ -589,7 +616,8 @@ int anna_mi_paged_attend(anna_mi_paged* h, int64_t layer, const anna_mi_paged_sp
                          int64_t query_stride_token, int64_t query_stride_head, const void* gate, int64_t gate_stride_token,
                          int64_t gate_stride_head, void* out, float scaling, int capacity_grid, void* stream) {
   return guarded(h, "paged_attend", [&]() -> int {
-    const int rc = check_layer(h, layer, span, "paged_attend");
+    int rc = check_layer(h, layer, span, "paged_attend");
+    if (rc == ANNA_MI_OK) rc = flush(h, stream);
     if (rc != ANNA_MI_OK || span->tokens == 0) return rc;
     ANNA_CHECK(query && out && (uintptr_t)out % 16 == 0, "paged_attend: null query or output, or an unaligned output");
     ANNA_CHECK(aligned(query, query_stride_token, query_stride_head) &&

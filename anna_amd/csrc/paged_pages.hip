@@ -6,8 +6,33 @@ namespace anna {
 namespace paged {
 namespace {
 
+// ---------------------------------------------------------------- page copies
+// A workgroup copies 16 KB of a page of a layer (all KV heads), 64 bytes a thread: 96 pages of 32 layers (442 MB read and
+// written) take 86 us, 5.2 TB/s; a resize of 409 pages 349 us, 5.5 TB/s.  Memory bounds it.
+constexpr int COPY_BYTES = 16384;
+
+__device__ __forceinline__ void copy_chunk(const uint8_t* from, uint8_t* to, int64_t page, int64_t chunk) {
+  const int64_t at = chunk * COPY_BYTES + threadIdx.x * 16;
+  u32x4 v[4];
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    v[k] = u32x4{0, 0, 0, 0};
+    if (from && at + k * 4096 < page) v[k] = __builtin_nontemporal_load((const u32x4*)(from + at + k * 4096));
+  }
+#pragma unroll
+  for (int k = 0; k < 4; k++)
+    if (at + k * 4096 < page) *(u32x4*)(to + at + k * 4096) = v[k];
+}
+
+__global__ __launch_bounds__(256) void paged_copy_kernel(const Copy c) {
+  const int source = c.words[2 * blockIdx.y], target = c.words[2 * blockIdx.y + 1];
+  copy_chunk(source < 0 ? nullptr : c.from + blockIdx.z * c.from_layer + source * c.page,
+             c.to + blockIdx.z * c.to_layer + target * c.page, c.page, blockIdx.x);
+}
+
 // ---------------------------------------------------------------- updates
-// One workgroup writes what a record says, one 256 table entries, one a whole table row.
+// One workgroup writes what a record says, one 256 table entries, one a whole table row, one copies 16 KB of a page of
+// a layer: all that a step needs before its first layer, in one launch.
 __global__ __launch_bounds__(256) void paged_update_kernel(const Update u) {
   const int tid = threadIdx.x;
   int blk = blockIdx.x;
@@ -44,33 +69,22 @@ __global__ __launch_bounds__(256) void paged_update_kernel(const Update u) {
     return;
   }
   blk -= entry_blocks;
-  words += 2 * u.entries + 3 * blk;
+  words += 2 * u.entries;
+  if (blk >= u.copies) {
+    blk -= u.copies;
+    words += 3 * u.copies;
+    const int chunks = (int)((u.page + COPY_BYTES - 1) / COPY_BYTES), pair = blk / (chunks * u.layers), layer = blk / chunks % u.layers;
+    uint8_t* base = u.pool + layer * u.pool_layer;
+    copy_chunk(base + words[2 * pair] * u.page, base + words[2 * pair + 1] * u.page, u.page, blk % chunks);
+    return;
+  }
+  words += 3 * blk;
   int32_t* row = u.table + words[0] * u.width;
   const int32_t* source = u.table + words[1] * u.width;
   for (int k = tid; k < u.width; k += 256) {
     if (k >= words[2]) row[k] = 0;
     else if (words[1] >= 0) row[k] = source[k];
   }
-}
-
-// ---------------------------------------------------------------- page copies
-// One workgroup copies 16 KB of a page of a layer (all KV heads), 64 bytes a thread.
-constexpr int COPY_BYTES = 16384;
-
-__global__ __launch_bounds__(256) void paged_copy_kernel(const Copy c) {
-  const int source = c.words[2 * blockIdx.y], target = c.words[2 * blockIdx.y + 1];
-  const int64_t at = (int64_t)blockIdx.x * COPY_BYTES + threadIdx.x * 16;
-  const uint8_t* from = c.from + blockIdx.z * c.from_layer + source * c.page + at;
-  uint8_t* to = c.to + blockIdx.z * c.to_layer + target * c.page + at;
-  u32x4 v[4];
-#pragma unroll
-  for (int k = 0; k < 4; k++) {
-    v[k] = u32x4{0, 0, 0, 0};
-    if (source >= 0 && at + k * 4096 < c.page) v[k] = __builtin_nontemporal_load((const u32x4*)(from + k * 4096));
-  }
-#pragma unroll
-  for (int k = 0; k < 4; k++)
-    if (at + k * 4096 < c.page) *(u32x4*)(to + k * 4096) = v[k];
 }
 
 // ---------------------------------------------------------------- store and read
@@ -288,8 +302,10 @@ __global__ __launch_bounds__(256) void paged_read_kernel(const uint8_t* __restri
 }  // namespace
 
 int launch_update(const Update& u, hipStream_t stream) {
-  const int blocks = u.records + (u.entries + 255) / 256 + u.copies;
-  if (blocks > 0) paged_update_kernel<<<blocks, 256, 0, stream>>>(u);
+  const int64_t blocks = u.records + (u.entries + 255) / 256 + u.copies +
+                         (int64_t)u.pairs * u.layers * ((u.page + COPY_BYTES - 1) / COPY_BYTES);
+  ANNA_CHECK(blocks <= INT32_MAX, "paged update: too many pages to copy");
+  if (blocks > 0) paged_update_kernel<<<(unsigned)blocks, 256, 0, stream>>>(u);
   ANNA_LAUNCH_CHECK("paged update");
   return ANNA_MI_OK;
 }

@@ -723,7 +723,8 @@ int anna_mi_paged_destroy(anna_mi_paged* handle);
 int anna_mi_paged_add(anna_mi_paged* handle, int64_t n, int32_t* seqs);
 int anna_mi_paged_fork(anna_mi_paged* handle, int64_t n, const int32_t* parents, int32_t* children, void* stream);
 /* Lengthens sequences by counts (0 allowed), whose old lengths go to starts (may be NULL).  A partly
- * filled last page that others share is copied first, in every layer. */
+ * filled last page that others share is copied first, in every layer.  The table entries and copies are
+ * launched by the next call that has a stream: a span's fill takes them along in its own launch. */
 int anna_mi_paged_extend(anna_mi_paged* handle, int64_t n, const int32_t* seqs, const int64_t* counts,
                          int64_t* starts, void* stream);
 int anna_mi_paged_truncate(anna_mi_paged* handle, int32_t seq, int64_t length, void* stream);
