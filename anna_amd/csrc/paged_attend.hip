@@ -18,6 +18,11 @@
 //   tokens of its query.  O^T = V^T P^T: the lane's eight tokens of two such tiles are its eight k of
 //   the second product, so P never leaves the lane; the value codes are stored in that order.
 // For fp16 activations ps is split into two bf16 terms: one alone is coarser than the output's type.
+// Memory bounds the long contexts: 4 sequences of 100K to 131K tokens (564 MB) take 113 us, 5.0 TB/s, a copy's rate.
+// Short ones are bound by the chain of a launch (item, table, first page: ~5 us), two or three steps of ~3 us and the
+// merge's launch (5 us): 8 sequences of 1K to 16K (45 MB, head_dim 256) take 27 us, one of 1000 tokens 10 us.
+//
+// Tile form, for more than 64 query rows of a KV head: further down.
 #include <type_traits>
 
 #include "paged.hpp"
@@ -29,6 +34,9 @@ namespace {
 typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 
 constexpr float NEG = -INFINITY;
+// Probabilities with bf16's exponents stay below 2^-ROOM: sums of a context's 2^24 of them, times what stands for a value
+// at most (31 times its scale, and a scale is up to 2^125), stay within fp32, as the values' mean does.
+constexpr float ROOM = 26.0f;
 
 __device__ __forceinline__ f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -246,7 +254,7 @@ __global__ __launch_bounds__(256, NQ * D <= 256 ? 2 : 1) void paged_split_kernel
       for (int t = 0; t < TT; t++)
 #pragma unroll
         for (int i = 0; i < 4; i++) top = fmaxf(top, z[n][t][i]);
-      top *= a.scale;
+      top = fmaf(top, a.scale, ROOM);
       top = fmaxf(top, lane_xor16(top));
       top = fmaxf(top, lane_xor32(top));
       top = fmaxf(top, m[n]);
@@ -347,11 +355,19 @@ __global__ __launch_bounds__(256, NQ * D <= 256 ? 2 : 1) void paged_split_kernel
 //
 // The operands are fp16 for both types: (code + zero) * scale rounded to 11 bits, probabilities (times 2^8, so
 // that small ones stay above fp16's subnormals) too, which keeps the result within a tenth of the output's
-// own rounding.  fp16 holds only so much: from the first page on with scales beyond the limits below, and for
-// queries above them from the first page on, an item goes on in bf16 instead, at bf16's precision.
+// own rounding for bf16 (fp16's own three roundings show: 3e-4 against 2e-4 of the plain form).  fp16 holds only so
+// much: from the first page on with scales beyond the limits below, and for queries above them from the first page on,
+// an item goes on in bf16 instead, at bf16's precision.
+//
+// The vector unit bounds it: of a page and wave (32 rows, head_dim 128) 32 matrix instructions (1024 cycles) stand against
+// ~320 vector ones, 32 of them exponentials, and with two waves a SIMD the two overlap in part.  2048 tokens at the end
+// of 32K (32 query heads on 8, head_dim 128): 1150 us, 926 TFLOP/s, 78% of a large product's rate.  head_dim 256 has room
+// for one wave a SIMD only (its sums alone are 128 registers): a page of 128 rows takes 3.9 us, ragged prompts of up to
+// 1500 tokens 130 us (310 TFLOP/s).
 constexpr float K_SCALE_MOST = 16.0f;                // |k| < 2^11: with |q| <= 2^11 subnormal roundings stay below 2^-14
 constexpr float V_SCALE_MOST = 256.0f;               // |v| < 2^15
 constexpr float V_SCALE_LEAST = 3.814697265625e-6f;  // 2^-18: subnormal roundings stay below a 2^-7th of a code's step
+constexpr float V_SHRINK = 0.0625f;                  // in bf16: rounded, a group's largest value may be past the type's largest
 constexpr float Q_MOST = 2048.0f;
 constexpr float P_SHIFT = 8.0f, P_SLACK = 4.0f;
 
@@ -468,7 +484,8 @@ template <int D> struct ValueShare {
     u32x4 v;
 #pragma unroll
     for (int i = 0; i < 4; i++)
-      v[i] = pack_bf16((bf16_lo(c[i]) + bf16_lo(offset[i])) * bf16_lo(scale[i]), (bf16_hi(c[i]) + bf16_hi(offset[i])) * bf16_hi(scale[i]));
+      v[i] = pack_bf16((bf16_lo(c[i]) + bf16_lo(offset[i])) * (bf16_lo(scale[i]) * V_SHRINK),
+                       (bf16_hi(c[i]) + bf16_hi(offset[i])) * (bf16_hi(scale[i]) * V_SHRINK));
     to[128 * (w / 2) + 16 * (w & 1)] = v;
   }
 };
@@ -482,12 +499,12 @@ template <int D> struct Rows {
   float m, l;
 };
 
-// The running maximum of a lane's query with the scores `top` added, less P_SHIFT: P_SHIFT above it the
-// probabilities would be 2^P_SHIFT.  It moves only when it has to, by more than P_SLACK, which leaves them within
-// fp16 and spares nearly all rescaling.  Returns the factor of everything summed so far.
-template <int D> __device__ __forceinline__ bool new_top(Rows<D>& w, float top, float scale, float& factor) {
+// The running maximum of a lane's query with the scores `top` added, for fp16 less P_SHIFT: P_SHIFT above it the
+// probabilities would be 2^P_SHIFT; for bf16 with ROOM instead.  It moves only when it has to, by more than P_SLACK,
+// which leaves them within fp16 and spares nearly all rescaling.  Returns the factor of everything summed so far.
+template <int D, bool F16> __device__ __forceinline__ bool new_top(Rows<D>& w, float top, float scale, float& factor) {
   top = fmaxf(top, lane_xor32(top));
-  top = fmaf(top, scale, -P_SHIFT);
+  top = fmaf(top, scale, F16 ? -P_SHIFT : ROOM);
   const bool moves = top > w.m + P_SLACK;
   factor = 1.0f;
   if (!__any(moves)) return false;
@@ -555,7 +572,7 @@ __device__ __forceinline__ void take_page(Rows<D>& w, const u32x4* lds, Q query,
       asm volatile("");  // a branch, not a select for every score of every page
       hide_from(z[half], half, hl, limit);
     }
-    moved[half] = new_top(w, top_of(z[half]), scale, factor[half]);
+    moved[half] = new_top<D, F16>(w, top_of(z[half]), scale, factor[half]);
     base = w.m == NEG ? 0.0f : w.m;
   };
   auto rescale = [&](int half) {
@@ -771,8 +788,14 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
     }
     barrier();
   }
-  // From the first page on that fp16 does not hold, in bf16: one buffer, nothing ahead.
+  // From the first page on that fp16 does not hold, in bf16: one buffer, nothing ahead; the probabilities with ROOM
+  // instead of P_SHIFT, the values at V_SHRINK until the end.
   if (p < it.page1) {
+    constexpr float LESS = 1.0f / (1ull << (int)(P_SHIFT + ROOM));
+    w.m += P_SHIFT + ROOM;
+    w.l *= LESS;
+#pragma unroll
+    for (int d = 0; d < D / 32; d++) w.acc[d] *= LESS * V_SHRINK;
 #pragma unroll
     for (int s = 0; s < KSTEPS; s++) {
       qf[s] = raw_query(s);
@@ -800,10 +823,12 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
         take_page<D, false, 1>(w, lds, query, sees - p * PAGE, p * PAGE + PAGE > seen_by_all, a.scale, lane, [](int) {}, [](int) {});
       barrier();
     }
+#pragma unroll
+    for (int d = 0; d < D / 32; d++) w.acc[d] *= 1.0f / V_SHRINK;
   }
 
   // A lane holds, of its query, dims 32 d + 8 b + 4 hl + i.  Through LDS, as fp32, to whole rows: lanes that write 8
-// bytes of 32 rows each took 13 us a workgroup (128 rows of head_dim 256, gated), this @@ us.
+  // bytes of 32 rows each took 13 us a workgroup (128 rows of head_dim 256, gated).
   const float total = w.l + lane_xor32(w.l);
   if (it.part >= 0) {
     if (!valid) return;

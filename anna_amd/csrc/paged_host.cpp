@@ -194,7 +194,7 @@ int make_plan(anna_mi_paged* h, int64_t n, const int32_t* seqs, const int64_t* s
   // a wave takes 32 rows: workgroups of 8 share a page's conversion among twice as many rows as those of
   // 4, which there are twice as many of
   if (large * H >= TILE_FILL && h->d.head_dim < 256) p.tile_rows = 256;
-  int64_t offset = 0, total[2] = {0, 0}, tiles[2] = {0, 0}, rows_of[2] = {0, 0};
+  int64_t offset = 0, tiles[2] = {0, 0}, rows_of[2] = {0, 0};  // tiles: those with tokens
   for (int64_t i = 0; i < n; i++) {
     const int64_t rows = counts[i] * G, f = rows > TILE_LEAST, R = f ? p.tile_rows : p.few_rows;
     for (int64_t t = 0; t < std::max<int64_t>(1, ceil_div(rows, R)); t++) {
@@ -203,8 +203,7 @@ int make_plan(anna_mi_paged* h, int64_t n, const int32_t* seqs, const int64_t* s
       r.offset = (int32_t)offset, r.tile = (int32_t)t, r.tiled = (int32_t)f;
       r.pages = rows ? (int32_t)((starts[i] + (std::min(rows, (t + 1) * R) - 1) / G) / PAGE + 1) : 0;
       r.touch0 = (int32_t)p.touches;
-      total[f] += r.pages;
-      tiles[f]++;
+      tiles[f] += rows > 0;
       rows_of[f] = std::max(rows_of[f], std::min(rows, R));
       p.records.push_back(r);
     }

@@ -7,8 +7,8 @@ namespace paged {
 namespace {
 
 // ---------------------------------------------------------------- page copies
-// A workgroup copies 16 KB of a page of a layer (all KV heads), 64 bytes a thread: 96 pages of 32 layers (442 MB read and
-// written) take 86 us, 5.2 TB/s; a resize of 409 pages 349 us, 5.5 TB/s.  Memory bounds it.
+// A workgroup copies 16 KB of a page of a layer (all KV heads), 64 bytes a thread: 94 pages of 32 layers (444 MB read and
+// written) take 86 us, 5.2 TB/s; a resize with 408 of them in use 349 us, 5.5 TB/s.  Memory bounds it.
 constexpr int COPY_BYTES = 16384;
 
 __device__ __forceinline__ void copy_chunk(const uint8_t* from, uint8_t* to, int64_t page, int64_t chunk) {
@@ -162,6 +162,10 @@ __device__ __forceinline__ uint32_t code_word(uint32_t lo, uint32_t hi) {
   return nibbles(__builtin_amdgcn_perm(hi, lo, 0x06040200)) | nibbles(__builtin_amdgcn_perm(hi, lo, 0x07050301)) << 16;
 }
 
+// Tokens of a page and KV head into the page: eight lanes a group, keys straight to their words, values by way of LDS,
+// where the codes of eight tokens meet in a word.  Prompts (7957 tokens of 8 heads, 42 MB): 17.6 us, 2.4 TB/s, bound by the
+// vector unit (~350 instructions for 16 values of 8 lanes, a third of them rounding) and the chain of a workgroup's
+// passes; one token of each of 64 sequences: 5 us, the chain alone.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void paged_store_kernel(uint8_t* __restrict__ pool, const int32_t* __restrict__ table, int64_t width,
                                                           const int32_t* __restrict__ header, const Touch* __restrict__ touch,
@@ -257,6 +261,7 @@ template <int DT> __device__ __forceinline__ u32x4 expand(uint32_t lo, uint32_t 
   return out;
 }
 
+// A page's tokens dense again, values by way of LDS.  7957 tokens of 8 heads (42 MB): 10 us, 4.3 TB/s; memory bounds it.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void paged_read_kernel(const uint8_t* __restrict__ pool, const int32_t* __restrict__ table,
                                                          int64_t width, const int32_t* __restrict__ header,

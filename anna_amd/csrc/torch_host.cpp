@@ -51,6 +51,7 @@ struct Library {
   decltype(&anna_mi_paged_fork) paged_fork = nullptr;
   decltype(&anna_mi_paged_free) paged_free = nullptr;
   decltype(&anna_mi_paged_extend) paged_extend = nullptr;
+  decltype(&anna_mi_paged_truncate) paged_truncate = nullptr;
   decltype(&anna_mi_paged_lengths) paged_lengths = nullptr;
   decltype(&anna_mi_paged_span_plan) paged_span_plan = nullptr;
   decltype(&anna_mi_paged_span_fill) paged_span_fill = nullptr;
@@ -80,6 +81,7 @@ void bind(const py::dict& d) {
   get("anna_mi_paged_fork", lib.paged_fork);
   get("anna_mi_paged_free", lib.paged_free);
   get("anna_mi_paged_extend", lib.paged_extend);
+  get("anna_mi_paged_truncate", lib.paged_truncate);
   get("anna_mi_paged_lengths", lib.paged_lengths);
   get("anna_mi_paged_span_plan", lib.paged_span_plan);
   get("anna_mi_paged_span_fill", lib.paged_span_fill);
@@ -517,6 +519,24 @@ bool paged_free(uintptr_t handle, const py::object& seqs, uintptr_t stream) {
   return true;
 }
 
+py::object filled_span(uintptr_t handle, uintptr_t span, const std::vector<int32_t>& s, const std::vector<int64_t>& starts,
+                       const std::vector<int64_t>& counts, int64_t kv_heads, int64_t head_dim, int64_t device, uintptr_t stream) {
+  const int64_t n = (int64_t)s.size();
+  anna_mi_paged_span* out = span_at(span);
+  check(lib.paged_span_plan(paged(handle), n, s.data(), starts.data(), counts.data(), out), "anna_mi_paged_span_plan");
+  const auto ints = at::TensorOptions().dtype(at::kInt).device(at::kCUDA, (c10::DeviceIndex)device);
+  std::vector<Tensor> held{at::empty({out->words}, ints)};
+  if (out->partial_rows > 0) {
+    held.push_back(at::empty({out->partial_rows, kv_heads, 2}, ints.dtype(at::kFloat)));
+    held.push_back(at::empty({out->partial_rows, kv_heads, head_dim}, ints.dtype(at::kFloat)));
+    out->partial_stats = (float*)ptr(held[1]);
+    out->partial_values = (float*)ptr(held[2]);
+  }
+  out->buf = (int32_t*)ptr(held[0]);
+  check(lib.paged_span_fill(paged(handle), n, s.data(), starts.data(), counts.data(), out, stream_ptr(stream)), "anna_mi_paged_span_fill");
+  return py::make_tuple(s, starts, counts, held);
+}
+
 // Fills a span anew, with its buffer and workspace: extend (starts is None) by counts, None for one each, or the
 // tokens that the sequences hold already.  -> (seqs, starts, counts, tensors), or None.
 py::object paged_span(uintptr_t handle, uintptr_t span, const py::object& seqs, const py::object& starts, const py::object& counts,
@@ -538,19 +558,13 @@ py::object paged_span(uintptr_t handle, uintptr_t span, const py::object& seqs, 
     at = whole<int64_t>(starts, 0, I64);
     if (!at || (int64_t)at->size() != n) return py::none();
   }
-  anna_mi_paged_span* out = span_at(span);
-  check(lib.paged_span_plan(paged(handle), n, s->data(), at->data(), c->data(), out), "anna_mi_paged_span_plan");
-  const auto ints = at::TensorOptions().dtype(at::kInt).device(at::kCUDA, (c10::DeviceIndex)device);
-  std::vector<Tensor> held{at::empty({out->words}, ints)};
-  if (out->partial_rows > 0) {
-    held.push_back(at::empty({out->partial_rows, kv_heads, 2}, ints.dtype(at::kFloat)));
-    held.push_back(at::empty({out->partial_rows, kv_heads, head_dim}, ints.dtype(at::kFloat)));
-    out->partial_stats = (float*)ptr(held[1]);
-    out->partial_values = (float*)ptr(held[2]);
+  try {
+    return filled_span(handle, span, *s, *at, *c, kv_heads, head_dim, device, stream);
+  } catch (...) {  // no memory for the span: the sequences as they were
+    if (starts.is_none())
+      for (int64_t i = 0; i < n; i++) lib.paged_truncate(paged(handle), (*s)[i], (*at)[i], stream_ptr(stream));
+    throw;
   }
-  out->buf = (int32_t*)ptr(held[0]);
-  check(lib.paged_span_fill(paged(handle), n, s->data(), at->data(), c->data(), out, stream_ptr(stream)), "anna_mi_paged_span_fill");
-  return py::make_tuple(*s, *at, *c, held);
 }
 
 // Rows [tokens, heads, head_dim] of the cache's type that the kernels read as they are

@@ -69,6 +69,7 @@ class PagedSpan:
         self._tensors: list[torch.Tensor] = []
         self._streams: set[int] = set()
         self._version = -1
+        self._ended: list[int] = []
 
     @property
     def tokens(self) -> int:
@@ -90,10 +91,10 @@ class PagedSpan:
                                      device=cache.device)
                 c.partial_stats, c.partial_values = stats.data_ptr(), values.data_ptr()
                 self._tensors += [stats, values]
-            self._streams = {cache._stream()}
+        self._used_on(cache._stream())
         cache._call("anna_mi_paged_span_fill", n, seqs, starts, counts, self._ref, cache._stream())
         self.seqs, self.starts, self.counts = list(seqs), list(starts), list(counts)
-        self._version = cache._version
+        self._ended, self._version = [cache._ended[s] for s in self.seqs], cache._version
 
     def _fresh(self, seqs, starts, counts) -> bool:
         """A new span's fill by the host module; False for calls that it leaves to the general way."""
@@ -106,8 +107,15 @@ class PagedSpan:
         if got is None:
             return False
         self.seqs, self.starts, self.counts, self._tensors = got
-        self._streams, self._version = {stream}, cache._version
+        self._ended, self._version = [cache._ended[s] for s in self.seqs], cache._version
+        self._streams = {stream}
         return True
+
+    def _used_on(self, stream: int) -> None:
+        if stream not in self._streams:
+            self._streams.add(stream)
+            for t in self._tensors:
+                t.record_stream(torch.cuda.current_stream(self.cache.device))
 
     @property
     def rows(self) -> torch.Tensor:
@@ -142,7 +150,9 @@ class PagedInt4Cache:
         width = -(-self.max_length // PAGE_TOKENS)
         self.pool = self._new_pool(self.num_pages, zero=True)
         self.table = torch.zeros((self.max_sequences, width), dtype=torch.int32, device=self.device)
-        self._version = 0  # counts the calls after which a span may name sequences that are no more
+        self._version = 0  # counts the calls after which a span may name tokens that are no more
+        self._ended = [0] * self.max_sequences  # how often a row's sequence has ended
+        self._streams: set[int] = set()  # that the pool and the table are used on
         d = _lib.PagedDesc(_lib.dtype_code(dtype), self.num_layers, self.num_pages, self.kv_heads, self.q_heads,
                            self.head_dim, self.max_sequences, width, self.pool.data_ptr(), self.table.data_ptr())
         self._handle = ctypes.c_void_p()
@@ -157,7 +167,12 @@ class PagedInt4Cache:
 
     # ---- calls
     def _stream(self) -> int:
-        return torch._C._cuda_getCurrentRawStream(self.device.index)
+        stream = torch._C._cuda_getCurrentRawStream(self.device.index)
+        if stream not in self._streams:
+            self._streams.add(stream)
+            for t in (self.pool, self.table):
+                t.record_stream(torch.cuda.current_stream(self.device))
+        return stream
 
     def _call(self, name: str, *args) -> None:
         if self._here():
@@ -201,7 +216,7 @@ class PagedInt4Cache:
     def extend(self, seqs, counts=None, *, span: PagedSpan | None = None) -> PagedSpan:
         """Lengthens sequences by ``counts`` tokens (one each by default, 0 allowed) and returns the span of
         the new tokens, which the caller then stores in every layer.  Nothing changes if the pool has
-        too few pages.  ``span``: an earlier span of as many sequences with the same counts, which is
+        too few pages or the span no memory.  ``span``: an earlier span of as many sequences with the same counts, which is
         filled again in place (a captured graph holds its addresses)."""
         self._counts("extend")
         if span is None:
@@ -223,7 +238,12 @@ class PagedInt4Cache:
                 if have + n > self.max_length:
                     raise RuntimeError(f"sequence {s} would hold {have + n} tokens, max_length is {self.max_length}")
             self._call("anna_mi_paged_extend", len(seqs), seqs, counts, starts, self._stream())
-            span._fill(seqs, starts, counts)
+            try:
+                span._fill(seqs, starts, counts)
+            except BaseException:  # no memory for the span: the sequences as they were
+                for s, have in zip(seqs, starts):
+                    self._call("anna_mi_paged_truncate", s, have, self._stream())
+                raise
         return span
 
     def span(self, seqs, starts, counts, *, span: PagedSpan | None = None) -> PagedSpan:
@@ -231,14 +251,16 @@ class PagedInt4Cache:
         self._counts("span")
         if span is None:
             span = PagedSpan(self)
-            if starts is not None and counts is not None and span._fresh(seqs, starts, counts):
-                return span
+            with self._lock:
+                if starts is not None and counts is not None and span._fresh(seqs, starts, counts):
+                    return span
             span = None
         seqs, starts, counts = _ints(seqs, ctypes.c_int32), _ints(starts, ctypes.c_int64), _ints(counts, ctypes.c_int64)
         if not len(seqs) == len(starts) == len(counts):
             raise ValueError(f"{len(seqs)} sequences, {len(starts)} starts and {len(counts)} counts")
         span = self._refilled(span, seqs, counts)
-        span._fill(seqs, starts, counts)
+        with self._lock:
+            span._fill(seqs, starts, counts)
         return span
 
     def _refilled(self, span: PagedSpan | None, seqs, counts) -> PagedSpan:
@@ -254,16 +276,21 @@ class PagedInt4Cache:
         """Forgets the tokens of a sequence from ``length`` on (drafted tokens that were not accepted)."""
         self._counts("truncate")
         seqs, length = _ints([seq], ctypes.c_int32), _ints([length], ctypes.c_int64)
-        self._call("anna_mi_paged_truncate", seqs[0], length[0], self._stream())
-        self._version += 1
+        with self._lock:
+            self._call("anna_mi_paged_truncate", seqs[0], length[0], self._stream())
+            self._version += 1
 
     def free(self, seqs) -> None:
         """Ends sequences; pages that no other sequence shares return to the pool."""
         self._counts("free")
-        if not (self._here() and _lib.host().paged_free(self._handle.value, seqs, self._stream())):
-            seqs = _ints(seqs, ctypes.c_int32)
-            self._call("anna_mi_paged_free", len(seqs), seqs, self._stream())
-        self._version += 1
+        seqs = list(seqs)
+        with self._lock:
+            if not (self._here() and _lib.host().paged_free(self._handle.value, seqs, self._stream())):
+                seqs = _ints(seqs, ctypes.c_int32)
+                self._call("anna_mi_paged_free", len(seqs), seqs, self._stream())
+            for s in seqs:
+                self._ended[s] += 1
+            self._version += 1
 
     def _lengths(self, seqs):
         lengths = (ctypes.c_int64 * len(seqs))()
@@ -305,8 +332,7 @@ class PagedInt4Cache:
                 raise RuntimeError(f"{num_pages} pages asked, {self.pages_in_use} are in use")
             pool = self._new_pool(num_pages, zero=False)
             self._call("anna_mi_paged_resize", num_pages, pool.data_ptr(), self._stream())
-            self.pool.record_stream(torch.cuda.current_stream(self.device))
-            self.pool, self.num_pages = pool, num_pages
+            self.pool, self.num_pages, self._streams = pool, num_pages, set()
 
     def page_table(self, span: PagedSpan) -> torch.Tensor:
         """The pages of the span's sequences, int32 [sequences, pages of max_length], 0 behind the last."""
@@ -319,15 +345,15 @@ class PagedInt4Cache:
         if not 0 <= layer < self.num_layers:
             raise IndexError(f"{what}: layer {layer} of {self.num_layers}")
         if span._version != self._version:
-            for s, start, n, have in zip(span.seqs, span.starts, span.counts, self._lengths((ctypes.c_int32 * len(span.seqs))(*span.seqs))):
+            if span._ended != [self._ended[s] for s in span.seqs]:
+                raise RuntimeError(f"{what}: a sequence of the span is not in use any more")
+            lengths = self._lengths((ctypes.c_int32 * len(span.seqs))(*span.seqs))
+            for s, start, n, have in zip(span.seqs, span.starts, span.counts, lengths):
                 if start + n > have:
                     raise RuntimeError(f"{what}: sequence {s} holds {have} tokens, the span reaches to {start + n}")
             span._version = self._version
         stream = self._stream()
-        if stream not in span._streams:
-            span._streams.add(stream)
-            for t in span._tensors:
-                t.record_stream(torch.cuda.current_stream(self.device))
+        span._used_on(stream)
         return stream
 
     def _rows(self, what: str, t: torch.Tensor, span: PagedSpan, heads: int) -> torch.Tensor:

@@ -252,6 +252,48 @@ def test_tiles_beyond_fp16(gpu, D, H, HQ, dtype, what):
         assert (err[:128] <= tol16[:128]).all()  # the tiles before that are the type's
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("n", [1, 3, 200])
+def test_values_at_the_types_limit(gpu, dtype, n):
+    """Values up to the largest number of the type, both signs, in both forms: what is finite stays finite."""
+    cache = make(D=64, H=1, HQ=2, dtype=dtype)
+    seqs = cache.add(1)
+    big = torch.finfo(dtype).max
+    k = rows((n, 1, 64), dtype, 1)
+    v = torch.where(rows((n, 1, 64), torch.float32, 2) > 0, big, -big).to(dtype)
+    v[:, :, 5] = 0.5 * big
+    cache.store(0, cache.extend(seqs, [n]), k, v)
+    m = Mirror()
+    m.store(seqs[0], 0, k.cpu(), v.cpu())
+    for count in {1, n}:
+        q = rows((count, 2, 64), dtype, 3)
+        got = cache.attend(0, cache.span(seqs, [n - count], [count]), q, scaling=0.125)
+        want, tol = attention(q.cpu(), *m.rows[seqs[0]], n - count, 0.125, dtype if dtype == FP and count == 1 else BF)
+        inside = want.abs() + tol < big
+        assert inside.any() and ((got.cpu().double() - want).abs() <= tol)[inside].all()
+
+
+@pytest.mark.parametrize("count", [1, 40])
+def test_what_a_page_held_before(gpu, count):
+    """A page taken again holds its last sequence's tokens behind the new one's, here values at the type's limit."""
+    cache = make(D=64, H=1, HQ=4, pages=2)
+    old, = cache.add()
+    big = torch.full((64, 1, 64), torch.finfo(BF).max, dtype=BF, device="cuda")
+    big[:, :, ::2] *= -1
+    cache.store(0, cache.extend([old], [64]), rows((64, 1, 64), BF, 1), big)
+    cache.free([old])
+    seqs, m = fill(cache, [40])
+    check_attend(cache, m, seqs, [40 - count], [count])
+
+
+def test_many_empty_sequences_beside_a_long_one(gpu):
+    cache = make(D=64, H=2, HQ=4, pages=100, sequences=320, length=6400)
+    seqs, m = fill(cache, [4000])
+    empty = cache.add(300)
+    check_attend(cache, m, seqs + empty, [3999] + [0] * 300, [1] + [0] * 300)
+    check_attend(cache, m, empty + seqs, [0] * 300 + [3900], [0] * 300 + [100])
+
+
 def test_attend_many_query_heads(gpu):
     """More query heads on a key/value head than a tile of the split form has rows."""
     cache = make(D=64, H=1, HQ=80)
@@ -302,6 +344,22 @@ def test_attend_is_the_same_every_time_and_alone(gpu):
         assert torch.equal(cache.attend(0, span, q, scaling=0.1), first)
     q[0] = float("nan")
     assert torch.equal(cache.attend(0, span, q, scaling=0.1)[1:], first[1:])
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("row", [0, 1, 40])  # of the split form, and at the front and in the middle of a tile
+def test_a_query_that_is_not_finite_is_alone(gpu, row, bad):
+    cache = make(D=128, H=2, HQ=8)
+    seqs = cache.add(3)
+    n = [200, 90, 300]
+    cache.store(0, cache.extend(seqs, n), rows((sum(n), 2, 128), BF, 1), rows((sum(n), 2, 128), BF, 2))
+    span = cache.span(seqs, [199, 0, 289], [1, 90, 11])
+    q = rows((102, 8, 128), BF, 3)
+    first = cache.attend(0, span, q, scaling=0.1)
+    q[row] = bad
+    got = cache.attend(0, span, q, scaling=0.1)
+    keep = [i for i in range(102) if i != row]
+    assert torch.equal(got[keep], first[keep]) and torch.isnan(got[row]).any()
 
 
 # ---------------------------------------------------------------- the pages' life
@@ -572,6 +630,42 @@ def test_refusals_leave_the_cache_as_it_was(gpu):
     cache.free([seqs[1]])
     with pytest.raises(RuntimeError, match="holds 0 tokens|not in use"):
         cache.read(0, span)
+
+
+def test_a_span_ends_with_its_sequences(gpu):
+    """Another sequence in the same row is none of the span's."""
+    cache = make(D=64, H=1, HQ=2)
+    seqs = cache.add(2)
+    cache.extend(seqs, [60, 30])
+    span = cache.span(seqs, [0, 0], [60, 30])
+    cache.free([seqs[1]])
+    with pytest.raises(RuntimeError, match="not in use"):
+        cache.read(0, span)
+    again, = cache.add()
+    cache.extend([again], [30])
+    cache.truncate(seqs[0], 0)
+    cache.extend([seqs[0]], [60])
+    assert again == seqs[1]
+    with pytest.raises(RuntimeError, match="not in use"):
+        cache.read(0, span)
+
+
+def test_no_memory_for_a_span(gpu, monkeypatch):
+    """An extend whose span cannot be allocated leaves the sequences as they were."""
+    np = pytest.importorskip("numpy")
+    cache = make(D=64, H=2, HQ=4, pages=8)
+    seqs, m = fill(cache, [100, 64])
+    free = cache.free_pages
+
+    def nothing(*args, **kwargs):
+        raise torch.OutOfMemoryError("none left")
+    with monkeypatch.context() as patch:
+        patch.setattr(torch, "empty", nothing)
+        with pytest.raises(torch.OutOfMemoryError):
+            cache.extend(np.array(seqs), [30, 1])
+    assert cache.lengths(seqs) == [100, 64] and cache.free_pages == free
+    check_held(cache, m, seqs)
+    check_attend(cache, m, seqs, [99, 0], [1, 64])
 
 
 def test_sequences_by_other_integers(gpu):
