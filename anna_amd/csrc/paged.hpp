@@ -9,6 +9,7 @@ namespace paged {
 
 constexpr int PAGE = 64;   // tokens of a page
 constexpr int GROUP = 64;  // values with one scale and zero
+constexpr int COPY_BYTES = 16384;  // of a page of all KV heads that a workgroup copies
 // What codes carry when they enter a matrix instruction, and offsets are without: 16 + code is exact in bf16's
 // eight bits by bit operations alone, and the smallest such number keeps the sums that cancel small.
 constexpr int CODE_BASE = 16;

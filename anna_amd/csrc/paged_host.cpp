@@ -42,6 +42,11 @@ constexpr int64_t SPLIT_ONCE = 512, TILE_ONCE = 256;
 // result is written and read again; up to TILE_LEAST query rows of a KV head are the split form's.
 constexpr int64_t TILE_FILL = 256, TILE_PAGES = 8, TILE_LEAST = 64;
 
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Workgroups of a launch, of up to 512 threads: 32 bits count its threads.
+constexpr int64_t MOST_GROUPS = UINT_MAX / 512;
+
 int hip_ok(hipError_t e, const char* what) { return e == hipSuccess ? ANNA_MI_OK : fail_hip(e, what); }
 
 // Batches words of the four kinds into as few launches as they need.
@@ -65,8 +70,8 @@ struct Updates {
     size_t r = 0, e = 0, c = 0, p = 0;
     while (r < records.size() || e < entries.size() || c < copies.size() || p < pairs.size()) {
       int n = 0;
-      auto take = [&](const std::vector<int32_t>& v, size_t& at, int step) {
-        const int k = (int)std::min<size_t>((v.size() - at) / step, (UPDATE_WORDS - n) / step);
+      auto take = [&](const std::vector<int32_t>& v, size_t& at, int step, size_t most = UPDATE_WORDS) {
+        const int k = (int)std::min({(v.size() - at) / step, (size_t)(UPDATE_WORDS - n) / step, most});
         if (k > 0) memcpy(u.words + n, v.data() + at, 4 * (size_t)k * step);
         n += k * step;
         at += (size_t)k * step;
@@ -75,7 +80,7 @@ struct Updates {
       u.records = take(records, r, R);
       u.entries = take(entries, e, 2);
       u.copies = take(copies, c, 3);
-      u.pairs = take(pairs, p, 2);
+      u.pairs = take(pairs, p, 2, std::max<int64_t>(1, MOST_GROUPS / 2 / (u.layers * ceil_div(u.page, COPY_BYTES))));
       const int rc = launch_update(u, stream);
       if (rc != ANNA_MI_OK) return rc;
     }
@@ -146,8 +151,6 @@ void give_back(anna_mi_paged* h, const std::vector<int32_t>& freed) {
   h->free_pages.insert(h->free_pages.end(), freed.rbegin(), freed.rend());
 }
 
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 // The layout of a span: its tiles, and the sizes that follow from them.  What a buffer has room for (the
 // bounds) depends on the counts alone, so that a span can be filled again as its sequences grow.
 struct Plan {
@@ -155,6 +158,7 @@ struct Plan {
   int64_t few_rows = 16, tile_rows = 128, units = 0, unit_rows = 0, touches = 0, tokens = 0;
   int64_t items[2] = {0, 0}, bound[2] = {0, 0};  // of the split form, of the tile form
   int64_t touch_bound = 0, partial_rows = 0, partial_bound = 0;
+  bool shared = false;  // a page with tokens of two sequences
 };
 
 // The fewest pages of an item of a form, `least` at least, with which there are at most `items` of them (or one a tile).
@@ -181,6 +185,7 @@ int make_plan(anna_mi_paged* h, int64_t n, const int32_t* seqs, const int64_t* s
   const int64_t G = h->d.q_heads / h->d.kv_heads, H = h->d.kv_heads;
   const int64_t most = 4096 / h->d.head_dim;  // rows of a split tile whose sums stay in registers
   int64_t large = 0;                          // tiles of 256 rows
+  std::vector<int32_t> held;                  // pages that others hold too
   for (int64_t i = 0; i < n; i++) {
     ANNA_CHECK(starts[i] >= 0 && counts[i] >= 0 && starts[i] <= h->length[seqs[i]] && counts[i] <= h->length[seqs[i]] - starts[i],
                "span: tokens %lld .. %lld of sequence %d, which holds %lld", (long long)starts[i],
@@ -207,10 +212,17 @@ int make_plan(anna_mi_paged* h, int64_t n, const int32_t* seqs, const int64_t* s
       rows_of[f] = std::max(rows_of[f], std::min(rows, R));
       p.records.push_back(r);
     }
-    if (counts[i] > 0) p.touches += (starts[i] + counts[i] - 1) / PAGE - starts[i] / PAGE + 1;
-    if (counts[i] > 0) p.touch_bound += (counts[i] + PAGE - 2) / PAGE + 1;
+    if (counts[i] > 0) {
+      const int64_t first = starts[i] / PAGE, last = (starts[i] + counts[i] - 1) / PAGE;
+      p.touches += last - first + 1;
+      p.touch_bound += (counts[i] + PAGE - 2) / PAGE + 1;
+      for (int64_t c = first; c <= last; c++)
+        if (h->refs[h->row(seqs[i])[c]] > 1) held.push_back(h->row(seqs[i])[c]);
+    }
     offset += counts[i];
   }
+  std::sort(held.begin(), held.end());
+  p.shared = std::adjacent_find(held.begin(), held.end()) != held.end();
   // Tiles of the tile form in falling order of their pages, so that the long ones start first.
   if (tiles[1] > 1)
     std::stable_sort(p.records.begin(), p.records.end(), [](const Record& a, const Record& b) {
@@ -239,7 +251,8 @@ int make_plan(anna_mi_paged* h, int64_t n, const int32_t* seqs, const int64_t* s
       p.bound[f] = std::max(target[f], tiles[f]);
       if (tiles[f] < target[f]) p.partial_bound += target[f] * rows_of[f];
     }
-  ANNA_CHECK(p.partial_bound <= INT_MAX && H * (p.bound[0] + p.bound[1]) <= INT_MAX / 64, "span: too many tokens");
+  ANNA_CHECK(p.partial_bound <= INT_MAX && H * std::max({p.bound[0], p.bound[1], p.touch_bound, (int64_t)p.records.size()}) <= MOST_GROUPS,
+             "span: too many tokens");
   return ANNA_MI_OK;
 }
 
@@ -272,6 +285,8 @@ int anna_mi_paged_create(const anna_mi_paged_desc* desc, anna_mi_paged** handle)
   ANNA_CHECK(d.num_layers > 0 && d.num_layers <= 65535 && d.num_pages > 0 && d.num_pages < INT_MAX, "paged_create: bad num_layers or num_pages");
   ANNA_CHECK(d.max_sequences > 0 && d.max_pages > 0 && d.max_sequences <= INT_MAX / d.max_pages && d.max_pages <= INT_MAX / (2 * PAGE),
              "paged_create: bad max_sequences or max_pages");
+  ANNA_CHECK(d.num_layers * ceil_div(d.kv_heads * page_bytes(d.head_dim), COPY_BYTES) <= MOST_GROUPS / 2,
+             "paged_create: a page of all layers is too large");
   ANNA_CHECK(d.pool && d.table, "paged_create: null pool or table");
   ANNA_CHECK((uintptr_t)d.pool % 16 == 0, "paged_create: the pool must be 16-byte aligned");
   try {
@@ -545,6 +560,7 @@ int anna_mi_paged_span_fill(anna_mi_paged* h, int64_t n, const int32_t* seqs, co
                    p.touches <= span->touch_capacity && p.partial_rows <= span->partial_rows && sections(*span).words <= span->words,
                "span: these tokens do not fit the span that is filled");
     ANNA_CHECK(p.partial_rows == 0 || (span->partial_stats && span->partial_values), "paged_span_fill: null partials");
+    span->shared = p.shared;
     span->split_items = p.items[0];
     span->tile_items = p.items[1];
     span->split_units = p.units;
@@ -587,6 +603,7 @@ int anna_mi_paged_store(anna_mi_paged* h, int64_t layer, const anna_mi_paged_spa
     int rc = check_layer(h, layer, span, "paged_store");
     if (rc == ANNA_MI_OK) rc = flush(h, stream);
     if (rc != ANNA_MI_OK || span->tokens == 0) return rc;
+    ANNA_CHECK(!span->shared, "paged_store: two sequences of the span share a page");
     ANNA_CHECK(keys && values, "paged_store: null keys or values");
     ANNA_CHECK(aligned(keys, key_stride_token, key_stride_head) && aligned(values, value_stride_token, value_stride_head),
                "paged_store: keys and values need rows of 16-byte alignment");

@@ -332,7 +332,7 @@ class PagedInt4Cache:
                 raise RuntimeError(f"{num_pages} pages asked, {self.pages_in_use} are in use")
             pool = self._new_pool(num_pages, zero=False)
             self._call("anna_mi_paged_resize", num_pages, pool.data_ptr(), self._stream())
-            self.pool, self.num_pages, self._streams = pool, num_pages, set()
+            self.pool, self.num_pages, self._streams = pool, num_pages, {self._stream()}
 
     def page_table(self, span: PagedSpan) -> torch.Tensor:
         """The pages of the span's sequences, int32 [sequences, pages of max_length], 0 behind the last."""
@@ -373,7 +373,8 @@ class PagedInt4Cache:
         return (t.stride(0) if t.shape[0] > 1 else 0), (t.stride(1) if t.shape[1] > 1 else 0)
 
     def store(self, layer: int, span: PagedSpan, keys: torch.Tensor, values: torch.Tensor) -> None:
-        """Quantizes the span's keys and values [tokens, kv_heads, head_dim] into the layer's pages."""
+        """Quantizes the span's keys and values [tokens, kv_heads, head_dim] into the layer's pages.  Refused where
+        tokens of two of the span's sequences stand in one page."""
         stream, capturing = self._check("store", layer, span), torch.cuda.is_current_stream_capturing()
         if self._here() and _lib.host().paged_store(self._handle.value, layer, span._address, keys, values, self.pool, self.dtype,
                                                     self.head_dim, capturing, stream):

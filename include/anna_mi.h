@@ -712,6 +712,7 @@ typedef struct {
   int64_t split_capacity, unit_capacity, touch_capacity;     /* and of the buffer's sections */
   int64_t tile_items, tile_capacity;
   int64_t few_rows, tile_rows; /* query rows of a tile: of the split form 16, 32 or 64, of the tile form 128 or 256 */
+  int64_t shared; /* 1: tokens of two of the sequences stand in the same page; such a span is not stored */
   int32_t* buf;
   float* partial_stats;  /* [partial_rows][kv_heads][2] */
   float* partial_values; /* [partial_rows][kv_heads][head_dim] */

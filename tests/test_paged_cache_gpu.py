@@ -650,6 +650,23 @@ def test_a_span_ends_with_its_sequences(gpu):
         cache.read(0, span)
 
 
+def test_sequences_that_share_a_page_are_not_stored_together(gpu):
+    cache = make(D=64, H=2, HQ=4)
+    seqs, m = fill(cache, [100])
+    child, = cache.fork(seqs)
+    m.rows[child] = m.rows[seqs[0]]
+    k = rows((8, 2, 64), BF, 5)
+    both = cache.span([seqs[0], child], [64, 68], [4, 4])
+    with pytest.raises(RuntimeError, match="share a page"):
+        cache.store(0, both, k, k)
+    check_held(cache, m, [seqs[0], child])
+    check_attend(cache, m, [seqs[0], child], [64, 68], [4, 4])
+    # one of them alone, both in pages of their own, and new tokens of both
+    cache.store(0, cache.span([child], [68], [4]), k[:4], k[:4])
+    cache.store(0, cache.span([seqs[0], child], [0, 68], [4, 4]), k, k)
+    cache.store(0, cache.extend([seqs[0], child], [4, 4]), k, k)
+
+
 def test_no_memory_for_a_span(gpu, monkeypatch):
     """An extend whose span cannot be allocated leaves the sequences as they were."""
     np = pytest.importorskip("numpy")
