@@ -344,14 +344,15 @@ class PagedInt4Cache:
             raise ValueError(f"{what}: the span belongs to another cache")
         if not 0 <= layer < self.num_layers:
             raise IndexError(f"{what}: layer {layer} of {self.num_layers}")
-        if span._version != self._version:
+        version = self._version
+        if span._version != version:
             if span._ended != [self._ended[s] for s in span.seqs]:
                 raise RuntimeError(f"{what}: a sequence of the span is not in use any more")
             lengths = self._lengths((ctypes.c_int32 * len(span.seqs))(*span.seqs))
             for s, start, n, have in zip(span.seqs, span.starts, span.counts, lengths):
                 if start + n > have:
                     raise RuntimeError(f"{what}: sequence {s} holds {have} tokens, the span reaches to {start + n}")
-            span._version = self._version
+            span._version = version
         stream = self._stream()
         span._used_on(stream)
         return stream

@@ -2,6 +2,7 @@
 them in all its forms, and the pages' life (copy on write, truncate, free, compact, resize)."""
 
 import random
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
@@ -707,3 +708,26 @@ def test_empty_spans(gpu):
         cache.store(0, span, q[:, :2], q[:, :2])
         assert cache.read(0, span)[0].shape == (0, 2, 64)
         assert cache.page_table(span).shape[0] == len(span.seqs)
+
+
+def test_threads_that_share_a_cache(gpu):
+    """Sequences that come, grow and go from several host threads, all on one stream."""
+    cache = make(D=64, H=2, HQ=4, pages=64, sequences=16)
+
+    def life(seed):
+        for turn in range(10):
+            n = 30 + 17 * ((seed + turn) % 8)
+            seqs = cache.add(2)
+            k, v = rows((2 * n, 2, 64), BF, seed), rows((2 * n, 2, 64), BF, seed + 1)
+            cache.store(0, cache.extend(seqs, [n, n]), k, v)
+            m = Mirror()
+            for i, s in enumerate(seqs):
+                m.store(s, 0, k[n * i:n * i + n].cpu(), v[n * i:n * i + n].cpu())
+            check_held(cache, m, seqs)
+            check_attend(cache, m, seqs, [n - 1, 0], [1, n])
+            cache.free(seqs)
+        return True
+
+    with ThreadPoolExecutor(4) as pool:
+        assert all(f.result() for f in [pool.submit(life, 10 * i) for i in range(4)])
+    assert cache.pages_in_use == 0
