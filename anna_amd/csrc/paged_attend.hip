@@ -75,13 +75,18 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 // 2^x of the difference to a running maximum that may still be -inf.
 __device__ __forceinline__ float weight(float m, float top) { return m == NEG ? 0.0f : __builtin_amdgcn_exp2f(m - top); }
 
-__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __expf(-x)); }
+// A reciprocal within a unit in the last place of fp32, where a division takes ten instructions.
+__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
+
+// Four neighbouring gates of an output row, asked for ahead of the sums that they meet.
+__device__ __forceinline__ u16x4 gates(const Attend& a, int64_t token, int head, int d) {
+  return *(const u16x4*)((const uint16_t*)a.gate + token * a.g_token + head * a.g_head + d);
+}
 
 // Four neighbouring values of an output row, gated.
 template <int DT>
-__device__ __forceinline__ void write_out(const Attend& a, int D, int64_t token, int head, int d, f32x4 v, int64_t heads) {
+__device__ __forceinline__ void write_out(const Attend& a, int D, int64_t token, int head, int d, f32x4 v, u16x4 g, int64_t heads) {
   if (a.gate) {
-    const u16x4 g = *(const u16x4*)((const uint16_t*)a.gate + token * a.g_token + head * a.g_head + d);
 #pragma unroll
     for (int i = 0; i < 4; i++) v[i] *= sigmoid(Elem<DT>::to_f32(g[i]));
   }
@@ -319,12 +324,19 @@ __global__ __launch_bounds__(256, NQ * D <= 256 ? 2 : 1) void paged_split_kernel
     float sum = l[n];
     sum += lane_xor16(sum);
     sum += lane_xor32(sum);
+    const int c = threadIdx.x / 16, row = it.tile * R + 16 * n + c;
     if (n > 0) __syncthreads();
     if (q == 0) wave_m[wave][r] = m[n], wave_l[wave][r] = sum;
 #pragma unroll
     for (int d = 0; d < DTILES; d++) *(f32x4*)&joined[wave][r][16 * d + 4 * q] = acc[n][d] + off[n][d / 4];
+    u16x4 gate[D / 64];
+#pragma unroll
+    for (int k = 0; k < D / 64; k++) {
+      gate[k] = u16x4{0, 0, 0, 0};
+      if (a.gate && it.part < 0 && row < rows)
+        gate[k] = gates(a, it.offset + row / G, h * G + row % G, 64 * k + 4 * (threadIdx.x % 16));
+    }
     __syncthreads();
-    const int c = threadIdx.x / 16, row = it.tile * R + 16 * n + c;
     if (row < rows) {
       const float top = fmaxf(fmaxf(wave_m[0][c], wave_m[1][c]), fmaxf(wave_m[2][c], wave_m[3][c]));
       float f[4], total = 0;
@@ -338,7 +350,7 @@ __global__ __launch_bounds__(256, NQ * D <= 256 ? 2 : 1) void paged_split_kernel
         f32x4 v = {0, 0, 0, 0};
 #pragma unroll
         for (int w = 0; w < 4; w++) v += f[w] * *(const f32x4*)&joined[w][c][d];
-        if (it.part < 0) write_out<DT>(a, D, it.offset + row / G, h * G + row % G, d, v * inv, (int64_t)H * G);
+        if (it.part < 0) write_out<DT>(a, D, it.offset + row / G, h * G + row % G, d, v * inv, gate[k], (int64_t)H * G);
         else *(f32x4*)(a.values + part * D + d) = v;
       }
       if (it.part >= 0 && threadIdx.x % 16 == 0) a.stats[2 * part] = top, a.stats[2 * part + 1] = total;
@@ -842,10 +854,30 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
     return;
   }
   constexpr int PART = 4 * D / NW, UNITS4 = PART / 4;  // dims of a pass: what the wave's share of LDS holds for 32 rows
+  constexpr int LANES = PART / 8, STEP = 64 / LANES, N = 32 / STEP;  // lanes of a row, eight dims each; rows at once
   f32x4* mine = (f32x4*)lds + wave * 32 * UNITS4;
   const float inv = 1.0f / total;
+  const int c = lane % LANES, r0 = lane / LANES, first_row = row0 + r0, step_t = STEP / G, step_h = STEP % G;
+  // what a lane writes: rows first_row + i STEP, their tokens and heads without a division each
+  auto each_row = [&](auto f) {
+    int token = first_row / G, out_head = first_row % G;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      f(i, first_row + i * STEP < rows, (int64_t)it.offset + token, h * G + out_head);
+      token += step_t;
+      out_head += step_h;
+      if (out_head >= G) out_head -= G, token++;
+    }
+  };
 #pragma unroll
   for (int pass = 0; pass < D / PART; pass++) {
+    const int dim = pass * PART + 8 * c;
+    u32x4 gate[N];  // all asked for at once
+    if (a.gate)
+      each_row([&](int i, bool ours, int64_t token, int head) {
+        gate[i] = u32x4{0, 0, 0, 0};
+        if (ours) gate[i] = *(const u32x4*)((const uint16_t*)a.gate + token * a.g_token + head * a.g_head + dim);
+      });
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last pass is read
 #pragma unroll
     for (int d = 0; d < PART / 32; d++)
@@ -856,29 +888,22 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
         mine[(lane % 32) * UNITS4 + (unit ^ (lane & 15))] = f32x4{x[4 * b], x[4 * b + 1], x[4 * b + 2], x[4 * b + 3]} * inv;
       }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    constexpr int LANES = PART / 8;  // of a row, eight dims each
-#pragma unroll
-    for (int i = 0; i < 32 * LANES / 64; i++) {
-      const int r = i * (64 / LANES) + lane / LANES, c = lane % LANES;
+    each_row([&](int i, bool ours, int64_t token, int head) {
+      const int r = r0 + i * STEP;
       const f32x4 x = mine[r * UNITS4 + ((2 * c) ^ (r & 15))], y = mine[r * UNITS4 + ((2 * c + 1) ^ (r & 15))];
-      const int out_row = row0 + r;
-      if (out_row >= rows) continue;
-      const int64_t token = it.offset + out_row / G;
-      const int out_head = h * G + out_row % G, dim = pass * PART + 8 * c;
       float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
       if (a.gate) {
-        const u32x4 g = *(const u32x4*)((const uint16_t*)a.gate + token * a.g_token + out_head * a.g_head + dim);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          v[2 * k] *= sigmoid(Elem<DT>::to_f32((uint16_t)g[k]));
-          v[2 * k + 1] *= sigmoid(Elem<DT>::to_f32((uint16_t)(g[k] >> 16)));
+          v[2 * k] *= sigmoid(Elem<DT>::to_f32((uint16_t)gate[i][k]));
+          v[2 * k + 1] *= sigmoid(Elem<DT>::to_f32((uint16_t)(gate[i][k] >> 16)));
         }
       }
       u32x4 o;
 #pragma unroll
       for (int k = 0; k < 4; k++) o[k] = Elem<DT>::cvt(v[2 * k]) | (uint32_t)Elem<DT>::cvt(v[2 * k + 1]) << 16;
-      *(u32x4*)((uint16_t*)a.out + (token * H * G + out_head) * D + dim) = o;
-    }
+      if (ours) *(u32x4*)((uint16_t*)a.out + (token * H * G + head) * D + dim) = o;
+    });
   }
 }
 
@@ -895,6 +920,10 @@ __global__ __launch_bounds__(2 * D) void paged_merge_kernel(const Attend a) {
   const int row = blockIdx.y;
   if (row >= u.rows) return;
   const int team = threadIdx.x / LANES, d = threadIdx.x % LANES * 4;
+  const int r = u.row0 + row, head = h * G + r % G;
+  const int64_t token = u.offset + r / G;
+  u16x4 gate = {0, 0, 0, 0};
+  if (a.gate && team == 0) gate = gates(a, token, head, d);
   float top = NEG, total = 0;
   f32x4 v = {0, 0, 0, 0};
   for (int k0 = team; k0 < u.splits; k0 += TEAMS * AHEAD) {
@@ -934,8 +963,7 @@ __global__ __launch_bounds__(2 * D) void paged_merge_kernel(const Attend a) {
     v = v * f0 + *(const f32x4*)&joined[k][d] * f1;
     top = next;
   }
-  const int r = u.row0 + row;
-  write_out<DT>(a, D, u.offset + r / G, h * G + r % G, d, v * (1.0f / total), (int64_t)H * G);
+  write_out<DT>(a, D, token, head, d, v * (1.0f / total), gate, (int64_t)H * G);
 }
 
 template <int DT, int D> int launch(const Attend& a, const Grid& g, hipStream_t stream) {
