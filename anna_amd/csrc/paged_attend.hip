@@ -216,13 +216,13 @@ __global__ __launch_bounds__(256, NQ * D <= 256 ? 2 : 1) void paged_split_kernel
   // memory every step (8 sequences of 1K to 16K: 27.4 us, so 23.3).
   constexpr bool QUERIES_IN_LDS = D == 256;
   u32x4* own = (u32x4*)joined[wave] + lane;
-  uint2* own_sums = (uint2*)((u32x4*)joined[wave] + 64 * KS) + lane;
+  u32x4* own_sums = (u32x4*)joined[wave] + 64 * KS + lane;
   if (QUERIES_IN_LDS) {
-    static_assert(D < 256 || (NQ == 1 && 1024 * KS + 512 * NG <= (int)sizeof(joined[0])), "the wave's part");
+    static_assert(D < 256 || (NQ == 1 && 1024 * (KS + NG) <= (int)sizeof(joined[0])), "the wave's part");
 #pragma unroll
     for (int s = 0; s < KS; s++) own[64 * s] = qf[0][s];
 #pragma unroll
-    for (int g = 0; g < NG; g++) own_sums[64 * g] = qsum[0][g];
+    for (int g = 0; g < NG; g++) own_sums[64 * g] = u32x4{qsum[0][g].x, qsum[0][g].y, 0, 0};
   }
   const uint32_t vmask = code_mask<ANNA_MI_BF16>(), kmask = DT == ANNA_MI_BF16 ? vmask : code_mask<DT>();
   for (; step < end; step += 4) {
@@ -231,8 +231,6 @@ __global__ __launch_bounds__(256, NQ * D <= 256 ? 2 : 1) void paged_split_kernel
       asm volatile("" ::: "memory");  // read here, not kept
 #pragma unroll
       for (int s = 0; s < KS; s++) qf[0][s] = own[64 * s];
-#pragma unroll
-      for (int g = 0; g < NG; g++) qsum[0][g] = own_sums[64 * g];
     }
 #pragma unroll
     for (int t = 0; t < TT; t++) {
@@ -243,7 +241,7 @@ __global__ __launch_bounds__(256, NQ * D <= 256 ? 2 : 1) void paged_split_kernel
         const u32x4 a0 = codes16<DT>(k.code[t][2 * g], kmask), a1 = codes16<DT>(k.code[t][2 * g + 1], kmask);
 #pragma unroll
         for (int n = 0; n < NQ; n++) {
-          f32x4 c = mfma_bf16(u32x4{o, o, 0, 0}, u32x4{qsum[n][g].x, qsum[n][g].y, 0, 0}, f32x4{0, 0, 0, 0});
+          f32x4 c = mfma_bf16(u32x4{o, o, 0, 0}, QUERIES_IN_LDS ? own_sums[64 * g] : u32x4{qsum[n][g].x, qsum[n][g].y, 0, 0}, f32x4{0, 0, 0, 0});
           c = mfma<DT>(a0, qf[n][2 * g], c);
           c = mfma<DT>(a1, qf[n][2 * g + 1], c);
           if (g == 0) z[n][t] = f32x4{bf16_lo(s.x) * c[0], bf16_hi(s.x) * c[1], bf16_lo(s.y) * c[2], bf16_hi(s.y) * c[3]};
