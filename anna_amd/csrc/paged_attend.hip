@@ -384,15 +384,17 @@ __global__ __launch_bounds__(256, NQ * D <= 256 ? 2 : 1) void paged_split_kernel
 //
 // The operands are fp16 for both types: (code + zero) * scale rounded to 11 bits, probabilities (times 2^8, so
 // that small ones stay above fp16's subnormals) too, which keeps the result within a tenth of the output's
-// own rounding for bf16 (fp16's own three roundings show: 3e-4 against 2e-4 of the plain form).  fp16 holds only so
-// much: from the first page on with scales beyond the limits below, and for queries above them from the first page on,
-// an item goes on in bf16 instead, at bf16's precision.
+// own rounding for bf16.  For fp16 they show beside it: 2.9e-4 in all against 2.1e-4 of the output's alone, from
+// the probabilities (a second term for them would give that back for 12% of the time), and up to 5e-4 where single
+// channels stand out of the keys, whose values then need more than fp16's bits, as a dense cache's would.
+// fp16 holds only so much: from the first page on with scales beyond the limits below, and for queries above them
+// from the first page on, an item goes on in bf16 instead, at bf16's precision.
 //
 // The vector unit bounds it: of a page and wave (32 rows, head_dim 128) 32 matrix instructions (1024 cycles) stand against
 // ~320 vector ones, 32 of them exponentials, and with two waves a SIMD the two overlap in part.  2048 tokens at the end
 // of 32K (32 query heads on 8, head_dim 128): 1150 us, 926 TFLOP/s, 78% of a large product's rate.  head_dim 256 has room
 // for one wave a SIMD only (its sums alone are 128 registers): a page of 128 rows takes 3.9 us, ragged prompts of up to
-// 1500 tokens 130 us (310 TFLOP/s).
+// 1500 tokens 116 us (340 TFLOP/s).
 constexpr float K_SCALE_MOST = 16.0f;                // |k| < 2^11: with |q| <= 2^11 subnormal roundings stay below 2^-14
 constexpr float V_SCALE_MOST = 256.0f;               // |v| < 2^15
 constexpr float V_SCALE_LEAST = 3.814697265625e-6f;  // 2^-18: subnormal roundings stay below a 2^-7th of a code's step
