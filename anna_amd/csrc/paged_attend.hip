@@ -524,6 +524,19 @@ template <int D> struct ValueShare {
 // LDS of a buffer: keys then values, 128 * D bytes each.
 template <int D> constexpr int buffer_words() { return 2 * 128 * D / 16; }
 
+// On their way out, 32 rows of UNITS four-value units stand in a wave's share of LDS, a row's units turned by the row's
+// number, so that neighbouring rows' same unit meets other banks; the turn stays within the row.
+template <int UNITS> constexpr int out_unit(int row, int unit) { return row * UNITS + (unit ^ (row & (UNITS < 16 ? UNITS - 1 : 15))); }
+template <int UNITS> constexpr bool one_to_one() {
+  bool taken[32 * UNITS] = {};
+  for (int i = 0; i < 32 * UNITS; i++) {
+    const int at = out_unit<UNITS>(i / UNITS, i % UNITS);
+    if (at < 0 || at >= 32 * UNITS || taken[at]) return false;
+    taken[at] = true;
+  }
+  return true;
+}
+
 // A wave's state: its 32 query rows.
 template <int D> struct Rows {
   f32x16 acc[D / 32];
@@ -874,6 +887,7 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
   }
   constexpr int PART = 4 * D / NW, UNITS4 = PART / 4;  // dims of a pass: what the wave's share of LDS holds for 32 rows
   constexpr int LANES = PART / 8, STEP = 64 / LANES, N = 32 / STEP;  // lanes of a row, eight dims each; rows at once
+  static_assert(one_to_one<UNITS4>() && NW * 32 * UNITS4 <= 2 * buffer_words<D>(), "a place of its own for every unit");
   f32x4* mine = (f32x4*)lds + wave * 32 * UNITS4;
   const float inv = 1.0f / total;
   const int c = lane % LANES, r0 = lane / LANES, first_row = row0 + r0, step_t = STEP / G, step_h = STEP % G;
@@ -904,12 +918,12 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
       for (int b = 0; b < 4; b++) {
         const f32x16& x = w.acc[pass * (PART / 32) + d];
         const int unit = 8 * d + 2 * b + hl;
-        mine[(lane % 32) * UNITS4 + (unit ^ (lane & 15))] = f32x4{x[4 * b], x[4 * b + 1], x[4 * b + 2], x[4 * b + 3]} * inv;
+        mine[out_unit<UNITS4>(lane % 32, unit)] = f32x4{x[4 * b], x[4 * b + 1], x[4 * b + 2], x[4 * b + 3]} * inv;
       }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     each_row([&](int i, bool ours, int64_t token, int head) {
       const int r = r0 + i * STEP;
-      const f32x4 x = mine[r * UNITS4 + ((2 * c) ^ (r & 15))], y = mine[r * UNITS4 + ((2 * c + 1) ^ (r & 15))];
+      const f32x4 x = mine[out_unit<UNITS4>(r, 2 * c)], y = mine[out_unit<UNITS4>(r, 2 * c + 1)];
       float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
       if (a.gate) {
 #pragma unroll
