@@ -430,6 +430,12 @@ template <int D> struct KeyShare {
       offset[g] = *(const uint16_t*)(row + (K_OFFSETS * D + r * NG * 2) + g * 2);
     }
   }
+  // The page's tokens from `seen` on become zeros.
+  __device__ __forceinline__ void hide_from(int seen, int quarter, uint32_t lane) {
+#pragma unroll
+    for (int g = 0; g < NG; g++)
+      if (16 * quarter + (int)(lane % 16) >= seen) scale[g] = 0;
+  }
   __device__ __forceinline__ bool wide() const {  // beyond what fp16 holds
     bool any = false;
 #pragma unroll
@@ -477,6 +483,14 @@ template <int D> struct ValueShare {
       const uint2 s = *(const uint2*)(row + u * 32 * NG + (V_SCALES * D + q * NG * 8));
       const uint2 o = *(const uint2*)(row + u * 32 * NG + (V_OFFSETS * D + q * NG * 8));
       scale[2 * u] = s.x, scale[2 * u + 1] = s.y, offset[2 * u] = o.x, offset[2 * u + 1] = o.y;
+    }
+  }
+  __device__ __forceinline__ void hide_from(int seen, int unit, uint32_t lane) {
+    const int first = unit / NG * 32 + (int)(lane / 16) * 4;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int token = first + k / 2 * 16 + k % 2 * 2;
+      scale[k] &= (token < seen ? 0xFFFFu : 0u) | (token + 1 < seen ? 0xFFFF0000u : 0u);
     }
   }
   __device__ __forceinline__ bool wide() const {
@@ -750,21 +764,29 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
 #pragma unroll
     for (int j = 0; j < 16; j++) w.acc[d][j] = 0;
 
-  // The loads are in: a flag if the page is none for fp16, and the scales as fp16.
-  auto convert_keys = [&](int slot) {
+  // The loads of page p are in: a flag if it is none for fp16, and the scales as fp16.  What no row of the tile sees has no
+  // say in that: it is the sequence's later tokens, or what the page held before.
+  const int seen_by_any = it.start + (min((it.tile + 1) * 32 * NW, rows) - 1) / G + 1;
+  auto not_ahead = [](int x) {  // nothing that follows from it is computed before the loop, to be kept in registers
+    asm volatile("" : "+v"(x));
+    return x;
+  };
+  auto convert_keys = [&](int p) {
     if (!has_keys) return;
-    if (__any(keys.wide())) wide[slot] = 1;
+    if (p * PAGE + PAGE > seen_by_any) keys.hide_from(seen_by_any - p * PAGE, wave & 3, not_ahead(lane));
+    if (__any(keys.wide())) wide[p & 3] = 1;
     keys.convert();
   };
-  auto convert_values = [&](int slot) {
+  auto convert_values = [&](int p) {
     bool beyond = false;
 #pragma unroll
     for (int n = 0; n < VALUES; n++)
       if (has_unit(n)) {
+        if (p * PAGE + PAGE > seen_by_any) values[n].hide_from(seen_by_any - p * PAGE, unit_of(n), not_ahead(lane));
         beyond |= values[n].wide();
         values[n].convert();
       }
-    if (__any(beyond)) wide[slot] = 1;
+    if (__any(beyond)) wide[p & 3] = 1;
   };
   const uint32_t mask = code_mask<ANNA_MI_F16>();
   const int key_at = KeyShare<D>::at(wave & 3, lane);
@@ -784,8 +806,8 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
   const int last = row0 < rows ? it.start + min(row0 + 31, rows - 1) / G + 1 : 0;  // and its last
   const int sees = valid ? it.start + t + 1 : 0;
 
-  convert_keys(it.page0 & 3);
-  convert_values(it.page0 & 3);
+  convert_keys(it.page0);
+  convert_values(it.page0);
 #pragma unroll
   for (int k = 0; k < KW; k++) put_key(lds, k);
 #pragma unroll
@@ -805,7 +827,7 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
     constexpr int KHALF = KSTEPS / 2, VHALF = D / 32;
     auto first = [&](int i) {
       constexpr int PER = (4 * VALUES + KHALF - 1) / KHALF;
-      if (i == 0) convert_values((p + 1) & 3);
+      if (i == 0) convert_values(p + 1);
 #pragma unroll
       for (int k = i * PER; k < (i + 1) * PER; k++)
         if (k < 4 * VALUES) put_value(then, k);
@@ -813,7 +835,7 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
     };
     auto second = [&](int i) {
       constexpr int PER = (KW + VHALF - 1) / VHALF;
-      if (i == 0) convert_keys((p + 1) & 3);
+      if (i == 0) convert_keys(p + 1);
 #pragma unroll
       for (int k = i * PER; k < (i + 1) * PER; k++)
         if (k < KW) put_key(then, k);

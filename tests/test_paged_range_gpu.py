@@ -1,0 +1,79 @@
+"""PagedInt4Cache's attention in tiles at the ends of what 16-bit operands hold: small and large queries, keys and values,
+and pages that held other tokens before.  Against the plain 64-bit counterpart."""
+
+import pytest
+import torch
+
+from _paged import Mirror, attention
+from test_paged_cache_gpu import BF, FP, make, rows
+
+pytestmark = pytest.mark.gpu
+
+
+def stored(cache, k, v):
+    """One sequence of these tokens (values of the cache's type, on the host) -> (sequences, its rows as held)."""
+    seqs = cache.add()
+    cache.store(0, cache.extend(seqs, [k.shape[0]]), k.cuda(), v.cuda())
+    m = Mirror()
+    m.store(0, 0, k, v)
+    return seqs, m.rows[0]
+
+
+def check(got, q, held, start, scaling, dtype):
+    want, tol = attention(q, *held, start, scaling, dtype)
+    err = (got.cpu().double() - want).abs()
+    assert (err <= tol).all(), float((err - tol).max())
+
+
+# ---------------------------------------------------------------- what no row sees
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("what", ["key", "value", "tiny value"])
+def test_tokens_that_a_page_held_before(gpu, D, dtype, what):
+    """What stands behind a sequence's end is nothing to its answers, bit by bit: neither tokens of another sequence that
+    had the page nor its own that are forgotten or not yet seen."""
+    factor = {"key": 2.0 ** 9, "value": 2.0 ** 12, "tiny value": 2.0 ** -22}[what]
+    k, v, q = (rows((n, h, D), dtype, i, "cpu") for i, n, h in ((1, 100, 2), (2, 100, 2), (3, 100, 4)))
+    k1, v1 = (rows((128, 2, D), torch.float32, i, "cpu") for i in (4, 5))
+    k1, v1 = ((k1 * factor).to(dtype), v1.to(dtype)) if what == "key" else (k1.to(dtype), (v1 * factor).to(dtype))
+
+    def answers(before):
+        cache = make(D=D, H=2, HQ=4, dtype=dtype, pages=2)
+        if before == "another":
+            old, _ = stored(cache, k1, v1)
+            cache.free(old)
+        elif before == "forgotten":
+            seqs = cache.add()
+            cache.store(0, cache.extend(seqs, [128]), torch.cat((k, k1[100:])).cuda(), torch.cat((v, v1[100:])).cuda())
+            cache.truncate(seqs[0], 100)
+        elif before == "later":
+            seqs = cache.add()
+            cache.store(0, cache.extend(seqs, [128]), torch.cat((k, k1[100:])).cuda(), torch.cat((v, v1[100:])).cuda())
+        if before in (None, "another"):
+            seqs, _ = stored(cache, k, v)
+        return cache.attend(0, cache.span(seqs, [0], [100]), q.cuda(), scaling=D ** -0.5)
+
+    first = answers(None)
+    for before in ("another", "forgotten", "later"):
+        assert torch.equal(answers(before), first), before
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_tokens_that_a_page_held_before_in_tiles_of_256(gpu, D):
+    lens = [70 + 5 * i % 60 for i in range(32)]
+    k, v, q = (rows((sum(lens), h, D), FP, i) for i, h in ((1, 8), (2, 8), (3, 32)))
+
+    def answers(before):
+        cache = make(D=D, H=8, HQ=32, dtype=FP, pages=96, sequences=32)
+        if before:
+            old = cache.add(32)
+            big = (rows((32 * 192, 8, D), torch.float32, 4) * 2.0 ** 9).to(FP)
+            cache.store(0, cache.extend(old, [192] * 32), big, big)
+            cache.free(old)
+        span = cache.extend(cache.add(32), lens)
+        assert span._c.tile_rows == 256
+        cache.store(0, span, k, v)
+        return cache.attend(0, span, q, scaling=D ** -0.5)
+
+    assert torch.equal(answers(True), answers(False))
