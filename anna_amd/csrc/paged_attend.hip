@@ -387,22 +387,22 @@ __global__ __launch_bounds__(256, NQ * D <= 256 ? 2 : 1) void paged_split_kernel
 // own rounding for bf16.  For fp16 they show beside it: 2.9e-4 in all against 2.1e-4 of the output's alone, from
 // the probabilities (a second term for them would give that back for 12% of the time), and up to 5e-4 where single
 // channels stand out of the keys, whose values then need more than fp16's bits, as a dense cache's would.
-// fp16 holds only so much: from the first page on with scales beyond the limits below, and for queries above them
-// from the first page on, an item goes on in bf16 instead, at bf16's precision.
+// fp16 holds only so much: from the first page on with scales beyond the limits below an item goes on in bf16 instead, at
+// bf16's precision.
 //
 // The vector unit bounds it: of a page and wave (32 rows, head_dim 128) 32 matrix instructions (1024 cycles) stand against
 // ~320 vector ones, 32 of them exponentials, and with two waves a SIMD the two overlap in part.  2048 tokens at the end
 // of 32K (32 query heads on 8, head_dim 128): 1150 us, 926 TFLOP/s, 78% of a large product's rate.  head_dim 256 has room
 // for one wave a SIMD only (its sums alone are 128 registers): a page of 128 rows takes 3.9 us, ragged prompts of up to
 // 1500 tokens 116 us (340 TFLOP/s).
-constexpr float K_SCALE_MOST = 16.0f;                // |k| < 2^11: with |q| <= 2^11 subnormal roundings stay below 2^-14
+constexpr float K_SCALE_MOST = 16.0f;                // |k| < 2^11.1
 constexpr float V_SCALE_MOST = 256.0f;               // |v| < 2^15
 constexpr float V_SCALE_LEAST = 3.814697265625e-6f;  // 2^-18: subnormal roundings stay below a 2^-7th of a code's step
 constexpr float V_SHRINK = 0.0625f;                  // in bf16: rounded, a group's largest value may be past the type's largest
-constexpr float Q_MOST = 2048.0f;
+constexpr int Q_BITS = 11;
+constexpr float SCALE_LEAST = 1.1754943508222875e-38f, SCALE_MOST = 3.4028234663852886e38f;  // 2^-126, the largest
 constexpr float P_SHIFT = 8.0f, P_SLACK = 4.0f;
 
-__device__ __forceinline__ f16x2 f16_pair(uint32_t v) { return f16x2{(_Float16)bf16_lo(v), (_Float16)bf16_hi(v)}; }
 // (code + zero) * scale of a pair: the sum is exact, the product rounded once.
 __device__ __forceinline__ uint32_t scaled(uint32_t code16, uint32_t offset, uint32_t scale) {
   return __builtin_bit_cast(uint32_t, (__builtin_bit_cast(f16x2, code16) + __builtin_bit_cast(f16x2, offset)) * __builtin_bit_cast(f16x2, scale));
@@ -741,20 +741,28 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
 #pragma unroll
   for (int s = 0; s < KSTEPS; s++) qf[s] = raw_query(s);
   if (threadIdx.x < 4) wide[threadIdx.x] = 0;
-  bool large = false;
-  auto too_large = [](float x) { return fabsf(x) > Q_MOST && fabsf(x) < INFINITY; };  // others spoil their own row alone
+  // A row's queries go in times a power of two that brings its largest to 2^(Q_BITS - 1) or above, below 2^Q_BITS, and its
+  // scores' scale takes that back: whatever their size, no value that could show is lost, and no row has a say in another's.
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 most = {0, 0};
+#pragma unroll
+  for (int s = 0; s < KSTEPS; s++)
+#pragma unroll
+    for (int k = 0; k < 4; k++) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, qf[s][k] & 0x7FFF7FFFu));
+  int largest = max(most[0], most[1]);
+  largest = max(largest, lane_xor32(largest));
+  // the exponent of zeros, infinities and NaN is 0
+  const int shift = Q_BITS - __builtin_amdgcn_frexp_expf(Elem<DT>::to_f32((uint16_t)largest));
 #pragma unroll
   for (int s = 0; s < KSTEPS; s++)
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-      if (DT == ANNA_MI_BF16) {
-        large |= too_large(bf16_lo(qf[s][k])) || too_large(bf16_hi(qf[s][k]));
-        qf[s][k] = __builtin_bit_cast(uint32_t, f16_pair(qf[s][k]));
-      } else {
-        large |= too_large(f16_bits_to_f32((uint16_t)qf[s][k])) || too_large(f16_bits_to_f32((uint16_t)(qf[s][k] >> 16)));
-      }
+      const float x = ldexpf(Elem<DT>::to_f32((uint16_t)qf[s][k]), shift), y = ldexpf(Elem<DT>::to_f32((uint16_t)(qf[s][k] >> 16)), shift);
+      qf[s][k] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)x, (_Float16)y});
     }
-  const bool all_wide = __syncthreads_or(large) != 0;
+  // neither 0 nor infinite, as scores that are not seen are -infinity: beyond these it makes no difference to finite ones
+  float scale = __builtin_amdgcn_fmed3f(ldexpf(a.scale, -shift), SCALE_LEAST, SCALE_MOST);
+  __syncthreads();
   auto query = [&](int s) { return qf[s]; };
 
   Rows<D> w;
@@ -817,7 +825,11 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
   next = page_id(it.page0 + 2);
   barrier();
   int p = it.page0;
-  for (; p < it.page1 && !all_wide && __builtin_amdgcn_readfirstlane(wide[p & 3]) == 0; p++) {
+  // A condition that always holds, but that the compiler takes to differ by lanes: without it, it keeps the two loops' sums
+  // apart, in 30 registers more (at 256 dims in memory).
+  int on = 1;
+  asm volatile("" : "+v"(on));
+  for (; p < it.page1 && on && __builtin_amdgcn_readfirstlane(wide[p & 3]) == 0; p++) {
     const int turn = (p - it.page0) & 1;
     u32x4 *now = lds + turn * buffer_words<D>(), *then = lds + (turn ^ 1) * buffer_words<D>();
     if (threadIdx.x == 0) wide[(p + 2) & 3] = 0;
@@ -845,7 +857,7 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
       }
     };
     if (p * PAGE < last) {
-      take_page<D, true, AHEAD>(w, now, query, sees - p * PAGE, p * PAGE + PAGE > seen_by_all, a.scale, lane, first, second);
+      take_page<D, true, AHEAD>(w, now, query, sees - p * PAGE, p * PAGE + PAGE > seen_by_all, scale, lane, first, second);
     } else {
 #pragma unroll
       for (int i = 0; i <= KHALF; i++) first(i);
@@ -860,6 +872,7 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
     constexpr float LESS = 1.0f / (1ull << (int)(P_SHIFT + ROOM));
     w.m += P_SHIFT + ROOM;
     w.l *= LESS;
+    scale = a.scale;
 #pragma unroll
     for (int d = 0; d < D / 32; d++) w.acc[d] *= LESS * V_SHRINK;
 #pragma unroll
@@ -886,7 +899,7 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
       }
       barrier();
       if (p * PAGE < last)
-        take_page<D, false, 1>(w, lds, query, sees - p * PAGE, p * PAGE + PAGE > seen_by_all, a.scale, lane, [](int) {}, [](int) {});
+        take_page<D, false, 1>(w, lds, query, sees - p * PAGE, p * PAGE + PAGE > seen_by_all, scale, lane, [](int) {}, [](int) {});
       barrier();
     }
 #pragma unroll

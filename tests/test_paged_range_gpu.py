@@ -77,3 +77,48 @@ def test_tokens_that_a_page_held_before_in_tiles_of_256(gpu, D):
         return cache.attend(0, span, q, scaling=D ** -0.5)
 
     assert torch.equal(answers(True), answers(False))
+
+
+# ---------------------------------------------------------------- queries
+
+SIZES = [(BF, 2.0 ** -30), (BF, 2.0 ** -100), (BF, 2.0 ** 40), (FP, 2.0 ** -12), (FP, 2.0 ** 11)]
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype,factor", SIZES)
+@pytest.mark.parametrize("count", [1, 100])
+def test_queries_of_any_size(gpu, D, dtype, factor, count):
+    """A query's size is taken back by the scaling, in both forms, to the type's own tolerance."""
+    cache = make(D=D, H=1, HQ=2, dtype=dtype)
+    seqs, held = stored(cache, *(rows((200, 1, D), dtype, i, "cpu") for i in (1, 2)))
+    q = (rows((count, 2, D), torch.float32, 3, "cpu") * factor).to(dtype)
+    scaling = D ** -0.5 / factor
+    got = cache.attend(0, cache.span(seqs, [200 - count], [count]), q.cuda(), scaling=scaling)
+    check(got, q, held, 200 - count, scaling, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_a_querys_size_is_its_own(gpu, dtype):
+    """A row far larger or smaller than the others, or all zeros, changes no other row's bits."""
+    cache = make(D=128, H=2, HQ=4, dtype=dtype)
+    seqs, held = stored(cache, *(rows((200, 2, 128), dtype, i, "cpu") for i in (1, 2)))
+    q = rows((200, 4, 128), dtype, 3, "cpu")
+    span = cache.span(seqs, [0], [200])
+    first = cache.attend(0, span, q.cuda(), scaling=0.1)
+    keep = [i for i in range(200) if i != 70]
+    for factor in (0.0, 2.0 ** -14, 2.0 ** 11):
+        p = q.clone()
+        p[70] *= factor
+        got = cache.attend(0, span, p.cuda(), scaling=0.1)
+        assert torch.equal(got[keep], first[keep]), factor
+        check(got, p, held, 0, 0.1, dtype)
+
+
+def test_scalings_at_the_ends(gpu):
+    """Scalings that leave fp32's normal numbers once the query's size is taken into them: flat or peaked, no NaN."""
+    cache = make(D=64, H=1, HQ=2)
+    seqs, held = stored(cache, *(rows((150, 1, 64), BF, i, "cpu") for i in (1, 2)))
+    for factor, scaling in ((2.0 ** -120, 1e-6), (2.0 ** -126, 1e-30), (2.0 ** 100, 2.0 ** -103), (2.0 ** -97, 2.0 ** 94), (0.0, 1e29)):
+        q = (rows((150, 2, 64), torch.float32, 3, "cpu") * factor).to(BF)
+        got = cache.attend(0, cache.span(seqs, [0], [150]), q.cuda(), scaling=scaling)
+        check(got, q, held, 0, scaling, BF)
