@@ -395,7 +395,13 @@ __global__ __launch_bounds__(256, NQ * D <= 256 ? 2 : 1) void paged_split_kernel
 // of 32K (32 query heads on 8, head_dim 128): 1150 us, 926 TFLOP/s, 78% of a large product's rate.  head_dim 256 has room
 // for one wave a SIMD only (its sums alone are 128 registers): a page of 128 rows takes 3.9 us, ragged prompts of up to
 // 1500 tokens 116 us (340 TFLOP/s).
-constexpr float K_SCALE_MOST = 16.0f;                // |k| < 2^11.1
+// Keys go in times 2^K_BITS.  A scale of K_SCALE_LEAST or more is exact so, and a key's subnormal rounding stays below a
+// 2^-8th of a code's step.  Smaller ones are off by up to 2^-25, a key by 136 times that, a score (D keys, queries below
+// 2^Q_BITS) by D * 2^-6.8 of its row's scale: up to scales of 2^-4 / D that is below half a step of fp16, and only tiles
+// with rows of larger ones need such keys as bf16 holds them.  (128 dims, scaling 128^-0.5: queries up to 64 do not.)
+constexpr float K_SCALE_MOST = 16.0f;  // |k| < 2^11.1
+constexpr int K_BITS = 4;
+constexpr uint32_t K_SCALE_LEAST = 0x3500;  // bf16's 2^-21
 constexpr float V_SCALE_MOST = 256.0f;               // |v| < 2^15
 constexpr float V_SCALE_LEAST = 3.814697265625e-6f;  // 2^-18: subnormal roundings stay below a 2^-7th of a code's step
 constexpr float V_SHRINK = 0.0625f;                  // in bf16: rounded, a group's largest value may be past the type's largest
@@ -436,16 +442,18 @@ template <int D> struct KeyShare {
     for (int g = 0; g < NG; g++)
       if (16 * quarter + (int)(lane % 16) >= seen) scale[g] = 0;
   }
-  __device__ __forceinline__ bool wide() const {  // beyond what fp16 holds
+  // Beyond what fp16 holds; least: bf16 bits of the smallest scale but 0.
+  __device__ __forceinline__ bool wide(uint32_t least) const {
     bool any = false;
 #pragma unroll
-    for (int g = 0; g < NG; g++) any |= bf16_lo(scale[g]) > K_SCALE_MOST;
+    for (int g = 0; g < NG; g++) any |= bf16_lo(scale[g]) > K_SCALE_MOST || scale[g] - 1 < least - 1;
     return any;
   }
   __device__ __forceinline__ void convert() {
 #pragma unroll
     for (int g = 0; g < NG; g++) {
-      scale[g] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)bf16_lo(scale[g]), (_Float16)bf16_lo(scale[g])});
+      const _Float16 s = (_Float16)(bf16_lo(scale[g]) * (1 << K_BITS));
+      scale[g] = __builtin_bit_cast(uint32_t, f16x2{s, s});
       offset[g] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)bf16_lo(offset[g]), (_Float16)bf16_lo(offset[g])});
     }
   }
@@ -761,8 +769,9 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
       qf[s][k] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)x, (_Float16)y});
     }
   // neither 0 nor infinite, as scores that are not seen are -infinity: beyond these it makes no difference to finite ones
-  float scale = __builtin_amdgcn_fmed3f(ldexpf(a.scale, -shift), SCALE_LEAST, SCALE_MOST);
-  __syncthreads();
+  float scale = __builtin_amdgcn_fmed3f(ldexpf(a.scale, -shift - K_BITS), SCALE_LEAST, SCALE_MOST);
+  const bool counts = largest > 0 && largest < (DT == ANNA_MI_BF16 ? 0x7F80 : 0x7C00);  // not for its row alone
+  const uint32_t key_least = __syncthreads_or(counts && scale > 0.0625f / D) ? K_SCALE_LEAST : 1;
   auto query = [&](int s) { return qf[s]; };
 
   Rows<D> w;
@@ -782,7 +791,7 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
   auto convert_keys = [&](int p) {
     if (!has_keys) return;
     if (p * PAGE + PAGE > seen_by_any) keys.hide_from(seen_by_any - p * PAGE, wave & 3, not_ahead(lane));
-    if (__any(keys.wide())) wide[p & 3] = 1;
+    if (__any(keys.wide(key_least))) wide[p & 3] = 1;
     keys.convert();
   };
   auto convert_values = [&](int p) {

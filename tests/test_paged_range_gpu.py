@@ -122,3 +122,48 @@ def test_scalings_at_the_ends(gpu):
         q = (rows((150, 2, 64), torch.float32, 3, "cpu") * factor).to(BF)
         got = cache.attend(0, cache.span(seqs, [0], [150]), q.cuda(), scaling=scaling)
         check(got, q, held, 0, scaling, BF)
+
+
+# ---------------------------------------------------------------- keys
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype,factor,as_type", [(BF, 2.0 ** -16, BF), (BF, 2.0 ** -24, BF), (BF, 2.0 ** -60, BF), (FP, 2.0 ** -12, FP),
+                                                  (FP, 2.0 ** -20, BF)])
+@pytest.mark.parametrize("count", [1, 100])
+def test_keys_of_any_size(gpu, D, dtype, factor, as_type, count):
+    """Small keys under a large scaling.  Where fp16 does not hold them, the tiles go on in bf16, to its tolerance."""
+    cache = make(D=D, H=1, HQ=2, dtype=dtype)
+    k = (rows((200, 1, D), torch.float32, 1, "cpu") * factor).to(dtype)
+    seqs, held = stored(cache, k, rows((200, 1, D), dtype, 2, "cpu"))
+    q = rows((count, 2, D), dtype, 3, "cpu")
+    scaling = D ** -0.5 / factor
+    got = cache.attend(0, cache.span(seqs, [200 - count], [count]), q.cuda(), scaling=scaling)
+    check(got, q, held, 200 - count, scaling, as_type)
+
+
+@pytest.mark.parametrize("dtype,factor", [(BF, 2.0 ** -26), (BF, 2.0 ** -20), (FP, 2.0 ** -20)])
+def test_a_small_group_that_alone_counts(gpu, dtype, factor):
+    """Queries that are zero where the keys are large: the scores come from a group of small keys alone."""
+    cache = make(D=128, H=1, HQ=2, dtype=dtype)
+    k = rows((200, 1, 128), torch.float32, 1, "cpu")
+    k[..., 64:] *= factor
+    k = k.to(dtype)
+    seqs, held = stored(cache, k, rows((200, 1, 128), dtype, 2, "cpu"))
+    q = rows((200, 2, 128), dtype, 3, "cpu")
+    q[..., :64] = 0
+    got = cache.attend(0, cache.span(seqs, [0], [200]), q.cuda(), scaling=0.125 / factor)
+    check(got, q, held, 0, 0.125 / factor, BF)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("D", [128, 256])
+def test_a_small_group_beside_ordinary_ones(gpu, D, dtype):
+    """Channels that are nearly dead cost no precision under an ordinary scaling: the type's own tolerance."""
+    cache = make(D=D, H=1, HQ=2, dtype=dtype)
+    k = rows((200, 1, D), torch.float32, 1, "cpu")
+    k[..., 64:128] *= 2.0 ** -21
+    k = k.to(dtype)
+    seqs, held = stored(cache, k, rows((200, 1, D), dtype, 2, "cpu"))
+    q = rows((200, 2, D), dtype, 3, "cpu")
+    got = cache.attend(0, cache.span(seqs, [0], [200]), q.cuda(), scaling=D ** -0.5)
+    check(got, q, held, 0, D ** -0.5, dtype)
