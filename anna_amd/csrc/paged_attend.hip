@@ -403,7 +403,7 @@ constexpr float K_SCALE_MOST = 16.0f;  // |k| < 2^11.1
 constexpr int K_BITS = 4;
 constexpr uint32_t K_SCALE_LEAST = 0x3500;  // bf16's 2^-21
 constexpr float V_SCALE_MOST = 256.0f;               // |v| < 2^15
-constexpr float V_SCALE_LEAST = 3.814697265625e-6f;  // 2^-18: subnormal roundings stay below a 2^-7th of a code's step
+constexpr float V_SCALE_LEAST = 7.62939453125e-6f;   // 2^-17: exact in fp16, subnormal roundings below a 2^-8th of a code's step
 constexpr float V_SHRINK = 0.0625f;                  // in bf16: rounded, a group's largest value may be past the type's largest
 constexpr int Q_BITS = 11;
 constexpr float SCALE_LEAST = 1.1754943508222875e-38f, SCALE_MOST = 3.4028234663852886e38f;  // 2^-126, the largest

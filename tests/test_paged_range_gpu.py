@@ -167,3 +167,21 @@ def test_a_small_group_beside_ordinary_ones(gpu, D, dtype):
     q = rows((200, 2, D), dtype, 3, "cpu")
     got = cache.attend(0, cache.span(seqs, [0], [200]), q.cuda(), scaling=D ** -0.5)
     check(got, q, held, 0, D ** -0.5, dtype)
+
+
+# ---------------------------------------------------------------- values
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_values_whose_scale_fp16_rounds(gpu, D):
+    """Values whose scale, 65.5 * 2^-24, lies between two of fp16's subnormal numbers: the first token's answer is its
+    value, to half a step of bf16 at most."""
+    cache = make(D=D, H=1, HQ=4, dtype=FP)
+    g = torch.Generator().manual_seed(1)
+    units = 1572 + 2 * (32.74 * torch.randint(0, 16, (100, 1, D), generator=g)).round()
+    units[..., ::64], units[..., 1::64] = 1572, 2554
+    v = (units * 2.0 ** -24).to(FP)
+    seqs, held = stored(cache, rows((100, 1, D), FP, 2, "cpu"), v)
+    assert (held[3] == 65.5 * 2.0 ** -24).all()
+    got = cache.attend(0, cache.span(seqs, [0], [100]), rows((100, 4, D), FP, 3).cuda(), scaling=D ** -0.5)
+    want = held[1][0].expand(4, D)
+    assert ((got[0].cpu().double() - want).abs() <= (2.0 ** -8 + 2.0 ** -11) * want.abs() + 2.0 ** -25).all()
