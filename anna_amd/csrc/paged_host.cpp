@@ -178,18 +178,28 @@ int64_t fewest_pages(const std::vector<Record>& records, int form, int64_t items
   return low;
 }
 
+// starts null: of the tokens that an extend by counts is going to add.  The bounds are those of its span.
 int make_plan(anna_mi_paged* h, int64_t n, const int32_t* seqs, const int64_t* starts, const int64_t* counts, Plan& p) {
-  ANNA_CHECK(n >= 0 && (n == 0 || (seqs && starts && counts)), "span: null arrays");
+  ANNA_CHECK(n >= 0 && (n == 0 || (seqs && counts)), "span: null arrays");
   int rc = check_seqs(h, n, seqs);
   if (rc != ANNA_MI_OK) return rc;
   const int64_t G = h->d.q_heads / h->d.kv_heads, H = h->d.kv_heads;
   const int64_t most = 4096 / h->d.head_dim;  // rows of a split tile whose sums stay in registers
   int64_t large = 0;                          // tiles of 256 rows
   std::vector<int32_t> held;                  // pages that others hold too
+  std::vector<int64_t> ends;
+  if (!starts) {
+    for (int64_t i = 0; i < n; i++) {
+      ends.push_back(h->length[seqs[i]]);
+      ANNA_CHECK(counts[i] >= 0 && counts[i] <= h->d.max_pages * PAGE - ends[i], "span: %lld tokens more than the %lld of sequence %d, at most %lld fit",
+                 (long long)counts[i], (long long)ends[i], (int)seqs[i], (long long)(h->d.max_pages * PAGE));
+    }
+  }
+  const int64_t* const at = starts ? starts : ends.data();
   for (int64_t i = 0; i < n; i++) {
-    ANNA_CHECK(starts[i] >= 0 && counts[i] >= 0 && starts[i] <= h->length[seqs[i]] && counts[i] <= h->length[seqs[i]] - starts[i],
-               "span: tokens %lld .. %lld of sequence %d, which holds %lld", (long long)starts[i],
-               (long long)(starts[i] + counts[i]), (int)seqs[i], (long long)h->length[seqs[i]]);
+    ANNA_CHECK(!starts || (starts[i] >= 0 && counts[i] >= 0 && starts[i] <= h->length[seqs[i]] && counts[i] <= h->length[seqs[i]] - starts[i]),
+               "span: tokens %lld .. %lld of sequence %d, which holds %lld", (long long)at[i],
+               (long long)(at[i] + counts[i]), (int)seqs[i], (long long)h->length[seqs[i]]);
     p.tokens += counts[i];
     const int64_t rows = counts[i] * G;
     if (rows > TILE_LEAST) large += ceil_div(rows, 256);
@@ -204,19 +214,19 @@ int make_plan(anna_mi_paged* h, int64_t n, const int32_t* seqs, const int64_t* s
     const int64_t rows = counts[i] * G, f = rows > TILE_LEAST, R = f ? p.tile_rows : p.few_rows;
     for (int64_t t = 0; t < std::max<int64_t>(1, ceil_div(rows, R)); t++) {
       Record r = {};
-      r.index = (int32_t)i, r.row = seqs[i], r.start = (int32_t)starts[i], r.count = (int32_t)counts[i];
+      r.index = (int32_t)i, r.row = seqs[i], r.start = (int32_t)at[i], r.count = (int32_t)counts[i];
       r.offset = (int32_t)offset, r.tile = (int32_t)t, r.tiled = (int32_t)f;
-      r.pages = rows ? (int32_t)((starts[i] + (std::min(rows, (t + 1) * R) - 1) / G) / PAGE + 1) : 0;
+      r.pages = rows ? (int32_t)((at[i] + (std::min(rows, (t + 1) * R) - 1) / G) / PAGE + 1) : 0;
       r.touch0 = (int32_t)p.touches;
       tiles[f] += rows > 0;
       rows_of[f] = std::max(rows_of[f], std::min(rows, R));
       p.records.push_back(r);
     }
     if (counts[i] > 0) {
-      const int64_t first = starts[i] / PAGE, last = (starts[i] + counts[i] - 1) / PAGE;
+      const int64_t first = at[i] / PAGE, last = (at[i] + counts[i] - 1) / PAGE;
       p.touches += last - first + 1;
       p.touch_bound += (counts[i] + PAGE - 2) / PAGE + 1;
-      for (int64_t c = first; c <= last; c++)
+      for (int64_t c = first; starts && c <= last; c++)
         if (h->refs[h->row(seqs[i])[c]] > 1) held.push_back(h->row(seqs[i])[c]);
     }
     offset += counts[i];
@@ -552,6 +562,7 @@ int anna_mi_paged_span_fill(anna_mi_paged* h, int64_t n, const int32_t* seqs, co
                             anna_mi_paged_span* span, void* stream) {
   return guarded(h, "paged_span_fill", [&]() -> int {
     ANNA_CHECK(span && span->buf && (uintptr_t)span->buf % 16 == 0, "paged_span_fill: null or unaligned buffer");
+    ANNA_CHECK(n <= 0 || starts, "paged_span_fill: null starts");
     Plan p;
     const int rc = make_plan(h, n, seqs, starts, counts, p);
     if (rc != ANNA_MI_OK) return rc;

@@ -51,7 +51,6 @@ struct Library {
   decltype(&anna_mi_paged_fork) paged_fork = nullptr;
   decltype(&anna_mi_paged_free) paged_free = nullptr;
   decltype(&anna_mi_paged_extend) paged_extend = nullptr;
-  decltype(&anna_mi_paged_truncate) paged_truncate = nullptr;
   decltype(&anna_mi_paged_lengths) paged_lengths = nullptr;
   decltype(&anna_mi_paged_span_plan) paged_span_plan = nullptr;
   decltype(&anna_mi_paged_span_fill) paged_span_fill = nullptr;
@@ -81,7 +80,6 @@ void bind(const py::dict& d) {
   get("anna_mi_paged_fork", lib.paged_fork);
   get("anna_mi_paged_free", lib.paged_free);
   get("anna_mi_paged_extend", lib.paged_extend);
-  get("anna_mi_paged_truncate", lib.paged_truncate);
   get("anna_mi_paged_lengths", lib.paged_lengths);
   get("anna_mi_paged_span_plan", lib.paged_span_plan);
   get("anna_mi_paged_span_fill", lib.paged_span_fill);
@@ -519,11 +517,10 @@ bool paged_free(uintptr_t handle, const py::object& seqs, uintptr_t stream) {
   return true;
 }
 
-py::object filled_span(uintptr_t handle, uintptr_t span, const std::vector<int32_t>& s, const std::vector<int64_t>& starts,
-                       const std::vector<int64_t>& counts, int64_t kv_heads, int64_t head_dim, int64_t device, uintptr_t stream) {
-  const int64_t n = (int64_t)s.size();
-  anna_mi_paged_span* out = span_at(span);
-  check(lib.paged_span_plan(paged(handle), n, s.data(), starts.data(), counts.data(), out), "anna_mi_paged_span_plan");
+// A span's memory, and the span's pointers to it; starts null: of an extend by counts.
+std::vector<Tensor> span_memory(uintptr_t handle, anna_mi_paged_span* out, const std::vector<int32_t>& s, const int64_t* starts,
+                                const std::vector<int64_t>& counts, int64_t kv_heads, int64_t head_dim, int64_t device) {
+  check(lib.paged_span_plan(paged(handle), (int64_t)s.size(), s.data(), starts, counts.data(), out), "anna_mi_paged_span_plan");
   const auto ints = at::TensorOptions().dtype(at::kInt).device(at::kCUDA, (c10::DeviceIndex)device);
   std::vector<Tensor> held{at::empty({out->words}, ints)};
   if (out->partial_rows > 0) {
@@ -533,8 +530,7 @@ py::object filled_span(uintptr_t handle, uintptr_t span, const std::vector<int32
     out->partial_values = (float*)ptr(held[2]);
   }
   out->buf = (int32_t*)ptr(held[0]);
-  check(lib.paged_span_fill(paged(handle), n, s.data(), starts.data(), counts.data(), out, stream_ptr(stream)), "anna_mi_paged_span_fill");
-  return py::make_tuple(s, starts, counts, held);
+  return held;
 }
 
 // Fills a span anew, with its buffer and workspace: extend (starts is None) by counts, None for one each, or the
@@ -544,7 +540,9 @@ py::object paged_span(uintptr_t handle, uintptr_t span, const py::object& seqs, 
   const auto s = whole<int32_t>(seqs, 0, I32);
   if (!s) return py::none();
   const int64_t n = (int64_t)s->size();
+  anna_mi_paged_span* out = span_at(span);
   std::optional<std::vector<int64_t>> c, at;
+  std::vector<Tensor> held;
   if (counts.is_none()) c = std::vector<int64_t>(n, 1);
   else c = whole<int64_t>(counts, 0, I64);
   if (!c || (int64_t)c->size() != n) return py::none();
@@ -553,18 +551,15 @@ py::object paged_span(uintptr_t handle, uintptr_t span, const py::object& seqs, 
     check(lib.paged_lengths(paged(handle), n, s->data(), at->data(), nullptr), "anna_mi_paged_lengths");
     for (int64_t i = 0; i < n; i++)
       if ((*at)[i] < 0 || (*c)[i] > max_length - (*at)[i]) return py::none();
+    held = span_memory(handle, out, *s, nullptr, *c, kv_heads, head_dim, device);  // before anything changes
     check(lib.paged_extend(paged(handle), n, s->data(), c->data(), at->data(), stream_ptr(stream)), "anna_mi_paged_extend");
   } else {
     at = whole<int64_t>(starts, 0, I64);
     if (!at || (int64_t)at->size() != n) return py::none();
+    held = span_memory(handle, out, *s, at->data(), *c, kv_heads, head_dim, device);
   }
-  try {
-    return filled_span(handle, span, *s, *at, *c, kv_heads, head_dim, device, stream);
-  } catch (...) {  // no memory for the span: the sequences as they were
-    if (starts.is_none())
-      for (int64_t i = 0; i < n; i++) lib.paged_truncate(paged(handle), (*s)[i], (*at)[i], stream_ptr(stream));
-    throw;
-  }
+  check(lib.paged_span_fill(paged(handle), n, s->data(), at->data(), c->data(), out, stream_ptr(stream)), "anna_mi_paged_span_fill");
+  return py::make_tuple(*s, *at, *c, held);
 }
 
 // Rows [tokens, heads, head_dim] of the cache's type that the kernels read as they are

@@ -76,12 +76,11 @@ class PagedSpan:
         """Tokens of all sequences."""
         return self._c.tokens
 
-    def _fill(self, seqs, starts, counts) -> None:
+    def _room(self, seqs, starts, counts) -> None:
+        """A new span's memory; starts None: of an extend by counts."""
         cache, c = self.cache, self._c
-        n = len(seqs)
-        fresh = c.buf is None
-        if fresh:
-            cache._call("anna_mi_paged_span_plan", n, seqs, starts, counts, self._ref)
+        if c.buf is None:
+            cache._call("anna_mi_paged_span_plan", len(seqs), seqs, starts, counts, self._ref)
             buf = torch.empty((c.words,), dtype=torch.int32, device=cache.device)
             c.buf = buf.data_ptr()
             self._tensors = [buf]
@@ -91,8 +90,11 @@ class PagedSpan:
                                      device=cache.device)
                 c.partial_stats, c.partial_values = stats.data_ptr(), values.data_ptr()
                 self._tensors += [stats, values]
+
+    def _fill(self, seqs, starts, counts) -> None:
+        cache = self.cache
         self._used_on(cache._stream())
-        cache._call("anna_mi_paged_span_fill", n, seqs, starts, counts, self._ref, cache._stream())
+        cache._call("anna_mi_paged_span_fill", len(seqs), seqs, starts, counts, self._ref, cache._stream())
         self.seqs, self.starts, self.counts = list(seqs), list(starts), list(counts)
         self._ended, self._version = [cache._ended[s] for s in self.seqs], cache._version
 
@@ -237,13 +239,9 @@ class PagedInt4Cache:
             for s, have, n in zip(seqs, starts, counts):
                 if have + n > self.max_length:
                     raise RuntimeError(f"sequence {s} would hold {have + n} tokens, max_length is {self.max_length}")
+            span._room(seqs, None, counts)  # before anything changes
             self._call("anna_mi_paged_extend", len(seqs), seqs, counts, starts, self._stream())
-            try:
-                span._fill(seqs, starts, counts)
-            except BaseException:  # no memory for the span: the sequences as they were
-                for s, have in zip(seqs, starts):
-                    self._call("anna_mi_paged_truncate", s, have, self._stream())
-                raise
+            span._fill(seqs, starts, counts)
         return span
 
     def span(self, seqs, starts, counts, *, span: PagedSpan | None = None) -> PagedSpan:
@@ -260,6 +258,7 @@ class PagedInt4Cache:
             raise ValueError(f"{len(seqs)} sequences, {len(starts)} starts and {len(counts)} counts")
         span = self._refilled(span, seqs, counts)
         with self._lock:
+            span._room(seqs, starts, counts)
             span._fill(seqs, starts, counts)
         return span
 

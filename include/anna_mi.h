@@ -739,7 +739,8 @@ int anna_mi_paged_resize(anna_mi_paged* handle, int64_t num_pages, void* pool, v
 int anna_mi_paged_lengths(anna_mi_paged* handle, int64_t n, const int32_t* seqs, int64_t* lengths, int64_t* live_pages);
 
 /* Sizes of a span (its capacities too); then, with buf and the partials allocated, its fill.  A fill
- * of the same sequences count and counts fits the buffer of an earlier one (its capacities). */
+ * of the same sequences count and counts fits the buffer of an earlier one (its capacities).  A plan without
+ * starts (NULL) is of the tokens that an extend by counts will add: with its memory at hand, the extend cannot fail for it. */
 int anna_mi_paged_span_plan(anna_mi_paged* handle, int64_t n, const int32_t* seqs, const int64_t* starts,
                             const int64_t* counts, anna_mi_paged_span* span);
 int anna_mi_paged_span_fill(anna_mi_paged* handle, int64_t n, const int32_t* seqs, const int64_t* starts,

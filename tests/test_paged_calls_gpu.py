@@ -1,0 +1,34 @@
+"""PagedInt4Cache's calls where they are refused or fail: what they leave behind."""
+
+import pytest
+import torch
+
+from test_paged_cache_gpu import BF, FP, check_attend, check_held, fill, make, rows
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("host", [True, False])
+def test_no_memory_for_the_span_of_forked_sequences(gpu, host):
+    """An extend whose span cannot be allocated leaves pages shared as they were; again and again."""
+    cache = make(D=256, H=8, HQ=8, pages=16)
+    parent, m = fill(cache, [100])
+    kids = cache.fork(parent * 3)
+    for s in kids:
+        m.rows[s] = m.rows[parent[0]]
+    seqs = kids if host else torch.tensor(kids)  # the host module takes plain lists alone
+    table = cache.page_table(cache.span(kids, [0] * 3, [1] * 3))
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.set_per_process_memory_fraction(0.0)  # the span's workspace (32 MiB) is not to be had
+    try:
+        for _ in range(20):
+            with pytest.raises(RuntimeError, match="out of memory"):
+                cache.extend(seqs, [130, 130, 130])
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert cache.pages_in_use == 2 and cache.lengths(kids) == [100] * 3
+    assert torch.equal(cache.page_table(cache.span(kids, [0] * 3, [1] * 3)), table) and torch.equal(table[0], table[1])
+    check_held(cache, m, kids)
+    cache.extend(seqs, [130, 130, 130])
+    assert cache.pages_in_use == 2 + 3 * 3 and cache.lengths(kids) == [230] * 3
