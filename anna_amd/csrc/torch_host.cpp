@@ -564,7 +564,7 @@ py::object paged_span(uintptr_t handle, uintptr_t span, const py::object& seqs, 
 
 // Rows [tokens, heads, head_dim] of the cache's type that the kernels read as they are
 bool paged_rows(const Tensor& t, const at::Device& dev, at::ScalarType dt, int64_t tokens, int64_t heads, int64_t head_dim) {
-  return plain(t, dev) && t.scalar_type() == dt && t.dim() == 3 && t.size(0) == tokens && t.size(1) == heads && t.size(2) == head_dim &&
+  return plain(t, dev) && !(t.requires_grad() && at::GradMode::is_enabled()) && t.scalar_type() == dt && t.dim() == 3 && t.size(0) == tokens && t.size(1) == heads && t.size(2) == head_dim &&
          t.stride(2) == 1 && (tokens <= 1 || t.stride(0) % 8 == 0) && (heads <= 1 || t.stride(1) % 8 == 0) &&
          reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }

@@ -18,10 +18,11 @@ include/anna_mi.h.
     span = cache.extend(seqs)                  # the next token of each
     answers = cache.fork([seqs[0]] * 4)        # four continuations of the first
 
-The host counts pages and lengths; ``extend`` and ``span`` lay out the step's launches once for all
-layers.  Calls that share a cache must not overlap on the GPU: run them on one stream, or order the
-streams.  A step can be captured in a graph (``store``, ``read`` and ``attend``, not the calls that
-count): refill its span with ``extend(..., span=span)`` before every replay.
+The cache is for inference: tensors that require grad are refused outside ``torch.no_grad()``.  The host
+counts pages and lengths; ``extend`` and ``span`` lay out the step's launches once for all layers.  Calls
+that share a cache must not overlap on the GPU: run them on one stream, or order the streams.  A step can be
+captured in a graph (``store``, ``read`` and ``attend``, not the calls that count): refill its span with
+``extend(..., span=span)`` before every replay.
 """
 
 from __future__ import annotations
@@ -362,11 +363,18 @@ class PagedInt4Cache:
             raise ValueError(f"{what} must be {self.dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
         if t.device != self.device:
             raise RuntimeError(f"{what} must be on {self.device}, got a tensor on {t.device}")
+        self._no_grad(what, t)
         # rows are read 16 bytes at a time; the stride of a single token or head is read by nobody
         if (t.stride(2) != 1 or t.data_ptr() % 16 or (t.shape[0] > 1 and t.stride(0) % 8)
                 or (heads > 1 and t.stride(1) % 8)):
             return t.clone(memory_format=torch.contiguous_format)
         return t
+
+    @staticmethod
+    def _no_grad(what: str, t: torch.Tensor) -> None:
+        if t.requires_grad and torch.is_grad_enabled():
+            # an answer without a graph would lose its gradient without a word
+            raise RuntimeError(f"{what} requires grad, but the cache has no backward pass: call it under torch.no_grad()")
 
     @staticmethod
     def _strides(t: torch.Tensor) -> tuple[int, int]:
@@ -414,6 +422,8 @@ class PagedInt4Cache:
         elif (out.dtype != self.dtype or tuple(out.shape) != tuple(query.shape) or out.device != self.device
               or not out.is_contiguous() or out.data_ptr() % 16):
             raise ValueError(f"out must be a contiguous, 16-byte aligned {self.dtype} tensor of the query's shape")
+        else:
+            self._no_grad("out", out)
         self._call("anna_mi_paged_attend", layer, span._ref, query.data_ptr(), *self._strides(query),
                    None if gate is None else gate.data_ptr(), *((0, 0) if gate is None else self._strides(gate)),
                    out.data_ptr(), scaling, capturing, stream)

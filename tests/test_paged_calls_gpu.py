@@ -32,3 +32,27 @@ def test_no_memory_for_the_span_of_forked_sequences(gpu, host):
     check_held(cache, m, kids)
     cache.extend(seqs, [130, 130, 130])
     assert cache.pages_in_use == 2 + 3 * 3 and cache.lengths(kids) == [230] * 3
+
+
+def test_what_requires_grad_is_refused(gpu):
+    """There is no backward pass: no call drops a gradient silently."""
+    cache = make(D=64, H=2, HQ=4)
+    seqs, m = fill(cache, [100])
+    span = cache.span(seqs, [90], [10])
+    q, kv = rows((10, 4, 64), BF, 5), rows((10, 2, 64), BF, 6)
+    want = cache.attend(0, span, q, scaling=0.1, gate=q)
+    with_grad, kv_grad = q.clone().requires_grad_(), kv.clone().requires_grad_()
+    wide = torch.cat((q, q), -1).requires_grad_()[..., 4:68]  # rows that are copied first
+    for name, call in [("query", lambda: cache.attend(0, span, with_grad, scaling=0.1)), ("query", lambda: cache.attend(0, span, wide, scaling=0.1)),
+                       ("gate", lambda: cache.attend(0, span, q, scaling=0.1, gate=with_grad)),
+                       ("out", lambda: cache.attend(0, span, q, scaling=0.1, out=with_grad)),
+                       ("keys", lambda: cache.store(0, span, kv_grad, kv)), ("values", lambda: cache.store(0, span, kv, kv_grad))]:
+        with pytest.raises(RuntimeError, match=name + " requires grad"):
+            call()
+    check_held(cache, m, seqs)
+    with torch.no_grad():
+        assert torch.equal(cache.attend(0, span, with_grad, scaling=0.1, gate=with_grad), want)
+        cache.store(0, span, kv_grad, kv_grad)
+    with torch.inference_mode():
+        assert cache.attend(0, span, with_grad, scaling=0.1, gate=with_grad).shape == want.shape
+    assert torch.equal(with_grad, q)
