@@ -221,8 +221,8 @@ class PagedSpan(ctypes.Structure):
         ("sequences", _I64), ("tokens", _I64), ("words", _I64), ("partial_rows", _I64), ("split_items", _I64),
         ("split_units", _I64), ("split_rows", _I64), ("touch_items", _I64), ("split_capacity", _I64),
         ("unit_capacity", _I64), ("touch_capacity", _I64), ("tile_items", _I64), ("tile_capacity", _I64),
-        ("few_rows", _I64), ("tile_rows", _I64), ("shared", _I64), ("buf", _P), ("partial_stats", _P),
-        ("partial_values", _P),
+        ("few_rows", _I64), ("tile_rows", _I64), ("shared", _I64), ("stored", _I64), ("buf", _P),
+        ("partial_stats", _P), ("partial_values", _P),
     ]
 
 

@@ -571,6 +571,7 @@ int anna_mi_paged_span_fill(anna_mi_paged* h, int64_t n, const int32_t* seqs, co
                    p.touches <= span->touch_capacity && p.partial_rows <= span->partial_rows && sections(*span).words <= span->words,
                "span: these tokens do not fit the span that is filled");
     ANNA_CHECK(p.partial_rows == 0 || (span->partial_stats && span->partial_values), "paged_span_fill: null partials");
+    ANNA_CHECK(!p.shared || !span->stored, "span: two sequences share a page that a captured store of this span would write");
     span->shared = p.shared;
     span->split_items = p.items[0];
     span->tile_items = p.items[1];
@@ -607,7 +608,7 @@ uint8_t* layer_pool(anna_mi_paged* h, int64_t layer) {
 bool aligned(const void* p, int64_t token, int64_t head) { return (uintptr_t)p % 16 == 0 && token % 8 == 0 && head % 8 == 0; }
 }  // namespace
 
-int anna_mi_paged_store(anna_mi_paged* h, int64_t layer, const anna_mi_paged_span* span, const void* keys, int64_t key_stride_token,
+int anna_mi_paged_store(anna_mi_paged* h, int64_t layer, anna_mi_paged_span* span, const void* keys, int64_t key_stride_token,
                         int64_t key_stride_head, const void* values, int64_t value_stride_token, int64_t value_stride_head,
                         int capacity_grid, void* stream) {
   return guarded(h, "paged_store", [&]() -> int {
@@ -618,6 +619,7 @@ int anna_mi_paged_store(anna_mi_paged* h, int64_t layer, const anna_mi_paged_spa
     ANNA_CHECK(keys && values, "paged_store: null keys or values");
     ANNA_CHECK(aligned(keys, key_stride_token, key_stride_head) && aligned(values, value_stride_token, value_stride_head),
                "paged_store: keys and values need rows of 16-byte alignment");
+    if (capacity_grid) span->stored = 1;
     return launch_store(h->d.dtype, h->d.head_dim, layer_pool(h, layer), h->d.table, h->d.max_pages, span->buf,
                         (const Touch*)(span->buf + sections(*span).touch),
                         capacity_grid ? span->touch_capacity : span->touch_items, h->d.kv_heads, keys, key_stride_token,

@@ -573,7 +573,7 @@ int64_t head_stride(const Tensor& t) { return t.size(1) > 1 ? t.stride(1) : 0; }
 
 bool paged_store(uintptr_t handle, int64_t layer, uintptr_t span, const Tensor& keys, const Tensor& values, const Tensor& pool,
                  at::ScalarType dtype, int64_t head_dim, bool capturing, uintptr_t stream) {
-  const anna_mi_paged_span* s = span_at(span);
+  anna_mi_paged_span* s = span_at(span);
   if (!paged_rows(keys, pool.device(), dtype, s->tokens, pool.size(2), head_dim) ||
       !paged_rows(values, pool.device(), dtype, s->tokens, pool.size(2), head_dim))
     return false;

@@ -713,6 +713,7 @@ typedef struct {
   int64_t tile_items, tile_capacity;
   int64_t few_rows, tile_rows; /* query rows of a tile: of the split form 16, 32 or 64, of the tile form 128 or 256 */
   int64_t shared; /* 1: tokens of two of the sequences stand in the same page; such a span is not stored */
+  int64_t stored; /* 1: a store with capacity_grid took this span, whose replays ask nothing; it is not filled so any more */
   int32_t* buf;
   float* partial_stats;  /* [partial_rows][kv_heads][2] */
   float* partial_values; /* [partial_rows][kv_heads][head_dim] */
@@ -750,7 +751,7 @@ int anna_mi_paged_span_fill(anna_mi_paged* handle, int64_t n, const int32_t* seq
  * captured graph), not for the last one.
  *
  * keys/values [tokens][kv_heads][head_dim] of a span into its pages of a layer, and back */
-int anna_mi_paged_store(anna_mi_paged* handle, int64_t layer, const anna_mi_paged_span* span, const void* keys,
+int anna_mi_paged_store(anna_mi_paged* handle, int64_t layer, anna_mi_paged_span* span, const void* keys,
                         int64_t key_stride_token, int64_t key_stride_head, const void* values,
                         int64_t value_stride_token, int64_t value_stride_head, int capacity_grid, void* stream);
 int anna_mi_paged_read(anna_mi_paged* handle, int64_t layer, const anna_mi_paged_span* span, void* keys, void* values,

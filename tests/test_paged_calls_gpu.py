@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+from _paged import held
 from test_paged_cache_gpu import BF, FP, check_attend, check_held, fill, make, rows
 
 pytestmark = pytest.mark.gpu
@@ -56,3 +57,30 @@ def test_what_requires_grad_is_refused(gpu):
     with torch.inference_mode():
         assert cache.attend(0, span, with_grad, scaling=0.1, gate=with_grad).shape == want.shape
     assert torch.equal(with_grad, q)
+
+
+def test_a_captured_store_is_not_replayed_over_shared_pages(gpu):
+    """A replay cannot refuse, so the fill before it does; the span then holds what it held."""
+    cache = make(D=64, H=2, HQ=4)
+    seqs, m = fill(cache, [100, 90])
+    span = cache.span(seqs, [70, 70], [4, 4])
+    k = rows((8, 2, 64), BF, 5)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.store(0, span, k, k)
+    child, = cache.fork(seqs[:1])
+    with pytest.raises(RuntimeError, match="share a page"):
+        cache.span([seqs[0], child], [70, 70], [4, 4], span=span)
+    assert span.seqs == seqs
+    read = cache.span([seqs[0], child], [70, 70], [4, 4])  # another one, not stored: as before
+    cache.attend(0, read, rows((8, 4, 64), BF, 6), scaling=0.1)
+    cache.span([seqs[0], child], [70, 70], [4, 4], span=read)
+    want = held(k.cpu(), k.cpu())[0].to(BF)
+    graph.replay()  # what the span was filled with last
+    for s, part in zip(seqs, want.split(4)):
+        assert torch.equal(cache.read(0, cache.span([s], [70], [4]))[0].cpu(), part)
+    cache.span([seqs[1], child], [80, 10], [4, 4], span=span)
+    graph.replay()
+    for s, at, part in zip([seqs[1], child], [80, 10], want.split(4)):
+        assert torch.equal(cache.read(0, cache.span([s], [at], [4]))[0].cpu(), part)
