@@ -188,8 +188,15 @@ class PagedInt4Cache:
         """Whether the cache's device is the current one, which the host module's calls take for granted."""
         return torch.cuda.current_device() == self.device.index
 
+    def _capturing(self) -> bool:
+        """Whether the current stream of the cache's device records a graph."""
+        if self._here():
+            return torch.cuda.is_current_stream_capturing()
+        with torch.cuda.device(self.device):
+            return torch.cuda.is_current_stream_capturing()
+
     def _counts(self, what: str) -> None:
-        if torch.cuda.is_current_stream_capturing():
+        if self._capturing():
             # lengths and pages are counted on the host: a replay would not count again
             raise RuntimeError(f"PagedInt4Cache.{what} cannot be captured in a graph")
 
@@ -383,7 +390,7 @@ class PagedInt4Cache:
     def store(self, layer: int, span: PagedSpan, keys: torch.Tensor, values: torch.Tensor) -> None:
         """Quantizes the span's keys and values [tokens, kv_heads, head_dim] into the layer's pages.  Refused where
         tokens of two of the span's sequences stand in one page."""
-        stream, capturing = self._check("store", layer, span), torch.cuda.is_current_stream_capturing()
+        stream, capturing = self._check("store", layer, span), self._capturing()
         if self._here() and _lib.host().paged_store(self._handle.value, layer, span._address, keys, values, self.pool, self.dtype,
                                                     self.head_dim, capturing, stream):
             return
@@ -393,7 +400,7 @@ class PagedInt4Cache:
 
     def read(self, layer: int, span: PagedSpan) -> tuple[torch.Tensor, torch.Tensor]:
         """The span's keys and values as the cache holds them, dense [tokens, kv_heads, head_dim]."""
-        stream, capturing = self._check("read", layer, span), torch.cuda.is_current_stream_capturing()
+        stream, capturing = self._check("read", layer, span), self._capturing()
         if self._here():
             return _lib.host().paged_read(self._handle.value, layer, span._address, self.pool, self.dtype, self.head_dim,
                                           capturing, stream)
@@ -406,7 +413,7 @@ class PagedInt4Cache:
                gate: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """Causal attention for the span's tokens: query [tokens, q_heads, head_dim] over all tokens of its
         sequence up to and with its own -> the same shape.  gate (optional, same shape as query): out *= sigmoid(gate)."""
-        stream, capturing = self._check("attend", layer, span), torch.cuda.is_current_stream_capturing()
+        stream, capturing = self._check("attend", layer, span), self._capturing()
         if self._here():
             got = _lib.host().paged_attend(self._handle.value, layer, span._address, query, gate, out, self.pool, self.dtype,
                                            self.q_heads, self.head_dim, scaling, capturing, stream)

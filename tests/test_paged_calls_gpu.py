@@ -84,3 +84,33 @@ def test_a_captured_store_is_not_replayed_over_shared_pages(gpu):
     graph.replay()
     for s, at, part in zip([seqs[1], child], [80, 10], want.split(4)):
         assert torch.equal(cache.read(0, cache.span([s], [at], [4]))[0].cpu(), part)
+
+
+@pytest.mark.parametrize("ours", [True, False])
+def test_captures_are_those_of_the_caches_device(gpu, monkeypatch, ours):
+    """With another device current, what counts is whether the cache's own records a graph (devices by proxy here)."""
+    cache = make(D=64, H=1, HQ=1)
+    seqs, _ = fill(cache, [3])
+    on_ours = []
+
+    class Device:
+        def __init__(self, device):
+            assert torch.device(device) == cache.device
+
+        def __enter__(self):
+            on_ours.append(1)
+
+        def __exit__(self, *args):
+            on_ours.pop()
+
+    with monkeypatch.context() as patch:
+        patch.setattr(torch.cuda, "current_device", lambda: cache.device.index + 1)
+        patch.setattr(torch.cuda, "device", Device)
+        patch.setattr(torch.cuda, "is_current_stream_capturing", lambda: bool(on_ours) == ours)
+        if ours:
+            for call in (lambda: cache.extend(seqs), lambda: cache.free(seqs), lambda: cache.compact()):
+                with pytest.raises(RuntimeError, match="captured"):
+                    call()
+        else:
+            cache.extend(seqs)
+    assert cache.lengths(seqs) == [3 if ours else 4]
