@@ -7,6 +7,7 @@
 #include <stddef.h>
 
 #include <algorithm>
+#include <memory>
 #include <mutex>
 #include <new>
 #include <vector>
@@ -300,8 +301,7 @@ int anna_mi_paged_create(const anna_mi_paged_desc* desc, anna_mi_paged** handle)
   ANNA_CHECK(d.pool && d.table, "paged_create: null pool or table");
   ANNA_CHECK((uintptr_t)d.pool % 16 == 0, "paged_create: the pool must be 16-byte aligned");
   try {
-    auto* h = new anna_mi_paged;
-    *handle = h;
+    auto h = std::make_unique<anna_mi_paged>();
     h->d = d;
     h->table.assign(d.max_sequences * d.max_pages, 0);
     h->length.assign(d.max_sequences, -1);
@@ -309,6 +309,7 @@ int anna_mi_paged_create(const anna_mi_paged_desc* desc, anna_mi_paged** handle)
     h->refs.assign(d.num_pages, 0);
     for (int64_t i = d.num_pages - 1; i >= 0; i--) h->free_pages.push_back((int32_t)i);
     for (int64_t i = d.max_sequences - 1; i >= 0; i--) h->free_seqs.push_back((int32_t)i);
+    *handle = h.release();
   } catch (const std::exception& e) {
     set_error("paged_create: %s", e.what());
     return ANNA_MI_EINVAL;

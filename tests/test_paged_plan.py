@@ -55,3 +55,31 @@ def test_refusals():
         _lib.call("anna_mi_paged_span_fill", h, 1, seqs, None, i64(1), ctypes.byref(_lib.PagedSpan(buf=64)), None)
     assert state(h, seqs) == ([100, 0], 2)
     _lib.call("anna_mi_paged_destroy", h)
+
+
+NO_MEMORY = """
+import ctypes, resource, sys
+sys.path[:0] = ["tests", "."]
+from anna_amd import _lib
+_lib.load()
+d = _lib.PagedDesc(0, 1, (1 << 30), 1, 1, 64, 1 << 10, 1 << 10, 64, 64)  # 4 GiB of counts for the pages
+h = ctypes.c_void_p(7)
+used = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (used + (1 << 30),) * 2)
+for _ in range(300):  # 4 MiB of table each, were they kept
+    try:
+        _lib.call("anna_mi_paged_create", ctypes.byref(d), ctypes.byref(h))
+        raise SystemExit("created")
+    except RuntimeError as e:
+        assert "paged_create" in str(e), e
+assert h.value == 7
+"""
+
+
+def test_a_cache_that_finds_no_memory_leaves_nothing():
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    done = subprocess.run([sys.executable, "-c", NO_MEMORY], cwd=Path(__file__).parents[1], capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, done.stdout + done.stderr
