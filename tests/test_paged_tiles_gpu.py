@@ -88,3 +88,55 @@ def test_rows_of_other_strides(gpu):
     want = cache.attend(0, span, q.contiguous(), scaling=0.1, gate=gate.contiguous())
     out = torch.empty_like(want)
     assert cache.attend(0, span, q, scaling=0.1, gate=gate, out=out) is out and torch.equal(out, want)
+
+
+@pytest.mark.parametrize("D,HQ,H,counts,lens,rows_of_a_tile", [
+    (64, 8, 2, [1, 3, 40, 100, 0], [2900, 10, 700, 64, 5], 128),
+    (256, 4, 2, [33, 1, 70], [1, 1800, 300], 128),
+    (128, 32, 8, [17 + i % 40 for i in range(32)] + [1, 2], [50 * (i % 7) for i in range(32)] + [2000, 3], 256),
+])
+def test_captured_mixed_steps_equal_eager_ones(gpu, D, HQ, H, counts, lens, rows_of_a_tile):
+    """store + attend of single tokens, drafts and prompts together, captured once: replays over other sequences, shorter and
+    longer ones, whose launches are laid out otherwise than those of the capture."""
+    n, total = len(counts), sum(counts)
+
+    def run(captured):
+        cache = PagedInt4Cache(num_layers=1, num_pages=sum(-(-(m + 8 * c) // 64) + 1 for m, c in zip(lens, counts)) + 64, kv_heads=H,
+                               q_heads=HQ, head_dim=D, max_sequences=n + 1, max_length=4096)
+        seqs, _ = fill(cache, lens)
+        k, v, q, out = (torch.zeros((total, h, D), dtype=BF, device="cuda") for h in (H, H, HQ, HQ))
+
+        def step(span):
+            cache.store(0, span, k, v)
+            cache.attend(0, span, q, scaling=0.1, gate=q, out=out)
+
+        seen, span, graph = [], None, None
+        for i in range(7):
+            if i == 3:  # other sequences, much longer or shorter than those of the capture
+                long = max(range(n), key=lambda j: lens[j])
+                kid, = cache.fork([seqs[long]])
+                cache.truncate(seqs[long], 7)
+                other = min(range(n), key=lambda j: lens[j])
+                cache.free([seqs[other]])
+                seqs[other] = kid
+                cache.compact()
+            if i == 5:
+                seqs.reverse()
+            span = cache.extend(seqs, counts, span=span)
+            assert span._c.tile_rows == rows_of_a_tile
+            for t, seed in ((k, 100), (v, 200), (q, 300)):
+                t.copy_(rows(t.shape, BF, seed + i))
+            if not captured or i == 0:
+                step(span)
+            else:
+                if graph is None:
+                    torch.cuda.synchronize()
+                    graph = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(graph):
+                        step(span)
+                graph.replay()
+            seen.append(out.clone())
+        return seen
+
+    for i, (a, b) in enumerate(zip(run(False), run(True))):
+        assert torch.equal(a, b) and torch.isfinite(a).all(), i
