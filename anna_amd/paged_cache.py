@@ -100,10 +100,8 @@ class PagedSpan:
         self._ended, self._version = [cache._ended[s] for s in self.seqs], cache._version
 
     def _fresh(self, seqs, starts, counts) -> bool:
-        """A new span's fill by the host module; False for calls that it leaves to the general way."""
+        """A new span's fill by the host module, on the current device; False for calls that it leaves to the general way."""
         cache = self.cache
-        if not cache._here():
-            return False
         stream = cache._stream()
         got = _lib.host().paged_span(cache._handle.value, self._address, seqs, starts, counts, cache.max_length,
                                      cache.kv_heads, cache.head_dim, cache.device.index, stream)
@@ -188,17 +186,18 @@ class PagedInt4Cache:
         """Whether the cache's device is the current one, which the host module's calls take for granted."""
         return torch.cuda.current_device() == self.device.index
 
-    def _capturing(self) -> bool:
-        """Whether the current stream of the cache's device records a graph."""
-        if self._here():
-            return torch.cuda.is_current_stream_capturing()
+    def _capturing_there(self) -> bool:
+        """Whether the current stream of the cache's device, which is not the current one, records a graph."""
         with torch.cuda.device(self.device):
             return torch.cuda.is_current_stream_capturing()
 
-    def _counts(self, what: str) -> None:
-        if self._capturing():
+    def _counts(self, what: str) -> bool:
+        """For calls that count on the host -> whether the cache's device is the current one."""
+        here = self._here()
+        if torch.cuda.is_current_stream_capturing() if here else self._capturing_there():
             # lengths and pages are counted on the host: a replay would not count again
             raise RuntimeError(f"PagedInt4Cache.{what} cannot be captured in a graph")
+        return here
 
     # ---- sequences
     def add(self, n: int = 1) -> list[int]:
@@ -213,8 +212,7 @@ class PagedInt4Cache:
     def fork(self, parents) -> list[int]:
         """A new sequence for every listed one (which may repeat), holding the same tokens in the same pages.
         A page is copied when one of the sequences that share it grows into it."""
-        self._counts("fork")
-        if self._here():
+        if self._counts("fork"):
             children = _lib.host().paged_fork(self._handle.value, parents, self._stream())
             if children is not None:
                 return children
@@ -228,8 +226,8 @@ class PagedInt4Cache:
         the new tokens, which the caller then stores in every layer.  Nothing changes if the pool has
         too few pages or the span no memory.  ``span``: an earlier span of as many sequences with the same counts, which is
         filled again in place (a captured graph holds its addresses)."""
-        self._counts("extend")
-        if span is None:
+        here = self._counts("extend")
+        if here and span is None:
             span = PagedSpan(self)
             with self._lock:
                 if span._fresh(seqs, None, counts):
@@ -254,8 +252,8 @@ class PagedInt4Cache:
 
     def span(self, seqs, starts, counts, *, span: PagedSpan | None = None) -> PagedSpan:
         """The span of tokens that the sequences hold already: to store them anew, read them, or attend for them."""
-        self._counts("span")
-        if span is None:
+        here = self._counts("span")
+        if here and span is None:
             span = PagedSpan(self)
             with self._lock:
                 if starts is not None and counts is not None and span._fresh(seqs, starts, counts):
@@ -289,10 +287,10 @@ class PagedInt4Cache:
 
     def free(self, seqs) -> None:
         """Ends sequences; pages that no other sequence shares return to the pool."""
-        self._counts("free")
+        here = self._counts("free")
         seqs = list(seqs)
         with self._lock:
-            if not (self._here() and _lib.host().paged_free(self._handle.value, seqs, self._stream())):
+            if not (here and _lib.host().paged_free(self._handle.value, seqs, self._stream())):
                 seqs = _ints(seqs, ctypes.c_int32)
                 self._call("anna_mi_paged_free", len(seqs), seqs, self._stream())
             for s in seqs:
@@ -390,9 +388,10 @@ class PagedInt4Cache:
     def store(self, layer: int, span: PagedSpan, keys: torch.Tensor, values: torch.Tensor) -> None:
         """Quantizes the span's keys and values [tokens, kv_heads, head_dim] into the layer's pages.  Refused where
         tokens of two of the span's sequences stand in one page."""
-        stream, capturing = self._check("store", layer, span), self._capturing()
-        if self._here() and _lib.host().paged_store(self._handle.value, layer, span._address, keys, values, self.pool, self.dtype,
-                                                    self.head_dim, capturing, stream):
+        stream, here = self._check("store", layer, span), self._here()
+        capturing = torch.cuda.is_current_stream_capturing() if here else self._capturing_there()
+        if here and _lib.host().paged_store(self._handle.value, layer, span._address, keys, values, self.pool, self.dtype,
+                                            self.head_dim, capturing, stream):
             return
         keys, values = self._rows("keys", keys, span, self.kv_heads), self._rows("values", values, span, self.kv_heads)
         self._call("anna_mi_paged_store", layer, span._ref, keys.data_ptr(), *self._strides(keys), values.data_ptr(),
@@ -400,8 +399,9 @@ class PagedInt4Cache:
 
     def read(self, layer: int, span: PagedSpan) -> tuple[torch.Tensor, torch.Tensor]:
         """The span's keys and values as the cache holds them, dense [tokens, kv_heads, head_dim]."""
-        stream, capturing = self._check("read", layer, span), self._capturing()
-        if self._here():
+        stream, here = self._check("read", layer, span), self._here()
+        capturing = torch.cuda.is_current_stream_capturing() if here else self._capturing_there()
+        if here:
             return _lib.host().paged_read(self._handle.value, layer, span._address, self.pool, self.dtype, self.head_dim,
                                           capturing, stream)
         keys, values = (torch.empty((span._c.tokens, self.kv_heads, self.head_dim), dtype=self.dtype, device=self.device)
@@ -413,8 +413,9 @@ class PagedInt4Cache:
                gate: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """Causal attention for the span's tokens: query [tokens, q_heads, head_dim] over all tokens of its
         sequence up to and with its own -> the same shape.  gate (optional, same shape as query): out *= sigmoid(gate)."""
-        stream, capturing = self._check("attend", layer, span), self._capturing()
-        if self._here():
+        stream, here = self._check("attend", layer, span), self._here()
+        capturing = torch.cuda.is_current_stream_capturing() if here else self._capturing_there()
+        if here:
             got = _lib.host().paged_attend(self._handle.value, layer, span._address, query, gate, out, self.pool, self.dtype,
                                            self.q_heads, self.head_dim, scaling, capturing, stream)
             if got is not None:
