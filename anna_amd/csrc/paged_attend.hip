@@ -444,10 +444,11 @@ template <int D> struct KeyShare {
   }
   // Beyond what fp16 holds; least: bf16 bits of the smallest scale but 0.
   __device__ __forceinline__ bool wide(uint32_t least) const {
-    bool any = false;
+    float most = bf16_lo(scale[0]);
+    uint32_t smallest = scale[0] - 1;
 #pragma unroll
-    for (int g = 0; g < NG; g++) any |= bf16_lo(scale[g]) > K_SCALE_MOST || scale[g] - 1 < least - 1;
-    return any;
+    for (int g = 1; g < NG; g++) most = fmaxf(most, bf16_lo(scale[g])), smallest = min(smallest, scale[g] - 1);
+    return most > K_SCALE_MOST || smallest < least - 1;
   }
   __device__ __forceinline__ void convert() {
 #pragma unroll
