@@ -114,3 +114,17 @@ def test_captures_are_those_of_the_caches_device(gpu, monkeypatch, ours):
         else:
             cache.extend(seqs)
     assert cache.lengths(seqs) == [3 if ours else 4]
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("start,count", [(2999, 1), (2992, 8), (2000, 100), (0, 130)])
+def test_answers_in_place_of_the_queries_or_gates(gpu, dtype, start, count):
+    """out may be the query or the gate itself, in every form, split over the context or not."""
+    cache = make(D=128, HQ=8, H=2, dtype=dtype)
+    seqs, _ = fill(cache, [3000, 40])
+    span = cache.span(seqs, [start, 39], [count, 1])
+    q, gate = (rows((count + 1, 8, 128), dtype, i) for i in (5, 6))
+    want = cache.attend(0, span, q, scaling=0.1, gate=gate)
+    for at in range(2):
+        x = [q.clone(), gate.clone()]
+        assert torch.equal(cache.attend(0, span, x[0], scaling=0.1, gate=x[1], out=x[at]), want)

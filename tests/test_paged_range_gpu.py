@@ -79,6 +79,32 @@ def test_tokens_that_a_page_held_before_in_tiles_of_256(gpu, D):
     assert torch.equal(answers(True), answers(False))
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("count", [1, 20, 100])
+def test_tokens_that_are_not_finite_and_that_no_row_sees(gpu, D, dtype, count):
+    """NaN and infinities of another sequence behind the end, and of its own later tokens: bit by bit as without them."""
+    k, v, q = (rows((n, h, D), dtype, i, "cpu") for i, n, h in ((1, 128, 1), (2, 128, 1), (3, count, 4)))
+
+    def answers(before):
+        cache = make(D=D, H=1, HQ=4, dtype=dtype, pages=2)
+        bad = torch.full((128, 1, D), float("nan"), dtype=dtype)
+        if before == "another":
+            old, _ = stored(cache, bad, -bad)
+            cache.free(old)
+        if before == "later":
+            bad[:] = float("inf")
+            seqs, _ = stored(cache, torch.cat((k[:110], bad[110:])), torch.cat((v[:110], bad[110:])))
+        else:
+            seqs, _ = stored(cache, k[:110], v[:110])
+        return cache.attend(0, cache.span(seqs, [110 - count], [count]), q.cuda(), scaling=D ** -0.5)
+
+    first = answers(None)
+    assert torch.isfinite(first).all()
+    for before in ("another", "later"):
+        assert torch.equal(answers(before), first), before
+
+
 # ---------------------------------------------------------------- queries
 
 SIZES = [(BF, 2.0 ** -30), (BF, 2.0 ** -100), (BF, 2.0 ** 40), (FP, 2.0 ** -12), (FP, 2.0 ** 11)]
