@@ -34,8 +34,9 @@ namespace {
 typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 
 constexpr float NEG = -INFINITY;
-// Probabilities with bf16's exponents stay below 2^-ROOM: sums of a context's 2^24 of them, times what stands for a value
-// at most (31 times its scale, and a scale is up to 2^125), stay within fp32, as the values' mean does.
+// Probabilities with bf16's exponents stay below 2^-ROOM, in the tile form, whose maximum may lag, 2^-(ROOM - P_SLACK): sums
+// of 2^24 of the former, times what stands for a value at most (31 times its scale, and a scale is up to 2^125), and of
+// 2^22 of the latter, times the type's largest value, stay within fp32, as the values' mean does.
 constexpr float ROOM = 26.0f;
 
 __device__ __forceinline__ f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
@@ -392,9 +393,9 @@ __global__ __launch_bounds__(256, NQ * D <= 256 ? 2 : 1) void paged_split_kernel
 //
 // The vector unit bounds it: of a page and wave (32 rows, head_dim 128) 32 matrix instructions (1024 cycles) stand against
 // ~320 vector ones, 32 of them exponentials, and with two waves a SIMD the two overlap in part.  2048 tokens at the end
-// of 32K (32 query heads on 8, head_dim 128): 1150 us, 926 TFLOP/s, 78% of a large product's rate.  head_dim 256 has room
-// for one wave a SIMD only (its sums alone are 128 registers): a page of 128 rows takes 3.9 us, ragged prompts of up to
-// 1500 tokens 116 us (340 TFLOP/s).
+// of 32K (32 query heads on 8, head_dim 128): 1119 us, 952 TFLOP/s, 80% of a large product's rate (by the card, up to
+// 1200); in bf16 from the first page on 1265.  head_dim 256 has room for one wave a SIMD only (its sums alone are 128
+// registers): a page of 128 rows takes 3.9 us, ragged prompts of up to 1500 tokens 116 us (343 TFLOP/s).
 // Keys go in times 2^K_BITS.  A scale of K_SCALE_LEAST or more is exact so, and a key's subnormal rounding stays below a
 // 2^-8th of a code's step.  Smaller ones are off by up to 2^-25, a key by 136 times that, a score (D keys, queries below
 // 2^Q_BITS) by D * 2^-6.8 of its row's scale: up to scales of 2^-4 / D that is below half a step of fp16, and only tiles

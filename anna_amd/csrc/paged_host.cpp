@@ -36,8 +36,8 @@ struct anna_mi_paged {
 namespace {
 
 // Workgroups of a launch that run at once on the 256 compute units: two on each of the split form, one of the tile
-// form.  A few more than that would leave most of the chip idle for a whole round: drafted tokens with 612 workgroups
-// 49 us, with 496 of them 42 us; 2048 tokens at the end of 32K with 512 of them 1340 us, with 256 1270 us.
+// form.  A few more than that would leave most of the chip idle for a whole round: with up to 640 and 512 of them drafted
+// tokens take 50 us, not 42, 8 sequences of 1K to 16K 27, not 24, 2048 tokens at the end of 32K 1196, not 1166.
 constexpr int64_t SPLIT_ONCE = 512, TILE_ONCE = 256;
 // Tiles of 256 rows when they fill the chip; an item of the tile form has TILE_PAGES pages at least, as its partial
 // result is written and read again; up to TILE_LEAST query rows of a KV head are the split form's.

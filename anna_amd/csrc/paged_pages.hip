@@ -8,7 +8,8 @@ namespace {
 
 // ---------------------------------------------------------------- page copies
 // A workgroup copies 16 KB (COPY_BYTES) of a page of a layer (all KV heads), 64 bytes a thread: 94 pages of 32 layers
-// (444 MB read and written) take 86 us, 5.2 TB/s; a resize with 408 of them in use 349 us, 5.5 TB/s.  Memory bounds it.
+// (444 MB read and written) take 70 us, 6.3 TB/s, some of it out of the last level's cache; a resize with 408 of them in use
+// 349 us, 5.5 TB/s.  Memory bounds it.
 __device__ __forceinline__ void copy_chunk(const uint8_t* from, uint8_t* to, int64_t page, int64_t chunk) {
   const int64_t at = chunk * COPY_BYTES + threadIdx.x * 16;
   u32x4 v[4];

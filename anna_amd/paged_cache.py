@@ -412,7 +412,8 @@ class PagedInt4Cache:
     def attend(self, layer: int, span: PagedSpan, query: torch.Tensor, *, scaling: float,
                gate: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """Causal attention for the span's tokens: query [tokens, q_heads, head_dim] over all tokens of its
-        sequence up to and with its own -> the same shape.  gate (optional, same shape as query): out *= sigmoid(gate)."""
+        sequence up to and with its own -> the same shape.  gate (optional, same shape as query): out *= sigmoid(gate).
+        out may be the query or the gate."""
         stream, here = self._check("attend", layer, span), self._here()
         capturing = torch.cuda.is_current_stream_capturing() if here else self._capturing_there()
         if here:
