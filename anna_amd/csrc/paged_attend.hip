@@ -396,13 +396,14 @@ __global__ __launch_bounds__(256, NQ * D <= 256 ? 2 : 1) void paged_split_kernel
 // of 32K (32 query heads on 8, head_dim 128): 1119 us, 952 TFLOP/s, 80% of a large product's rate (by the card, up to
 // 1200); in bf16 from the first page on 1265.  head_dim 256 has room for one wave a SIMD only (its sums alone are 128
 // registers): a page of 128 rows takes 3.9 us, ragged prompts of up to 1500 tokens 116 us (343 TFLOP/s).
-// Keys go in times 2^K_BITS.  A scale of K_SCALE_LEAST or more is exact so, and a key's subnormal rounding stays below a
-// 2^-8th of a code's step.  Smaller ones are off by up to 2^-25, a key by 136 times that, a score (D keys, queries below
-// 2^Q_BITS) by D * 2^-6.8 of its row's scale: up to scales of 2^-4 / D that is below half a step of fp16, and only tiles
-// with rows of larger ones need such keys as bf16 holds them.  (128 dims, scaling 128^-0.5: queries up to 64 do not.)
-constexpr float K_SCALE_MOST = 16.0f;  // |k| < 2^11.1
-constexpr int K_BITS = 4;
-constexpr uint32_t K_SCALE_LEAST = 0x3500;  // bf16's 2^-21
+// Keys go in times 2^K_BITS, up to 121 scales each: below 2^16.  A scale of K_SCALE_LEAST or more is exact so, and a key's
+// subnormal rounding stays below a 2^-8th of a code's step.  Smaller ones are off by up to 2^-25, a key by 121 times that, a
+// score (D keys, queries below 2^Q_BITS) by D * 2^-7 of its row's scale: with scales up to 2^-3 / D that moves a probability
+// by 2^-10.6 of itself at the very most, and only tiles with rows of larger scales need such keys as bf16 holds them.
+// (128 dims, scaling 128^-0.5: queries below 64 do not.)
+constexpr float K_SCALE_MOST = 64.0f;
+constexpr int K_BITS = 3;
+constexpr uint32_t K_SCALE_LEAST = 0x3580;  // bf16's 2^-20
 constexpr float V_SCALE_MOST = 256.0f;               // |v| < 2^15
 constexpr float V_SCALE_LEAST = 7.62939453125e-6f;   // 2^-17: exact in fp16, subnormal roundings below a 2^-8th of a code's step
 constexpr float V_SHRINK = 0.0625f;                  // in bf16: rounded, a group's largest value may be past the type's largest
@@ -773,7 +774,7 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(const Attend a) {
   // neither 0 nor infinite, as scores that are not seen are -infinity: beyond these it makes no difference to finite ones
   float scale = __builtin_amdgcn_fmed3f(ldexpf(a.scale, -shift - K_BITS), SCALE_LEAST, SCALE_MOST);
   const bool counts = largest > 0 && largest < (DT == ANNA_MI_BF16 ? 0x7F80 : 0x7C00);  // not for its row alone
-  const uint32_t key_least = __syncthreads_or(counts && scale > 0.0625f / D) ? K_SCALE_LEAST : 1;
+  const uint32_t key_least = __syncthreads_or(counts && scale > 0.125f / D) ? K_SCALE_LEAST : 1;
   auto query = [&](int s) { return qf[s]; };
 
   Rows<D> w;

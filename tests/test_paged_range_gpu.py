@@ -167,6 +167,20 @@ def test_keys_of_any_size(gpu, D, dtype, factor, as_type, count):
     check(got, q, held, 200 - count, scaling, as_type)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_keys_with_large_channels(gpu, D, dtype):
+    """Channels of keys in the hundreds, as biased projections make them: the type's own tolerance."""
+    cache = make(D=D, H=2, HQ=4, dtype=dtype)
+    k = (rows((200, 2, D), torch.float32, 1, "cpu") * 8).to(dtype)
+    seqs, held = stored(cache, k, rows((200, 2, D), dtype, 2, "cpu"))
+    assert 16 < held[2].max() < 64
+    q = rows((200, 4, D), dtype, 3, "cpu")
+    for scaling in (D ** -0.5 / 8, 1e-5):  # and with scores near 0, whose errors do not hide those of the values
+        got = cache.attend(0, cache.span(seqs, [0], [200]), q.cuda(), scaling=scaling)
+        check(got, q, held, 0, scaling, dtype)
+
+
 @pytest.mark.parametrize("dtype,factor", [(BF, 2.0 ** -26), (BF, 2.0 ** -20), (FP, 2.0 ** -20)])
 def test_a_small_group_that_alone_counts(gpu, dtype, factor):
     """Queries that are zero where the keys are large: the scores come from a group of small keys alone."""
