@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from _paged import held
-from test_paged_cache_gpu import BF, FP, check_attend, check_held, fill, make, rows
+from test_paged_cache_gpu import BF, FP, check_held, fill, make, rows
 
 pytestmark = pytest.mark.gpu
 
