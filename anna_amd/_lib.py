@@ -244,6 +244,49 @@ PROTOTYPES.update({
     "anna_mi_paged_read": [_P, _I64, _SPAN, _P, _P, _I, _P],
     "anna_mi_paged_attend": [_P, _I64, _SPAN, _P, _I64, _I64, _P, _I64, _I64, _P, _F, _I, _P],
 })
+
+
+class StateSpan(ctypes.Structure):
+    """anna_mi_state_span."""
+
+    _fields_ = [
+        ("sequences", _I64), ("tokens", _I64), ("words", _I64), ("steps", _I64), ("chains", _I64), ("chunks", _I64),
+        ("max_slot", _I64), ("buf", _P),
+    ]
+
+
+class GatedDeltaArgs(ctypes.Structure):
+    """anna_mi_gated_delta_args."""
+
+    _fields_ = [
+        ("dtype", _I), ("gates_dtype", _I), ("normalize", _I), ("scaling", _F), ("key_heads", _I64),
+        ("value_heads", _I64), ("key_dim", _I64), ("value_dim", _I64),
+        ("query", _P), ("query_stride_token", _I64), ("query_stride_head", _I64),
+        ("key", _P), ("key_stride_token", _I64), ("key_stride_head", _I64),
+        ("value", _P), ("value_stride_token", _I64), ("value_stride_head", _I64),
+        ("decay", _P), ("decay_stride", _I64), ("beta", _P), ("beta_stride", _I64), ("a_log", _P), ("dt_bias", _P),
+        ("state", _P), ("slots", _I64), ("state_stride_slot", _I64), ("out", _P), ("workspace", _P),
+    ]
+
+
+class RmsNormArgs(ctypes.Structure):
+    """anna_mi_rms_norm_args."""
+
+    _fields_ = [
+        ("dtype", _I), ("out_format", _I), ("rows", _I64), ("cols", _I64), ("group", _I64), ("x", _P), ("x_stride", _I64),
+        ("weight", _P), ("residual", _P), ("residual_stride", _I64), ("gate", _P), ("gate_stride", _I64), ("eps", _F),
+        ("weight_offset", _F), ("out", _P), ("out_stride", _I64), ("scales", _P),
+    ]
+
+
+_STATE_SPAN = ctypes.POINTER(StateSpan)
+PROTOTYPES.update({
+    "anna_mi_state_span_plan": [_I64, _P, _P, _P, _STATE_SPAN],
+    "anna_mi_state_span_fill": [_I64, _P, _P, _P, _STATE_SPAN, _P],
+    "anna_mi_gated_delta": [ctypes.POINTER(GatedDeltaArgs), _STATE_SPAN, _P],
+    "anna_mi_causal_conv1d": [_P, _I, _I64, _I64, _P, _I64, _P, _P, _I64, _I64, _I, _STATE_SPAN, _P, _I64, _P],
+    "anna_mi_rms_norm": [ctypes.POINTER(RmsNormArgs), _P],
+})
 # entry points that do not return a status code
 RAW_PROTOTYPES: dict[str, tuple] = {
     "anna_mi_sizeof_moe_mlp_args": (_I64, []),
@@ -261,6 +304,10 @@ RAW_PROTOTYPES: dict[str, tuple] = {
     "anna_mi_sizeof_tq_store_args": (_I64, []),
     "anna_mi_sizeof_paged_desc": (_I64, []),
     "anna_mi_sizeof_paged_span": (_I64, []),
+    "anna_mi_sizeof_state_span": (_I64, []),
+    "anna_mi_sizeof_gated_delta_args": (_I64, []),
+    "anna_mi_sizeof_rms_norm_args": (_I64, []),
+    "anna_mi_gated_delta_workspace": (_I64, [ctypes.POINTER(GatedDeltaArgs), _STATE_SPAN]),
     "anna_mi_tq_decode_workgroups": (_I64, [_I64, _I64, _P, _I64]),
 }
 

@@ -1,0 +1,99 @@
+// Layout of the packed tokens of sequences that continue states (anna_mi_state_span).
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "delta.hpp"
+
+namespace anna {
+
+// Sizes of a span, and with `words` its content.  Sequences of at most STEP_TOKENS tokens are taken token by
+// token, longer ones ("chains") in chunks.
+static int lay_out(int64_t n, const int32_t* slots, const int64_t* counts, const int32_t* fresh, anna_mi_state_span* s,
+                   int32_t* words) {
+  ANNA_CHECK(s != nullptr, "state span: null span");
+  ANNA_CHECK(n >= 0 && n <= INT32_MAX / 4, "state span: %lld sequences", (long long)n);
+  ANNA_CHECK(n == 0 || (slots && counts), "state span: null slots or counts");
+  int64_t tokens = 0, steps = 0, chains = 0, chunks = 0, max_slot = -1;
+  for (int64_t i = 0; i < n; i++) {
+    ANNA_CHECK(slots[i] >= -1, "state span: slot %d of sequence %lld", (int)slots[i], (long long)i);
+    ANNA_CHECK(counts[i] >= 0 && counts[i] <= INT32_MAX, "state span: sequence %lld of %lld tokens", (long long)i, (long long)counts[i]);
+    tokens += counts[i];
+    ANNA_CHECK(tokens <= INT32_MAX, "state span: more than 2^31 - 1 tokens");
+    max_slot = std::max<int64_t>(max_slot, slots[i]);
+    if (counts[i] > STEP_TOKENS) {
+      chains++;
+      chunks += (counts[i] + CHUNK - 1) / CHUNK;
+    } else if (counts[i] > 0) {
+      steps++;
+    }
+  }
+  try {
+    std::vector<int32_t> used(slots, slots + n);
+    std::sort(used.begin(), used.end());
+    for (int64_t i = 1; i < n; i++)
+      ANNA_CHECK(used[i] != used[i - 1] || used[i] < 0, "state span: slot %d is named twice", (int)used[i]);
+  } catch (const std::bad_alloc&) {
+    set_error("state span: out of host memory");
+    return ANNA_MI_EINVAL;
+  }
+  const int64_t total = 4 * n + steps + 2 * chains + 2 * chunks;
+  if (words) {
+    ANNA_CHECK(s->sequences == n && s->tokens == tokens && s->steps == steps && s->chains == chains && s->chunks == chunks &&
+                   s->words == std::max<int64_t>(1, total),
+               "state span: filled with other counts than it was planned for");
+    s->max_slot = max_slot;
+    int32_t* step = words + 4 * n;
+    int32_t* chain = step + steps;
+    int32_t* chunk = chain + 2 * chains;
+    int64_t first = 0, first_chunk = 0;
+    for (int64_t i = 0; i < n; i++) {
+      const int32_t record[4] = {slots[i], (int32_t)first, (int32_t)counts[i], fresh && fresh[i] ? 1 : 0};
+      std::copy(record, record + 4, words + 4 * i);
+      first += counts[i];
+      if (counts[i] > STEP_TOKENS) {
+        *chain++ = (int32_t)i;
+        *chain++ = (int32_t)first_chunk;
+        const int64_t m = (counts[i] + CHUNK - 1) / CHUNK;
+        for (int64_t c = 0; c < m; c++) {
+          *chunk++ = (int32_t)i;
+          *chunk++ = (int32_t)c;
+        }
+        first_chunk += m;
+      } else if (counts[i] > 0) {
+        *step++ = (int32_t)i;
+      }
+    }
+    if (total == 0) words[0] = 0;
+    return ANNA_MI_OK;
+  }
+  s->sequences = n;
+  s->tokens = tokens;
+  s->words = std::max<int64_t>(1, total);
+  s->steps = steps;
+  s->chains = chains;
+  s->chunks = chunks;
+  s->max_slot = max_slot;
+  return ANNA_MI_OK;
+}
+
+}  // namespace anna
+
+extern "C" {
+
+int anna_mi_state_span_plan(int64_t n, const int32_t* slots, const int64_t* counts, const int32_t* fresh,
+                            anna_mi_state_span* span) {
+  return anna::lay_out(n, slots, counts, fresh, span, nullptr);
+}
+
+int anna_mi_state_span_fill(int64_t n, const int32_t* slots, const int64_t* counts, const int32_t* fresh,
+                            anna_mi_state_span* span, int32_t* words) {
+  ANNA_CHECK(words != nullptr, "state span: null words");
+  return anna::lay_out(n, slots, counts, fresh, span, words);
+}
+
+int64_t anna_mi_sizeof_state_span(void) { return (int64_t)sizeof(anna_mi_state_span); }
+int64_t anna_mi_sizeof_gated_delta_args(void) { return (int64_t)sizeof(anna_mi_gated_delta_args); }
+int64_t anna_mi_sizeof_rms_norm_args(void) { return (int64_t)sizeof(anna_mi_rms_norm_args); }
+
+}  // extern "C"

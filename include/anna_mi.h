@@ -765,6 +765,88 @@ int anna_mi_paged_attend(anna_mi_paged* handle, int64_t layer, const anna_mi_pag
 int64_t anna_mi_sizeof_paged_desc(void);
 int64_t anna_mi_sizeof_paged_span(void);
 
+/* ------------------------------------------------------------- linear attention
+ * The operators of a linear-attention layer between its projections: the short causal convolution,
+ * the gated delta rule over a state of every value head, and the root-mean-square norms (the
+ * reference's SYCL library holds counterparts of a batch of equal lengths: sycl:5618-7600, 3345-3714,
+ * 1764-1986; these take packed tokens of ragged sequences whose states are rows of a pool). */
+
+/* Packed tokens of sequences, one sequence after the other, and the rows ("slots") of the state
+ * pools that they continue.  Laid out once for all layers of a step. */
+typedef struct {
+  int64_t sequences, tokens;
+  int64_t words;                  /* int32 words of buf */
+  int64_t steps, chains, chunks;  /* sequences taken token by token, in chunks of 64; chunks of all chains */
+  int64_t max_slot;               /* the largest slot, -1 without any */
+  const int32_t* buf;             /* device: [sequences][4] slot, first token, tokens, fresh; [steps] sequence;
+                                     [chains][2] sequence, first chunk; [chunks][2] sequence, chunk of it */
+} anna_mi_state_span;
+
+/* Sizes of a span of n sequences.  slots: rows of the states, each at most once, or -1 for a sequence
+ * that is computed for nobody (padding of a captured batch: its outputs are zeros); counts: tokens,
+ * 0 allowed (such a sequence's state stays as it is); fresh (may be NULL): nonzero where the state's
+ * content is taken as zeros.  fill writes the words of buf to host memory; the caller copies them.
+ * Fills of the same counts have the same sizes. */
+int anna_mi_state_span_plan(int64_t n, const int32_t* slots, const int64_t* counts, const int32_t* fresh,
+                            anna_mi_state_span* span);
+int anna_mi_state_span_fill(int64_t n, const int32_t* slots, const int64_t* counts, const int32_t* fresh,
+                            anna_mi_state_span* span, int32_t* words);
+
+/* The gated delta rule.  With k^ = k / sqrt(|k|^2 + 1e-6) and q^ = scaling * q / sqrt(|q|^2 + 1e-6) (normalize;
+ * else k and scaling * q), a value head's state S [key_dim][value_dim] takes a token by
+ *   u = beta (v - e^g S^T k^),  S <- e^g S + k^ u^T,  out = S^T q^
+ * key_dim 64 or 128; value_dim a multiple of 32 up to 256; value head h reads key head h / (value_heads /
+ * key_heads).  Rows of query, key and value are 16-byte aligned. */
+typedef struct {
+  int dtype;       /* of query, key, value and out: bf16 or fp16 */
+  int gates_dtype; /* of decay and beta: bf16, fp16 or fp32 */
+  int normalize;
+  float scaling;
+  int64_t key_heads, value_heads, key_dim, value_dim;
+  const void* query; int64_t query_stride_token, query_stride_head; /* [tokens][key_heads][key_dim] */
+  const void* key; int64_t key_stride_token, key_stride_head;
+  const void* value; int64_t value_stride_token, value_stride_head; /* [tokens][value_heads][value_dim] */
+  const void* decay; int64_t decay_stride; /* [tokens][value_heads]: g, or a where a_log is given */
+  const void* beta; int64_t beta_stride;   /* [tokens][value_heads]: beta, or its logit where a_log is given */
+  const float* a_log;   /* [value_heads] or NULL: g = -exp(a_log) softplus(a + dt_bias), beta = sigmoid(b) */
+  const float* dt_bias; /* with a_log */
+  float* state; int64_t slots, state_stride_slot; /* [slots][value_heads][key_dim][value_dim] */
+  void* out;            /* [tokens][value_heads][value_dim] */
+  void* workspace;      /* anna_mi_gated_delta_workspace bytes, 256-byte aligned (NULL for 0) */
+} anna_mi_gated_delta_args;
+
+int64_t anna_mi_gated_delta_workspace(const anna_mi_gated_delta_args* args, const anna_mi_state_span* span);
+int anna_mi_gated_delta(const anna_mi_gated_delta_args* args, const anna_mi_state_span* span, void* stream);
+int64_t anna_mi_sizeof_state_span(void);
+int64_t anna_mi_sizeof_gated_delta_args(void);
+
+/* out[t][c] = act(bias[c] + sum_j weight[c][j] x[t - width + 1 + j][c]) over a sequence's tokens, with the rows
+ * of its state [slots][width - 1][channels] (oldest first) in front of them; the state then holds the
+ * last width - 1 inputs.  width 2 to 8; x, out, weight, bias and state of one dtype (bf16, fp16, fp32);
+ * out must not overlap x.  activation: 0 none, 1 SiLU. */
+int anna_mi_causal_conv1d(const void* x, int dtype, int64_t channels, int64_t x_stride, const void* weight,
+                          int64_t width, const void* bias, void* state, int64_t slots, int64_t state_stride_slot,
+                          int activation, const anna_mi_state_span* span, void* out, int64_t out_stride, void* stream);
+
+/* y = h / sqrt(mean(h^2) + eps) * (weight + weight_offset) [* silu(gate)] of every row, with h = x, or
+ * h = x + residual, rounded to the dtype and written back to residual.  out_format 0: out in dtype; 1: out e4m3
+ * codes and scales fp32 [rows][cols / group]: scale = max|y| / 448 of the group's columns, code = e4m3(y / scale),
+ * both 0 where max|y| < 2^-100.  group: 32, 64 or 128 (a divisor of cols, rows 16-byte aligned) or cols. */
+typedef struct {
+  int dtype, out_format;
+  int64_t rows, cols, group;
+  const void* x; int64_t x_stride;
+  const void* weight;
+  void* residual; int64_t residual_stride;     /* or NULL */
+  const void* gate; int64_t gate_stride;       /* or NULL */
+  float eps, weight_offset;
+  void* out; int64_t out_stride;
+  float* scales;
+} anna_mi_rms_norm_args;
+
+int anna_mi_rms_norm(const anna_mi_rms_norm_args* args, void* stream);
+int64_t anna_mi_sizeof_rms_norm_args(void);
+
 #ifdef __cplusplus
 }
 #endif
