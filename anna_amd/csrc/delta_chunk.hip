@@ -9,12 +9,12 @@
 // one head's state and needs no other wave: columns of S, u and out depend on the same column of v only.
 //
 // Precision: the state stays fp32.  Products run on the fp16 matrix instructions with fp32 sums; an fp32
-// operand x enters as two fp16 values, hi = fp16(x / s) and lo = fp16(x / s - hi), 22 bits of it, with s a power
-// of two that brings the largest of its column (of T': of the chunk) to 2^14, so values down to 2^-28 of the
-// largest keep all 22 bits.  q and k are exact in one fp16 value once a row's power of two is taken out.
+// operand x enters as two fp16 values, hi = fp16(x / s) and lo = fp16(x / s - hi), 22 bits of it or 2^-25 where that is
+// more, with s a power of two of its column (of T': of the chunk).  q and k are exact in one fp16 value once a row's
+// power of two is taken out.
 //
-// A chunk with a token that is not finite (of the operands that a wave sees) is taken token by token: zeros above
-// the diagonals times what is not finite would reach the tokens in front of it.
+// Zeros above the diagonals times what is not finite would reach the tokens in front of it.  It also reaches the whole
+// of its column's update, where a wave sees it and then takes the chunk token by token from the state that it still has.
 //
 // Operands are held in the order of the matrix instruction's registers: fragment (mt, ks) of an M x K operand
 // gives lane (n = lane % 16, g = lane / 16) the 8 values of row (mt, n) at k = 32 ks + 8 g + 0..7.  Rows of tile mt are
@@ -33,29 +33,26 @@ __device__ __forceinline__ void t_frag(int f, int& mt, int& ks) {
   mt = ks ? f - 2 : f;
 }
 
-// Factors of a chunk and value head: of K S, of Q S, of u on its way to the state, and {e^{a_63}, scale of T', of P}
+// Factors of a chunk and value head: of K S, of Q S, of (T' / its scale) x on its way to the state, and {e^{a_63}, scale of T', of P}
 struct Factors {
   float decayed_k[CHUNK], decayed_q[CHUNK], to_end[CHUNK];
-  float end, t_scale, p_scale;
-  int not_finite;  // a q, k, g or beta of the chunk is not
-  float pad[60];
+  float end, t_scale, p_scale, pad[61];
 };
 
-// The workspace: K, Q and K^T of every chunk and key head, T' (hi, lo), P (hi, and lo for fp16) and the factors
-// of every chunk and value head
+// The workspace: K and Q of every chunk and key head, T' (hi, lo), the factors and P (hi, and lo for fp16) of every
+// chunk and value head
 template <int DK> struct Places {
   static constexpr int64_t MAT = CHUNK * DK * 2;
   char* base;
   int64_t HK, HV, chunks;
   int p_parts;
   __host__ __device__ int64_t head_bytes() const { return T_FRAGS * FRAG * (2 + p_parts) + (int64_t)sizeof(Factors); }
-  __host__ __device__ int64_t bytes() const { return chunks * (HK * 3 * MAT + HV * head_bytes()); }
-  __device__ char* k(int64_t chunk, int64_t hk) const { return base + (chunk * HK + hk) * 3 * MAT; }
+  __host__ __device__ int64_t bytes() const { return chunks * (HK * 2 * MAT + HV * head_bytes()); }
+  __device__ char* k(int64_t chunk, int64_t hk) const { return base + (chunk * HK + hk) * 2 * MAT; }
   __device__ char* q(int64_t chunk, int64_t hk) const { return k(chunk, hk) + MAT; }
-  __device__ char* kt(int64_t chunk, int64_t hk) const { return k(chunk, hk) + 2 * MAT; }
-  __device__ char* t(int64_t chunk, int64_t hv) const { return base + chunks * HK * 3 * MAT + (chunk * HV + hv) * head_bytes(); }
-  __device__ char* p(int64_t chunk, int64_t hv) const { return t(chunk, hv) + 2 * T_FRAGS * FRAG; }
-  __device__ Factors* factors(int64_t chunk, int64_t hv) const { return (Factors*)(p(chunk, hv) + p_parts * T_FRAGS * FRAG); }
+  __device__ char* t(int64_t chunk, int64_t hv) const { return base + chunks * HK * 2 * MAT + (chunk * HV + hv) * head_bytes(); }
+  __device__ Factors* factors(int64_t chunk, int64_t hv) const { return (Factors*)(t(chunk, hv) + 2 * T_FRAGS * FRAG); }
+  __device__ char* p(int64_t chunk, int64_t hv) const { return (char*)(factors(chunk, hv) + 1); }
 };
 
 // ---------------------------------------------------------------- powers of two
@@ -72,245 +69,304 @@ __device__ __forceinline__ Pow2 pow2_of(float largest) {
 __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
-// hi and lo of eight values
+// hi and lo of eight values.  The pair of hi passes through a register of its own: a value that is a product may
+// be rounded in one step or two, and lo has to be what is left of the hi that the matrix instruction gets.  `one`
+// is 1, which the compiler does not know: x - hi is then one instruction with its rounding (v_fma_mix).
 __device__ __forceinline__ void split(const float (&x)[8], f16x8& hi, f16x8& lo) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  float one = 1.f;
+  asm("" : "+s"(one));
 #pragma unroll
-  for (int e = 0; e < 8; e++) {
-    hi[e] = (_Float16)x[e];
-    lo[e] = (_Float16)(x[e] - (float)hi[e]);
+  for (int e = 0; e < 8; e += 2) {
+    f16x2 h = {(_Float16)x[e], (_Float16)x[e + 1]};
+    asm("" : "+v"(h));
+    hi[e] = h[0];
+    hi[e + 1] = h[1];
+    lo[e] = (_Float16)fmaf(x[e], one, -(float)h[0]);
+    lo[e + 1] = (_Float16)fmaf(x[e + 1], one, -(float)h[1]);
   }
 }
 
 // ---------------------------------------------------------------- what needs no state
 
+// 2^t of t <= 0, or of any t: its whole part apart, so that a long sum's fraction keeps its bits
+__device__ __forceinline__ float exp2_of(double t) {
+  const double whole = __builtin_rint(t);
+  return ldexpf(__builtin_amdgcn_exp2f((float)(t - whole)), (int)fmin(fmax(whole, -10000.), 10000.));
+}
+
+// A workgroup takes a chunk, a key head and `per` of its value heads.  A wave has the rows row_of(wave, 0..15) of K and Q,
+// which are at once their fragments and the left operands of K K^T and Q K^T.
 template <int DT, int DK>
-__global__ __launch_bounds__(256) void delta_prepare_kernel(const anna_mi_gated_delta_args a, const int32_t* __restrict__ buf,
+__global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gated_delta_args a, const int32_t* __restrict__ buf,
                                                             int64_t sequences, const int32_t* __restrict__ chunks,
-                                                            const Places<DK> ws) {
+                                                            const Places<DK> ws, int per) {
   typedef typename Elem<DT>::T T;
-  constexpr int LD = DK + 8;    // halves of a row of K and Q in LDS
-  constexpr int LF = CHUNK + 4; // floats of a row of A, T and P
-  __shared__ _Float16 K[CHUNK][LD], Q[CHUNK][LD];
-  __shared__ float A[CHUNK][LF], TI[CHUNK][LF];
-  __shared__ double at[CHUNK];  // a
-  __shared__ float kf[CHUNK], qf[CHUNK], beta[CHUNK], tops[2][4];
-  __shared__ int not_finite;
+  constexpr int KS = DK / 32;
+  constexpr int LD = DK + 8;     // halves of a row of K in LDS
+  constexpr int LF = CHUNK + 4;  // floats of a row of A, then T in its place, then P
+  __shared__ _Float16 K[CHUNK][LD];
+  __shared__ float A[CHUNK][LF];
+  __shared__ double sums[4][CHUNK];  // a / ln 2 of the next four value heads
+  __shared__ float betas[4][CHUNK], kf[CHUNK], qf[CHUNK], tops[2][4];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
-  const int64_t HV = a.value_heads, chunk = blockIdx.x / HV, hv = blockIdx.x % HV, hk = hv / (HV / a.key_heads);
-  const bool writes_k = hv % (HV / a.key_heads) == 0;
+  const uint32_t ratio = (uint32_t)a.value_heads / (uint32_t)a.key_heads, parts = (uint32_t)a.value_heads / (uint32_t)per;
+  const uint32_t chunk = blockIdx.x / parts, hv0 = blockIdx.x % parts * per, hk = hv0 / ratio;
+  const bool writes_k = hv0 % ratio == 0;
   const SpanSeq seq = ((const SpanSeq*)buf)[chunks[2 * chunk]];
   if (seq.slot < 0) return;
   const int64_t first = seq.first + (int64_t)chunks[2 * chunk + 1] * CHUNK;
   const int tokens = min(CHUNK, seq.tokens - chunks[2 * chunk + 1] * CHUNK);
-  if (tid == 0) not_finite = 0;
-  __syncthreads();
 
-  // rows of K and Q: a power of two taken out of each, what is left to make the unit vector kept as a factor
-  constexpr int RL = DK / 8, RR = 256 / RL;  // lanes of a row, rows at a time
-  for (int which = 0; which < 2; which++) {
-    const T* src = (const T*)(which ? a.query : a.key);
-    const int64_t st = which ? a.query_stride_token : a.key_stride_token, sh = which ? a.query_stride_head : a.key_stride_head;
+  const int mine = row_of(wave, n);
+  u32x4 raw[2][KS];
+  if (mine < tokens) {
+    const T* kp = (const T*)a.key + (first + mine) * a.key_stride_token + hk * a.key_stride_head + 8 * g;
+    const T* qp = (const T*)a.query + (first + mine) * a.query_stride_token + hk * a.query_stride_head + 8 * g;
 #pragma unroll
-    for (int i = 0; i < CHUNK / RR; i++) {
-      const int row = tid / RL + RR * i, c = tid % RL * 8;
-      float x[8] = {}, ss = 0.f, top = 0.f;
-      if (row < tokens) {
-        const u32x4 raw = *(const u32x4*)(src + (first + row) * st + hk * sh + c);
-        const T* h = (const T*)&raw;
+    for (int s = 0; s < KS; s++) raw[0][s] = *(const u32x4*)(kp + 32 * s);
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = Elem<DT>::to_f32(h[e]);
+    for (int s = 0; s < KS; s++) raw[1][s] = *(const u32x4*)(qp + 32 * s);
+  } else {
+#pragma unroll
+    for (int s = 0; s < KS; s++) raw[0][s] = raw[1][s] = u32x4{0, 0, 0, 0};
+  }
+
+  // decays of four value heads, a wave each: sums of logarithms in 64 bits, as their differences count; -inf stands
+  // for e^-10^4 = 0
+  auto gates = [&](int h) {
+    if (h < per) {
+      Gate gate{0.f, 0.f};
+      if (lane < tokens) gate = gate_of(a, first + lane, hv0 + h);
+      double s = gate.g < -1e4f ? -1e4 : (double)gate.g;
+#pragma unroll
+      for (int off = 1; off < 64; off *= 2) {
+        const double o = __shfl_up(s, off, 64);
+        if (lane >= off) s += o;
       }
+      sums[wave][lane] = s * 1.4426950408889634;
+      betas[wave][lane] = gate.beta;
+    }
+  };
+  gates(wave);
+
+  // a power of two is taken out of every row, and what is left to make the unit vector kept as a factor
+  f16x8 kr[KS], qr[KS];
+#pragma unroll
+  for (int which = 0; which < 2; which++) {
+    float ss = 0.f, top = 0.f, x[KS][8];
+#pragma unroll
+    for (int s = 0; s < KS; s++)
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        ss = fmaf(x[e], x[e], ss);
-        top = fmaxf(top, fabsf(x[e]));
+        const uint32_t w = raw[which][s][e / 2];
+        x[s][e] = Elem<DT>::to_f32((T)(e & 1 ? w >> 16 : w & 0xffffu));
+        ss = fmaf(x[s][e], x[s][e], ss);
+        top = fmaxf(top, fabsf(x[s][e]));
       }
+    ss += lane_xor16(ss);
+    ss += lane_xor32(ss);
+    top = fmaxf(top, lane_xor16(top));
+    top = fmaxf(top, lane_xor32(top));
+    // the largest value goes to 1 .. 2, where what fp16 rounds off the small ones, 2^-25, is below fp32's
+    // roundings of the row's products
+    const int e = top > 0.f && top < INFINITY ? 1 - __builtin_amdgcn_frexp_expf(top) : 0;
 #pragma unroll
-      for (int off = 1; off < RL; off *= 2) {
-        ss += __shfl_xor(ss, off, 64);
-        top = fmaxf(top, __shfl_xor(top, off, 64));
-      }
-      // the largest value goes to 2^8: no sum of 128 products of two rows comes near fp32's limits, and fp16 holds
-      // what is 2^-22 of the largest with all its bits
-      const int e = top > 0.f && top < INFINITY ? 8 - ilogbf(top) : 0;
-      f16x8 h8;
+    for (int s = 0; s < KS; s++)
 #pragma unroll
-      for (int j = 0; j < 8; j++) h8[j] = (_Float16)ldexpf(x[j], e);
-      *(f16x8*)&(which ? Q : K)[row][c] = h8;
-      if (tid % RL == 0) {
-        if (!isfinite(ss)) not_finite = 1;
-        const float f = ldexpf(a.normalize ? rsqrtf(ss + NORM_EPS) : 1.f, -e);
-        if (which) qf[row] = f * a.scaling;
-        else kf[row] = f;
-      }
+      for (int j = 0; j < 8; j++) (which ? qr : kr)[s][j] = (_Float16)ldexpf(x[s][j], e);
+    if (g == 0) {
+      const float f = ldexpf(a.normalize ? rsqrtf(ss + NORM_EPS) : 1.f, -e);
+      if (which) qf[mine] = f * a.scaling;
+      else kf[mine] = f;
     }
   }
-  if (wave == 0) {  // decays: sums of logarithms in 64 bits, as their differences count; -inf stands for e^-10^4 = 0
-    Gate gate{0.f, 0.f};
-    if (lane < tokens) gate = gate_of(a, first + lane, hv);
-    double s = gate.g < -1e4f ? -1e4 : (double)gate.g;
-    if (!isfinite(s) || !isfinite(gate.beta)) not_finite = 1;
 #pragma unroll
-    for (int off = 1; off < 64; off *= 2) {
-      const double o = __shfl_up(s, off, 64);
-      if (lane >= off) s += o;
+  for (int s = 0; s < KS; s++) *(f16x8*)&K[mine][32 * s + 8 * g] = kr[s];
+  if (writes_k) {
+    char* const k_to = ws.k(chunk, hk) + wave * KS * FRAG + 16 * lane;
+    char* const q_to = ws.q(chunk, hk) + wave * KS * FRAG + 16 * lane;
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      *(f16x8*)(k_to + s * FRAG) = kr[s];
+      *(f16x8*)(q_to + s * FRAG) = qr[s];
     }
-    at[lane] = s;
-    beta[lane] = gate.beta;
   }
-  for (int i = tid; i < CHUNK * LF; i += 256) (&TI[0][0])[i] = 0.f;
   __syncthreads();
 
-  // A and P, 16 rows a wave; P's rows are kept in registers until A has been used up
-  f32x4 P[4];
-  float p_top = 0.f;
-  {
-    f16x8 kr[DK / 32], qr[DK / 32];
+  // K K^T and Q K^T of the wave's rows, as far as the tokens that they see: of waves 0 and 1 the first 32
+  const int tiles = wave < 2 ? 2 : 4;
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  f32x4 kk[4] = {zero, zero, zero, zero}, qk[4] = {zero, zero, zero, zero};
 #pragma unroll
-    for (int s = 0; s < DK / 32; s++) {
-      kr[s] = *(const f16x8*)&K[16 * wave + n][32 * s + 8 * g];
-      qr[s] = *(const f16x8*)&Q[16 * wave + n][32 * s + 8 * g];
+  for (int ct = 0; ct < 4; ct++)
+    if (ct < tiles)
+#pragma unroll
+      for (int s = 0; s < KS; s++) {
+        const f16x8 col = *(const f16x8*)&K[16 * ct + n][32 * s + 8 * g];
+        kk[ct] = mfma16(kr[s], col, kk[ct]);
+        qk[ct] = mfma16(qr[s], col, qk[ct]);
+      }
+  float ki[4], qi[4];
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    ki[r] = kf[row_of(wave, 4 * g + r)];
+    qi[r] = qf[row_of(wave, 4 * g + r)];
+  }
+
+  for (int h = 0; h < per; h++) {
+    const int64_t hv = hv0 + h;
+    if (h > 0) {
+      __syncthreads();  // the head before is done with LDS
+      if (h % 4 == 0) {
+        gates(h + wave);
+        __syncthreads();
+      }
+    }
+    const double* const at = sums[h % 4];
+    const float* const beta = betas[h % 4];
+
+    // A and P; P's rows are kept in registers until A's place is free
+    f32x4 P[4];
+    float p_top = 0.f, t_top = 0.f;
+    double ai[4];
+    float bi[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      ai[r] = at[row_of(wave, 4 * g + r)];
+      bi[r] = beta[row_of(wave, 4 * g + r)];
     }
 #pragma unroll
     for (int ct = 0; ct < 4; ct++) {
-      f32x4 kk = {0.f, 0.f, 0.f, 0.f}, qk = {0.f, 0.f, 0.f, 0.f};
-      if (ct <= wave) {
-#pragma unroll
-        for (int s = 0; s < DK / 32; s++) {
-          const f16x8 col = *(const f16x8*)&K[16 * ct + n][32 * s + 8 * g];
-          kk = mfma16(kr[s], col, kk);
-          qk = mfma16(qr[s], col, qk);
-        }
-      }
       const int j = 16 * ct + n;
-      const double aj = at[j];
-      const float cj = kf[j];
+      if (ct < tiles) {
+        const double aj = at[j];
+        const float cj = kf[j];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int i = row_of(wave, 4 * g + r);
+          const float d = i >= j ? exp2_of(ai[r] - aj) * cj : 0.f;
+          A[i][j] = i > j ? bi[r] * (ki[r] * kk[ct][r]) * d : 0.f;
+          P[ct][r] = (qi[r] * qk[ct][r]) * d;
+          p_top = fmaxf(p_top, fabsf(P[ct][r]));
+        }
+      } else {
+        P[ct] = zero;
+#pragma unroll
+        for (int r = 0; r < 4; r++) A[row_of(wave, 4 * g + r)][j] = 0.f;
+      }
+    }
+    __syncthreads();
+
+    // T = (1 + A)^-1 in A's place: the diagonal blocks by substitution, a lane a column; then larger ones from
+    // products, T21 = -T22 (A21 T11)
+    if (wave == 0) {
+      float x[16];
+      const float b = beta[16 * g + n];
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        float s = i == n ? 1.f : 0.f;
+#pragma unroll
+        for (int k = 0; k < i; k++) s = fmaf(-A[16 * g + i][16 * g + k], x[k], s);
+        x[i] = s;
+        t_top = fmaxf(t_top, fabsf(s * b));
+      }
+#pragma unroll
+      for (int i = 0; i < 16; i++) A[16 * g + i][16 * g + n] = x[i];
+    }
+    __syncthreads();
+    // product of 16 x 16 blocks; the second form takes a result of the instruction as its right operand: its lane
+    // (n, g) holds the rows 4 g + r
+    auto block = [&](int lb, int lc, int rb, int rc, f32x4 c) {
+#pragma unroll
+      for (int k = 0; k < 4; k++) c = mfma4(A[16 * lb + n][16 * lc + 4 * g + k], A[16 * rb + 4 * g + k][16 * rc + n], c);
+      return c;
+    };
+    auto times = [&](int lb, int lc, f32x4 x, f32x4 c) {
+#pragma unroll
+      for (int k = 0; k < 4; k++) c = mfma4(A[16 * lb + n][16 * lc + 4 * g + k], x[k], c);
+      return c;
+    };
+    auto put = [&](int rb, int cb, f32x4 y) {
+      const float b = beta[16 * cb + n];
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        const int i = 16 * wave + 4 * g + r;
-        const float d = i >= j ? expf((float)(at[i] - aj)) : 0.f;
-        A[i][j] = i > j ? beta[i] * d * (kf[i] * kk[r] * cj) : 0.f;
-        P[ct][r] = i >= j ? d * (qf[i] * qk[r] * cj) : 0.f;
-        p_top = fmaxf(p_top, fabsf(P[ct][r]));
+        A[16 * rb + 4 * g + r][16 * cb + n] = -y[r];
+        t_top = fmaxf(t_top, fabsf(y[r] * b));
+      }
+    };
+    if (wave < 2) {
+      const int b = 2 * wave;
+      const f32x4 y = times(b + 1, b + 1, block(b + 1, b, b, b, zero), zero);
+      put(b + 1, b, y);
+    }
+    __syncthreads();
+    {
+      const int b = wave & 1, row = 2 + (wave >> 1);  // block column, block row of the result
+      f32x4 x2 = zero, x3 = zero;
+      for (int c = b; c < 2; c++) {
+        x2 = block(2, c, c, b, x2);
+        x3 = block(3, c, c, b, x3);
+      }
+      f32x4 y = times(row, 2, x2, zero);
+      if (row == 3) y = times(row, 3, x3, y);
+      __syncthreads();  // A21 is read
+      put(row, b, y);
+    }
+    t_top = wave_max(t_top);
+    p_top = wave_max(p_top);
+    if (lane == 0) {
+      tops[0][wave] = t_top;
+      tops[1][wave] = p_top;
+    }
+    __syncthreads();
+    const Pow2 ts = pow2_of(fmaxf(fmaxf(tops[0][0], tops[0][1]), fmaxf(tops[0][2], tops[0][3])));
+    const Pow2 ps = pow2_of(fmaxf(fmaxf(tops[1][0], tops[1][1]), fmaxf(tops[1][2], tops[1][3])));
+    char* const t_to = ws.t(chunk, hv);
+    char* const p_to = ws.p(chunk, hv);
+    for (int f = wave; f < T_FRAGS; f += 4) {
+      int mt, ks;
+      t_frag(f, mt, ks);
+      const int i = row_of(mt, n), j = 32 * ks + 8 * g;
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = A[i][j + e] * beta[j + e] * ts.down;
+      f16x8 hi, lo;
+      split(x, hi, lo);
+      *(f16x8*)(t_to + (2 * f) * FRAG + 16 * lane) = hi;
+      *(f16x8*)(t_to + (2 * f + 1) * FRAG + 16 * lane) = lo;
+    }
+    if (tid < CHUNK) {
+      Factors* to = ws.factors(chunk, hv);
+      const float e = exp2_of(at[tid]);
+      to->decayed_k[tid] = e * kf[tid];
+      to->decayed_q[tid] = e * qf[tid];
+      to->to_end[tid] = exp2_of(at[CHUNK - 1] - at[tid]) * kf[tid] * ts.up;
+      if (tid == CHUNK - 1) to->end = e;
+      if (tid == 0) {
+        to->t_scale = ts.up;
+        to->p_scale = ps.up;
       }
     }
-  }
-  __syncthreads();
-
-  // (1 + A)^-1: the diagonal blocks by substitution, a lane a column; then larger ones from products,
-  // T21 = -T22 (A21 T11)
-  if (wave == 0) {
-    float x[16];
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-      float s = i == n ? 1.f : 0.f;
-#pragma unroll
-      for (int k = 0; k < i; k++) s = fmaf(-A[16 * g + i][16 * g + k], x[k], s);
-      x[i] = s;
-      TI[16 * g + i][16 * g + n] = s;
-    }
-  }
-  __syncthreads();
-  // product of 16 x 16 blocks in LDS; the second form takes a result of the instruction as its right operand: its lane
-  // (n, g) holds the rows 4 g + r
-  auto block = [&](const float (*L)[LF], int lb, int lc, const float (*R)[LF], int rb, int rc, f32x4 c) {
-#pragma unroll
-    for (int k = 0; k < 4; k++) c = mfma4(L[16 * lb + n][16 * lc + 4 * g + k], R[16 * rb + 4 * g + k][16 * rc + n], c);
-    return c;
-  };
-  auto times = [&](const float (*L)[LF], int lb, int lc, f32x4 x, f32x4 c) {
-#pragma unroll
-    for (int k = 0; k < 4; k++) c = mfma4(L[16 * lb + n][16 * lc + 4 * g + k], x[k], c);
-    return c;
-  };
-  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  if (wave < 2) {
-    const int b = 2 * wave;
-    const f32x4 x = block(A, b + 1, b, TI, b, b, zero), y = times(TI, b + 1, b + 1, x, zero);
-#pragma unroll
-    for (int r = 0; r < 4; r++) TI[16 * (b + 1) + 4 * g + r][16 * b + n] = -y[r];
-  }
-  __syncthreads();
-  {
-    const int b = wave & 1, row = 2 + (wave >> 1);  // block column, block row of the result
-    f32x4 x2 = zero, x3 = zero;
-    for (int c = b; c < 2; c++) {
-      x2 = block(A, 2, c, TI, c, b, x2);
-      x3 = block(A, 3, c, TI, c, b, x3);
-    }
-    f32x4 y = times(TI, row, 2, x2, zero);
-    if (row == 3) y = times(TI, row, 3, x3, y);
-    __syncthreads();  // A and T11, T22 are read
-#pragma unroll
-    for (int r = 0; r < 4; r++) TI[16 * row + 4 * g + r][16 * b + n] = -y[r];
+    __syncthreads();
 #pragma unroll
     for (int ct = 0; ct < 4; ct++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) A[16 * wave + 4 * g + r][16 * ct + n] = P[ct][r];  // P in A's place
-  }
-  __syncthreads();
-
-  float t_top = 0.f;
-  for (int i = tid; i < CHUNK * CHUNK; i += 256) t_top = fmaxf(t_top, fabsf(TI[i / CHUNK][i % CHUNK] * beta[i % CHUNK]));
-  t_top = wave_max(t_top);
-  p_top = wave_max(p_top);
-  if (lane == 0) {
-    tops[0][wave] = t_top;
-    tops[1][wave] = p_top;
-  }
-  __syncthreads();
-  const Pow2 ts = pow2_of(fmaxf(fmaxf(tops[0][0], tops[0][1]), fmaxf(tops[0][2], tops[0][3])));
-  const Pow2 ps = pow2_of(fmaxf(fmaxf(tops[1][0], tops[1][1]), fmaxf(tops[1][2], tops[1][3])));
-
-  char* const t_to = ws.t(chunk, hv);
-  char* const p_to = ws.p(chunk, hv);
-  for (int f = wave; f < T_FRAGS; f += 4) {
-    int mt, ks;
-    t_frag(f, mt, ks);
-    const int i = row_of(mt, n), j = 32 * ks + 8 * g;
-    float x[8], y[8];
+      for (int r = 0; r < 4; r++) A[row_of(wave, 4 * g + r)][16 * ct + n] = P[ct][r];
+    __syncthreads();
+    for (int f = wave; f < T_FRAGS; f += 4) {
+      int mt, ks;
+      t_frag(f, mt, ks);
+      const int i = row_of(mt, n), j = 32 * ks + 8 * g;
+      float y[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      x[e] = TI[i][j + e] * beta[j + e] * ts.down;
-      y[e] = A[i][j + e] * ps.down;
+      for (int e = 0; e < 8; e++) y[e] = A[i][j + e] * ps.down;
+      f16x8 hi, lo;
+      split(y, hi, lo);
+      *(f16x8*)(p_to + ws.p_parts * f * FRAG + 16 * lane) = hi;
+      if (ws.p_parts == 2) *(f16x8*)(p_to + (2 * f + 1) * FRAG + 16 * lane) = lo;
     }
-    f16x8 hi, lo;
-    split(x, hi, lo);
-    *(f16x8*)(t_to + (2 * f) * FRAG + 16 * lane) = hi;
-    *(f16x8*)(t_to + (2 * f + 1) * FRAG + 16 * lane) = lo;
-    split(y, hi, lo);
-    *(f16x8*)(p_to + ws.p_parts * f * FRAG + 16 * lane) = hi;
-    if (ws.p_parts == 2) *(f16x8*)(p_to + (2 * f + 1) * FRAG + 16 * lane) = lo;
-  }
-  if (tid < CHUNK) {
-    Factors* to = ws.factors(chunk, hv);
-    const float e = expf((float)at[tid]);
-    to->decayed_k[tid] = e * kf[tid];
-    to->decayed_q[tid] = e * qf[tid];
-    to->to_end[tid] = expf((float)(at[CHUNK - 1] - at[tid])) * kf[tid];
-    if (tid == 0) {
-      to->end = expf((float)at[CHUNK - 1]);
-      to->t_scale = ts.up;
-      to->p_scale = ps.up;
-      to->not_finite = not_finite;
-    }
-  }
-  if (!writes_k) return;
-  char* const k_to = ws.k(chunk, hk);
-  char* const q_to = ws.q(chunk, hk);
-  char* const kt_to = ws.kt(chunk, hk);
-  for (int f = wave; f < 4 * (DK / 32); f += 4) {
-    const int mt = f / (DK / 32), ks = f % (DK / 32), i = row_of(mt, n), d = 32 * ks + 8 * g;
-    *(f16x8*)(k_to + f * FRAG + 16 * lane) = *(const f16x8*)&K[i][d];
-    *(f16x8*)(q_to + f * FRAG + 16 * lane) = *(const f16x8*)&Q[i][d];
-  }
-  for (int f = wave; f < DK / 16 * 2; f += 4) {
-    const int mt = f / 2, ks = f % 2, d = row_of(mt, n), i = 32 * ks + 8 * g;
-    f16x8 h;
-#pragma unroll
-    for (int e = 0; e < 8; e++) h[e] = K[i + e][d];
-    *(f16x8*)(kt_to + f * FRAG + 16 * lane) = h;
   }
 }
 
@@ -323,9 +379,9 @@ __device__ __forceinline__ float column_max(float v) {
   v = fmaxf(v, lane_xor16(v));
   return fmaxf(v, lane_xor32(v));
 }
-// Tiles 2 s and 2 s + 1 of a product's result as the operand of the next: hi and lo of x * down
-__device__ __forceinline__ void operand(f32x4 x, f32x4 y, float down, f16x8& hi, f16x8& lo) {
-  const float f[8] = {x[0] * down, x[1] * down, x[2] * down, x[3] * down, y[0] * down, y[1] * down, y[2] * down, y[3] * down};
+// Tiles 2 s and 2 s + 1 of a product's result as the operand of the next
+__device__ __forceinline__ void operand(f32x4 x, f32x4 y, f16x8& hi, f16x8& lo) {
+  const float f[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
   split(f, hi, lo);
 }
 __device__ __forceinline__ float largest(const f32x4& x) { return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))); }
@@ -370,163 +426,386 @@ __device__ __forceinline__ void delta_tokens(const anna_mi_gated_delta_args& a, 
   }
 }
 
-template <int DT, int DK>
-__global__ __launch_bounds__(64) void delta_chain_kernel(const anna_mi_gated_delta_args a, const int32_t* __restrict__ buf,
-                                                         int64_t sequences, const int32_t* __restrict__ chains,
-                                                         const Places<DK> ws) {
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef const __attribute__((address_space(1))) void* global_ptr;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+
+// Four 16-bit values of a column: of every 16 lanes, lane j brings 8 bytes of row j / 4, columns 4 (j % 4) .., and
+// takes column j of the four rows
+__device__ __forceinline__ s16x4 read_column(const char* p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)p); }
+
+// A workgroup of CW groups of 16 columns.  Its LDS: two chunks' operands of the state (K, T', the factors, v), two of
+// the output (Q, the factors, P), and with SPLIT what a state's wave hands to the output's.
+//   SPLIT: a wave for the state and one for the output of every column group, the output's a chunk behind, and one
+//     wave that copies operands from the workspace into LDS a chunk ahead.  For few sequences: the chain of states is
+//     all that counts, and what is not in it runs beside it.
+//   else: a wave for every column group, that takes the output too, and one for the copies.
+template <int DT, int DK, int CW, bool SPLIT> struct Stage {
+  static constexpr bool EXACT_OUT = DT == ANNA_MI_F16;  // an fp16 output shows the second parts of its operands
+  static constexpr int PARTS = EXACT_OUT ? 2 : 1, KS = DK / 32;
+  static constexpr int MAT = CHUNK * DK * 2, TS = 2 * T_FRAGS * FRAG, PS = PARTS * T_FRAGS * FRAG, FAC = (int)sizeof(Factors);
+  static constexpr int TILE = 16 * (CHUNK * 2 + 8);  // of v [64][16], and of the output's columns [16][64 + 4]
+  static constexpr int STATE = MAT + TS + FAC + CW * TILE;  // K, T', factors, v
+  static constexpr int OUT = MAT + (SPLIT ? FAC : 0) + PS;  // Q, factors, P
+  static constexpr int MAIL = SPLIT ? PARTS * (KS + 2) * FRAG + 256 + 64 : 0;  // S, u; their unit a lane; a flag
+  static constexpr int MAILS = 2 * STATE + 2 * OUT, TILES = MAILS + 2 * CW * MAIL, TOUCHED = TILES + (SPLIT ? CW * TILE : 0);
+  static constexpr int COPIERS = SPLIT && CW == 1 ? 2 : 1, FIRST_COPIER = (SPLIT ? 2 : 1) * CW;
+  static constexpr int WAVES = FIRST_COPIER + COPIERS, BYTES = TOUCHED + COPIERS * 256;
+};
+
+template <int DT, int DK, int CW, bool SPLIT>
+__global__ __launch_bounds__((64 * Stage<DT, DK, CW, SPLIT>::WAVES), 2) void delta_chain_kernel(
+    const anna_mi_gated_delta_args a, const int32_t* __restrict__ buf, int64_t sequences, const int32_t* __restrict__ chains,
+    const Places<DK> ws, uint32_t units) {
   typedef typename Elem<DT>::T T;
+  typedef Stage<DT, DK, CW, SPLIT> St;
   constexpr int NT = DK / 16, KS = DK / 32;
-  constexpr bool EXACT_OUT = DT == ANNA_MI_F16;  // an fp16 output shows the second parts of its operands
-  const int lane = threadIdx.x, n = lane & 15, g = lane >> 4;
+  constexpr bool EXACT_OUT = St::EXACT_OUT;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t HV = a.value_heads, DV = a.value_dim;
-  const int slices = (int)(DV / 16);
-  const int64_t item = blockIdx.x / slices, hv = item % HV, hk = hv / (HV / a.key_heads);
-  const int64_t col = blockIdx.x % slices * 16 + n;
-  const int32_t* chain = chains + 2 * (item / HV);
+  // a key head's workgroups on one XCD (workgroup b runs on XCD b % 8), whose L2 then has K and Q once for all of them,
+  // and T' and P for a value head's slices
+  const uint32_t ratio = (uint32_t)HV / (uint32_t)a.key_heads, slices = (uint32_t)DV / (16 * CW), each = ratio * slices;
+  const uint32_t unit_of = blockIdx.x / (8 * each) * 8 + blockIdx.x % 8, part = blockIdx.x / 8 % each;
+  if (unit_of >= units) return;
+  const uint32_t hk = unit_of % (uint32_t)a.key_heads, hv = hk * ratio + part / slices, col0 = part % slices * (16 * CW);
+  const int32_t* chain = chains + 2 * (unit_of / (uint32_t)a.key_heads);
   const SpanSeq seq = ((const SpanSeq*)buf)[chain[0]];
-  T* const out = (T*)a.out + hv * DV + col;
+  const int64_t chunk0 = chain[1];
+  const int count = (seq.tokens + CHUNK - 1) / CHUNK;
   if (seq.slot < 0) {
-    for (int t = g; t < seq.tokens; t += 4) out[(seq.first + (int64_t)t) * HV * DV] = Elem<DT>::cvt(0.f);
+    for (int64_t i = threadIdx.x; i < (int64_t)seq.tokens * 16 * CW; i += 64 * St::WAVES)
+      ((T*)a.out)[((seq.first + i / (16 * CW)) * HV + hv) * DV + col0 + i % (16 * CW)] = Elem<DT>::cvt(0.f);
     return;
   }
-  float* const state = a.state + seq.slot * a.state_stride_slot + hv * DK * DV + col;
+
+  // ---- copies of the operands, one piece of FRAG bytes an instruction, the pieces dealt to COPIERS waves
+  int piece = 0;
+  auto copy = [&](const char* from, int to, int bytes) {
+#pragma unroll
+    for (int i = 0; i < bytes; i += FRAG)
+      if (piece++ % St::COPIERS == wave - St::FIRST_COPIER)
+        __builtin_amdgcn_global_load_lds((global_ptr)(from + i + 16 * lane), (lds_ptr)(lds + to + i), 16, 0, 0);
+  };
+  auto fetch_state = [&](int c) {
+    const int to = (c & 1) * St::STATE;
+    piece = 0;
+    copy(ws.k(chunk0 + c, hk), to, St::MAT);
+    copy(ws.t(chunk0 + c, hv), to + St::MAT, St::TS + St::FAC);
+    const int tokens = min(CHUNK, seq.tokens - c * CHUNK);
+    const T* v = (const T*)a.value + (seq.first + (int64_t)c * CHUNK) * a.value_stride_token + hv * a.value_stride_head + col0;
+#pragma unroll
+    for (int i = 0; i < 2 * CW; i++)
+      if (piece++ % St::COPIERS == wave - St::FIRST_COPIER) {
+        // rows behind the last token hold the last one's again; their row of T' is zero
+        const int t = min(32 * (i & 1) + lane / 2, tokens - 1);
+        __builtin_amdgcn_global_load_lds((global_ptr)(v + t * a.value_stride_token + 16 * (i >> 1) + 8 * (lane & 1)),
+                                         (lds_ptr)(lds + to + St::MAT + St::TS + St::FAC + (i >> 1) * St::TILE + (i & 1) * FRAG), 16, 0, 0);
+      }
+  };
+  auto fetch_out = [&](int c) {
+    const int to = 2 * St::STATE + (c & 1) * St::OUT;
+    copy(ws.q(chunk0 + c, hk), to, St::MAT);
+    if constexpr (SPLIT) copy((const char*)ws.factors(chunk0 + c, hv), to + St::MAT, St::FAC + St::PS);
+    else copy(ws.p(chunk0 + c, hv), to + St::MAT, St::PS);
+  };
+  if (wave >= St::FIRST_COPIER) {
+    // A chunk's time is short of memory's latency: a word of each line of the chunk after the next is asked for, which
+    // brings the line to L2.  A value head's workgroups share its lines among them.  The words go to a corner of LDS that nobody
+    // reads.
+    constexpr int TOUCHES = CW == 1 ? 1 : CW == 2 ? 2 : 4;
+    constexpr int LK = St::MAT / 128, LT = LK + (St::TS + St::FAC) / 128, LQ = LT + St::MAT / 128, LP = LQ + St::PS / 128;
+    auto touch = [&](int c) {
+      c = min(c, count - 1);
+      const char *const k = ws.k(chunk0 + c, hk), *const t = ws.t(chunk0 + c, hv), *const q = ws.q(chunk0 + c, hk), *const p = ws.p(chunk0 + c, hv);
+#pragma unroll
+      for (int i = 0; i < TOUCHES; i++) {
+        const int line = (i * slices + part % slices) * 64 + lane;
+        const char* at = line < LK ? k + 128 * line : line < LT ? t + 128 * (line - LK) : line < LQ ? q + 128 * (line - LT) : p + 128 * min(line - LQ, LP - LQ - 1);
+        __builtin_amdgcn_global_load_lds((global_ptr)at, (lds_ptr)(lds + St::TOUCHED + 256 * (wave - St::FIRST_COPIER)), 4, 0, 0);
+      }
+    };
+    // the newest are the words, of the first copier alone
+    auto wait = [&] {
+      if (wave == St::FIRST_COPIER) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(TOUCHES) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    fetch_state(0);
+    if constexpr (!SPLIT) fetch_out(0);
+    if (wave == St::FIRST_COPIER) touch(1);
+    for (int c = 0; c < count + SPLIT; c++) {
+      wait();
+      if (c + 1 < count) {
+        fetch_state(c + 1);
+        if constexpr (!SPLIT) fetch_out(c + 1);
+      }
+      if constexpr (SPLIT)
+        if (c < count) fetch_out(c);
+      if (wave == St::FIRST_COPIER) touch(c + 2);
+    }
+    return;
+  }
+  // chunk c (the output's waves: c - 1) is in LDS, and nobody reads the one before any more
+  auto meet = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+
+  const int cg = wave % CW;
+  const uint32_t col = col0 + 16 * cg + n;
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  // A wave that takes everything has the registers for it if operands are not asked for earlier than this
+#define PHASE() __builtin_amdgcn_sched_barrier(0)
+
+  // ---- out = e^a Q S + P u
+  auto load_q = [&](const char* at, f16x8 (&Q)[4 * KS]) {
+#pragma unroll
+    for (int f = 0; f < 4 * KS; f++) Q[f] = frag(at, f, lane);
+  };
+  auto q_times = [&](const f16x8 (&Q)[4 * KS], const f16x8 (&sh)[KS], const f16x8 (&sl)[KS], f32x4 (&qs)[4]) {
+#pragma unroll
+    for (int mt = 0; mt < 4; mt++) qs[mt] = zero;
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      if constexpr (EXACT_OUT)
+#pragma unroll
+        for (int mt = 0; mt < 4; mt++) qs[mt] = mfma16(Q[mt * KS + s], sl[s], qs[mt]);
+#pragma unroll
+      for (int mt = 0; mt < 4; mt++) qs[mt] = mfma16(Q[mt * KS + s], sh[s], qs[mt]);
+    }
+  };
+  auto load_p = [&](const char* at, const Factors* fac, f16x8 (&PF)[St::PARTS * T_FRAGS], f32x4 (&fq)[4]) {
+#pragma unroll
+    for (int f = 0; f < St::PARTS * T_FRAGS; f++) PF[f] = frag(at, f, lane);
+#pragma unroll
+    for (int mt = 0; mt < 4; mt++) fq[mt] = *(const f32x4*)&fac->decayed_q[row_of(mt, 4 * g)];
+  };
+  auto finish = [&](int c, const f16x8 (&PF)[St::PARTS * T_FRAGS], const f32x4 (&fq)[4], const f16x8 (&uh)[2], const f16x8 (&ul)[2],
+                    const f32x4 (&qs)[4], float unit, float p_scale, char* tile) {
+    f32x4 o[4] = {zero, zero, zero, zero};
+#pragma unroll
+    for (int part = EXACT_OUT ? 0 : 2; part < 3; part++)
+#pragma unroll
+      for (int f = 0; f < T_FRAGS; f++) {
+        const int s = f >= 4, mt = s ? f - 2 : f;
+        o[mt] = mfma16(PF[St::PARTS * f + (part == 0)], part == 1 ? ul[s] : uh[s], o[mt]);
+      }
+    // through LDS by columns, so that a lane takes a token's row of 32 bytes
+#pragma unroll
+    for (int mt = 0; mt < 4; mt++) {
+      uint32_t w[2];
+#pragma unroll
+      for (int r = 0; r < 4; r += 2) {
+        const float y0 = fmaf(o[mt][r], p_scale, fq[mt][r] * qs[mt][r]), y1 = fmaf(o[mt][r + 1], p_scale, fq[mt][r + 1] * qs[mt][r + 1]);
+        w[r / 2] = (uint32_t)Elem<DT>::cvt(y0 * unit) | (uint32_t)Elem<DT>::cvt(y1 * unit) << 16;
+      }
+      *(uint2*)(tile + n * (CHUNK * 2 + 8) + 2 * row_of(mt, 4 * g)) = make_uint2(w[0], w[1]);
+    }
+    s16x4 row[4];
+#pragma unroll
+    for (int b = 0; b < 4; b++) row[b] = read_column(tile + (4 * b + n / 4) * (CHUNK * 2 + 8) + 2 * (16 * g + 4 * (n % 4)));
+    const int tokens = min(CHUNK, seq.tokens - c * CHUNK);
+    if (lane < tokens) {
+      T* const to = (T*)a.out + ((seq.first + (int64_t)c * CHUNK + lane) * HV + hv) * DV + col0 + 16 * cg;
+      *(u32x4*)to = __builtin_bit_cast(u32x4, __builtin_shufflevector(row[0], row[1], 0, 1, 2, 3, 4, 5, 6, 7));
+      *(u32x4*)(to + 8) = __builtin_bit_cast(u32x4, __builtin_shufflevector(row[2], row[3], 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  };
+
+  if constexpr (SPLIT) {
+    if (wave >= CW) {
+      meet();
+      for (int c = 0; c < count; c++) {
+        meet();
+        const char *const st = lds + 2 * St::STATE + (c & 1) * St::OUT, *const mail = lds + St::MAILS + (2 * cg + (c & 1)) * St::MAIL;
+        const Factors* const fac = (const Factors*)(st + St::MAT);
+        f16x8 sh[KS], sl[KS], uh[2], ul[2], Q[4 * KS], PF[St::PARTS * T_FRAGS];
+        f32x4 qs[4], fq[4];
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+          sh[s] = frag(mail, s, lane);
+          if constexpr (EXACT_OUT) sl[s] = frag(mail, KS + 2 + s, lane);
+        }
+        load_q(st, Q);
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+          uh[s] = frag(mail, KS + s, lane);
+          if constexpr (EXACT_OUT) ul[s] = frag(mail, 2 * KS + 2 + s, lane);
+        }
+        const float unit = *(const float*)(mail + St::PARTS * (KS + 2) * FRAG + 4 * lane);
+        const int taken = *(const int*)(mail + St::PARTS * (KS + 2) * FRAG + 256);
+        load_p(st + St::MAT + St::FAC, fac, PF, fq);
+        const float p_scale = fac->p_scale;
+        if (taken) continue;  // token by token, by the state's wave
+        q_times(Q, sh, sl, qs);
+        finish(c, PF, fq, uh, ul, qs, unit, p_scale, lds + St::TILES + cg * St::TILE);
+      }
+      return;
+    }
+  }
+
+  // ---- the state
+  float* const state = a.state + seq.slot * a.state_stride_slot + (int64_t)hv * DK * DV + col;
   f32x4 S[NT];
 #pragma unroll
   for (int t = 0; t < NT; t++)
 #pragma unroll
     for (int r = 0; r < 4; r++) S[t][r] = seq.fresh ? 0.f : state[row_of(t, 4 * g + r) * DV];
+  // S, x and u of a column are held in its unit, a power of two, kept so that the largest of S and v is 2^3 to 2^11:
+  // what is computed from them is then short of fp16's upper end, and 2^-25 below their roundings
+  float unit = 1.f, per_unit = 1.f;
+  bool lost = false;  // the column is not finite any more
 
-  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  const int count = (seq.tokens + CHUNK - 1) / CHUNK;
   for (int c = 0; c < count; c++) {
-    const int64_t chunk = chain[1] + (int64_t)c, first = seq.first + (int64_t)c * CHUNK;
-    const int tokens = min(CHUNK, seq.tokens - c * CHUNK);
-    const char *kf = ws.k(chunk, hk), *qf = ws.q(chunk, hk), *ktf = ws.kt(chunk, hk), *tf = ws.t(chunk, hv), *pf = ws.p(chunk, hv);
-    const Factors* fac = ws.factors(chunk, hv);
-    float v[4][4], zeros = 0.f;
+    meet();
+    const char* const st = lds + (c & 1) * St::STATE;
+    const char* const so = lds + 2 * St::STATE + (c & 1) * St::OUT;
+    char* const mail = lds + St::MAILS + (2 * cg + (c & 1)) * St::MAIL;
+    const Factors* const fac = (const Factors*)(st + St::MAT + St::TS);
+    char* const tile = lds + (c & 1) * St::STATE + St::MAT + St::TS + St::FAC + cg * St::TILE;
+    s16x4 v[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; mt++) v[mt] = read_column(tile + 32 * (row_of(mt, 4 * g) + n / 4) + 8 * (n % 4));
+    f16x8 K[4 * KS];
+#pragma unroll
+    for (int f = 0; f < 4 * KS; f++) K[f] = frag(st, f, lane);
+    f32x4 fk[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; mt++) fk[mt] = *(const f32x4*)&fac->decayed_k[row_of(mt, 4 * g)];
+    f32x4 x[4];
+    float top = 0.f, v_top = 0.f;
+#pragma unroll
+    for (int t = 0; t < NT; t++) top = fmaxf(top, largest(S[t]));
+#pragma unroll
+    for (int mt = 0; mt < 4; mt++) {
+#pragma unroll
+      for (int r = 0; r < 4; r++) x[mt][r] = Elem<DT>::to_f32((T)v[mt][r]);
+      v_top = fmaxf(v_top, largest(x[mt]));
+    }
+    top = column_max(fmaxf(top, v_top * per_unit));
+    if (__any(top > 2048.f || (top < 8.f && top > 0.f))) {
+      const uint32_t e = min(max((__float_as_uint(top) >> 23) & 255u, 10u), 250u);
+      const float up = __uint_as_float((e - 7u) << 23);  // the largest becomes 2^7
+      const bool change = (top > 2048.f || top < 8.f) && unit * up >= 0x1p-100f && unit * up <= 0x1p100f;
+      const float down = change ? __uint_as_float((261u - e) << 23) : 1.f;
+      unit *= change ? up : 1.f;
+      per_unit *= down;
+#pragma unroll
+      for (int t = 0; t < NT; t++) S[t] *= down;
+    }
+    // K S
+    f16x8 sh[KS], sl[KS];
+#pragma unroll
+    for (int s = 0; s < KS; s++) operand(S[2 * s], S[2 * s + 1], sh[s], sl[s]);
+    f32x4 ks[4] = {zero, zero, zero, zero}, qs[4];
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+#pragma unroll
+      for (int mt = 0; mt < 4; mt++) ks[mt] = mfma16(K[mt * KS + s], sl[s], ks[mt]);
+#pragma unroll
+      for (int mt = 0; mt < 4; mt++) ks[mt] = mfma16(K[mt * KS + s], sh[s], ks[mt]);
+    }
+    f16x8 TF[2 * T_FRAGS];
+#pragma unroll
+    for (int f = 0; f < 2 * T_FRAGS; f++) TF[f] = frag(st + St::MAT, f, lane);
+    f32x4 fe[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; mt++) fe[mt] = *(const f32x4*)&fac->to_end[row_of(mt, 4 * g)];
+    const float t_scale = fac->t_scale, end = fac->end;
+    if constexpr (SPLIT) {
+#pragma unroll
+      for (int s = 0; s < KS; s++) {
+        *(f16x8*)(mail + s * FRAG + 16 * lane) = sh[s];
+        if constexpr (EXACT_OUT) *(f16x8*)(mail + (KS + 2 + s) * FRAG + 16 * lane) = sl[s];
+      }
+    }
+    if constexpr (!SPLIT) {
+      PHASE();
+      f16x8 Q[4 * KS];
+      load_q(so, Q);
+      q_times(Q, sh, sl, qs);
+      PHASE();
+    }
+    // x = v - e^a K S
 #pragma unroll
     for (int mt = 0; mt < 4; mt++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int t = row_of(mt, 4 * g + r);
-        v[mt][r] = t < tokens ? Elem<DT>::load((const T*)a.value, (first + t) * a.value_stride_token + hv * a.value_stride_head + col) : 0.f;
-        zeros = fmaf(v[mt][r], 0.f, zeros);
-      }
-    if (fac->not_finite || __any(zeros != 0.f)) {  // a NaN differs from 0 too
-      delta_tokens<DT, DK>(a, first, tokens, hv, hk, col, g, S);
-      continue;
-    }
-
-    // K S and Q S
-    float top = 0.f;
-#pragma unroll
-    for (int t = 0; t < NT; t++) top = fmaxf(top, largest(S[t]));
-    const Pow2 ss = pow2_of(column_max(top));
-    f32x4 ks[4] = {zero, zero, zero, zero}, qs[4] = {zero, zero, zero, zero};
-#pragma unroll
-    for (int s = 0; s < KS; s++) {
-      f16x8 hi, lo;
-      operand(S[2 * s], S[2 * s + 1], ss.down, hi, lo);
-#pragma unroll
-      for (int mt = 0; mt < 4; mt++) {
-        const f16x8 k = frag(kf, mt * KS + s, lane), q = frag(qf, mt * KS + s, lane);
-        ks[mt] = mfma16(k, hi, ks[mt]);
-        ks[mt] = mfma16(k, lo, ks[mt]);
-        qs[mt] = mfma16(q, hi, qs[mt]);
-        if constexpr (EXACT_OUT) qs[mt] = mfma16(q, lo, qs[mt]);
-      }
-    }
-    // v - e^a K S
-    f32x4 x[4];
-    top = 0.f;
-#pragma unroll
-    for (int mt = 0; mt < 4; mt++) {
-      const f32x4 f = *(const f32x4*)&fac->decayed_k[row_of(mt, 4 * g)];
-#pragma unroll
-      for (int r = 0; r < 4; r++) x[mt][r] = fmaf(-f[r] * ss.up, ks[mt][r], v[mt][r]);
-      top = fmaxf(top, largest(x[mt]));
-    }
-    // u = T' x
-    const Pow2 xs = pow2_of(column_max(top));
-    f32x4 u[4] = {zero, zero, zero, zero};
-    {
-      f16x8 hi[2], lo[2];
-      operand(x[0], x[1], xs.down, hi[0], lo[0]);
-      operand(x[2], x[3], xs.down, hi[1], lo[1]);
-#pragma unroll
-      for (int f = 0; f < T_FRAGS; f++) {
-        const int s = f >= 4, mt = s ? f - 2 : f;
-        const f16x8 th = frag(tf, 2 * f, lane), tl = frag(tf, 2 * f + 1, lane);
-        u[mt] = mfma16(tl, hi[s], u[mt]);
-        u[mt] = mfma16(th, lo[s], u[mt]);
-        u[mt] = mfma16(th, hi[s], u[mt]);
-      }
-    }
-    const float us = fac->t_scale * xs.up;
-    top = 0.f;
-#pragma unroll
-    for (int mt = 0; mt < 4; mt++) {
-#pragma unroll
-      for (int r = 0; r < 4; r++) u[mt][r] *= us;
-      top = fmaxf(top, largest(u[mt]));
-    }
-    // out = e^a Q S + P u
-    const Pow2 os = pow2_of(column_max(top));
-    f32x4 o[4] = {zero, zero, zero, zero};
-    {
-      f16x8 hi[2], lo[2];
-      operand(u[0], u[1], os.down, hi[0], lo[0]);
-      operand(u[2], u[3], os.down, hi[1], lo[1]);
-#pragma unroll
-      for (int f = 0; f < T_FRAGS; f++) {
-        const int s = f >= 4, mt = s ? f - 2 : f;
-        const f16x8 ph = frag(pf, (EXACT_OUT ? 2 : 1) * f, lane);
-        if constexpr (EXACT_OUT) {
-          o[mt] = mfma16(frag(pf, 2 * f + 1, lane), hi[s], o[mt]);
-          o[mt] = mfma16(ph, lo[s], o[mt]);
-        }
-        o[mt] = mfma16(ph, hi[s], o[mt]);
-      }
-    }
-    const float ps = fac->p_scale * os.up;
-#pragma unroll
-    for (int mt = 0; mt < 4; mt++) {
-      const f32x4 f = *(const f32x4*)&fac->decayed_q[row_of(mt, 4 * g)];
-#pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int t = row_of(mt, 4 * g + r);
-        if (t < tokens) out[(first + t) * HV * DV] = Elem<DT>::cvt(fmaf(f[r] * ss.up, qs[mt][r], ps * o[mt][r]));
-      }
-    }
-    // S' = e^{a_63} S + K^T (e^{a_63 - a} u)
-    top = 0.f;
-#pragma unroll
-    for (int mt = 0; mt < 4; mt++) {
-      u[mt] *= *(const f32x4*)&fac->to_end[row_of(mt, 4 * g)];
-      top = fmaxf(top, largest(u[mt]));
-    }
-    const Pow2 es = pow2_of(column_max(top));
-    const float end = fac->end;
+      for (int r = 0; r < 4; r++) x[mt][r] = fmaf(x[mt][r], per_unit, -(fk[mt][r] * ks[mt][r]));
     f16x8 hi[2], lo[2];
-    operand(u[0], u[1], es.down, hi[0], lo[0]);
-    operand(u[2], u[3], es.down, hi[1], lo[1]);
+    operand(x[0], x[1], hi[0], lo[0]);
+    operand(x[2], x[3], hi[1], lo[1]);
+    // K^T: row (t, n) at tokens 32 j + 8 g + 0..7, as columns of K's fragments (2 j and 2 j + 1, t / 2)
+    f16x8 KT[2 * NT];
 #pragma unroll
-    for (int t = 0; t < NT; t++) {
-      f32x4 s = zero;
+    for (int f = 0; f < 2 * NT; f++) {
+      const int t = f / 2, j = f % 2;
+      s16x4 h[2];
 #pragma unroll
-      for (int j = 0; j < 2; j++) {
-        const f16x8 k = frag(ktf, 2 * t + j, lane);
-        s = mfma16(k, lo[j], s);
-        s = mfma16(k, hi[j], s);
+      for (int i = 0; i < 2; i++)
+        h[i] = read_column(st + ((2 * j + i) * KS + t / 2) * FRAG + (16 * (n % 4) + 4 * g + n / 4) * 16 + 8 * (t % 2));
+      KT[f] = __builtin_bit_cast(f16x8, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    // u = T' x, the small parts first
+    f32x4 u[4] = {zero, zero, zero, zero};
+#pragma unroll
+    for (int part = 0; part < 3; part++)
+#pragma unroll
+      for (int f = 0; f < T_FRAGS; f++) {
+        const int s = f >= 4, mt = s ? f - 2 : f;
+        u[mt] = mfma16(TF[2 * f + (part == 0)], part == 1 ? lo[s] : hi[s], u[mt]);
       }
+    f32x4 w[4];
 #pragma unroll
-      for (int r = 0; r < 4; r++) S[t][r] = fmaf(s[r], es.up, S[t][r] * end);
+    for (int mt = 0; mt < 4; mt++) w[mt] = u[mt] * fe[mt];
+    operand(w[0], w[1], hi[0], lo[0]);
+    operand(w[2], w[3], hi[1], lo[1]);
+    const float p_scale = fac->p_scale;
+    // S' = e^{a_63} S + K^T (e^{a_63 - a} u)
+    f32x4 add[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) add[t] = S[t] * end;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+      for (int t = 0; t < NT; t++) add[t] = mfma16(KT[2 * t + (j & 1)], j < 2 ? lo[j & 1] : hi[j & 1], add[t]);
+    f16x8 uh[2], ul[2];
+#pragma unroll
+    for (int mt = 0; mt < 4; mt++) u[mt] *= t_scale;
+    operand(u[0], u[1], uh[0], ul[0]);
+    operand(u[2], u[3], uh[1], ul[1]);
+    const bool bad = !(fabsf(add[0][0]) < INFINITY) && !lost;
+    const bool taken = __any(bad);
+    if constexpr (SPLIT) {
+#pragma unroll
+      for (int s = 0; s < 2; s++) {
+        *(f16x8*)(mail + (KS + s) * FRAG + 16 * lane) = uh[s];
+        if constexpr (EXACT_OUT) *(f16x8*)(mail + (2 * KS + 2 + s) * FRAG + 16 * lane) = ul[s];
+      }
+      *(float*)(mail + St::PARTS * (KS + 2) * FRAG + 4 * lane) = unit;
+      *(int*)(mail + St::PARTS * (KS + 2) * FRAG + 256) = taken;
+    }
+    if (taken) {
+#pragma unroll
+      for (int t = 0; t < NT; t++) S[t] *= unit;
+      unit = per_unit = 1.f;
+      delta_tokens<DT, DK>(a, seq.first + (int64_t)c * CHUNK, min(CHUNK, seq.tokens - c * CHUNK), hv, hk, col, g, S);
+      lost = lost || bad;
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; t++) S[t] = add[t];
+      if constexpr (!SPLIT) {
+        PHASE();
+        f16x8 PF[St::PARTS * T_FRAGS];
+        f32x4 fq[4];
+        load_p(so + St::MAT, fac, PF, fq);
+        finish(c, PF, fq, uh, ul, qs, unit, p_scale, tile);
+      }
     }
   }
+  if constexpr (SPLIT) meet();
 #pragma unroll
   for (int t = 0; t < NT; t++)
 #pragma unroll
-    for (int r = 0; r < 4; r++) state[row_of(t, 4 * g + r) * DV] = S[t][r];
+    for (int r = 0; r < 4; r++) state[row_of(t, 4 * g + r) * DV] = S[t][r] * unit;
 }
 
 // ---------------------------------------------------------------- host
@@ -540,11 +819,31 @@ static int delta_chunks(const anna_mi_gated_delta_args& a, const anna_mi_state_s
   const Places<DK> ws = places<DK>(a, s);
   const int32_t* chains = s.buf + 4 * s.sequences + s.steps;
   const int32_t* chunks = chains + 2 * s.chains;
-  const int64_t prepare = s.chunks * a.value_heads, chain = s.chains * a.value_heads * (a.value_dim / 16);
-  ANNA_CHECK(prepare <= INT32_MAX / 256 && chain <= INT32_MAX / 64, "gated delta rule: too many tokens and heads for a launch");
-  delta_prepare_kernel<DT, DK><<<prepare, 256, 0, stream>>>(a, s.buf, s.sequences, chunks, ws);
+  // a key head's value heads in one workgroup share the products of K, where that still fills the chip
+  const int64_t ratio = a.value_heads / a.key_heads;
+  const int per = s.chunks * a.key_heads >= 1024 ? (int)ratio : 1;
+  const int64_t prepare = s.chunks * (a.value_heads / per), groups = s.chains * a.value_heads * (a.value_dim / 16);
+  ANNA_CHECK(prepare <= INT32_MAX / 256 && groups <= INT32_MAX / 128, "gated delta rule: too many tokens and heads for a launch");
+  delta_prepare_kernel<DT, DK><<<prepare, 256, 0, stream>>>(a, s.buf, s.sequences, chunks, ws, per);
   ANNA_LAUNCH_CHECK("delta_prepare");
-  delta_chain_kernel<DT, DK><<<chain, 64, 0, stream>>>(a, s.buf, s.sequences, chains, ws);
+  const uint32_t units = (uint32_t)(s.chains * a.key_heads);
+  hipError_t allowed = hipSuccess;
+#define ANNA_CHAIN(CW, SPLIT)                                                                                             \
+  {                                                                                                                       \
+    typedef Stage<DT, DK, CW, SPLIT> St;                                                                                  \
+    static_assert(St::BYTES <= 160 * 1024, "LDS");                                                                        \
+    const auto kern = &delta_chain_kernel<DT, DK, CW, SPLIT>;                                                             \
+    allowed = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, St::BYTES);              \
+    if (allowed == hipSuccess)                                                                                            \
+      kern<<<8 * ((units + 7) / 8) * (groups / units / CW), 64 * St::WAVES, St::BYTES, stream>>>(a, s.buf, s.sequences,   \
+                                                                                                 chains, ws, units);     \
+  }
+  constexpr bool TWO = Stage<DT, DK, 2, true>::BYTES <= 160 * 1024;  // fp16 at 128 key dims: the second parts leave no room
+  if (a.value_dim % 64 == 0 && groups >= 1024) ANNA_CHAIN(4, false)
+  else if (TWO && groups > 256) ANNA_CHAIN((TWO ? 2 : 1), true)
+  else ANNA_CHAIN(1, true)
+#undef ANNA_CHAIN
+  if (allowed != hipSuccess) return fail_hip(allowed, "delta_chain");
   ANNA_LAUNCH_CHECK("delta_chain");
   return ANNA_MI_OK;
 }
@@ -584,6 +883,7 @@ int anna_mi_gated_delta(const anna_mi_gated_delta_args* args, const anna_mi_stat
   ANNA_CHECK(rows16(a.query, a.query_stride_token, a.query_stride_head) && rows16(a.key, a.key_stride_token, a.key_stride_head) &&
                  rows16(a.value, a.value_stride_token, a.value_stride_head),
              "gated delta rule: rows of query, key and value must be 16-byte aligned");
+  ANNA_CHECK((uintptr_t)a.out % 16 == 0, "gated delta rule: out must be 16-byte aligned");
   ANNA_CHECK((uintptr_t)a.state % 16 == 0 && a.state_stride_slot % 4 == 0, "gated delta rule: states must be 16-byte aligned");
   ANNA_CHECK(a.slots <= 1 || a.state_stride_slot >= a.value_heads * a.key_dim * a.value_dim, "gated delta rule: states overlap");
   ANNA_CHECK(span->chunks == 0 || (a.workspace && (uintptr_t)a.workspace % 256 == 0), "gated delta rule: no workspace, or not 256-byte aligned");

@@ -22,11 +22,11 @@ __global__ __launch_bounds__(256) void delta_step_kernel(const anna_mi_gated_del
   __shared__ float part[2][4][TC][SUMS + 1];
 
   const int tid = threadIdx.x, c = tid % TC, r = tid / TC, wave = tid / 64;
-  const int slice = blockIdx.x % slices;
-  const int64_t item = blockIdx.x / slices;
-  const int64_t HV = a.value_heads, hv = item % HV, hk = hv / (HV / a.key_heads);
+  const uint32_t heads = (uint32_t)a.value_heads, slice = blockIdx.x % (uint32_t)slices, item = blockIdx.x / (uint32_t)slices;
+  const uint32_t hv = item % heads, hk = hv / (heads / (uint32_t)a.key_heads);
+  const int64_t HV = a.value_heads;
   const int dv = slices * COLS, col = slice * COLS + 4 * c;
-  const SpanSeq seq = ((const SpanSeq*)buf)[buf[4 * sequences + item / HV]];
+  const SpanSeq seq = ((const SpanSeq*)buf)[buf[4 * sequences + item / heads]];
 
   if (seq.slot < 0) {  // a sequence of nobody
     for (int i = tid; i < seq.tokens * COLS; i += 256)

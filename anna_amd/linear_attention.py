@@ -287,8 +287,8 @@ def gated_delta_rule(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     stream = _check_span("gated_delta_rule", span, tokens, device)
     if out is None:
         out = torch.empty((tokens, value_heads, value_dim), dtype=query.dtype, device=device)
-    elif out.dtype != query.dtype or out.shape != value.shape or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous {query.dtype} {list(value.shape)}")
+    elif out.dtype != query.dtype or out.shape != value.shape or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError(f"out must be a contiguous, 16-byte aligned {query.dtype} {list(value.shape)}")
     else:
         _apart(out, query=q, key=k, value=v, decay=decay, beta=beta, state=state, a_log=a_log, dt_bias=dt_bias)
     g, b = (t if t.stride(1) == 1 or value_heads == 1 else t.contiguous() for t in (decay, beta))

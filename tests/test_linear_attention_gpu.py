@@ -93,6 +93,58 @@ def test_delta_rule(gpu, case):
     check_delta(c, counts, fresh, DK ** -0.5, out, state)
 
 
+# Workgroups of the chunks' form take 1, 2 or 4 groups of 16 columns, by sequences * value heads * columns / 16:
+# up to 256, to 1023, and more
+MANY = [
+    (20, 2, 4, 128, 128, BF), (20, 4, 4, 64, 128, HF), (40, 2, 4, 128, 128, BF), (40, 1, 4, 128, 128, HF), (70, 2, 4, 64, 64, BF),
+    (70, 1, 4, 64, 64, HF), (60, 2, 3 * 2, 128, 96, BF), (45, 2, 2, 128, 256, HF),
+]
+
+
+@pytest.mark.parametrize("case", MANY, ids=["x".join(map(str, c[:5])) + str(c[5])[6:] for c in MANY])
+def test_delta_rule_of_many_sequences(gpu, case):
+    n, HK, HV, DK, DV, dtype = case
+    counts = [13 + (7 * i) % 90 if i % 9 else 1 for i in range(n)]
+    fresh = [i % 3 == 0 for i in range(n)]
+    c = delta_case(n, counts, HK, HV, DK, DV, dtype, True)
+    c["slots"][5] = -1
+    out, state = run_delta(gpu, c, counts, fresh, DK ** -0.5)
+    check_delta(c, counts, fresh, DK ** -0.5, out, state)
+
+
+@pytest.mark.parametrize("n", [20, 40])
+def test_delta_rule_of_many_sequences_with_some_not_finite(gpu, n):
+    counts = [70] * n
+    c = delta_case(n, counts, 2, 4, 128, 128, BF, False)
+    c["v"][70 * 3 + 40, 2, 17] = float("nan")
+    c["k"][70 * 5 + 66, 0, 3] = float("inf")
+    out, state = run_delta(gpu, c, counts, [False] * n, 0.1)
+    bad = {3: (40, [2]), 5: (66, [0, 1])}
+    for i in bad:
+        at, heads = bad[i]
+        part = out[70 * i:70 * i + 70].float()
+        assert torch.isfinite(part[:at]).all() and not torch.isfinite(part[at:, heads]).all(-1).any()
+        rest = [h for h in range(4) if h not in heads]
+        assert torch.isfinite(part[:, rest]).all() and torch.isfinite(state[c["slots"][i]][rest]).all()
+    assert torch.isfinite(state[c["slots"][3]][2][:, [j for j in range(128) if j != 17]]).all()
+    # the tokens in front, and all other sequences
+    c["v"][70 * 3 + 40:70 * 4] = 0
+    c["k"][70 * 5 + 66:70 * 6] = 0
+    c["k"][70 * 3 + 40:70 * 4] = 0
+    clean, _ = run_delta(gpu, c, counts, [False] * n, 0.1)
+    g, beta = c["decay"].double(), c["beta"].double()
+    for i in range(n):
+        m = bad[i][0] if i in bad else 70
+        rows = slice(70 * i, 70 * i + m)
+        want, S, sums, errors, E, eps = plain.delta_rule(c["q"][rows], c["k"][rows], c["v"][rows], g[rows], beta[rows], c["state"][c["slots"][i]], 0.1,
+                                                         chunked=True)
+        tol = plain.delta_tolerance(want, sums, errors, eps, BF, 0.1, True)
+        for got in (out, clean):
+            assert ((got[rows].double() - want).abs() <= tol).all(), i
+        if i not in bad:
+            assert ((state[c["slots"][i]].double() - S).norm(dim=1) <= E).all()
+
+
 @pytest.mark.parametrize("counts", [[4, 1], [100, 20]])
 def test_delta_rule_precision(gpu, counts):
     """The state is as exact as fp32 sums make it.  An operand split in two fp16 values is off by 2^-24 to 2^-23 of
