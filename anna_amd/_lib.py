@@ -366,7 +366,8 @@ _HOST_ENTRIES = ("anna_mi_last_error", "anna_mi_int4_linear", "anna_mi_decode_nu
                  "anna_mi_moe_router", "anna_mi_moe_dispatch", "anna_mi_moe_grouped_int4_mlp", "anna_mi_moe_combine",
                  "anna_mi_moe_prefill_workspace", "anna_mi_moe_prefill", "anna_mi_paged_fork", "anna_mi_paged_free",
                  "anna_mi_paged_extend", "anna_mi_paged_lengths",
-                 "anna_mi_paged_span_plan", "anna_mi_paged_span_fill", "anna_mi_paged_store", "anna_mi_paged_read", "anna_mi_paged_attend")
+                 "anna_mi_paged_span_plan", "anna_mi_paged_span_fill", "anna_mi_paged_store", "anna_mi_paged_read", "anna_mi_paged_attend",
+                 "anna_mi_gated_delta_workspace", "anna_mi_gated_delta", "anna_mi_causal_conv1d", "anna_mi_rms_norm")
 _host = None
 
 

@@ -57,6 +57,10 @@ struct Library {
   decltype(&anna_mi_paged_store) paged_store = nullptr;
   decltype(&anna_mi_paged_read) paged_read = nullptr;
   decltype(&anna_mi_paged_attend) paged_attend = nullptr;
+  decltype(&anna_mi_gated_delta_workspace) gated_delta_workspace = nullptr;
+  decltype(&anna_mi_gated_delta) gated_delta = nullptr;
+  decltype(&anna_mi_causal_conv1d) causal_conv1d = nullptr;
+  decltype(&anna_mi_rms_norm) rms_norm = nullptr;
 } lib;
 
 void bind(const py::dict& d) {
@@ -86,6 +90,10 @@ void bind(const py::dict& d) {
   get("anna_mi_paged_store", lib.paged_store);
   get("anna_mi_paged_read", lib.paged_read);
   get("anna_mi_paged_attend", lib.paged_attend);
+  get("anna_mi_gated_delta_workspace", lib.gated_delta_workspace);
+  get("anna_mi_gated_delta", lib.gated_delta);
+  get("anna_mi_causal_conv1d", lib.causal_conv1d);
+  get("anna_mi_rms_norm", lib.rms_norm);
 }
 
 void check(int rc, const char* name) {
@@ -607,6 +615,117 @@ OptTensor paged_attend(uintptr_t handle, int64_t layer, uintptr_t span, const Te
   return o;
 }
 
+// ---------------------------------------------------------------- linear attention
+
+// Without a gradient to lose
+bool given(const Tensor& t, const at::Device& dev) { return plain(t, dev) && !(t.requires_grad() && at::GradMode::is_enabled()); }
+bool given(const OptTensor& t, const at::Device& dev) { return !t || given(*t, dev); }
+
+// A pool of states [slots][shape], contiguous in each slot; -> elements from one slot to the next, or -1
+int64_t pool_stride(const Tensor& t, const at::Device& dev, at::ScalarType dt, at::IntArrayRef shape) {
+  if (!given(t, dev) || t.scalar_type() != dt || t.dim() != (int64_t)shape.size() + 1) return -1;
+  int64_t size = 1;
+  for (int64_t i = (int64_t)shape.size(); i > 0; i--) {
+    if (t.size(i) != shape[i - 1] || (t.size(i) > 1 && t.stride(i) != size)) return -1;
+    size *= t.size(i);
+  }
+  return t.size(0) > 1 ? (t.stride(0) >= size ? t.stride(0) : -1) : size;
+}
+
+OptTensor gated_delta(const Tensor& query, const Tensor& key, const Tensor& value, const Tensor& decay, const Tensor& beta,
+                      const Tensor& state, const OptTensor& a_log, const OptTensor& dt_bias, uintptr_t span_address, double scaling,
+                      bool normalize, uintptr_t stream) {
+  const auto* span = reinterpret_cast<const anna_mi_state_span*>(span_address);
+  const at::Device dev = query.device();
+  const at::ScalarType dt = query.scalar_type();
+  if (query.dim() != 3 || value.dim() != 3 || (dt != at::kBFloat16 && dt != at::kHalf) || span->tokens != query.size(0)) return std::nullopt;
+  const int64_t tokens = query.size(0), HK = query.size(1), DK = query.size(2), HV = value.size(1), DV = value.size(2);
+  if (!paged_rows(query, dev, dt, tokens, HK, DK) || !paged_rows(key, dev, dt, tokens, HK, DK) || !paged_rows(value, dev, dt, tokens, HV, DV))
+    return std::nullopt;
+  auto rows = [&](const Tensor& t) {
+    return given(t, dev) && t.scalar_type() == decay.scalar_type() && dtype_code(t) >= 0 && t.dim() == 2 && t.size(0) == tokens &&
+           t.size(1) == HV && (t.stride(1) == 1 || HV == 1);
+  };
+  auto heads = [&](const OptTensor& t) { return !t || (given(*t, dev) && is(*t, dev, at::kFloat) && t->dim() == 1 && t->size(0) == HV); };
+  if (!rows(decay) || !rows(beta) || a_log.has_value() != dt_bias.has_value() || !heads(a_log) || !heads(dt_bias) ||
+      (DK != 64 && DK != 128) || DV % 32 || DV < 32 || DV > 256 || HK < 1 || HV < 1 || HV % HK || !(scaling > -1e30 && scaling < 1e30))
+    return std::nullopt;
+  const int64_t stride = pool_stride(state, dev, at::kFloat, {HV, DK, DV});
+  if (stride < 0 || stride % 4 || reinterpret_cast<uintptr_t>(ptr(state)) % 16) return std::nullopt;
+  Tensor out = at::empty({tokens, HV, DV}, value.options().requires_grad(false)), workspace;
+  anna_mi_gated_delta_args a{};
+  a.dtype = dtype_code(query), a.gates_dtype = dtype_code(decay), a.normalize = normalize, a.scaling = (float)scaling;
+  a.key_heads = HK, a.value_heads = HV, a.key_dim = DK, a.value_dim = DV;
+  a.query = ptr(query), a.query_stride_token = token_stride(query), a.query_stride_head = head_stride(query);
+  a.key = ptr(key), a.key_stride_token = token_stride(key), a.key_stride_head = head_stride(key);
+  a.value = ptr(value), a.value_stride_token = token_stride(value), a.value_stride_head = head_stride(value);
+  a.decay = ptr(decay), a.decay_stride = token_stride(decay), a.beta = ptr(beta), a.beta_stride = token_stride(beta);
+  a.a_log = (const float*)ptr(a_log), a.dt_bias = (const float*)ptr(dt_bias);
+  a.state = (float*)ptr(state), a.slots = state.size(0), a.state_stride_slot = stride, a.out = ptr(out);
+  if (span->chunks > 0) {
+    workspace = at::empty({lib.gated_delta_workspace(&a, span)}, value.options().dtype(at::kByte).requires_grad(false));
+    a.workspace = ptr(workspace);
+  }
+  check(lib.gated_delta(&a, span, stream_ptr(stream)), "anna_mi_gated_delta");
+  return out;
+}
+
+OptTensor causal_conv1d(const Tensor& x, const Tensor& weight, const OptTensor& bias, const Tensor& state, uintptr_t span_address,
+                        bool silu, uintptr_t stream) {
+  const auto* span = reinterpret_cast<const anna_mi_state_span*>(span_address);
+  const at::Device dev = x.device();
+  const at::ScalarType dt = x.scalar_type();
+  if (x.dim() != 2 || dtype_code(x) < 0 || !given(x, dev) || span->tokens != x.size(0)) return std::nullopt;
+  const int64_t tokens = x.size(0), channels = x.size(1);
+  if (channels < 1 || (channels > 1 && x.stride(1) != 1) || (tokens > 1 && x.stride(0) < channels) || !given(weight, dev) ||
+      !is(weight, dev, dt) || weight.dim() != 2 || weight.size(0) != channels || weight.size(1) < 2 || weight.size(1) > 8 ||
+      !given(bias, dev) || (bias && (!is(*bias, dev, dt) || bias->dim() != 1 || bias->size(0) != channels)))
+    return std::nullopt;
+  const int64_t width = weight.size(1), stride = pool_stride(state, dev, dt, {width - 1, channels});
+  if (stride < 0) return std::nullopt;
+  Tensor out = at::empty({tokens, channels}, x.options().requires_grad(false));
+  check(lib.causal_conv1d(ptr(x), dtype_code(x), channels, tokens > 1 ? x.stride(0) : channels, ptr(weight), width, ptr(bias), ptr(state),
+                          state.size(0), stride, silu, span, ptr(out), channels, stream_ptr(stream)),
+        "anna_mi_causal_conv1d");
+  return out;
+}
+
+// out, or codes and scales with a group; both undefined for calls that are left to the caller
+std::pair<OptTensor, OptTensor> rms_norm(const Tensor& x, const Tensor& weight, double eps, double weight_offset, const OptTensor& residual,
+                                         const OptTensor& gate, int64_t group, uintptr_t stream) {
+  const std::pair<OptTensor, OptTensor> none;
+  const at::Device dev = x.device();
+  const at::ScalarType dt = x.scalar_type();
+  if (x.dim() < 1 || dtype_code(x) < 0 || x.numel() == 0 || !(eps >= 0.0 && eps < 1e30)) return none;
+  const int64_t cols = x.size(-1), rows = x.numel() / cols;
+  // rows with one stride: contiguous tensors, and matrices
+  auto lies = [&](const Tensor& t, int64_t& stride) {
+    if (!given(t, dev) || t.scalar_type() != dt || t.sizes() != x.sizes()) return false;
+    if (t.is_contiguous()) return stride = cols, true;
+    if (t.dim() != 2 || (cols > 1 && t.stride(1) != 1) || (rows > 1 && t.stride(0) < cols)) return false;
+    return stride = rows > 1 ? t.stride(0) : cols, true;
+  };
+  anna_mi_rms_norm_args a{};
+  if (!lies(x, a.x_stride) || (residual && !lies(*residual, a.residual_stride)) || (gate && !lies(*gate, a.gate_stride)) ||
+      !given(weight, dev) || !is(weight, dev, dt) || weight.dim() != 1 || weight.size(0) != cols)
+    return none;
+  a.dtype = dtype_code(x), a.out_format = group > 0, a.rows = rows, a.cols = cols, a.group = group;
+  a.x = ptr(x), a.weight = ptr(weight), a.residual = ptr(residual), a.gate = ptr(gate);
+  a.eps = (float)eps, a.weight_offset = (float)weight_offset, a.out_stride = cols;
+  const auto options = x.options().requires_grad(false);
+  Tensor out = at::empty(x.sizes(), group > 0 ? options.dtype(at::kFloat8_e4m3fn) : options);
+  OptTensor scales;
+  a.out = ptr(out);
+  if (group > 0) {
+    auto shape = x.sizes().vec();
+    shape.back() = cols / group;
+    scales = at::empty(shape, options.dtype(at::kFloat));
+    a.scales = (float*)ptr(*scales);
+  }
+  check(lib.rms_norm(&a, stream_ptr(stream)), "anna_mi_rms_norm");
+  return {out, scales};
+}
+
 }  // namespace
 
 #ifndef ANNA_MI_SOURCE_HASH
@@ -630,4 +749,7 @@ PYBIND11_MODULE(_torch_host, m) {
   m.def("paged_store", &paged_store, no_gil);
   m.def("paged_read", &paged_read, no_gil);
   m.def("paged_attend", &paged_attend, no_gil);
+  m.def("gated_delta", &gated_delta, no_gil);
+  m.def("causal_conv1d", &causal_conv1d, no_gil);
+  m.def("rms_norm", &rms_norm, no_gil);
 }
