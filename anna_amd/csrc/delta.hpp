@@ -8,10 +8,27 @@ namespace anna {
 constexpr int CHUNK = 64;        // tokens of a chunk
 constexpr int STEP_TOKENS = 12;  // sequences of at most so many tokens are taken token by token
 
-// A sequence's record in a span's buffer
+// The records of a span's buffer: a sequence, one taken in chunks, a chunk of it
 struct SpanSeq {
   int32_t slot, first, tokens, fresh;
 };
+struct SpanChain {
+  SpanSeq seq;
+  int32_t first_chunk, pad[3];
+};
+struct SpanChunk {
+  int32_t slot, first, tokens, pad;
+};
+inline const SpanSeq* span_seqs(const anna_mi_state_span& s) { return (const SpanSeq*)s.buf; }
+inline const SpanSeq* span_steps(const anna_mi_state_span& s) { return span_seqs(s) + s.sequences; }
+inline const SpanChain* span_chains(const anna_mi_state_span& s) { return (const SpanChain*)(span_steps(s) + s.steps); }
+inline const SpanChunk* span_chunks(const anna_mi_state_span& s) { return (const SpanChunk*)(span_chains(s) + s.chains); }
+inline const int32_t* span_owners(const anna_mi_state_span& s) { return (const int32_t*)(span_chunks(s) + s.chunks); }
+
+// x / (1 + e^-x), off by a few 2^-24 of itself (|x| 2^-24 where x is far below 0)
+__device__ __forceinline__ float silu_of(float x) {
+  return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * x));
+}
 
 // The decay's logarithm and beta of a token and value head, from what the caller gave
 struct Gate {
@@ -22,15 +39,19 @@ __device__ __forceinline__ float gate_value(const void* p, int dtype, int64_t i)
   const uint16_t h = ((const uint16_t*)p)[i];
   return dtype == ANNA_MI_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
 }
-__device__ __forceinline__ Gate gate_of(const anna_mi_gated_delta_args& a, int64_t token, int64_t head) {
-  Gate r{gate_value(a.decay, a.gates_dtype, token * a.decay_stride + head),
-         gate_value(a.beta, a.gates_dtype, token * a.beta_stride + head)};
+__device__ __forceinline__ Gate gate_of(const anna_mi_gated_delta_args& a, Gate r, int64_t head) {
   if (a.a_log) {
     const float x = r.g + a.dt_bias[head];
     r.g = -expf(a.a_log[head]) * (fmaxf(x, 0.f) + log1pf(expf(-fabsf(x))));  // softplus without overflow
     r.beta = 1.f / (1.f + expf(-r.beta));
   }
   return r;
+}
+__device__ __forceinline__ Gate gate_of(const anna_mi_gated_delta_args& a, int64_t token, int64_t head) {
+  return gate_of(a,
+                 Gate{gate_value(a.decay, a.gates_dtype, token * a.decay_stride + head),
+                      gate_value(a.beta, a.gates_dtype, token * a.beta_stride + head)},
+                 head);
 }
 
 constexpr float NORM_EPS = 1e-6f;

@@ -98,9 +98,8 @@ __device__ __forceinline__ float exp2_of(double t) {
 // A workgroup takes a chunk, a key head and `per` of its value heads.  A wave has the rows row_of(wave, 0..15) of K and Q,
 // which are at once their fragments and the left operands of K K^T and Q K^T.
 template <int DT, int DK>
-__global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gated_delta_args a, const int32_t* __restrict__ buf,
-                                                            int64_t sequences, const int32_t* __restrict__ chunks,
-                                                            const Places<DK> ws, int per) {
+__global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gated_delta_args a,
+                                                               const SpanChunk* __restrict__ chunks, const Places<DK> ws, int per) {
   typedef typename Elem<DT>::T T;
   constexpr int KS = DK / 32;
   constexpr int LD = DK + 8;     // halves of a row of K in LDS
@@ -114,10 +113,10 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
   const uint32_t ratio = (uint32_t)a.value_heads / (uint32_t)a.key_heads, parts = (uint32_t)a.value_heads / (uint32_t)per;
   const uint32_t chunk = blockIdx.x / parts, hv0 = blockIdx.x % parts * per, hk = hv0 / ratio;
   const bool writes_k = hv0 % ratio == 0;
-  const SpanSeq seq = ((const SpanSeq*)buf)[chunks[2 * chunk]];
-  if (seq.slot < 0) return;
-  const int64_t first = seq.first + (int64_t)chunks[2 * chunk + 1] * CHUNK;
-  const int tokens = min(CHUNK, seq.tokens - chunks[2 * chunk + 1] * CHUNK);
+  const SpanChunk here = chunks[chunk];
+  if (here.slot < 0) return;
+  const int64_t first = here.first;
+  const int tokens = here.tokens;
 
   const int mine = row_of(wave, n);
   u32x4 raw[2][KS];
@@ -456,8 +455,7 @@ template <int DT, int DK, int CW, bool SPLIT> struct Stage {
 
 template <int DT, int DK, int CW, bool SPLIT>
 __global__ __launch_bounds__((64 * Stage<DT, DK, CW, SPLIT>::WAVES), 2) void delta_chain_kernel(
-    const anna_mi_gated_delta_args a, const int32_t* __restrict__ buf, int64_t sequences, const int32_t* __restrict__ chains,
-    const Places<DK> ws, uint32_t units) {
+    const anna_mi_gated_delta_args a, const SpanChain* __restrict__ chains, const Places<DK> ws, uint32_t units) {
   typedef typename Elem<DT>::T T;
   typedef Stage<DT, DK, CW, SPLIT> St;
   constexpr int NT = DK / 16, KS = DK / 32;
@@ -471,9 +469,9 @@ __global__ __launch_bounds__((64 * Stage<DT, DK, CW, SPLIT>::WAVES), 2) void del
   const uint32_t unit_of = blockIdx.x / (8 * each) * 8 + blockIdx.x % 8, part = blockIdx.x / 8 % each;
   if (unit_of >= units) return;
   const uint32_t hk = unit_of % (uint32_t)a.key_heads, hv = hk * ratio + part / slices, col0 = part % slices * (16 * CW);
-  const int32_t* chain = chains + 2 * (unit_of / (uint32_t)a.key_heads);
-  const SpanSeq seq = ((const SpanSeq*)buf)[chain[0]];
-  const int64_t chunk0 = chain[1];
+  const SpanChain chain = chains[unit_of / (uint32_t)a.key_heads];
+  const SpanSeq seq = chain.seq;
+  const int64_t chunk0 = chain.first_chunk;
   const int count = (seq.tokens + CHUNK - 1) / CHUNK;
   if (seq.slot < 0) {
     for (int64_t i = threadIdx.x; i < (int64_t)seq.tokens * 16 * CW; i += 64 * St::WAVES)
@@ -817,14 +815,12 @@ template <int DK> static Places<DK> places(const anna_mi_gated_delta_args& a, co
 template <int DT, int DK>
 static int delta_chunks(const anna_mi_gated_delta_args& a, const anna_mi_state_span& s, hipStream_t stream) {
   const Places<DK> ws = places<DK>(a, s);
-  const int32_t* chains = s.buf + 4 * s.sequences + s.steps;
-  const int32_t* chunks = chains + 2 * s.chains;
   // a key head's value heads in one workgroup share the products of K, where that still fills the chip
   const int64_t ratio = a.value_heads / a.key_heads;
   const int per = s.chunks * a.key_heads >= 1024 ? (int)ratio : 1;
   const int64_t prepare = s.chunks * (a.value_heads / per), groups = s.chains * a.value_heads * (a.value_dim / 16);
   ANNA_CHECK(prepare <= INT32_MAX / 256 && groups <= INT32_MAX / 128, "gated delta rule: too many tokens and heads for a launch");
-  delta_prepare_kernel<DT, DK><<<prepare, 256, 0, stream>>>(a, s.buf, s.sequences, chunks, ws, per);
+  delta_prepare_kernel<DT, DK><<<prepare, 256, 0, stream>>>(a, span_chunks(s), ws, per);
   ANNA_LAUNCH_CHECK("delta_prepare");
   const uint32_t units = (uint32_t)(s.chains * a.key_heads);
   hipError_t allowed = hipSuccess;
@@ -835,8 +831,7 @@ static int delta_chunks(const anna_mi_gated_delta_args& a, const anna_mi_state_s
     const auto kern = &delta_chain_kernel<DT, DK, CW, SPLIT>;                                                             \
     allowed = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, St::BYTES);              \
     if (allowed == hipSuccess)                                                                                            \
-      kern<<<8 * ((units + 7) / 8) * (groups / units / CW), 64 * St::WAVES, St::BYTES, stream>>>(a, s.buf, s.sequences,   \
-                                                                                                 chains, ws, units);     \
+      kern<<<8 * ((units + 7) / 8) * (groups / units / CW), 64 * St::WAVES, St::BYTES, stream>>>(a, span_chains(s), ws, units); \
   }
   constexpr bool TWO = Stage<DT, DK, 2, true>::BYTES <= 160 * 1024;  // fp16 at 128 key dims: the second parts leave no room
   if (a.value_dim % 64 == 0 && groups >= 1024) ANNA_CHAIN(4, false)

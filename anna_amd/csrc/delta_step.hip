@@ -3,7 +3,8 @@
 // A workgroup owns COLS columns of one head's state for all rows, in registers: thread (r, c) the
 // columns 4 c .. 4 c + 3 of the rows r, r + RG, ...  Both products of a token with the state are sums over rows,
 // and S'^T q = e^g S^T q + (k . q) u with u = beta (v - e^g S^T k), so one round of sums over the old state
-// serves both.
+// serves both.  While the state is on its way, the waves make the unit vectors and the factors of all tokens, a
+// wave a token, in LDS.
 //
 // It is bound by the state's bytes (key_dim * value_dim * 4 read and written a sequence and head); a
 // token's q, k and v are a hundredth of them.
@@ -12,66 +13,81 @@
 namespace anna {
 
 template <int DT, int DK, int COLS>
-__global__ __launch_bounds__(256) void delta_step_kernel(const anna_mi_gated_delta_args a, const int32_t* __restrict__ buf,
-                                                         int64_t sequences, int slices) {
+__global__ __launch_bounds__(256) void delta_step_kernel(const anna_mi_gated_delta_args a, const SpanSeq* __restrict__ steps,
+                                                         int slices) {
   typedef typename Elem<DT>::T T;
   constexpr int TC = COLS / 4;     // threads on a row
   constexpr int RG = 256 / TC;     // rows at a time
   constexpr int NR = DK / RG;      // rows of a thread
   constexpr int SUMS = 8;          // S^T k and S^T q of four columns
   __shared__ float part[2][4][TC][SUMS + 1];
+  __shared__ float ks[STEP_TOKENS][DK], qs[STEP_TOKENS][DK], vs[STEP_TOKENS][COLS];
+  __shared__ float decays[STEP_TOKENS], betas[STEP_TOKENS], kqs[STEP_TOKENS];
 
-  const int tid = threadIdx.x, c = tid % TC, r = tid / TC, wave = tid / 64;
+  const int tid = threadIdx.x, c = tid % TC, r = tid / TC, wave = tid / 64, lane = tid % 64;
   const uint32_t heads = (uint32_t)a.value_heads, slice = blockIdx.x % (uint32_t)slices, item = blockIdx.x / (uint32_t)slices;
   const uint32_t hv = item % heads, hk = hv / (heads / (uint32_t)a.key_heads);
   const int64_t HV = a.value_heads;
   const int dv = slices * COLS, col = slice * COLS + 4 * c;
-  const SpanSeq seq = ((const SpanSeq*)buf)[buf[4 * sequences + item / heads]];
+  const SpanSeq seq = steps[item / heads];
 
   if (seq.slot < 0) {  // a sequence of nobody
     for (int i = tid; i < seq.tokens * COLS; i += 256)
       ((T*)a.out)[((int64_t)(seq.first + i / COLS) * HV + hv) * dv + slice * COLS + i % COLS] = Elem<DT>::cvt(0.f);
     return;
   }
-  float* state = a.state + seq.slot * a.state_stride_slot + hv * DK * dv + col;
+  float* state = a.state + seq.slot * a.state_stride_slot + (int64_t)hv * DK * dv + col;
   f32x4 S[NR];
 #pragma unroll
   for (int i = 0; i < NR; i++) S[i] = seq.fresh ? f32x4{0.f, 0.f, 0.f, 0.f} : *(const f32x4*)(state + (int64_t)(r + RG * i) * dv);
 
-  for (int t = 0; t < seq.tokens; t++) {
+  for (int t = wave; t < seq.tokens; t += 4) {
     const int64_t token = seq.first + t;
     const T* qp = (const T*)a.query + token * a.query_stride_token + hk * a.query_stride_head;
     const T* kp = (const T*)a.key + token * a.key_stride_token + hk * a.key_stride_head;
-    const T* vp = (const T*)a.value + token * a.value_stride_token + hv * a.value_stride_head + col;
-    // every wave for itself: |k|^2, |q|^2, k . q
-    float kk = 0.f, qq = 0.f, kq = 0.f;
+    const T* vp = (const T*)a.value + token * a.value_stride_token + hv * a.value_stride_head + slice * COLS;
+    float k[DK / 64], q[DK / 64], kk = 0.f, qq = 0.f, kq = 0.f;
 #pragma unroll
     for (int i = 0; i < DK / 64; i++) {
-      const float x = Elem<DT>::load(kp, (tid & 63) + 64 * i), y = Elem<DT>::load(qp, (tid & 63) + 64 * i);
-      kk = fmaf(x, x, kk);
-      qq = fmaf(y, y, qq);
-      kq = fmaf(x, y, kq);
-    }
-    float k[NR], q[NR], v[4], sum[SUMS] = {};
-#pragma unroll
-    for (int i = 0; i < NR; i++) {
-      k[i] = Elem<DT>::load(kp, r + RG * i);
-      q[i] = Elem<DT>::load(qp, r + RG * i);
+      k[i] = Elem<DT>::load(kp, lane + 64 * i);
+      q[i] = Elem<DT>::load(qp, lane + 64 * i);
     }
 #pragma unroll
-    for (int j = 0; j < 4; j++) v[j] = Elem<DT>::load(vp, j);
+    for (int i = 0; i < (COLS + 63) / 64; i++)
+      if (lane + 64 * i < COLS) vs[t][lane + 64 * i] = Elem<DT>::load(vp, lane + 64 * i);
     const Gate gate = gate_of(a, token, hv);
+#pragma unroll
+    for (int i = 0; i < DK / 64; i++) {
+      kk = fmaf(k[i], k[i], kk);
+      qq = fmaf(q[i], q[i], qq);
+      kq = fmaf(k[i], q[i], kq);
+    }
     const float ck = a.normalize ? rsqrtf(wave_sum_rows(kk) + NORM_EPS) : 1.f;
     const float cq = a.scaling * (a.normalize ? rsqrtf(wave_sum_rows(qq) + NORM_EPS) : 1.f);
     kq = wave_sum_rows(kq) * ck * cq;
 #pragma unroll
+    for (int i = 0; i < DK / 64; i++) {
+      ks[t][lane + 64 * i] = k[i] * ck;
+      qs[t][lane + 64 * i] = q[i] * cq;
+    }
+    if (lane == 0) {
+      decays[t] = expf(gate.g);
+      betas[t] = gate.beta;
+      kqs[t] = kq;
+    }
+  }
+  __syncthreads();
+
+  for (int t = 0; t < seq.tokens; t++) {
+    float k[NR], sum[SUMS] = {};
+#pragma unroll
     for (int i = 0; i < NR; i++) {
-      k[i] *= ck;
-      q[i] *= cq;
+      k[i] = ks[t][r + RG * i];
+      const float q = qs[t][r + RG * i];
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         sum[j] = fmaf(S[i][j], k[i], sum[j]);
-        sum[4 + j] = fmaf(S[i][j], q[i], sum[4 + j]);
+        sum[4 + j] = fmaf(S[i][j], q, sum[4 + j]);
       }
     }
     // over the row groups: of a wave, then of the four waves
@@ -82,25 +98,29 @@ __global__ __launch_bounds__(256) void delta_step_kernel(const anna_mi_gated_del
       sum[s] += lane_xor32(sum[s]);
     }
     auto& mine = part[t & 1];
-    if ((tid & 63) < TC)
+    if (lane < TC)
 #pragma unroll
       for (int s = 0; s < SUMS; s++) mine[wave][c][s] = sum[s];
     __syncthreads();
 #pragma unroll
     for (int s = 0; s < SUMS; s++) sum[s] = (mine[0][c][s] + mine[1][c][s]) + (mine[2][c][s] + mine[3][c][s]);
 
-    const float e = expf(gate.g);
+    const float e = decays[t], beta = betas[t];
     float u[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) u[j] = gate.beta * (v[j] - e * sum[j]);
+    for (int j = 0; j < 4; j++) u[j] = beta * (vs[t][4 * c + j] - e * sum[j]);
 #pragma unroll
     for (int i = 0; i < NR; i++)
 #pragma unroll
       for (int j = 0; j < 4; j++) S[i][j] = fmaf(k[i], u[j], e * S[i][j]);
     if (r == 0) {
-      T* out = (T*)a.out + (token * HV + hv) * dv + col;
+      const float kq = kqs[t];
+      uint32_t w[2];
 #pragma unroll
-      for (int j = 0; j < 4; j++) out[j] = Elem<DT>::cvt(fmaf(kq, u[j], e * sum[4 + j]));
+      for (int j = 0; j < 4; j += 2)
+        w[j / 2] = (uint32_t)Elem<DT>::cvt(fmaf(kq, u[j], e * sum[4 + j])) |
+                   (uint32_t)Elem<DT>::cvt(fmaf(kq, u[j + 1], e * sum[5 + j])) << 16;
+      *(uint2*)((T*)a.out + ((seq.first + (int64_t)t) * HV + hv) * dv + col) = make_uint2(w[0], w[1]);
     }
   }
 #pragma unroll
@@ -108,15 +128,22 @@ __global__ __launch_bounds__(256) void delta_step_kernel(const anna_mi_gated_del
 }
 
 int delta_step(const anna_mi_gated_delta_args& a, const anna_mi_state_span& s, hipStream_t stream) {
-  constexpr int COLS = 32;
-  const int slices = (int)(a.value_dim / COLS);
-  const int64_t grid = s.steps * a.value_heads * slices;
+  // The widest slices that leave a workgroup for every compute unit: rows of 128 columns are whole lines, and
+  // fewer workgroups make the unit vectors (heads of 64 x 128, 24 sequences of up to 6 tokens: 19.2 us at 32 columns,
+  // 14.8 at 128); for few sequences narrow ones are sooner done (one sequence: 4.9 us, 6.0 at 128).
+  const int64_t states = s.steps * a.value_heads;
+  int cols = 32;
+  for (int wide = 64; wide <= 128; wide *= 2)
+    if (a.value_dim % wide == 0 && states * (a.value_dim / wide) >= 256) cols = wide;
+  const int slices = (int)(a.value_dim / cols);
+  const int64_t grid = states * slices;
   if (grid == 0) return ANNA_MI_OK;
   ANNA_CHECK(grid <= INT32_MAX / 256, "gated delta rule: too many sequences and heads for a launch");
   ANNA_DISPATCH_DTYPE(a.dtype, DT, {
     if constexpr (DT != ANNA_MI_F32) {
-      if (a.key_dim == 64) delta_step_kernel<DT, 64, COLS><<<grid, 256, 0, stream>>>(a, s.buf, s.sequences, slices);
-      else delta_step_kernel<DT, 128, COLS><<<grid, 256, 0, stream>>>(a, s.buf, s.sequences, slices);
+      auto go = [&](auto kern) { kern<<<grid, 256, 0, stream>>>(a, span_steps(s), slices); };
+      if (a.key_dim == 64) go(cols == 32 ? delta_step_kernel<DT, 64, 32> : cols == 64 ? delta_step_kernel<DT, 64, 64> : delta_step_kernel<DT, 64, 128>);
+      else go(cols == 32 ? delta_step_kernel<DT, 128, 32> : cols == 64 ? delta_step_kernel<DT, 128, 64> : delta_step_kernel<DT, 128, 128>);
     }
   });
   ANNA_LAUNCH_CHECK("delta_step");

@@ -4,7 +4,7 @@
 // rows longer than the registers of a workgroup are read twice.  Sums of squares and the scales are fp32.  The
 // sum with the residual is rounded to the type before it is normalised: what is normalised is what the stream
 // holds, as in a model that adds and normalises in two steps.  Bound by the rows' bytes.
-#include "common.hpp"
+#include "delta.hpp"
 
 namespace anna {
 
@@ -164,7 +164,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(const anna_mi_rms_norm_ar
         float g[8];
         load8<DT>(a.gate, row * a.gate_stride + c, n, vec, g);
 #pragma unroll
-        for (int e = 0; e < 8; e++) h[i][e] *= g[e] / (1.f + expf(-g[e]));
+        for (int e = 0; e < 8; e++) h[i][e] *= silu_of(g[e]);
       }
     }
     if constexpr (!CODES) {
@@ -231,7 +231,7 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(const anna_mi_rms_no
       float g[8];
       load8<DT>(a.gate, row * a.gate_stride + c, n, vec, g);
 #pragma unroll
-      for (int e = 0; e < 8; e++) h[e] *= g[e] / (1.f + expf(-g[e]));
+      for (int e = 0; e < 8; e++) h[e] *= silu_of(g[e]);
     }
   };
   const bool by_row = a.group == cols;

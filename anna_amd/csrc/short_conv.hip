@@ -1,8 +1,8 @@
 // The short causal convolution of a linear-attention layer over packed, ragged sequences, with the last
 // width - 1 inputs of every sequence kept in a row of a state pool.
 //
-// A thread takes 8 channels (16 bytes of the 16-bit types) and walks down TILE tokens with the window in
-// registers, so an input is read once and width - 1 times more at a tile's border.  Bound by the bytes of x and out.
+// A thread takes 8 channels (16 bytes of the 16-bit types) and walks down `tile` tokens with the window in
+// registers, so an input is read once, and the width - 1 in front of a tile once more.  Bound by the bytes of x and out.
 // The thread that has a sequence's first token also takes the width - 2 tokens behind it, also past its tile:
 // it alone reads the state of its channels, and then writes the new one.
 #include "delta.hpp"
@@ -18,119 +18,131 @@ template <int DT, int W>
 __global__ __launch_bounds__(256) void short_conv_kernel(const typename Elem<DT>::T* __restrict__ x, int64_t x_stride,
                                                          const typename Elem<DT>::T* __restrict__ weight,
                                                          const typename Elem<DT>::T* __restrict__ bias,
-                                                         typename Elem<DT>::T* state, int64_t state_stride, int64_t channels,
-                                                         int silu, const SpanSeq* __restrict__ seqs, int sequences, int tokens,
-                                                         int tile, int vec, typename Elem<DT>::T* __restrict__ out,
-                                                         int64_t out_stride) {
+                                                         typename Elem<DT>::T* state, int64_t state_stride, uint32_t channels,
+                                                         int silu, const SpanSeq* __restrict__ seqs,
+                                                         const int32_t* __restrict__ owners, int tokens, int tile, int vec,
+                                                         typename Elem<DT>::T* __restrict__ out, int64_t out_stride) {
   typedef typename Elem<DT>::T T;
-  const int64_t groups = (channels + 7) / 8, item = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t c0 = item % groups * 8;
-  const int64_t first = item / groups * tile;
-  if (first >= tokens) return;
-  const int n = (int)min((int64_t)8, channels - c0), last = (int)min(first + tile, (int64_t)tokens);
+  typedef Vec8<DT> Row;
+  constexpr int FOUR = 4;  // tokens whose loads go together, a group ahead of their use
+  const uint32_t groups = (channels + 7) / 8, item = blockIdx.x * 256 + threadIdx.x, c0 = item % groups * 8;
+  const int64_t begin = (int64_t)(item / groups) * tile;
+  if (begin >= tokens) return;
+  const int first = (int)begin, last = (int)min(begin + tile, (int64_t)tokens), n = min(8u, channels - c0);
 
-  auto load = [&](const T* p, float (&f)[8]) {
+  auto load = [&](const T* p) {
+    Row r;
     if (vec) {
-      const Vec8<DT> v = *(const Vec8<DT>*)__builtin_assume_aligned(p, 16);
-#pragma unroll
-      for (int e = 0; e < 8; e++) f[e] = Elem<DT>::to_f32(v.v[e]);
+      r = *(const Row*)__builtin_assume_aligned(p, 16);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; e++) f[e] = e < n ? Elem<DT>::load(p, e) : 0.f;
+      for (int e = 0; e < 8; e++) r.v[e] = e < n ? p[e] : (T)0;
     }
+    return r;
   };
-  auto save = [&](T* p, const float (&f)[8]) {
+  auto save = [&](T* p, const Row& r) {
     if (vec) {
-      Vec8<DT> v;
-#pragma unroll
-      for (int e = 0; e < 8; e++) v.v[e] = Elem<DT>::cvt(f[e]);
-      *(Vec8<DT>*)__builtin_assume_aligned(p, 16) = v;
+      *(Row*)__builtin_assume_aligned(p, 16) = r;
     } else {
 #pragma unroll
       for (int e = 0; e < 8; e++)
-        if (e < n) p[e] = Elem<DT>::cvt(f[e]);
+        if (e < n) p[e] = r.v[e];
     }
   };
 
+  int s = owners[first];
+  SpanSeq seq = seqs[s];
   float w[W][8], b[8] = {};
+  if (vec) {  // eight channels' taps lie together
 #pragma unroll
-  for (int e = 0; e < 8; e++)
+    for (int i = 0; i < W; i++) {
+      const Row r = load(weight + (int64_t)c0 * W + 8 * i);
 #pragma unroll
-    for (int j = 0; j < W; j++) w[j][e] = e < n ? Elem<DT>::load(weight, (c0 + e) * W + j) : 0.f;
+      for (int e = 0; e < 8; e++) w[(8 * i + e) % W][(8 * i + e) / W] = Elem<DT>::to_f32(r.v[e]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+#pragma unroll
+      for (int j = 0; j < W; j++) w[j][e] = e < n ? Elem<DT>::load(weight, (int64_t)(c0 + e) * W + j) : 0.f;
+  }
   if (bias)
 #pragma unroll
     for (int e = 0; e < 8; e++) b[e] = e < n ? Elem<DT>::load(bias, c0 + e) : 0.f;
 
-  // the last sequence that begins at or before the tile and is not empty
-  int lo = 0, hi = sequences - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (seqs[mid].first <= first) lo = mid;
-    else hi = mid - 1;
-  }
-  int s = lo;
-  SpanSeq seq = seqs[s];
-
-  float win[W][8];  // inputs t - W + 1 .. t
-  bool begins = true;
-  int t = (int)first;
+  int t = first;
   if (t > seq.first && t < seq.first + W - 1) t = min(seq.first + min(W - 1, seq.tokens), last);  // another thread's
-  for (;; t++) {
-    if (t >= last && (begins || t >= min(seq.first + W - 1, seq.first + seq.tokens))) break;
-    while (t >= seq.first + seq.tokens) {
-      seq = seqs[++s];
-      begins = true;
+  while (t < last) {
+    while (t >= seq.first + seq.tokens) seq = seqs[++s];
+    const int pos = t - seq.first, end = seq.first + seq.tokens;
+    // to the tile's end, and from a sequence's first token through the width - 2 behind it
+    const int stop = min(end, pos == 0 ? max(last, seq.first + W - 1) : last), run = stop - t;
+    if (seq.slot < 0) {
+      Row zeros;
+#pragma unroll
+      for (int e = 0; e < 8; e++) zeros.v[e] = Elem<DT>::cvt(0.f);
+      for (; t < stop; t++) save(out + (int64_t)t * out_stride + c0, zeros);
+      continue;
     }
-    const int pos = t - seq.first;
-    if (begins) {
-      begins = false;
+    const T* const from = x + (int64_t)t * x_stride + c0;
+    Row next[FOUR], win[W - 1];  // win: the inputs in front of the next one
+#pragma unroll
+    for (int i = 0; i < FOUR; i++) next[i] = load(from + (int64_t)min(i, run - 1) * x_stride);
+#pragma unroll
+    for (int j = 0; j < W - 1; j++) {
+      const int at = pos - (W - 1) + j;
+      if (at >= 0) {
+        win[j] = load(x + (int64_t)(seq.first + at) * x_stride + c0);
+      } else if (!seq.fresh) {
+        win[j] = load(state + seq.slot * state_stride + (int64_t)(W - 1 + at) * channels + c0);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) win[j].v[e] = Elem<DT>::cvt(0.f);
+      }
+    }
+    if (pos == 0) {
+      // the state after the sequence's tokens: all of the old one that is needed is in the window
+      T* to = state + seq.slot * state_stride + c0;
 #pragma unroll
       for (int j = 0; j < W - 1; j++) {
-        const int at = pos - (W - 1) + j;
+        const int at = seq.tokens - (W - 1) + j;
+        Row r = win[W - 2];
         if (at >= 0) {
-          load(x + (int64_t)(seq.first + at) * x_stride + c0, win[j + 1]);
-        } else if (seq.slot >= 0 && !seq.fresh) {
-          load(state + seq.slot * state_stride + (int64_t)(W - 1 + at) * channels + c0, win[j + 1]);
+          r = load(x + (int64_t)(seq.first + at) * x_stride + c0);
         } else {
 #pragma unroll
-          for (int e = 0; e < 8; e++) win[j + 1][e] = 0.f;
+          for (int i = 0; i < W - 1; i++)  // window entry i is position i - (W - 1)
+            if (i == W - 1 + at) r = win[i];
         }
+        save(to + (int64_t)j * channels, r);
       }
-      if (pos == 0 && seq.slot >= 0) {
-        // the state after the sequence's tokens: all of the old one that is needed is in the window
-        T* to = state + seq.slot * state_stride + c0;
+    }
+    for (int k = 0; k < run; k += FOUR) {
+      Row rows[W - 1 + FOUR];
 #pragma unroll
-        for (int j = 0; j < W - 1; j++) {
-          const int at = seq.tokens - (W - 1) + j;
-          float f[8];
-          if (at >= 0) {
-            load(x + (int64_t)(seq.first + at) * x_stride + c0, f);
-          } else {
+      for (int j = 0; j < W - 1; j++) rows[j] = win[j];
 #pragma unroll
-            for (int i = 0; i < W - 1; i++)  // window entry 1 + i is position i - (W - 1)
-              if (i == W - 1 + at)
+      for (int i = 0; i < FOUR; i++) rows[W - 1 + i] = next[i];
 #pragma unroll
-                for (int e = 0; e < 8; e++) f[e] = win[1 + i][e];
+      for (int j = 0; j < W - 1; j++) win[j] = rows[FOUR + j];
+      if (k + FOUR < run)
+#pragma unroll
+        for (int i = 0; i < FOUR; i++) next[i] = load(from + (int64_t)min(k + FOUR + i, run - 1) * x_stride);
+#pragma unroll
+      for (int i = 0; i < FOUR; i++)
+        if (k + i < run) {
+          Row r;
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            float y = b[e];
+#pragma unroll
+            for (int j = 0; j < W; j++) y = fmaf(Elem<DT>::to_f32(rows[i + j].v[e]), w[j][e], y);
+            r.v[e] = Elem<DT>::cvt(silu ? silu_of(y) : y);
           }
-          save(to + (int64_t)j * channels, f);
+          save(out + (int64_t)(t + k + i) * out_stride + c0, r);
         }
-      }
     }
-#pragma unroll
-    for (int j = 0; j + 1 < W; j++)
-#pragma unroll
-      for (int e = 0; e < 8; e++) win[j][e] = win[j + 1][e];
-    load(x + (int64_t)t * x_stride + c0, win[W - 1]);
-    float y[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      y[e] = b[e];
-#pragma unroll
-      for (int j = 0; j < W; j++) y[e] = fmaf(win[j][e], w[j][e], y[e]);
-      if (silu) y[e] = y[e] / (1.f + expf(-y[e]));
-      if (seq.slot < 0) y[e] = 0.f;
-    }
-    save(out + (int64_t)t * out_stride + c0, y);
+    t = stop;
   }
 }
 
@@ -141,18 +153,19 @@ static int launch(const void* x, int64_t channels, int64_t x_stride, const void*
   typedef typename Elem<DT>::T T;
   constexpr int64_t unit = 16 / sizeof(T);
   auto rows16 = [&](const void* p, int64_t stride) { return (uintptr_t)p % 16 == 0 && stride % unit == 0; };
-  const int vec = channels % 8 == 0 && rows16(x, x_stride) && rows16(out, out_stride) && rows16(state, state_stride);
-  // 16 tokens a thread once that fills the chip with 8 waves a compute unit, fewer otherwise
+  const int vec = channels % 8 == 0 && rows16(x, x_stride) && rows16(out, out_stride) && rows16(state, state_stride) &&
+                  (uintptr_t)weight % 16 == 0;
+  // 64 tokens a thread once that fills the chip with 8 waves a compute unit, fewer otherwise
   const int64_t groups = (channels + 7) / 8;
-  int tile = 16;
+  int tile = 64;
   while (tile > 1 && groups * ((s->tokens + tile - 1) / tile) < 256 * 8 * 64) tile /= 2;
   const int64_t items = groups * ((s->tokens + tile - 1) / tile), grid = (items + 255) / 256;
   ANNA_CHECK(grid <= INT32_MAX / 256, "causal_conv1d: too many tokens and channels for a launch");
 #define ANNA_CONV(W)                                                                                                       \
   case W:                                                                                                                  \
     short_conv_kernel<DT, W><<<grid, 256, 0, stream>>>((const T*)x, x_stride, (const T*)weight, (const T*)bias, (T*)state, \
-                                                       state_stride, channels, activation, (const SpanSeq*)s->buf,         \
-                                                       (int)s->sequences, (int)s->tokens, tile, vec, (T*)out, out_stride); \
+                                                       state_stride, (uint32_t)channels, activation, span_seqs(*s), span_owners(*s), \
+                                                       (int)s->tokens, tile, vec, (T*)out, out_stride);                    \
     break;
   switch (width) {
     ANNA_CONV(2) ANNA_CONV(3) ANNA_CONV(4) ANNA_CONV(5) ANNA_CONV(6) ANNA_CONV(7) ANNA_CONV(8)

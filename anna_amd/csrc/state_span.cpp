@@ -37,32 +37,32 @@ static int lay_out(int64_t n, const int32_t* slots, const int64_t* counts, const
     set_error("state span: out of host memory");
     return ANNA_MI_EINVAL;
   }
-  const int64_t total = 4 * n + steps + 2 * chains + 2 * chunks;
+  const int64_t total = 4 * n + 4 * steps + 8 * chains + 4 * chunks + tokens;
   if (words) {
     ANNA_CHECK(s->sequences == n && s->tokens == tokens && s->steps == steps && s->chains == chains && s->chunks == chunks &&
                    s->words == std::max<int64_t>(1, total),
                "state span: filled with other counts than it was planned for");
     s->max_slot = max_slot;
     int32_t* step = words + 4 * n;
-    int32_t* chain = step + steps;
-    int32_t* chunk = chain + 2 * chains;
-    int64_t first = 0, first_chunk = 0;
+    int32_t* chain = step + 4 * steps;
+    int32_t* chunk = chain + 8 * chains;
+    int32_t* owner = chunk + 4 * chunks;
+    int32_t first = 0, first_chunk = 0;
     for (int64_t i = 0; i < n; i++) {
-      const int32_t record[4] = {slots[i], (int32_t)first, (int32_t)counts[i], fresh && fresh[i] ? 1 : 0};
+      const int32_t count = (int32_t)counts[i];
+      const int32_t record[8] = {slots[i], first, count, fresh && fresh[i] ? 1 : 0, first_chunk, 0, 0, 0};
       std::copy(record, record + 4, words + 4 * i);
-      first += counts[i];
-      if (counts[i] > STEP_TOKENS) {
-        *chain++ = (int32_t)i;
-        *chain++ = (int32_t)first_chunk;
-        const int64_t m = (counts[i] + CHUNK - 1) / CHUNK;
-        for (int64_t c = 0; c < m; c++) {
-          *chunk++ = (int32_t)i;
-          *chunk++ = (int32_t)c;
+      if (count > STEP_TOKENS) {
+        chain = std::copy(record, record + 8, chain);
+        for (int32_t at = 0; at < count; at += CHUNK, first_chunk++) {
+          const int32_t part[4] = {slots[i], first + at, std::min(CHUNK, count - at), 0};
+          chunk = std::copy(part, part + 4, chunk);
         }
-        first_chunk += m;
-      } else if (counts[i] > 0) {
-        *step++ = (int32_t)i;
+      } else if (count > 0) {
+        step = std::copy(record, record + 4, step);
       }
+      owner = std::fill_n(owner, count, (int32_t)i);
+      first += count;
     }
     if (total == 0) words[0] = 0;
     return ANNA_MI_OK;

@@ -778,8 +778,9 @@ typedef struct {
   int64_t words;                  /* int32 words of buf */
   int64_t steps, chains, chunks;  /* sequences taken token by token, in chunks of 64; chunks of all chains */
   int64_t max_slot;               /* the largest slot, -1 without any */
-  const int32_t* buf;             /* device: [sequences][4] slot, first token, tokens, fresh; [steps] sequence;
-                                     [chains][2] sequence, first chunk; [chunks][2] sequence, chunk of it */
+  const int32_t* buf;             /* device: [sequences][4] slot, first token, tokens, fresh; [steps][4] the same of
+                                     the sequences taken token by token; [chains][8] the same, first chunk, 0, 0, 0;
+                                     [chunks][4] slot, first token, tokens, 0; [tokens] the token's sequence */
 } anna_mi_state_span;
 
 /* Sizes of a span of n sequences.  slots: rows of the states, each at most once, or -1 for a sequence
