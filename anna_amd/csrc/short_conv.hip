@@ -9,66 +9,68 @@
 
 namespace anna {
 
+constexpr int NC = 4;  // channels of a thread
+
 template <int DT>
-struct Vec8 {
-  typename Elem<DT>::T v[8];
+struct alignas(NC * sizeof(typename Elem<DT>::T)) Vec {
+  typename Elem<DT>::T v[NC];
 };
 
-template <int DT, int W>
+template <int DT, int W, bool VEC>
 __global__ __launch_bounds__(256) void short_conv_kernel(const typename Elem<DT>::T* __restrict__ x, int64_t x_stride,
                                                          const typename Elem<DT>::T* __restrict__ weight,
                                                          const typename Elem<DT>::T* __restrict__ bias,
                                                          typename Elem<DT>::T* state, int64_t state_stride, uint32_t channels,
                                                          int silu, const SpanSeq* __restrict__ seqs,
-                                                         const int32_t* __restrict__ owners, int tokens, int tile, int vec,
+                                                         const int32_t* __restrict__ owners, int tokens, int tile,
                                                          typename Elem<DT>::T* __restrict__ out, int64_t out_stride) {
   typedef typename Elem<DT>::T T;
-  typedef Vec8<DT> Row;
+  typedef Vec<DT> Row;
   constexpr int FOUR = 4;  // tokens whose loads go together, a group ahead of their use
-  const uint32_t groups = (channels + 7) / 8, item = blockIdx.x * 256 + threadIdx.x, c0 = item % groups * 8;
+  const uint32_t groups = (channels + NC - 1) / NC, item = blockIdx.x * 256 + threadIdx.x, c0 = item % groups * NC;
   const int64_t begin = (int64_t)(item / groups) * tile;
   if (begin >= tokens) return;
-  const int first = (int)begin, last = (int)min(begin + tile, (int64_t)tokens), n = min(8u, channels - c0);
+  const int first = (int)begin, last = (int)min(begin + tile, (int64_t)tokens), n = min((uint32_t)NC, channels - c0);
 
   auto load = [&](const T* p) {
     Row r;
-    if (vec) {
-      r = *(const Row*)__builtin_assume_aligned(p, 16);
+    if constexpr (VEC) {
+      r = *(const Row*)p;
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; e++) r.v[e] = e < n ? p[e] : (T)0;
+      for (int e = 0; e < NC; e++) r.v[e] = e < n ? p[e] : (T)0;
     }
     return r;
   };
   auto save = [&](T* p, const Row& r) {
-    if (vec) {
-      *(Row*)__builtin_assume_aligned(p, 16) = r;
+    if constexpr (VEC) {
+      *(Row*)p = r;
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; e++)
+      for (int e = 0; e < NC; e++)
         if (e < n) p[e] = r.v[e];
     }
   };
 
   int s = owners[first];
   SpanSeq seq = seqs[s];
-  float w[W][8], b[8] = {};
-  if (vec) {  // eight channels' taps lie together
+  float w[W][NC], b[NC] = {};
+  if constexpr (VEC) {  // the channels' taps lie together
 #pragma unroll
     for (int i = 0; i < W; i++) {
-      const Row r = load(weight + (int64_t)c0 * W + 8 * i);
+      const Row r = load(weight + (int64_t)c0 * W + NC * i);
 #pragma unroll
-      for (int e = 0; e < 8; e++) w[(8 * i + e) % W][(8 * i + e) / W] = Elem<DT>::to_f32(r.v[e]);
+      for (int e = 0; e < NC; e++) w[(NC * i + e) % W][(NC * i + e) / W] = Elem<DT>::to_f32(r.v[e]);
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; e++)
+    for (int e = 0; e < NC; e++)
 #pragma unroll
       for (int j = 0; j < W; j++) w[j][e] = e < n ? Elem<DT>::load(weight, (int64_t)(c0 + e) * W + j) : 0.f;
   }
   if (bias)
 #pragma unroll
-    for (int e = 0; e < 8; e++) b[e] = e < n ? Elem<DT>::load(bias, c0 + e) : 0.f;
+    for (int e = 0; e < NC; e++) b[e] = e < n ? Elem<DT>::load(bias, c0 + e) : 0.f;
 
   int t = first;
   if (t > seq.first && t < seq.first + W - 1) t = min(seq.first + min(W - 1, seq.tokens), last);  // another thread's
@@ -80,7 +82,7 @@ __global__ __launch_bounds__(256) void short_conv_kernel(const typename Elem<DT>
     if (seq.slot < 0) {
       Row zeros;
 #pragma unroll
-      for (int e = 0; e < 8; e++) zeros.v[e] = Elem<DT>::cvt(0.f);
+      for (int e = 0; e < NC; e++) zeros.v[e] = Elem<DT>::cvt(0.f);
       for (; t < stop; t++) save(out + (int64_t)t * out_stride + c0, zeros);
       continue;
     }
@@ -97,7 +99,7 @@ __global__ __launch_bounds__(256) void short_conv_kernel(const typename Elem<DT>
         win[j] = load(state + seq.slot * state_stride + (int64_t)(W - 1 + at) * channels + c0);
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; e++) win[j].v[e] = Elem<DT>::cvt(0.f);
+        for (int e = 0; e < NC; e++) win[j].v[e] = Elem<DT>::cvt(0.f);
       }
     }
     if (pos == 0) {
@@ -117,7 +119,7 @@ __global__ __launch_bounds__(256) void short_conv_kernel(const typename Elem<DT>
         save(to + (int64_t)j * channels, r);
       }
     }
-    for (int k = 0; k < run; k += FOUR) {
+    auto outputs = [&](int k, int m) {  // of `m` tokens from k on; the next ones' rows are asked for in front of the stores
       Row rows[W - 1 + FOUR];
 #pragma unroll
       for (int j = 0; j < W - 1; j++) rows[j] = win[j];
@@ -125,23 +127,26 @@ __global__ __launch_bounds__(256) void short_conv_kernel(const typename Elem<DT>
       for (int i = 0; i < FOUR; i++) rows[W - 1 + i] = next[i];
 #pragma unroll
       for (int j = 0; j < W - 1; j++) win[j] = rows[FOUR + j];
-      if (k + FOUR < run)
+      if (m == FOUR)
 #pragma unroll
         for (int i = 0; i < FOUR; i++) next[i] = load(from + (int64_t)min(k + FOUR + i, run - 1) * x_stride);
+      Row y[FOUR];
 #pragma unroll
       for (int i = 0; i < FOUR; i++)
-        if (k + i < run) {
-          Row r;
 #pragma unroll
-          for (int e = 0; e < 8; e++) {
-            float y = b[e];
+        for (int e = 0; e < NC; e++) {
+          float sum = b[e];
 #pragma unroll
-            for (int j = 0; j < W; j++) y = fmaf(Elem<DT>::to_f32(rows[i + j].v[e]), w[j][e], y);
-            r.v[e] = Elem<DT>::cvt(silu ? silu_of(y) : y);
-          }
-          save(out + (int64_t)(t + k + i) * out_stride + c0, r);
+          for (int j = 0; j < W; j++) sum = fmaf(Elem<DT>::to_f32(rows[i + j].v[e]), w[j][e], sum);
+          y[i].v[e] = Elem<DT>::cvt(silu ? silu_of(sum) : sum);
         }
-    }
+#pragma unroll
+      for (int i = 0; i < FOUR; i++)
+        if (i < m) save(out + (int64_t)(t + k + i) * out_stride + c0, y[i]);
+    };
+    int k = 0;
+    for (; k + FOUR <= run; k += FOUR) outputs(k, FOUR);
+    if (k < run) outputs(k, run - k);
     t = stop;
   }
 }
@@ -151,21 +156,19 @@ static int launch(const void* x, int64_t channels, int64_t x_stride, const void*
                   void* state, int64_t state_stride, int activation, const anna_mi_state_span* s, void* out,
                   int64_t out_stride, hipStream_t stream) {
   typedef typename Elem<DT>::T T;
-  constexpr int64_t unit = 16 / sizeof(T);
-  auto rows16 = [&](const void* p, int64_t stride) { return (uintptr_t)p % 16 == 0 && stride % unit == 0; };
-  const int vec = channels % 8 == 0 && rows16(x, x_stride) && rows16(out, out_stride) && rows16(state, state_stride) &&
-                  (uintptr_t)weight % 16 == 0;
-  // 64 tokens a thread once that fills the chip with 8 waves a compute unit, fewer otherwise
-  const int64_t groups = (channels + 7) / 8;
-  int tile = 64;
+  auto rows = [&](const void* p, int64_t stride) { return (uintptr_t)p % (NC * sizeof(T)) == 0 && stride % NC == 0; };
+  const bool vec = channels % NC == 0 && rows(x, x_stride) && rows(out, out_stride) && rows(state, state_stride) && rows(weight, NC);
+  // 24 tokens a thread once that fills the chip with 8 waves a compute unit, fewer otherwise
+  const int64_t groups = (channels + NC - 1) / NC;
+  int tile = 24;
   while (tile > 1 && groups * ((s->tokens + tile - 1) / tile) < 256 * 8 * 64) tile /= 2;
   const int64_t items = groups * ((s->tokens + tile - 1) / tile), grid = (items + 255) / 256;
   ANNA_CHECK(grid <= INT32_MAX / 256, "causal_conv1d: too many tokens and channels for a launch");
 #define ANNA_CONV(W)                                                                                                       \
   case W:                                                                                                                  \
-    short_conv_kernel<DT, W><<<grid, 256, 0, stream>>>((const T*)x, x_stride, (const T*)weight, (const T*)bias, (T*)state, \
+    (vec ? short_conv_kernel<DT, W, true> : short_conv_kernel<DT, W, false>)<<<grid, 256, 0, stream>>>((const T*)x, x_stride, (const T*)weight, (const T*)bias, (T*)state, \
                                                        state_stride, (uint32_t)channels, activation, span_seqs(*s), span_owners(*s), \
-                                                       (int)s->tokens, tile, vec, (T*)out, out_stride);                    \
+                                                       (int)s->tokens, tile, (T*)out, out_stride);                    \
     break;
   switch (width) {
     ANNA_CONV(2) ANNA_CONV(3) ANNA_CONV(4) ANNA_CONV(5) ANNA_CONV(6) ANNA_CONV(7) ANNA_CONV(8)
