@@ -17,30 +17,33 @@ struct Row8 {
   typename Elem<DT>::T v[8];
 };
 
-template <int DT>
-__device__ __forceinline__ void load8(const void* base, int64_t at, int n, bool vec, float (&f)[8]) {
+// VEC: eight columns at a time, 16-byte aligned; else `n` of them one by one
+template <int DT, bool VEC>
+__device__ __forceinline__ Row8<DT> load8(const void* base, int64_t at, int n) {
   const typename Elem<DT>::T* p = (const typename Elem<DT>::T*)base + at;
-  if (vec) {
-    const Row8<DT> v = *(const Row8<DT>*)__builtin_assume_aligned(p, 16);
+  if constexpr (VEC) return *(const Row8<DT>*)__builtin_assume_aligned(p, 16);
+  Row8<DT> r;
 #pragma unroll
-    for (int e = 0; e < 8; e++) f[e] = Elem<DT>::to_f32(v.v[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; e++) f[e] = e < n ? Elem<DT>::load(p, e) : 0.f;
-  }
+  for (int e = 0; e < 8; e++) r.v[e] = e < n ? p[e] : (typename Elem<DT>::T)0;
+  return r;
 }
 template <int DT>
-__device__ __forceinline__ void save8(void* base, int64_t at, int n, bool vec, const float (&f)[8]) {
-  typename Elem<DT>::T* p = (typename Elem<DT>::T*)base + at;
-  if (vec) {
-    Row8<DT> v;
+__device__ __forceinline__ void widen(const Row8<DT>& r, float (&f)[8]) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) v.v[e] = Elem<DT>::cvt(f[e]);
-    *(Row8<DT>*)__builtin_assume_aligned(p, 16) = v;
+  for (int e = 0; e < 8; e++) f[e] = Elem<DT>::to_f32(r.v[e]);
+}
+template <int DT, bool VEC>
+__device__ __forceinline__ void save8(void* base, int64_t at, int n, const float (&f)[8]) {
+  typename Elem<DT>::T* p = (typename Elem<DT>::T*)base + at;
+  Row8<DT> r;
+#pragma unroll
+  for (int e = 0; e < 8; e++) r.v[e] = Elem<DT>::cvt(f[e]);
+  if constexpr (VEC) {
+    *(Row8<DT>*)__builtin_assume_aligned(p, 16) = r;
   } else {
 #pragma unroll
     for (int e = 0; e < 8; e++)
-      if (e < n) p[e] = Elem<DT>::cvt(f[e]);
+      if (e < n) p[e] = r.v[e];
   }
 }
 
@@ -79,7 +82,8 @@ __device__ __forceinline__ uint32_t abs_max(const float (&y)[8], int n) {
   return m;
 }
 // Codes of eight values; `to_unit`: 448 / the group's largest
-__device__ __forceinline__ void save_codes(uint8_t* p, int n, bool vec, const float (&y)[8], float to_unit) {
+template <bool VEC>
+__device__ __forceinline__ void save_codes(uint8_t* p, int n, const float (&y)[8], float to_unit) {
   uint32_t w[2];
 #pragma unroll
   for (int h = 0; h < 2; h++) {
@@ -92,7 +96,7 @@ __device__ __forceinline__ void save_codes(uint8_t* p, int n, bool vec, const fl
     int packed = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
     w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], packed, true);
   }
-  if (vec) {
+  if constexpr (VEC) {
     *(uint2*)p = make_uint2(w[0], w[1]);
   } else {
 #pragma unroll
@@ -115,18 +119,29 @@ __device__ __forceinline__ uint32_t group_max(uint32_t m, int lanes) {
   return m;
 }
 
-template <int DT, int LANES, int VECS, bool CODES>
-__global__ __launch_bounds__(256) void rms_norm_kernel(const anna_mi_rms_norm_args a, int vec_in) {
+template <int DT, int LANES, int VECS, bool CODES, bool VEC>
+__global__ __launch_bounds__(256) void rms_norm_kernel(const anna_mi_rms_norm_args a) {
   constexpr int ROWS = 256 / LANES;
   __shared__ float sums[4];
   __shared__ uint32_t tops[4];
-  const bool vec = vec_in;
   const int lane = threadIdx.x % LANES;
   int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES;
   const bool live = row < a.rows;
   if (!live) row = a.rows - 1;  // its lanes take part in the exchanges, and store nothing
   const int64_t cols = a.cols;
 
+  // everything is asked for in front of the sum
+  Row8<DT> x[VECS], old[VECS], gate[VECS], weight[VECS];
+#pragma unroll
+  for (int i = 0; i < VECS; i++) {
+    const int64_t c = 8 * (int64_t)(lane + LANES * i);
+    const int n = (int)min((int64_t)8, max((int64_t)0, cols - c));
+    if (n == 0) continue;
+    x[i] = load8<DT, VEC>(a.x, row * a.x_stride + c, n);
+    if (a.residual) old[i] = load8<DT, VEC>(a.residual, row * a.residual_stride + c, n);
+    if (a.gate) gate[i] = load8<DT, VEC>(a.gate, row * a.gate_stride + c, n);
+    weight[i] = load8<DT, VEC>(a.weight, c, n);
+  }
   float h[VECS][8], ss = 0.f;
 #pragma unroll
   for (int i = 0; i < VECS; i++) {
@@ -137,13 +152,13 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(const anna_mi_rms_norm_ar
       for (int e = 0; e < 8; e++) h[i][e] = 0.f;
       continue;
     }
-    load8<DT>(a.x, row * a.x_stride + c, n, vec, h[i]);
+    widen<DT>(x[i], h[i]);
     if (a.residual) {
-      float old[8];
-      load8<DT>(a.residual, row * a.residual_stride + c, n, vec, old);
+      float r[8];
+      widen<DT>(old[i], r);
 #pragma unroll
-      for (int e = 0; e < 8; e++) h[i][e] = Elem<DT>::to_f32(Elem<DT>::cvt(h[i][e] + old[e]));
-      if (live) save8<DT>(a.residual, row * a.residual_stride + c, n, vec, h[i]);
+      for (int e = 0; e < 8; e++) h[i][e] = Elem<DT>::to_f32(Elem<DT>::cvt(h[i][e] + r[e]));
+      if (live) save8<DT, VEC>(a.residual, row * a.residual_stride + c, n, h[i]);
     }
 #pragma unroll
     for (int e = 0; e < 8; e++) ss = fmaf(h[i][e], h[i][e], ss);
@@ -157,18 +172,18 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(const anna_mi_rms_norm_ar
     const int n = (int)min((int64_t)8, max((int64_t)0, cols - c));
     if (n > 0) {
       float w[8];
-      load8<DT>(a.weight, c, n, vec, w);
+      widen<DT>(weight[i], w);
 #pragma unroll
       for (int e = 0; e < 8; e++) h[i][e] = h[i][e] * rs * (w[e] + a.weight_offset);
       if (a.gate) {
         float g[8];
-        load8<DT>(a.gate, row * a.gate_stride + c, n, vec, g);
+        widen<DT>(gate[i], g);
 #pragma unroll
         for (int e = 0; e < 8; e++) h[i][e] *= silu_of(g[e]);
       }
     }
     if constexpr (!CODES) {
-      if (live && n > 0) save8<DT>(a.out, row * a.out_stride + c, n, vec, h[i]);
+      if (live && n > 0) save8<DT, VEC>(a.out, row * a.out_stride + c, n, h[i]);
     } else {
       const uint32_t m = abs_max(h[i], n);
       if (a.group == cols) {
@@ -176,7 +191,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(const anna_mi_rms_norm_ar
       } else {  // every group lies in neighbouring lanes of one vector row
         const Scale s = scale_of(group_max(m, (int)a.group / 8));
         if (live && n > 0) {
-          save_codes((uint8_t*)a.out + row * a.out_stride + c, n, vec, h[i], s.to_unit);
+          save_codes<VEC>((uint8_t*)a.out + row * a.out_stride + c, n, h[i], s.to_unit);
           if (c % a.group == 0) a.scales[row * (cols / a.group) + c / a.group] = s.scale;
         }
       }
@@ -190,18 +205,17 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(const anna_mi_rms_norm_ar
       for (int i = 0; i < VECS; i++) {
         const int64_t c = 8 * (int64_t)(lane + LANES * i);
         const int n = (int)min((int64_t)8, max((int64_t)0, cols - c));
-        if (live && n > 0) save_codes((uint8_t*)a.out + row * a.out_stride + c, n, vec, h[i], s.to_unit);
+        if (live && n > 0) save_codes<VEC>((uint8_t*)a.out + row * a.out_stride + c, n, h[i], s.to_unit);
       }
     }
   }
 }
 
 // Rows of any length: a workgroup a row, read again for every pass (the second from L2)
-template <int DT, bool CODES>
-__global__ __launch_bounds__(256) void rms_norm_long_kernel(const anna_mi_rms_norm_args a, int vec_in) {
+template <int DT, bool CODES, bool VEC>
+__global__ __launch_bounds__(256) void rms_norm_long_kernel(const anna_mi_rms_norm_args a) {
   __shared__ float sums[4];
   __shared__ uint32_t tops[4];
-  const bool vec = vec_in;
   const int64_t row = blockIdx.x, cols = a.cols;
   const void* src = a.residual ? a.residual : a.x;
   const int64_t src_stride = a.residual ? a.residual_stride : a.x_stride;
@@ -209,13 +223,13 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(const anna_mi_rms_no
   for (int64_t c = 8 * (int64_t)threadIdx.x; c < cols; c += 2048) {
     const int n = (int)min((int64_t)8, cols - c);
     float h[8];
-    load8<DT>(a.x, row * a.x_stride + c, n, vec, h);
+    widen<DT>(load8<DT, VEC>(a.x, row * a.x_stride + c, n), h);
     if (a.residual) {
       float old[8];
-      load8<DT>(a.residual, row * a.residual_stride + c, n, vec, old);
+      widen<DT>(load8<DT, VEC>(a.residual, row * a.residual_stride + c, n), old);
 #pragma unroll
       for (int e = 0; e < 8; e++) h[e] = Elem<DT>::to_f32(Elem<DT>::cvt(h[e] + old[e]));
-      save8<DT>(a.residual, row * a.residual_stride + c, n, vec, h);  // read again below by the same thread
+      save8<DT, VEC>(a.residual, row * a.residual_stride + c, n, h);  // read again below by the same thread
     }
 #pragma unroll
     for (int e = 0; e < 8; e++) ss = fmaf(h[e], h[e], ss);
@@ -223,13 +237,13 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(const anna_mi_rms_no
   const float rs = rsqrtf(row_sum<256>(ss, sums) / (float)cols + a.eps);
   auto value = [&](int64_t c, int n, float (&h)[8]) {
     float w[8];
-    load8<DT>(src, row * src_stride + c, n, vec, h);
-    load8<DT>(a.weight, c, n, vec, w);
+    widen<DT>(load8<DT, VEC>(src, row * src_stride + c, n), h);
+    widen<DT>(load8<DT, VEC>(a.weight, c, n), w);
 #pragma unroll
     for (int e = 0; e < 8; e++) h[e] = h[e] * rs * (w[e] + a.weight_offset);
     if (a.gate) {
       float g[8];
-      load8<DT>(a.gate, row * a.gate_stride + c, n, vec, g);
+      widen<DT>(load8<DT, VEC>(a.gate, row * a.gate_stride + c, n), g);
 #pragma unroll
       for (int e = 0; e < 8; e++) h[e] *= silu_of(g[e]);
     }
@@ -255,11 +269,11 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(const anna_mi_rms_no
     float h[8] = {};
     if (n > 0) value(c, n, h);
     if constexpr (!CODES) {
-      if (n > 0) save8<DT>(a.out, row * a.out_stride + c, n, vec, h);
+      if (n > 0) save8<DT, VEC>(a.out, row * a.out_stride + c, n, h);
     } else {
       if (!by_row) s = scale_of(group_max(abs_max(h, n), (int)a.group / 8));
       if (n > 0) {
-        save_codes((uint8_t*)a.out + row * a.out_stride + c, n, vec, h, s.to_unit);
+        save_codes<VEC>((uint8_t*)a.out + row * a.out_stride + c, n, h, s.to_unit);
         if (!by_row && c % a.group == 0) a.scales[row * (cols / a.group) + c / a.group] = s.scale;
       }
     }
@@ -274,7 +288,9 @@ template <int DT, bool CODES> static int launch_norm(const anna_mi_rms_norm_args
                    (CODES ? (uintptr_t)a.out % 8 == 0 && (a.rows == 1 || a.out_stride % 8 == 0) : rows16(a.out, a.out_stride));
   const int64_t vecs = (a.cols + 7) / 8;
   auto blocks = [&](int rows) { return (a.rows + rows - 1) / rows; };
-#define ANNA_NORM(LANES, VECS) rms_norm_kernel<DT, LANES, VECS, CODES><<<blocks(256 / LANES), 256, 0, stream>>>(a, vec)
+#define ANNA_NORM(LANES, VECS)                                                                                          \
+  (vec ? rms_norm_kernel<DT, LANES, VECS, CODES, true> : rms_norm_kernel<DT, LANES, VECS, CODES, false>)<<<blocks(256 / LANES), \
+                                                                                                           256, 0, stream>>>(a)
   if (vecs <= 8) ANNA_NORM(8, 1);
   else if (vecs <= 16) ANNA_NORM(16, 1);
   else if (vecs <= 32) ANNA_NORM(32, 1);
@@ -282,7 +298,7 @@ template <int DT, bool CODES> static int launch_norm(const anna_mi_rms_norm_args
   else if (vecs <= 256) ANNA_NORM(256, 1);
   else if (vecs <= 512) ANNA_NORM(256, 2);
   else if (vecs <= 1024) ANNA_NORM(256, 4);
-  else rms_norm_long_kernel<DT, CODES><<<a.rows, 256, 0, stream>>>(a, vec);
+  else (vec ? rms_norm_long_kernel<DT, CODES, true> : rms_norm_long_kernel<DT, CODES, false>)<<<a.rows, 256, 0, stream>>>(a);
 #undef ANNA_NORM
   ANNA_LAUNCH_CHECK("rms_norm");
   return ANNA_MI_OK;
