@@ -89,10 +89,34 @@ __device__ __forceinline__ void split(const float (&x)[8], f16x8& hi, f16x8& lo)
 
 // ---------------------------------------------------------------- what needs no state
 
-// 2^t of t <= 0, or of any t: its whole part apart, so that a long sum's fraction keeps its bits
-__device__ __forceinline__ float exp2_of(double t) {
-  const double whole = __builtin_rint(t);
-  return ldexpf(__builtin_amdgcn_exp2f((float)(t - whole)), (int)fmin(fmax(whole, -10000.), 10000.));
+// A sum of logarithms to base 2 in two floats: the difference of two such sums is short of fp32 only by 2^-24 of itself,
+// however long the sums are
+struct Log2 {
+  float hi, lo;
+};
+__device__ __forceinline__ float exp2_of(Log2 a, Log2 b) { return __builtin_amdgcn_exp2f((a.hi - b.hi) + (a.lo - b.lo)); }
+__device__ __forceinline__ float exp2_of(Log2 a) { return __builtin_amdgcn_exp2f(a.hi + a.lo); }
+
+// Sums up to and with every lane
+template <int SHIFT>
+__device__ __forceinline__ double from_lane_before(double v) {  // of the lane SHIFT before in 16 lanes, 0 where there is none
+  const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)bits, 0x110 + SHIFT, 0xf, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(bits >> 32), 0x110 + SHIFT, 0xf, 0xf, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double lane_value(double v, int lane) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)bits, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(bits >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double running_sum(double v, int row) {
+  v += from_lane_before<1>(v);
+  v += from_lane_before<2>(v);
+  v += from_lane_before<4>(v);
+  v += from_lane_before<8>(v);
+  const double t0 = lane_value(v, 15), t1 = lane_value(v, 31), t2 = lane_value(v, 47);
+  return v + (row > 2 ? t0 + t1 + t2 : row > 1 ? t0 + t1 : row > 0 ? t0 : 0.);
 }
 
 // A workgroup takes a chunk, a key head and `per` of its value heads.  A wave has the rows row_of(wave, 0..15) of K and Q,
@@ -106,7 +130,7 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
   constexpr int LF = CHUNK + 4;  // floats of a row of A, then T in its place, then P
   __shared__ _Float16 K[CHUNK][LD];
   __shared__ float A[CHUNK][LF];
-  __shared__ double sums[4][CHUNK];  // a / ln 2 of the next four value heads
+  __shared__ Log2 sums[4][CHUNK];  // a / ln 2 of the next four value heads
   __shared__ float betas[4][CHUNK], kf[CHUNK], qf[CHUNK], tops[2][4];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
@@ -117,6 +141,24 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
   if (here.slot < 0) return;
   const int64_t first = here.first;
   const int tokens = here.tokens;
+
+  // decays of four value heads, a wave each: sums of logarithms in 64 bits, as their differences count; -inf stands
+  // for e^-10^4 = 0
+  auto gate_raw = [&](int h) {
+    return h < per && lane < tokens ? Gate{gate_value(a.decay, a.gates_dtype, (first + lane) * a.decay_stride + hv0 + h),
+                                           gate_value(a.beta, a.gates_dtype, (first + lane) * a.beta_stride + hv0 + h)}
+                                    : Gate{0.f, 0.f};
+  };
+  auto gates = [&](int h, Gate gate) {
+    if (h < per) {
+      gate = lane < tokens ? gate_of(a, gate, hv0 + h) : Gate{0.f, 0.f};
+      const double s = running_sum(gate.g < -1e4f ? -1e4 : (double)gate.g, g) * 1.4426950408889634;
+      const float hi = (float)s;
+      sums[wave][lane] = {hi, (float)(s - hi)};
+      betas[wave][lane] = gate.beta;
+    }
+  };
+  const Gate mine_raw = gate_raw(wave);
 
   const int mine = row_of(wave, n);
   u32x4 raw[2][KS];
@@ -132,23 +174,7 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
     for (int s = 0; s < KS; s++) raw[0][s] = raw[1][s] = u32x4{0, 0, 0, 0};
   }
 
-  // decays of four value heads, a wave each: sums of logarithms in 64 bits, as their differences count; -inf stands
-  // for e^-10^4 = 0
-  auto gates = [&](int h) {
-    if (h < per) {
-      Gate gate{0.f, 0.f};
-      if (lane < tokens) gate = gate_of(a, first + lane, hv0 + h);
-      double s = gate.g < -1e4f ? -1e4 : (double)gate.g;
-#pragma unroll
-      for (int off = 1; off < 64; off *= 2) {
-        const double o = __shfl_up(s, off, 64);
-        if (lane >= off) s += o;
-      }
-      sums[wave][lane] = s * 1.4426950408889634;
-      betas[wave][lane] = gate.beta;
-    }
-  };
-  gates(wave);
+  gates(wave, mine_raw);
 
   // a power of two is taken out of every row, and what is left to make the unit vector kept as a factor
   f16x8 kr[KS], qr[KS];
@@ -219,35 +245,36 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
     if (h > 0) {
       __syncthreads();  // the head before is done with LDS
       if (h % 4 == 0) {
-        gates(h + wave);
+        gates(h + wave, gate_raw(h + wave));
         __syncthreads();
       }
     }
-    const double* const at = sums[h % 4];
+    const Log2* const at = sums[h % 4];
     const float* const beta = betas[h % 4];
 
     // A and P; P's rows are kept in registers until A's place is free
     f32x4 P[4];
     float p_top = 0.f, t_top = 0.f;
-    double ai[4];
-    float bi[4];
+    Log2 ai[4], aj[4];
+    float bi[4], cj[4];
 #pragma unroll
     for (int r = 0; r < 4; r++) {
       ai[r] = at[row_of(wave, 4 * g + r)];
       bi[r] = beta[row_of(wave, 4 * g + r)];
+      aj[r] = at[16 * r + n];
+      cj[r] = kf[16 * r + n];
     }
 #pragma unroll
     for (int ct = 0; ct < 4; ct++) {
       const int j = 16 * ct + n;
       if (ct < tiles) {
-        const double aj = at[j];
-        const float cj = kf[j];
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
+        for (int r = 0; r < 4; r++) {  // without branches: tokens that are not seen have a decay of e^-inf
           const int i = row_of(wave, 4 * g + r);
-          const float d = i >= j ? exp2_of(ai[r] - aj) * cj : 0.f;
-          A[i][j] = i > j ? bi[r] * (ki[r] * kk[ct][r]) * d : 0.f;
-          P[ct][r] = (qi[r] * qk[ct][r]) * d;
+          const float t = (ai[r].hi - aj[ct].hi) + (ai[r].lo - aj[ct].lo), d = __builtin_amdgcn_exp2f(i >= j ? t : -INFINITY) * cj[ct];
+          const float x = bi[r] * (ki[r] * kk[ct][r]) * d, y = (qi[r] * qk[ct][r]) * d;
+          A[i][j] = i > j ? x : 0.f;
+          P[ct][r] = i >= j ? y : 0.f;
           p_top = fmaxf(p_top, fabsf(P[ct][r]));
         }
       } else {
@@ -341,7 +368,7 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
       const float e = exp2_of(at[tid]);
       to->decayed_k[tid] = e * kf[tid];
       to->decayed_q[tid] = e * qf[tid];
-      to->to_end[tid] = exp2_of(at[CHUNK - 1] - at[tid]) * kf[tid] * ts.up;
+      to->to_end[tid] = exp2_of(at[CHUNK - 1], at[tid]) * kf[tid] * ts.up;
       if (tid == CHUNK - 1) to->end = e;
       if (tid == 0) {
         to->t_scale = ts.up;
