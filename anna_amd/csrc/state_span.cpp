@@ -44,16 +44,16 @@ static int lay_out(int64_t n, const int32_t* slots, const int64_t* counts, const
                "state span: filled with other counts than it was planned for");
     s->max_slot = max_slot;
     int32_t* step = words + 4 * n;
-    int32_t* chain = step + 4 * steps;
+    int32_t* const chain = step + 4 * steps;
     int32_t* chunk = chain + 8 * chains;
     int32_t* owner = chunk + 4 * chunks;
     int32_t first = 0, first_chunk = 0;
-    for (int64_t i = 0; i < n; i++) {
+    for (int64_t i = 0, c = 0; i < n; i++) {
       const int32_t count = (int32_t)counts[i];
       const int32_t record[8] = {slots[i], first, count, fresh && fresh[i] ? 1 : 0, first_chunk, 0, 0, 0};
       std::copy(record, record + 4, words + 4 * i);
       if (count > STEP_TOKENS) {
-        chain = std::copy(record, record + 8, chain);
+        std::copy(record, record + 8, chain + 8 * c++);
         for (int32_t at = 0; at < count; at += CHUNK, first_chunk++) {
           const int32_t part[4] = {slots[i], first + at, std::min(CHUNK, count - at), 0};
           chunk = std::copy(part, part + 4, chunk);
@@ -64,6 +64,12 @@ static int lay_out(int64_t n, const int32_t* slots, const int64_t* counts, const
       owner = std::fill_n(owner, count, (int32_t)i);
       first += count;
     }
+    // the longest chains first: their workgroups start first, and the short ones fill what is left
+    struct Record {
+      int32_t v[8];
+    };
+    Record* const sorted = (Record*)chain;
+    std::stable_sort(sorted, sorted + chains, [](const Record& a, const Record& b) { return a.v[2] > b.v[2]; });
     if (total == 0) words[0] = 0;
     return ANNA_MI_OK;
   }

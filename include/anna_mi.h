@@ -779,7 +779,8 @@ typedef struct {
   int64_t steps, chains, chunks;  /* sequences taken token by token, in chunks of 64; chunks of all chains */
   int64_t max_slot;               /* the largest slot, -1 without any */
   const int32_t* buf;             /* device: [sequences][4] slot, first token, tokens, fresh; [steps][4] the same of
-                                     the sequences taken token by token; [chains][8] the same, first chunk, 0, 0, 0;
+                                     the sequences taken token by token; [chains][8] the same, first chunk, 0, 0, 0,
+                                     the longest first;
                                      [chunks][4] slot, first token, tokens, 0; [tokens] the token's sequence */
 } anna_mi_state_span;
 

@@ -34,7 +34,7 @@ def test_layout():
     assert (span.sequences, span.tokens, span.steps, span.chains, span.chunks, span.max_slot) == (5, 155, 2, 2, 4, 9)
     assert words[:20] == [5, 0, 1, 0, -1, 1, 12, 1, 0, 13, 0, 0, 9, 13, 13, 0, 2, 26, 129, 1]
     assert words[20:28] == [5, 0, 1, 0, -1, 1, 12, 1]
-    assert words[28:44] == [9, 13, 13, 0, 0, 0, 0, 0, 2, 26, 129, 1, 1, 0, 0, 0]
+    assert words[28:44] == [2, 26, 129, 1, 1, 0, 0, 0, 9, 13, 13, 0, 0, 0, 0, 0]
     assert words[44:60] == [9, 13, 13, 0, 2, 26, 64, 0, 2, 90, 64, 0, 2, 154, 1, 0]
     assert words[60:] == [0] + [1] * 12 + [3] * 13 + [4] * 129
     span, words = plan([], [])
