@@ -633,12 +633,12 @@ int64_t pool_stride(const Tensor& t, const at::Device& dev, at::ScalarType dt, a
 }
 
 OptTensor gated_delta(const Tensor& query, const Tensor& key, const Tensor& value, const Tensor& decay, const Tensor& beta,
-                      const Tensor& state, const OptTensor& a_log, const OptTensor& dt_bias, uintptr_t span_address, double scaling,
-                      bool normalize, uintptr_t stream) {
+                      const Tensor& state, const OptTensor& a_log, const OptTensor& dt_bias, uintptr_t span_address, int64_t device,
+                      double scaling, bool normalize, uintptr_t stream) {
   const auto* span = reinterpret_cast<const anna_mi_state_span*>(span_address);
   const at::Device dev = query.device();
   const at::ScalarType dt = query.scalar_type();
-  if (query.dim() != 3 || value.dim() != 3 || (dt != at::kBFloat16 && dt != at::kHalf) || span->tokens != query.size(0)) return std::nullopt;
+  if (!query.is_cuda() || dev.index() != device || query.dim() != 3 || value.dim() != 3 || (dt != at::kBFloat16 && dt != at::kHalf) || span->tokens != query.size(0)) return std::nullopt;
   const int64_t tokens = query.size(0), HK = query.size(1), DK = query.size(2), HV = value.size(1), DV = value.size(2);
   if (!paged_rows(query, dev, dt, tokens, HK, DK) || !paged_rows(key, dev, dt, tokens, HK, DK) || !paged_rows(value, dev, dt, tokens, HV, DV))
     return std::nullopt;
@@ -671,11 +671,11 @@ OptTensor gated_delta(const Tensor& query, const Tensor& key, const Tensor& valu
 }
 
 OptTensor causal_conv1d(const Tensor& x, const Tensor& weight, const OptTensor& bias, const Tensor& state, uintptr_t span_address,
-                        bool silu, uintptr_t stream) {
+                        int64_t device, bool silu, uintptr_t stream) {
   const auto* span = reinterpret_cast<const anna_mi_state_span*>(span_address);
   const at::Device dev = x.device();
   const at::ScalarType dt = x.scalar_type();
-  if (x.dim() != 2 || dtype_code(x) < 0 || !given(x, dev) || span->tokens != x.size(0)) return std::nullopt;
+  if (!x.is_cuda() || dev.index() != device || x.dim() != 2 || dtype_code(x) < 0 || !given(x, dev) || span->tokens != x.size(0)) return std::nullopt;
   const int64_t tokens = x.size(0), channels = x.size(1);
   if (channels < 1 || (channels > 1 && x.stride(1) != 1) || (tokens > 1 && x.stride(0) < channels) || !given(weight, dev) ||
       !is(weight, dev, dt) || weight.dim() != 2 || weight.size(0) != channels || weight.size(1) < 2 || weight.size(1) > 8 ||
@@ -690,13 +690,13 @@ OptTensor causal_conv1d(const Tensor& x, const Tensor& weight, const OptTensor& 
   return out;
 }
 
-// out, or codes and scales with a group; both undefined for calls that are left to the caller
-std::pair<OptTensor, OptTensor> rms_norm(const Tensor& x, const Tensor& weight, double eps, double weight_offset, const OptTensor& residual,
-                                         const OptTensor& gate, int64_t group, uintptr_t stream) {
-  const std::pair<OptTensor, OptTensor> none;
+// out, or with a group codes, and scales; undefined for calls that are left to the caller
+Tensor norm(const Tensor& x, const Tensor& weight, double eps, double weight_offset, const OptTensor& residual, const OptTensor& gate,
+            int64_t group, Tensor* scales, int64_t device, uintptr_t stream) {
+  const Tensor none;
   const at::Device dev = x.device();
   const at::ScalarType dt = x.scalar_type();
-  if (x.dim() < 1 || dtype_code(x) < 0 || x.numel() == 0 || !(eps >= 0.0 && eps < 1e30)) return none;
+  if (!x.is_cuda() || dev.index() != device || x.dim() < 1 || dtype_code(x) < 0 || x.numel() == 0 || !(eps >= 0.0 && eps < 1e30)) return none;
   const int64_t cols = x.size(-1), rows = x.numel() / cols;
   // rows with one stride: contiguous tensors, and matrices
   auto lies = [&](const Tensor& t, int64_t& stride) {
@@ -714,16 +714,29 @@ std::pair<OptTensor, OptTensor> rms_norm(const Tensor& x, const Tensor& weight, 
   a.eps = (float)eps, a.weight_offset = (float)weight_offset, a.out_stride = cols;
   const auto options = x.options().requires_grad(false);
   Tensor out = at::empty(x.sizes(), group > 0 ? options.dtype(at::kFloat8_e4m3fn) : options);
-  OptTensor scales;
   a.out = ptr(out);
   if (group > 0) {
     auto shape = x.sizes().vec();
     shape.back() = cols / group;
-    scales = at::empty(shape, options.dtype(at::kFloat));
+    *scales = at::empty(shape, options.dtype(at::kFloat));
     a.scales = (float*)ptr(*scales);
   }
   check(lib.rms_norm(&a, stream_ptr(stream)), "anna_mi_rms_norm");
-  return {out, scales};
+  return out;
+}
+
+OptTensor rms_norm(const Tensor& x, const Tensor& weight, double eps, double weight_offset, const OptTensor& residual, const OptTensor& gate,
+                   int64_t device, uintptr_t stream) {
+  Tensor out = norm(x, weight, eps, weight_offset, residual, gate, 0, nullptr, device, stream);
+  return out.defined() ? OptTensor(std::move(out)) : std::nullopt;
+}
+
+std::optional<std::pair<Tensor, Tensor>> rms_norm_e4m3(const Tensor& x, const Tensor& weight, double eps, double weight_offset,
+                                                       const OptTensor& residual, const OptTensor& gate, int64_t group, int64_t device,
+                                                       uintptr_t stream) {
+  Tensor scales, codes = norm(x, weight, eps, weight_offset, residual, gate, group, &scales, device, stream);
+  if (!codes.defined()) return std::nullopt;
+  return std::make_pair(std::move(codes), std::move(scales));
 }
 
 }  // namespace
@@ -752,4 +765,5 @@ PYBIND11_MODULE(_torch_host, m) {
   m.def("gated_delta", &gated_delta, no_gil);
   m.def("causal_conv1d", &causal_conv1d, no_gil);
   m.def("rms_norm", &rms_norm, no_gil);
+  m.def("rms_norm_e4m3", &rms_norm_e4m3, no_gil);
 }

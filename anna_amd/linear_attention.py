@@ -52,7 +52,8 @@ class StateSpan:
         device = torch.device(device)
         if device.type != "cuda":
             raise RuntimeError(f"StateSpan needs a ROCm device, got {device}")
-        self.device = torch.device("cuda", torch.cuda.current_device() if device.index is None else device.index)
+        self._index = torch.cuda.current_device() if device.index is None else device.index
+        self.device = torch.device("cuda", self._index)
         self._counts = None
         self._c = _lib.StateSpan()
         self._ref = ctypes.byref(self._c)
@@ -94,11 +95,11 @@ class StateSpan:
             return torch.cuda.is_current_stream_capturing()
 
     def _stream(self) -> int:
-        return torch._C._cuda_getCurrentRawStream(self.device.index)
+        return torch._C._cuda_getCurrentRawStream(self._index)
 
     def _used(self) -> int:
         """The current stream, on which the span's buffer is used from now on."""
-        stream = self._stream()
+        stream = _raw_stream(self._index)
         if stream not in self._streams:
             self._streams.add(stream)
             self._buf.record_stream(torch.cuda.current_stream(self.device))
@@ -190,10 +191,9 @@ def _check_span(what: str, span: StateSpan, tokens: int, device: torch.device) -
     return span._used()
 
 
-def _here(t: torch.Tensor, span: StateSpan | None = None) -> bool:
-    """Whether a call is on the current device, which the host module takes for granted; it answers None to
-    calls that the general way below converts or refuses."""
-    return t.is_cuda and t.device.index == torch.cuda.current_device() and (span is None or span.device == t.device)
+# The host module takes the plain calls on the current device; it answers None to those that the general way
+# below converts or refuses.
+_host, _cuda_device, _raw_stream = _lib.host, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 # ---------------------------------------------------------------- operators
@@ -208,8 +208,8 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | No
     with the rows of the sequence's state in front.  weight [channels, width], width 2 to 8; state [slots, width - 1,
     channels], the last inputs of every sequence, oldest first, updated in place; all of one type (bf16, fp16
     or fp32; sums in fp32).  x may be strided by rows (a slice of a projection).  activation: "silu" or None.  out must not overlap x."""
-    if out is None and span is not None and _here(x, span):
-        got = _lib.host().causal_conv1d(x, weight, bias, state, span._address, activation == "silu", span._used()) if activation in ("silu", None) else None
+    if out is None and span is not None and x.is_cuda and _cuda_device() == span._index and (activation == "silu" or activation is None):
+        got = _host().causal_conv1d(x, weight, bias, state, span._address, span._index, activation is not None, span._used())
         if got is not None:
             return got
     if x.dim() != 2 or x.dtype not in _lib._DTYPE_CODES:
@@ -262,8 +262,8 @@ def gated_delta_rule(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
 
     Sequences of up to 12 tokens go token by token, longer ones in chunks of 64 tokens, with a
     workspace of about 20 KB a chunk and value head.  Sums, products and the state are fp32 or as exact."""
-    if out is None and span is not None and _here(query, span):
-        got = _lib.host().gated_delta(query, key, value, decay, beta, state, a_log, dt_bias, span._address, scaling, normalize, span._used())
+    if out is None and span is not None and query.is_cuda and _cuda_device() == span._index:
+        got = _host().gated_delta(query, key, value, decay, beta, state, a_log, dt_bias, span._address, span._index, scaling, normalize, span._used())
         if got is not None:
             return got
     if query.dim() != 3 or value.dim() != 3 or query.dtype not in (torch.bfloat16, torch.float16):
@@ -372,8 +372,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, weight
     residual (same shape): x is added to it first, in place, and the sum, as the type holds it, is what is
     normalised.  out (contiguous) may be x or gate themselves, and overlaps nothing else."""
     if out is None:
-        if _here(x):
-            got = _lib.host().rms_norm(x, weight, eps, weight_offset, residual, gate, 0, _lib.stream_of(x))[0]
+        if x.is_cuda:
+            device = _cuda_device()
+            got = _host().rms_norm(x, weight, eps, weight_offset, residual, gate, device, _raw_stream(device))
             if got is not None:
                 return got
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
@@ -399,10 +400,11 @@ def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, w
     group = cols if group_size is None else operator.index(group_size)
     if group != cols and (group not in E4M3_GROUPS or cols % group):
         raise ValueError(f"group_size {group} of {cols} columns: 32, 64 or 128 (a divisor) or all columns are supported")
-    if _here(x):
-        codes, scales = _lib.host().rms_norm(x, weight, eps, weight_offset, residual, gate, group, _lib.stream_of(x))
-        if codes is not None:
-            return codes, scales
+    if x.is_cuda:
+        device = _cuda_device()
+        got = _host().rms_norm_e4m3(x, weight, eps, weight_offset, residual, gate, group, device, _raw_stream(device))
+        if got is not None:
+            return got
     codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
     scales = torch.empty((*x.shape[:-1], cols // group), dtype=torch.float32, device=x.device)
     _norm(x, weight, float(eps), float(weight_offset), residual, gate, codes, scales, group)
