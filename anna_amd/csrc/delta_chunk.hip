@@ -33,10 +33,11 @@ __device__ __forceinline__ void t_frag(int f, int& mt, int& ks) {
   mt = ks ? f - 2 : f;
 }
 
-// Factors of a chunk and value head: of K S, of Q S, of (T' / its scale) x on its way to the state, and {e^{a_63}, scale of T', of P}
+// Factors of a chunk and value head: e^a and k's for K S; of (T' / its scale) x on its way to the state; e^a for Q S; q's
+// for the output (P and Q are without them, so rows of any size keep their bits); e^{a_63}, the scales of T' and P
 struct Factors {
-  float decayed_k[CHUNK], decayed_q[CHUNK], to_end[CHUNK];
-  float end, t_scale, p_scale, pad[61];
+  float decayed_k[CHUNK], to_end[CHUNK], decay[CHUNK], q[CHUNK];
+  float end, t_scale, p_scale, pad[253];
 };
 
 // The workspace: K and Q of every chunk and key head, T' (hi, lo), the factors and P (hi, and lo for fp16) of every
@@ -138,7 +139,7 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
   const uint32_t chunk = blockIdx.x / parts, hv0 = blockIdx.x % parts * per, hk = hv0 / ratio;
   const bool writes_k = hv0 % ratio == 0;
   const SpanChunk here = chunks[chunk];
-  if (here.slot < 0) return;
+  if ((uint32_t)here.slot >= (uint32_t)a.slots) return;
   const int64_t first = here.first;
   const int tokens = here.tokens;
 
@@ -233,12 +234,9 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
         kk[ct] = mfma16(kr[s], col, kk[ct]);
         qk[ct] = mfma16(qr[s], col, qk[ct]);
       }
-  float ki[4], qi[4];
+  float ki[4];
 #pragma unroll
-  for (int r = 0; r < 4; r++) {
-    ki[r] = kf[row_of(wave, 4 * g + r)];
-    qi[r] = qf[row_of(wave, 4 * g + r)];
-  }
+  for (int r = 0; r < 4; r++) ki[r] = kf[row_of(wave, 4 * g + r)];
 
   for (int h = 0; h < per; h++) {
     const int64_t hv = hv0 + h;
@@ -272,10 +270,10 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
         for (int r = 0; r < 4; r++) {  // without branches: tokens that are not seen have a decay of e^-inf
           const int i = row_of(wave, 4 * g + r);
           const float t = (ai[r].hi - aj[ct].hi) + (ai[r].lo - aj[ct].lo), d = __builtin_amdgcn_exp2f(i >= j ? t : -INFINITY) * cj[ct];
-          const float x = bi[r] * (ki[r] * kk[ct][r]) * d, y = (qi[r] * qk[ct][r]) * d;
+          const float x = bi[r] * (ki[r] * kk[ct][r]) * d, y = qk[ct][r] * d;
           A[i][j] = i > j ? x : 0.f;
           P[ct][r] = i >= j ? y : 0.f;
-          p_top = fmaxf(p_top, fabsf(P[ct][r]));
+          p_top = fmaxf(p_top, fabsf(P[ct][r]) < INFINITY ? fabsf(P[ct][r]) : 0.f);  // a q that is not finite is its row's affair
         }
       } else {
         P[ct] = zero;
@@ -367,7 +365,8 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
       Factors* to = ws.factors(chunk, hv);
       const float e = exp2_of(at[tid]);
       to->decayed_k[tid] = e * kf[tid];
-      to->decayed_q[tid] = e * qf[tid];
+      to->decay[tid] = e;
+      to->q[tid] = qf[tid];
       to->to_end[tid] = exp2_of(at[CHUNK - 1], at[tid]) * kf[tid] * ts.up;
       if (tid == CHUNK - 1) to->end = e;
       if (tid == 0) {
@@ -399,6 +398,16 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
 // ---------------------------------------------------------------- the chain of states
 
 __device__ __forceinline__ f16x8 frag(const char* base, int f, int lane) { return *(const f16x8*)(base + f * FRAG + 16 * lane); }
+
+// Two values rounded to the type, in one register
+template <int DT> __device__ __forceinline__ uint32_t pair_of(float x, float y) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  const f32x2 v = {x, y};
+  if constexpr (DT == ANNA_MI_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+}
 
 // Largest of a column, over the four lanes that hold it
 __device__ __forceinline__ float column_max(float v) {
@@ -500,7 +509,7 @@ __global__ __launch_bounds__((64 * Stage<DT, DK, CW, SPLIT>::WAVES), 2) void del
   const SpanSeq seq = chain.seq;
   const int64_t chunk0 = chain.first_chunk;
   const int count = (seq.tokens + CHUNK - 1) / CHUNK;
-  if (seq.slot < 0) {
+  if ((uint32_t)seq.slot >= (uint32_t)a.slots) {
     for (int64_t i = threadIdx.x; i < (int64_t)seq.tokens * 16 * CW; i += 64 * St::WAVES)
       ((T*)a.out)[((seq.first + i / (16 * CW)) * HV + hv) * DV + col0 + i % (16 * CW)] = Elem<DT>::cvt(0.f);
     return;
@@ -570,6 +579,7 @@ __global__ __launch_bounds__((64 * Stage<DT, DK, CW, SPLIT>::WAVES), 2) void del
         if (c < count) fetch_out(c);
       if (wave == St::FIRST_COPIER) touch(c + 2);
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last words have landed: LDS may go to another workgroup
     return;
   }
   // chunk c (the output's waves: c - 1) is in LDS, and nobody reads the one before any more
@@ -598,14 +608,17 @@ __global__ __launch_bounds__((64 * Stage<DT, DK, CW, SPLIT>::WAVES), 2) void del
       for (int mt = 0; mt < 4; mt++) qs[mt] = mfma16(Q[mt * KS + s], sh[s], qs[mt]);
     }
   };
-  auto load_p = [&](const char* at, const Factors* fac, f16x8 (&PF)[St::PARTS * T_FRAGS], f32x4 (&fq)[4]) {
+  auto load_p = [&](const char* at, const Factors* fac, f16x8 (&PF)[St::PARTS * T_FRAGS], f32x4 (&fd)[4], f32x4 (&fq)[4]) {
 #pragma unroll
     for (int f = 0; f < St::PARTS * T_FRAGS; f++) PF[f] = frag(at, f, lane);
 #pragma unroll
-    for (int mt = 0; mt < 4; mt++) fq[mt] = *(const f32x4*)&fac->decayed_q[row_of(mt, 4 * g)];
+    for (int mt = 0; mt < 4; mt++) {
+      fd[mt] = *(const f32x4*)&fac->decay[row_of(mt, 4 * g)];
+      fq[mt] = *(const f32x4*)&fac->q[row_of(mt, 4 * g)];
+    }
   };
-  auto finish = [&](int c, const f16x8 (&PF)[St::PARTS * T_FRAGS], const f32x4 (&fq)[4], const f16x8 (&uh)[2], const f16x8 (&ul)[2],
-                    const f32x4 (&qs)[4], float unit, float p_scale, char* tile) {
+  auto finish = [&](int c, const f16x8 (&PF)[St::PARTS * T_FRAGS], const f32x4 (&fd)[4], const f32x4 (&fq)[4], const f16x8 (&uh)[2],
+                    const f16x8 (&ul)[2], const f32x4 (&qs)[4], float unit, float p_scale, char* tile) {
     f32x4 o[4] = {zero, zero, zero, zero};
 #pragma unroll
     for (int part = EXACT_OUT ? 0 : 2; part < 3; part++)
@@ -620,8 +633,8 @@ __global__ __launch_bounds__((64 * Stage<DT, DK, CW, SPLIT>::WAVES), 2) void del
       uint32_t w[2];
 #pragma unroll
       for (int r = 0; r < 4; r += 2) {
-        const float y0 = fmaf(o[mt][r], p_scale, fq[mt][r] * qs[mt][r]), y1 = fmaf(o[mt][r + 1], p_scale, fq[mt][r + 1] * qs[mt][r + 1]);
-        w[r / 2] = (uint32_t)Elem<DT>::cvt(y0 * unit) | (uint32_t)Elem<DT>::cvt(y1 * unit) << 16;
+        const float y0 = fmaf(o[mt][r], p_scale, fd[mt][r] * qs[mt][r]), y1 = fmaf(o[mt][r + 1], p_scale, fd[mt][r + 1] * qs[mt][r + 1]);
+        w[r / 2] = pair_of<DT>(y0 * (fq[mt][r] * unit), y1 * (fq[mt][r + 1] * unit));
       }
       *(uint2*)(tile + n * (CHUNK * 2 + 8) + 2 * row_of(mt, 4 * g)) = make_uint2(w[0], w[1]);
     }
@@ -644,7 +657,7 @@ __global__ __launch_bounds__((64 * Stage<DT, DK, CW, SPLIT>::WAVES), 2) void del
         const char *const st = lds + 2 * St::STATE + (c & 1) * St::OUT, *const mail = lds + St::MAILS + (2 * cg + (c & 1)) * St::MAIL;
         const Factors* const fac = (const Factors*)(st + St::MAT);
         f16x8 sh[KS], sl[KS], uh[2], ul[2], Q[4 * KS], PF[St::PARTS * T_FRAGS];
-        f32x4 qs[4], fq[4];
+        f32x4 qs[4], fd[4], fq[4];
 #pragma unroll
         for (int s = 0; s < KS; s++) {
           sh[s] = frag(mail, s, lane);
@@ -658,11 +671,11 @@ __global__ __launch_bounds__((64 * Stage<DT, DK, CW, SPLIT>::WAVES), 2) void del
         }
         const float unit = *(const float*)(mail + St::PARTS * (KS + 2) * FRAG + 4 * lane);
         const int taken = *(const int*)(mail + St::PARTS * (KS + 2) * FRAG + 256);
-        load_p(st + St::MAT + St::FAC, fac, PF, fq);
+        load_p(st + St::MAT + St::FAC, fac, PF, fd, fq);
         const float p_scale = fac->p_scale;
         if (taken) continue;  // token by token, by the state's wave
         q_times(Q, sh, sl, qs);
-        finish(c, PF, fq, uh, ul, qs, unit, p_scale, lds + St::TILES + cg * St::TILE);
+        finish(c, PF, fd, fq, uh, ul, qs, unit, p_scale, lds + St::TILES + cg * St::TILE);
       }
       return;
     }
@@ -820,9 +833,9 @@ __global__ __launch_bounds__((64 * Stage<DT, DK, CW, SPLIT>::WAVES), 2) void del
       if constexpr (!SPLIT) {
         PHASE();
         f16x8 PF[St::PARTS * T_FRAGS];
-        f32x4 fq[4];
-        load_p(so + St::MAT, fac, PF, fq);
-        finish(c, PF, fq, uh, ul, qs, unit, p_scale, tile);
+        f32x4 fd[4], fq[4];
+        load_p(so + St::MAT, fac, PF, fd, fq);
+        finish(c, PF, fd, fq, uh, ul, qs, unit, p_scale, tile);
       }
     }
   }
@@ -881,6 +894,7 @@ static int check_delta(const anna_mi_gated_delta_args* args, const anna_mi_state
   ANNA_CHECK(a.key_heads >= 1 && a.value_heads >= a.key_heads && a.value_heads % a.key_heads == 0 && a.value_heads <= 65536,
              "gated delta rule: %lld value heads on %lld key heads", (long long)a.value_heads, (long long)a.key_heads);
   ANNA_CHECK(span->tokens >= 0 && span->tokens <= INT32_MAX, "gated delta rule: %lld tokens", (long long)span->tokens);
+  ANNA_CHECK(a.slots >= 0 && a.slots <= INT32_MAX, "gated delta rule: %lld slots", (long long)a.slots);
   ANNA_CHECK(span->max_slot < a.slots, "gated delta rule: slot %lld of a state of %lld", (long long)span->max_slot, (long long)a.slots);
   return ANNA_MI_OK;
 }
@@ -894,7 +908,7 @@ int64_t anna_mi_gated_delta_workspace(const anna_mi_gated_delta_args* args, cons
   return args->key_dim == 64 ? anna::places<64>(*args, *span).bytes() : anna::places<128>(*args, *span).bytes();
 }
 
-int anna_mi_gated_delta(const anna_mi_gated_delta_args* args, const anna_mi_state_span* span, void* stream) {
+int anna_mi_gated_delta(const anna_mi_gated_delta_args* args, anna_mi_state_span* span, void* stream) {
   if (const int rc = anna::check_delta(args, span)) return rc;
   const anna_mi_gated_delta_args& a = *args;
   if (span->tokens == 0) return ANNA_MI_OK;
@@ -909,6 +923,7 @@ int anna_mi_gated_delta(const anna_mi_gated_delta_args* args, const anna_mi_stat
   ANNA_CHECK((uintptr_t)a.state % 16 == 0 && a.state_stride_slot % 4 == 0, "gated delta rule: states must be 16-byte aligned");
   ANNA_CHECK(a.slots <= 1 || a.state_stride_slot >= a.value_heads * a.key_dim * a.value_dim, "gated delta rule: states overlap");
   ANNA_CHECK(span->chunks == 0 || (a.workspace && (uintptr_t)a.workspace % 256 == 0), "gated delta rule: no workspace, or not 256-byte aligned");
+  span->least_slots = a.slots < span->least_slots ? a.slots : span->least_slots;
   hipStream_t st = anna::as_stream(stream);
   if (const int rc = anna::delta_step(a, *span, st)) return rc;
   if (span->chains == 0) return ANNA_MI_OK;

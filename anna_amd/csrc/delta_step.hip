@@ -31,7 +31,7 @@ __global__ __launch_bounds__(256) void delta_step_kernel(const anna_mi_gated_del
   const int dv = slices * COLS, col = slice * COLS + 4 * c;
   const SpanSeq seq = steps[item / heads];
 
-  if (seq.slot < 0) {  // a sequence of nobody
+  if ((uint32_t)seq.slot >= (uint32_t)a.slots) {  // a sequence of nobody
     for (int i = tid; i < seq.tokens * COLS; i += 256)
       ((T*)a.out)[((int64_t)(seq.first + i / COLS) * HV + hv) * dv + slice * COLS + i % COLS] = Elem<DT>::cvt(0.f);
     return;

@@ -288,6 +288,8 @@ template <int DT, bool CODES> static int launch_norm(const anna_mi_rms_norm_args
                    (CODES ? (uintptr_t)a.out % 8 == 0 && (a.rows == 1 || a.out_stride % 8 == 0) : rows16(a.out, a.out_stride));
   const int64_t vecs = (a.cols + 7) / 8;
   auto blocks = [&](int rows) { return (a.rows + rows - 1) / rows; };
+  const int64_t grid = blocks(vecs <= 8 ? 32 : vecs <= 16 ? 16 : vecs <= 32 ? 8 : vecs <= 64 ? 4 : 1);
+  ANNA_CHECK(grid <= INT32_MAX / 256, "rms_norm: %lld rows of %lld columns are too many for a launch", (long long)a.rows, (long long)a.cols);
 #define ANNA_NORM(LANES, VECS)                                                                                          \
   (vec ? rms_norm_kernel<DT, LANES, VECS, CODES, true> : rms_norm_kernel<DT, LANES, VECS, CODES, false>)<<<blocks(256 / LANES), \
                                                                                                            256, 0, stream>>>(a)
@@ -312,7 +314,6 @@ extern "C" int anna_mi_rms_norm(const anna_mi_rms_norm_args* args, void* stream)
   ANNA_CHECK(anna::valid_dtype(a.dtype), "rms_norm: dtype %d", a.dtype);
   ANNA_CHECK(a.out_format == 0 || a.out_format == 1, "rms_norm: out_format %d", a.out_format);
   ANNA_CHECK(a.rows >= 0 && a.cols >= 1 && a.cols <= (1 << 28), "rms_norm: %lld rows of %lld", (long long)a.rows, (long long)a.cols);
-  ANNA_CHECK(a.rows <= INT32_MAX / 256, "rms_norm: %lld rows, at most 2^23 - 1 a call", (long long)a.rows);
   if (a.rows == 0) return ANNA_MI_OK;
   ANNA_CHECK(a.x && a.weight && a.out && (a.out_format == 0 || a.scales), "rms_norm: null pointer");
   ANNA_CHECK(a.rows == 1 || (a.x_stride >= a.cols && a.out_stride >= a.cols && (!a.residual || a.residual_stride >= a.cols) &&

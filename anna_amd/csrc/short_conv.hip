@@ -20,7 +20,7 @@ template <int DT, int W, bool VEC>
 __global__ __launch_bounds__(256) void short_conv_kernel(const typename Elem<DT>::T* __restrict__ x, int64_t x_stride,
                                                          const typename Elem<DT>::T* __restrict__ weight,
                                                          const typename Elem<DT>::T* __restrict__ bias,
-                                                         typename Elem<DT>::T* state, int64_t state_stride, uint32_t channels,
+                                                         typename Elem<DT>::T* state, uint32_t slots, int64_t state_stride, uint32_t channels,
                                                          int silu, const SpanSeq* __restrict__ seqs,
                                                          const int32_t* __restrict__ owners, int tokens, int tile,
                                                          typename Elem<DT>::T* __restrict__ out, int64_t out_stride) {
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256) void short_conv_kernel(const typename Elem<DT>
     const int pos = t - seq.first, end = seq.first + seq.tokens;
     // to the tile's end, and from a sequence's first token through the width - 2 behind it
     const int stop = min(end, pos == 0 ? max(last, seq.first + W - 1) : last), run = stop - t;
-    if (seq.slot < 0) {
+    if ((uint32_t)seq.slot >= slots) {
       Row zeros;
 #pragma unroll
       for (int e = 0; e < NC; e++) zeros.v[e] = Elem<DT>::cvt(0.f);
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(256) void short_conv_kernel(const typename Elem<DT>
 
 template <int DT>
 static int launch(const void* x, int64_t channels, int64_t x_stride, const void* weight, int64_t width, const void* bias,
-                  void* state, int64_t state_stride, int activation, const anna_mi_state_span* s, void* out,
+                  void* state, int64_t slots, int64_t state_stride, int activation, const anna_mi_state_span* s, void* out,
                   int64_t out_stride, hipStream_t stream) {
   typedef typename Elem<DT>::T T;
   auto rows = [&](const void* p, int64_t stride) { return (uintptr_t)p % (NC * sizeof(T)) == 0 && stride % NC == 0; };
@@ -166,7 +166,7 @@ static int launch(const void* x, int64_t channels, int64_t x_stride, const void*
   ANNA_CHECK(grid <= INT32_MAX / 256, "causal_conv1d: too many tokens and channels for a launch");
 #define ANNA_CONV(W)                                                                                                       \
   case W:                                                                                                                  \
-    (vec ? short_conv_kernel<DT, W, true> : short_conv_kernel<DT, W, false>)<<<grid, 256, 0, stream>>>((const T*)x, x_stride, (const T*)weight, (const T*)bias, (T*)state, \
+    (vec ? short_conv_kernel<DT, W, true> : short_conv_kernel<DT, W, false>)<<<grid, 256, 0, stream>>>((const T*)x, x_stride, (const T*)weight, (const T*)bias, (T*)state, (uint32_t)slots, \
                                                        state_stride, (uint32_t)channels, activation, span_seqs(*s), span_owners(*s), \
                                                        (int)s->tokens, tile, (T*)out, out_stride);                    \
     break;
@@ -183,19 +183,20 @@ static int launch(const void* x, int64_t channels, int64_t x_stride, const void*
 
 extern "C" int anna_mi_causal_conv1d(const void* x, int dtype, int64_t channels, int64_t x_stride, const void* weight,
                                      int64_t width, const void* bias, void* state, int64_t slots, int64_t state_stride_slot,
-                                     int activation, const anna_mi_state_span* span, void* out, int64_t out_stride,
-                                     void* stream) {
+                                     int activation, anna_mi_state_span* span, void* out, int64_t out_stride, void* stream) {
   ANNA_CHECK(span != nullptr, "causal_conv1d: null span");
   ANNA_CHECK(anna::valid_dtype(dtype), "causal_conv1d: dtype %d", dtype);
   ANNA_CHECK(width >= 2 && width <= 8, "causal_conv1d: width %lld, 2 to 8 are supported", (long long)width);
   ANNA_CHECK(channels >= 1 && channels <= (1 << 24), "causal_conv1d: %lld channels", (long long)channels);
   ANNA_CHECK(activation == 0 || activation == 1, "causal_conv1d: activation %d", activation);
+  ANNA_CHECK(slots >= 0 && slots <= INT32_MAX, "causal_conv1d: %lld slots", (long long)slots);
   ANNA_CHECK(span->max_slot < slots, "causal_conv1d: slot %lld of a state of %lld", (long long)span->max_slot, (long long)slots);
   if (span->tokens == 0) return ANNA_MI_OK;
   ANNA_CHECK(span->tokens <= INT32_MAX && x && weight && out && span->buf && (state || span->max_slot < 0), "causal_conv1d: null pointer");
   ANNA_CHECK(x_stride >= channels || span->tokens == 1, "causal_conv1d: rows of x overlap");
   ANNA_CHECK(out_stride >= channels || span->tokens == 1, "causal_conv1d: rows of out overlap");
   ANNA_CHECK(slots <= 1 || state_stride_slot >= (width - 1) * channels, "causal_conv1d: rows of the state overlap");
-  ANNA_DISPATCH_DTYPE(dtype, DT, return anna::launch<DT>(x, channels, x_stride, weight, width, bias, state, state_stride_slot,
+  span->least_slots = slots < span->least_slots ? slots : span->least_slots;
+  ANNA_DISPATCH_DTYPE(dtype, DT, return anna::launch<DT>(x, channels, x_stride, weight, width, bias, state, slots, state_stride_slot,
                                                          activation, span, out, out_stride, anna::as_stream(stream)));
 }

@@ -80,6 +80,7 @@ static int lay_out(int64_t n, const int32_t* slots, const int64_t* counts, const
   s->chains = chains;
   s->chunks = chunks;
   s->max_slot = max_slot;
+  s->least_slots = INT64_MAX;
   return ANNA_MI_OK;
 }
 

@@ -635,7 +635,7 @@ int64_t pool_stride(const Tensor& t, const at::Device& dev, at::ScalarType dt, a
 OptTensor gated_delta(const Tensor& query, const Tensor& key, const Tensor& value, const Tensor& decay, const Tensor& beta,
                       const Tensor& state, const OptTensor& a_log, const OptTensor& dt_bias, uintptr_t span_address, int64_t device,
                       double scaling, bool normalize, uintptr_t stream) {
-  const auto* span = reinterpret_cast<const anna_mi_state_span*>(span_address);
+  auto* span = reinterpret_cast<anna_mi_state_span*>(span_address);
   const at::Device dev = query.device();
   const at::ScalarType dt = query.scalar_type();
   if (!query.is_cuda() || dev.index() != device || query.dim() != 3 || value.dim() != 3 || (dt != at::kBFloat16 && dt != at::kHalf) || span->tokens != query.size(0)) return std::nullopt;
@@ -672,7 +672,7 @@ OptTensor gated_delta(const Tensor& query, const Tensor& key, const Tensor& valu
 
 OptTensor causal_conv1d(const Tensor& x, const Tensor& weight, const OptTensor& bias, const Tensor& state, uintptr_t span_address,
                         int64_t device, bool silu, uintptr_t stream) {
-  const auto* span = reinterpret_cast<const anna_mi_state_span*>(span_address);
+  auto* span = reinterpret_cast<anna_mi_state_span*>(span_address);
   const at::Device dev = x.device();
   const at::ScalarType dt = x.scalar_type();
   if (!x.is_cuda() || dev.index() != device || x.dim() != 2 || dtype_code(x) < 0 || !given(x, dev) || span->tokens != x.size(0)) return std::nullopt;

@@ -778,6 +778,8 @@ typedef struct {
   int64_t words;                  /* int32 words of buf */
   int64_t steps, chains, chunks;  /* sequences taken token by token, in chunks of 64; chunks of all chains */
   int64_t max_slot;               /* the largest slot, -1 without any */
+  int64_t least_slots;            /* of the pools that calls took this span with: a captured call is replayed with slots
+                                     below it (the kernels take others for a sequence of nobody) */
   const int32_t* buf;             /* device: [sequences][4] slot, first token, tokens, fresh; [steps][4] the same of
                                      the sequences taken token by token; [chains][8] the same, first chunk, 0, 0, 0,
                                      the longest first;
@@ -818,7 +820,7 @@ typedef struct {
 } anna_mi_gated_delta_args;
 
 int64_t anna_mi_gated_delta_workspace(const anna_mi_gated_delta_args* args, const anna_mi_state_span* span);
-int anna_mi_gated_delta(const anna_mi_gated_delta_args* args, const anna_mi_state_span* span, void* stream);
+int anna_mi_gated_delta(const anna_mi_gated_delta_args* args, anna_mi_state_span* span, void* stream);
 int64_t anna_mi_sizeof_state_span(void);
 int64_t anna_mi_sizeof_gated_delta_args(void);
 
@@ -828,7 +830,7 @@ int64_t anna_mi_sizeof_gated_delta_args(void);
  * out must not overlap x.  activation: 0 none, 1 SiLU. */
 int anna_mi_causal_conv1d(const void* x, int dtype, int64_t channels, int64_t x_stride, const void* weight,
                           int64_t width, const void* bias, void* state, int64_t slots, int64_t state_stride_slot,
-                          int activation, const anna_mi_state_span* span, void* out, int64_t out_stride, void* stream);
+                          int activation, anna_mi_state_span* span, void* out, int64_t out_stride, void* stream);
 
 /* y = h / sqrt(mean(h^2) + eps) * (weight + weight_offset) [* silu(gate)] of every row, with h = x, or
  * h = x + residual, rounded to the dtype and written back to residual.  out_format 0: out in dtype; 1: out e4m3

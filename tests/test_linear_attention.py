@@ -171,7 +171,7 @@ def test_e4m3_refuses_groups(cols, group):
 
 def test_c_entries_refuse():
     lib = _lib.load()
-    span = _lib.StateSpan(1, 1, 5, 1, 0, 0, 0, None)
+    span = _lib.StateSpan(1, 1, 9, 1, 0, 0, 0, 1 << 40, None)
     args = _lib.GatedDeltaArgs(dtype=_lib.F32)
     assert lib.anna_mi_gated_delta(None, ctypes.byref(span), None) == 1
     assert lib.anna_mi_gated_delta(ctypes.byref(args), ctypes.byref(span), None) == 1
@@ -181,6 +181,6 @@ def test_c_entries_refuse():
     assert b"slot 0 of a state of 0" in lib.anna_mi_last_error()
     assert lib.anna_mi_causal_conv1d(None, _lib.BF16, 8, 8, None, 4, None, None, 1, 24, 1, ctypes.byref(span), None, 8, None) == 1
     assert b"null pointer" in lib.anna_mi_last_error()
-    norm = _lib.RmsNormArgs(dtype=_lib.BF16, out_format=1, rows=1 << 24, cols=8)
+    norm = _lib.RmsNormArgs(dtype=_lib.BF16, out_format=0, rows=1 << 24, cols=8192, x=16, x_stride=8192, weight=16, out=16, out_stride=8192)
     assert lib.anna_mi_rms_norm(ctypes.byref(norm), None) == 1
-    assert b"rows" in lib.anna_mi_last_error()
+    assert b"too many for a launch" in lib.anna_mi_last_error()

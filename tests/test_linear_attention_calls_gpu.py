@@ -234,6 +234,9 @@ def test_device_refusals(gpu):
         span._lay_out([0, 1], [2, 1], None)
     with pytest.raises(RuntimeError, match="slot 5 is named twice"):
         span.refill([5, 5])
+    la.causal_conv1d(x, layer.conv_weight, None, layer.conv_state, span)
+    with pytest.raises(RuntimeError, match="slot 2: the span was used with states of 2 slots"):
+        span.refill([2, 0])  # a graph captured with it would write behind the pool
     assert span.slots == [0, 1] and span.counts == [1, 2] and span.tokens == 3
     la.causal_conv1d(x, layer.conv_weight, None, layer.conv_state, span)  # as it was
 

@@ -249,6 +249,48 @@ def test_delta_rule_what_is_not_finite_reaches_nothing_before_it(gpu, what, coun
         first += n
 
 
+@pytest.mark.parametrize("normalize", [True, False])
+def test_delta_rule_a_query_has_a_say_in_its_own_row_only(gpu, normalize):
+    """Queries of very different size, one of them not finite, in one chunk: each row is as exact as alone."""
+    counts = [100]
+    c = delta_case(71, counts, 2, 4, 64, 64, HF, False)
+    c["k"] = (c["k"].float() / (1.01 * c["k"].float().norm(dim=-1, keepdim=True))).to(HF)
+    c["q"] = c["q"].to(BF)
+    c["k"], c["v"] = c["k"].to(BF), c["v"].to(BF)
+    c["k"] = (c["k"].float() * 0.99).to(BF)
+    c["q"][::3] = (c["q"][::3].float() * 2.0 ** 60).to(BF)
+    c["q"][1::3] = (c["q"][1::3].float() * 2.0 ** -40).to(BF)
+    if not normalize:
+        c["q"][31, 0, 5] = float("inf")
+    else:
+        c["q"][31, 0, 5] = float("nan")
+    out, state = run_delta(gpu, c, counts, [False], 0.1, normalize=normalize)
+    g, beta = plain.gates(c["decay"], c["beta"])
+    clean = c["q"].clone()
+    clean[31, 0] = 0
+    want, S, sums, errors, E, eps = plain.delta_rule(clean, c["k"], c["v"], g, beta, c["state"][c["slots"][0]], 0.1, normalize, chunked=True)
+    q_norm = clean.double().norm(dim=-1, keepdim=True).repeat_interleave(2, 1) if not normalize else 1.0
+    tol = plain.delta_tolerance(want, sums, errors * q_norm, eps, BF, 0.1, True)
+    ok = torch.ones_like(want, dtype=torch.bool)
+    ok[31, :2] = False
+    assert ((out.double() - want).abs() <= tol)[ok].all()
+    assert not torch.isfinite(out[31, :2].float()).any()
+    assert ((state[c["slots"][0]].double() - S).norm(dim=1) <= E).all()
+
+
+# A key head's value heads go in one workgroup from 1024 chunks and key heads on
+GROUPED = [(128, 8, 48, 64, 32, BF), (64, 16, 32, 64, 32, HF)]
+
+
+@pytest.mark.parametrize("case", GROUPED, ids=["x".join(map(str, c[:3])) for c in GROUPED])
+def test_delta_rule_of_many_chunks(gpu, case):
+    n, HK, HV, DK, DV, dtype = case
+    counts = [13 + i % 3 for i in range(n)]
+    c = delta_case(n, counts, HK, HV, DK, DV, dtype, True)
+    out, state = run_delta(gpu, c, counts, [False] * n, DK ** -0.5)
+    check_delta(c, counts, [False] * n, DK ** -0.5, out, state)
+
+
 def test_delta_rule_in_pieces(gpu):
     """A sequence in one call, and in calls that continue each other through both forms."""
     counts = [150]
@@ -452,6 +494,18 @@ def test_norm_values_that_are_not_finite_or_tiny(gpu):
     codes, scales = la.rms_norm_e4m3(randn(4, 3, 256).to(gpu), w.to(gpu), group_size=128)
     assert torch.isfinite(codes.cpu().float()[:, :128]).all() and torch.isfinite(scales[:, 0]).all()
     assert torch.isnan(codes.cpu().float()[:, 130]).all() and torch.isnan(scales[:, 1]).all()
+
+
+def test_norm_of_many_short_rows(gpu):
+    rows = (1 << 23) + 5  # more than a launch has workgroups of one row
+    x, w = randn(1, 64, 8).to(BF), randn(2, 8).to(BF)
+    wide = x.to(gpu).repeat(rows // 64 + 1, 1)[:rows]
+    got = la.rms_norm(wide, w.to(gpu))
+    want, _ = plain.norm(x, w, 1e-6, 0.0)
+    tol = (2.0 ** -8 + 40 * 2.0 ** -24) * want.abs() + 2.0 ** -140
+    assert ((got[:64].cpu().double() - want).abs() <= tol).all()
+    assert torch.equal(got[64:rows // 64 * 64].view(-1, 64, 8), got[:64].expand(rows // 64 - 1, 64, 8))
+    assert torch.equal(got[rows // 64 * 64:], got[:rows % 64])
 
 
 def test_norm_layouts(gpu):
