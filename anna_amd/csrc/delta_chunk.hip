@@ -20,6 +20,14 @@
 // gives lane (n = lane % 16, g = lane / 16) the 8 values of row (mt, n) at k = 32 ks + 8 g + 0..7.  Rows of tile mt are
 // numbered so that the instruction's result, rows 4 g + r of a tile in lane (n, g), is at once the other operand of
 // the next product: row m of tile mt stands for index 32 (mt / 2) + 8 (m / 4) + 4 (mt % 2) + m % 4.
+//
+// What bounds it, 16 key and 32 value heads of 128, bf16.  One sequence of 16384 tokens: preparation 107 us, chain 425.
+// The preparation writes 0.3 GB of workspace (58 us at a copy's rate); the rest is latency, about 36000 cycles a
+// workgroup of loads, products and the inverse's steps with three workgroups a compute unit to cover for each other (two: 121 us).
+// The chain is 256 chunks in a row at 1.65 us each on every compute unit: 82 matrix instructions of the state's
+// wave are a third of that, what makes their operands (splits, scales, LDS) another; the bytes alone would take 80 us.
+// Eight sequences of 25344 tokens together, fp16: preparation 160 us, chain 350, of which the operands that pass
+// through LDS once for every four column groups are the larger part.
 #include "delta.hpp"
 
 namespace anna {
@@ -855,9 +863,11 @@ template <int DK> static Places<DK> places(const anna_mi_gated_delta_args& a, co
 template <int DT, int DK>
 static int delta_chunks(const anna_mi_gated_delta_args& a, const anna_mi_state_span& s, hipStream_t stream) {
   const Places<DK> ws = places<DK>(a, s);
-  // a key head's value heads in one workgroup share the products of K, where that still fills the chip
+  // a key head's value heads in one workgroup share the products of K, where that still fills the chip: 256 chunks of
+  // 16 key heads take 107 us with both value heads and 143 with one; with the chains 32 chunks take 80 and 85, 16
+  // chunks 50 both ways
   const int64_t ratio = a.value_heads / a.key_heads;
-  const int per = s.chunks * a.key_heads >= 1024 ? (int)ratio : 1;
+  const int per = s.chunks * a.key_heads >= 512 ? (int)ratio : 1;
   const int64_t prepare = s.chunks * (a.value_heads / per), groups = s.chains * a.value_heads * (a.value_dim / 16);
   ANNA_CHECK(prepare <= INT32_MAX / 256 && groups <= INT32_MAX / 128, "gated delta rule: too many tokens and heads for a launch");
   delta_prepare_kernel<DT, DK><<<prepare, 256, 0, stream>>>(a, span_chunks(s), ws, per);
@@ -874,6 +884,10 @@ static int delta_chunks(const anna_mi_gated_delta_args& a, const anna_mi_state_s
       kern<<<8 * ((units + 7) / 8) * (groups / units / CW), 64 * St::WAVES, St::BYTES, stream>>>(a, span_chains(s), ws, units); \
   }
   constexpr bool TWO = Stage<DT, DK, 2, true>::BYTES <= 160 * 1024;  // fp16 at 128 key dims: the second parts leave no room
+  // One workgroup fits a compute unit's LDS in each form.  Up to 256 column groups all have one to themselves: 419 us for
+  // 16384 tokens of 32 heads of 128, 461 with two groups in a workgroup, which in turn takes up to 512 groups in one go
+  // where one would need two.  From 1024 groups on four share the copies: 65 us for prompts of 1115 to 1500
+  // tokens, 77 with two; 350 for eight sequences in fp16, 714 with one.
   if (a.value_dim % 64 == 0 && groups >= 1024) ANNA_CHAIN(4, false)
   else if (TWO && groups > 256) ANNA_CHAIN((TWO ? 2 : 1), true)
   else ANNA_CHAIN(1, true)

@@ -7,7 +7,8 @@
 // wave a token, in LDS.
 //
 // It is bound by the state's bytes (key_dim * value_dim * 4 read and written a sequence and head); a
-// token's q, k and v are a hundredth of them.
+// token's q, k and v are a hundredth of them.  64 sequences' next tokens, 32 value heads of 128 x 128 (0.27 GB): 59 us =
+// 4.6 TB/s; a copy of 1 GiB runs at 5.2.  One sequence (4.2 MB): 5.3 us, the loads' latency and a launch.
 #include "delta.hpp"
 
 namespace anna {

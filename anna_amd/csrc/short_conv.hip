@@ -1,10 +1,18 @@
 // The short causal convolution of a linear-attention layer over packed, ragged sequences, with the last
 // width - 1 inputs of every sequence kept in a row of a state pool.
 //
-// A thread takes 8 channels (16 bytes of the 16-bit types) and walks down `tile` tokens with the window in
-// registers, so an input is read once, and the width - 1 in front of a tile once more.  Bound by the bytes of x and out.
+//   out[t, c] = act(bias[c] + sum_j weight[c, j] x[t - (width - 1) + j, c]),   x in front of a sequence: its state
+//
+// A thread takes 4 channels (8 bytes of the 16-bit types) and walks down `tile` tokens with the window in
+// registers, so an input is read once, and the width - 1 in front of a tile once more.  The next four tokens' rows are asked
+// for in front of a group's stores, and full groups have no branches.  Sums are fp32, rounded to the type once, after
+// the activation; the state keeps inputs as they came, so nothing is rounded there.
 // The thread that has a sequence's first token also takes the width - 2 tokens behind it, also past its tile:
 // it alone reads the state of its channels, and then writes the new one.
+//
+// Bound by the bytes of x and out.  12787 tokens of 8192 channels in 6 sequences, bf16, width 4 (0.42 GB): 85 us =
+// 4.9 TB/s; a copy of 1 GiB runs at 5.2.  8 channels a thread took 165 us (half the waves, so that loads wait for
+// stores), groups of four with branches in them 134.  One token of 64 sequences: 4.0 us, an empty launch takes 3.6.
 #include "delta.hpp"
 
 namespace anna {
@@ -158,7 +166,8 @@ static int launch(const void* x, int64_t channels, int64_t x_stride, const void*
   typedef typename Elem<DT>::T T;
   auto rows = [&](const void* p, int64_t stride) { return (uintptr_t)p % (NC * sizeof(T)) == 0 && stride % NC == 0; };
   const bool vec = channels % NC == 0 && rows(x, x_stride) && rows(out, out_stride) && rows(state, state_stride) && rows(weight, NC);
-  // 24 tokens a thread once that fills the chip with 8 waves a compute unit, fewer otherwise
+  // 24 tokens a thread once that fills the chip with 8 waves a compute unit, fewer otherwise.  At 12787 tokens of 8192
+  // channels 16 and 48 are within 3% of it; below the limit a call takes as long as one wave's chain of loads.
   const int64_t groups = (channels + NC - 1) / NC;
   int tile = 24;
   while (tile > 1 && groups * ((s->tokens + tile - 1) / tile) < 256 * 8 * 64) tile /= 2;

@@ -19,7 +19,7 @@ static int lay_out(int64_t n, const int32_t* slots, const int64_t* counts, const
     ANNA_CHECK(slots[i] >= -1, "state span: slot %d of sequence %lld", (int)slots[i], (long long)i);
     ANNA_CHECK(counts[i] >= 0 && counts[i] <= INT32_MAX, "state span: sequence %lld of %lld tokens", (long long)i, (long long)counts[i]);
     tokens += counts[i];
-    ANNA_CHECK(tokens <= INT32_MAX, "state span: more than 2^31 - 1 tokens");
+    ANNA_CHECK(tokens <= INT32_MAX - 4095, "state span: more than 2^31 - 4096 tokens");  // kernels count a little further
     max_slot = std::max<int64_t>(max_slot, slots[i]);
     if (counts[i] > STEP_TOKENS) {
       chains++;
