@@ -13,6 +13,15 @@ from anna_amd import linear_attention as la
 from anna_amd.quantization import XPUInt4Linear
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def nothing_cached():
+    """The large tensors' segments go back to the device, so that nobody's lasting tensors come to lie in them."""
+    yield
+    torch.cuda.empty_cache()
+
+
 BF = torch.bfloat16
 
 

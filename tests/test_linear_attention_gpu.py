@@ -7,6 +7,15 @@ import _linear as plain
 from anna_amd import linear_attention as la
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def nothing_cached():
+    """The large tensors' segments go back to the device, so that nobody's lasting tensors come to lie in them."""
+    yield
+    torch.cuda.empty_cache()
+
+
 BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
 STEPS = 12  # sequences of more tokens go in chunks
 
