@@ -21,13 +21,18 @@
 // numbered so that the instruction's result, rows 4 g + r of a tile in lane (n, g), is at once the other operand of
 // the next product: row m of tile mt stands for index 32 (mt / 2) + 8 (m / 4) + 4 (mt % 2) + m % 4.
 //
-// What bounds it, 16 key and 32 value heads of 128, bf16.  One sequence of 16384 tokens: preparation 107 us, chain 425.
+// What bounds it, 16 key and 32 value heads of 128, bf16.  One sequence of 16384 tokens: preparation 107 us, chain 415.
 // The preparation writes 0.3 GB of workspace (58 us at a copy's rate); the rest is latency, about 36000 cycles a
 // workgroup of loads, products and the inverse's steps with three workgroups a compute unit to cover for each other (two: 121 us).
-// The chain is 256 chunks in a row at 1.65 us each on every compute unit: 82 matrix instructions of the state's
+// The chain is 256 chunks in a row at 1.6 us each on every compute unit: 82 matrix instructions of the state's
 // wave are a third of that, what makes their operands (splits, scales, LDS) another; the bytes alone would take 80 us.
-// Eight sequences of 25344 tokens together, fp16: preparation 160 us, chain 350, of which the operands that pass
-// through LDS once for every four column groups are the larger part.
+// Eight sequences of 25344 tokens together, fp16: preparation 160 us, chain 350. Four waves a compute unit there read all
+// operands from LDS, 2.7 to 2.9 us a chunk: without copies from memory it is as long, vector unit 41% and matrix cores 26%
+// busy, a third of the cycles with LDS, an eighth in its conflicts. Two column groups a wave, which halves what is
+// read, took 650: the vector unit of half the SIMDs is then too little. A wave more for every group's output, with operands in
+// single buffers that the output's waves fill, took 430.
+#include <type_traits>
+
 #include "delta.hpp"
 
 namespace anna {
@@ -524,34 +529,35 @@ __global__ __launch_bounds__((64 * Stage<DT, DK, CW, SPLIT>::WAVES), 2) void del
   }
 
   // ---- copies of the operands, one piece of FRAG bytes an instruction, the pieces dealt to COPIERS waves
-  int piece = 0;
-  auto copy = [&](const char* from, int to, int bytes) {
+  const int copier = wave - St::FIRST_COPIER;
+  auto copy = [&](const char* from, int to, auto bytes) {
+    constexpr int N = decltype(bytes)::value / FRAG;
 #pragma unroll
-    for (int i = 0; i < bytes; i += FRAG)
-      if (piece++ % St::COPIERS == wave - St::FIRST_COPIER)
-        __builtin_amdgcn_global_load_lds((global_ptr)(from + i + 16 * lane), (lds_ptr)(lds + to + i), 16, 0, 0);
+    for (int i = 0; i < (N + St::COPIERS - 1) / St::COPIERS; i++) {
+      const int at = (St::COPIERS * i + copier) * FRAG;
+      if (N % St::COPIERS == 0 || at < N * FRAG)
+        __builtin_amdgcn_global_load_lds((global_ptr)(from + at + 16 * lane), (lds_ptr)(lds + to + at), 16, 0, 0);
+    }
   };
   auto fetch_state = [&](int c) {
     const int to = (c & 1) * St::STATE;
-    piece = 0;
-    copy(ws.k(chunk0 + c, hk), to, St::MAT);
-    copy(ws.t(chunk0 + c, hv), to + St::MAT, St::TS + St::FAC);
+    copy(ws.k(chunk0 + c, hk), to, std::integral_constant<int, St::MAT>());
+    copy(ws.t(chunk0 + c, hv), to + St::MAT, std::integral_constant<int, St::TS + St::FAC>());
     const int tokens = min(CHUNK, seq.tokens - c * CHUNK);
     const T* v = (const T*)a.value + (seq.first + (int64_t)c * CHUNK) * a.value_stride_token + hv * a.value_stride_head + col0;
 #pragma unroll
-    for (int i = 0; i < 2 * CW; i++)
-      if (piece++ % St::COPIERS == wave - St::FIRST_COPIER) {
-        // rows behind the last token hold the last one's again; their row of T' is zero
-        const int t = min(32 * (i & 1) + lane / 2, tokens - 1);
-        __builtin_amdgcn_global_load_lds((global_ptr)(v + t * a.value_stride_token + 16 * (i >> 1) + 8 * (lane & 1)),
-                                         (lds_ptr)(lds + to + St::MAT + St::TS + St::FAC + (i >> 1) * St::TILE + (i & 1) * FRAG), 16, 0, 0);
-      }
+    for (int i = 0; i < 2 * CW / St::COPIERS; i++) {
+      // rows behind the last token hold the last one's again; their row of T' is zero
+      const int at = St::COPIERS * i + copier, t = min(32 * (at & 1) + lane / 2, tokens - 1);
+      __builtin_amdgcn_global_load_lds((global_ptr)(v + t * a.value_stride_token + 16 * (at >> 1) + 8 * (lane & 1)),
+                                       (lds_ptr)(lds + to + St::MAT + St::TS + St::FAC + (at >> 1) * St::TILE + (at & 1) * FRAG), 16, 0, 0);
+    }
   };
   auto fetch_out = [&](int c) {
     const int to = 2 * St::STATE + (c & 1) * St::OUT;
-    copy(ws.q(chunk0 + c, hk), to, St::MAT);
-    if constexpr (SPLIT) copy((const char*)ws.factors(chunk0 + c, hv), to + St::MAT, St::FAC + St::PS);
-    else copy(ws.p(chunk0 + c, hv), to + St::MAT, St::PS);
+    copy(ws.q(chunk0 + c, hk), to, std::integral_constant<int, St::MAT>());
+    if constexpr (SPLIT) copy((const char*)ws.factors(chunk0 + c, hv), to + St::MAT, std::integral_constant<int, St::FAC + St::PS>());
+    else copy(ws.p(chunk0 + c, hv), to + St::MAT, std::integral_constant<int, St::PS>());
   };
   if (wave >= St::FIRST_COPIER) {
     // A chunk's time is short of memory's latency: a word of each line of the chunk after the next is asked for, which
@@ -884,7 +890,7 @@ static int delta_chunks(const anna_mi_gated_delta_args& a, const anna_mi_state_s
       kern<<<8 * ((units + 7) / 8) * (groups / units / CW), 64 * St::WAVES, St::BYTES, stream>>>(a, span_chains(s), ws, units); \
   }
   constexpr bool TWO = Stage<DT, DK, 2, true>::BYTES <= 160 * 1024;  // fp16 at 128 key dims: the second parts leave no room
-  // One workgroup fits a compute unit's LDS in each form.  Up to 256 column groups all have one to themselves: 419 us for
+  // One workgroup fits a compute unit's LDS in each form.  Up to 256 column groups all have one to themselves: 415 us for
   // 16384 tokens of 32 heads of 128, 461 with two groups in a workgroup, which in turn takes up to 512 groups in one go
   // where one would need two.  From 1024 groups on four share the copies: 65 us for prompts of 1115 to 1500
   // tokens, 77 with two; 350 for eight sequences in fp16, 714 with one.
