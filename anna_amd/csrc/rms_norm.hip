@@ -8,8 +8,8 @@
 //   h = x + residual,   y = h / sqrt(mean(h^2) + eps) * (weight + offset) * silu(gate)
 //   e4m3: code = round(y 448 / m), scale = m / 448, m the largest |y| of a group
 //
-// Bound by the rows' bytes.  8192 rows of 4096 with residual and e4m3 codes (0.24 GB): 53 us = 4.5 TB/s; a copy of
-// 1 GiB runs at 5.2.  262144 rows of 128 with gate (0.2 GB): 41 us = 4.9 TB/s.  64 rows of 2048: 3.1 us, less
+// Bound by the rows' bytes.  8192 rows of 4096 with residual and e4m3 codes (0.24 GB): 49 us = 4.8 TB/s; a copy of
+// 1 GiB runs at 5.2 (55 us with a clamp of every code, which branches, and divisions by the group).  262144 rows of 128 with gate (0.2 GB): 41 us = 4.9 TB/s.  64 rows of 2048: 3.1 us, less
 // than an empty launch from the host takes.
 #include "delta.hpp"
 
@@ -32,6 +32,12 @@ __device__ __forceinline__ Row8<DT> load8(const void* base, int64_t at, int n) {
 #pragma unroll
   for (int e = 0; e < 8; e++) r.v[e] = e < n ? p[e] : (typename Elem<DT>::T)0;
   return r;
+}
+// Columns from c on, up to eight; of aligned rows eight or none
+template <bool VEC>
+__device__ __forceinline__ int columns(int64_t cols, int64_t c) {
+  if constexpr (VEC) return c < cols ? 8 : 0;
+  return (int)min((int64_t)8, max((int64_t)0, cols - c));
 }
 template <int DT>
 __device__ __forceinline__ void widen(const Row8<DT>& r, float (&f)[8]) {
@@ -80,14 +86,16 @@ template <int LANES> __device__ __forceinline__ uint32_t row_max(uint32_t v, uin
   return v;
 }
 
+template <bool VEC>
 __device__ __forceinline__ uint32_t abs_max(const float (&y)[8], int n) {
   uint32_t m = 0;
 #pragma unroll
   for (int e = 0; e < 8; e++)
-    if (e < n) m = max(m, __float_as_uint(y[e]) & 0x7fffffffu);
+    if (VEC || e < n) m = max(m, __float_as_uint(y[e]) & 0x7fffffffu);
   return m;
 }
-// Codes of eight values; `to_unit`: 448 / the group's largest
+// Codes of eight values; `to_unit`: 448 / the group's largest, so that what two roundings add to a product is far from
+// 464, where e4m3 would end
 template <bool VEC>
 __device__ __forceinline__ void save_codes(uint8_t* p, int n, const float (&y)[8], float to_unit) {
   uint32_t w[2];
@@ -95,10 +103,7 @@ __device__ __forceinline__ void save_codes(uint8_t* p, int n, const float (&y)[8
   for (int h = 0; h < 2; h++) {
     float c[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      c[e] = y[4 * h + e] * to_unit;
-      c[e] = c[e] > E4M3_MAX ? E4M3_MAX : c[e] < -E4M3_MAX ? -E4M3_MAX : c[e];  // a NaN stays
-    }
+    for (int e = 0; e < 4; e++) c[e] = y[4 * h + e] * to_unit;
     int packed = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
     w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], packed, true);
   }
@@ -141,7 +146,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(const anna_mi_rms_norm_ar
 #pragma unroll
   for (int i = 0; i < VECS; i++) {
     const int64_t c = 8 * (int64_t)(lane + LANES * i);
-    const int n = (int)min((int64_t)8, max((int64_t)0, cols - c));
+    const int n = columns<VEC>(cols, c);
     if (n == 0) continue;
     x[i] = load8<DT, VEC>(a.x, row * a.x_stride + c, n);
     if (a.residual) old[i] = load8<DT, VEC>(a.residual, row * a.residual_stride + c, n);
@@ -152,7 +157,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(const anna_mi_rms_norm_ar
 #pragma unroll
   for (int i = 0; i < VECS; i++) {
     const int64_t c = 8 * (int64_t)(lane + LANES * i);
-    const int n = (int)min((int64_t)8, max((int64_t)0, cols - c));
+    const int n = columns<VEC>(cols, c);
     if (n == 0) {
 #pragma unroll
       for (int e = 0; e < 8; e++) h[i][e] = 0.f;
@@ -172,10 +177,11 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(const anna_mi_rms_norm_ar
   const float rs = rsqrtf(row_sum<LANES>(ss, sums) / (float)cols + a.eps);
 
   uint32_t top = 0;
+  const int shift = __builtin_ctz((uint32_t)a.group);  // of groups that are not whole rows
 #pragma unroll
   for (int i = 0; i < VECS; i++) {
     const int64_t c = 8 * (int64_t)(lane + LANES * i);
-    const int n = (int)min((int64_t)8, max((int64_t)0, cols - c));
+    const int n = columns<VEC>(cols, c);
     if (n > 0) {
       float w[8];
       widen<DT>(weight[i], w);
@@ -191,14 +197,14 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(const anna_mi_rms_norm_ar
     if constexpr (!CODES) {
       if (live && n > 0) save8<DT, VEC>(a.out, row * a.out_stride + c, n, h[i]);
     } else {
-      const uint32_t m = abs_max(h[i], n);
+      const uint32_t m = abs_max<VEC>(h[i], n);
       if (a.group == cols) {
         top = max(top, m);
       } else {  // every group lies in neighbouring lanes of one vector row
         const Scale s = scale_of(group_max(m, (int)a.group / 8));
         if (live && n > 0) {
           save_codes<VEC>((uint8_t*)a.out + row * a.out_stride + c, n, h[i], s.to_unit);
-          if (c % a.group == 0) a.scales[row * (cols / a.group) + c / a.group] = s.scale;
+          if ((c & (a.group - 1)) == 0) a.scales[row * (cols >> shift) + (c >> shift)] = s.scale;
         }
       }
     }
@@ -210,7 +216,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(const anna_mi_rms_norm_ar
 #pragma unroll
       for (int i = 0; i < VECS; i++) {
         const int64_t c = 8 * (int64_t)(lane + LANES * i);
-        const int n = (int)min((int64_t)8, max((int64_t)0, cols - c));
+        const int n = columns<VEC>(cols, c);
         if (live && n > 0) save_codes<VEC>((uint8_t*)a.out + row * a.out_stride + c, n, h[i], s.to_unit);
       }
     }
@@ -227,7 +233,7 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(const anna_mi_rms_no
   const int64_t src_stride = a.residual ? a.residual_stride : a.x_stride;
   float ss = 0.f;
   for (int64_t c = 8 * (int64_t)threadIdx.x; c < cols; c += 2048) {
-    const int n = (int)min((int64_t)8, cols - c);
+    const int n = columns<VEC>(cols, c);
     float h[8];
     widen<DT>(load8<DT, VEC>(a.x, row * a.x_stride + c, n), h);
     if (a.residual) {
@@ -255,15 +261,16 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(const anna_mi_rms_no
     }
   };
   const bool by_row = a.group == cols;
+  const int shift = __builtin_ctz((uint32_t)a.group);  // of groups that are not whole rows
   Scale s{0.f, 0.f};
   if constexpr (CODES) {
     if (by_row) {
       uint32_t top = 0;
       for (int64_t c = 8 * (int64_t)threadIdx.x; c < cols; c += 2048) {
-        const int n = (int)min((int64_t)8, cols - c);
+        const int n = columns<VEC>(cols, c);
         float h[8];
         value(c, n, h);
-        top = max(top, abs_max(h, n));
+        top = max(top, abs_max<VEC>(h, n));
       }
       s = scale_of(row_max<256>(top, tops));
       if (threadIdx.x == 0) a.scales[row] = s.scale;
@@ -271,16 +278,16 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(const anna_mi_rms_no
   }
   for (int64_t base = 0; base < cols; base += 2048) {  // whole workgroups: a group's lanes meet below
     const int64_t c = base + 8 * (int64_t)threadIdx.x;
-    const int n = (int)min((int64_t)8, max((int64_t)0, cols - c));
+    const int n = columns<VEC>(cols, c);
     float h[8] = {};
     if (n > 0) value(c, n, h);
     if constexpr (!CODES) {
       if (n > 0) save8<DT, VEC>(a.out, row * a.out_stride + c, n, h);
     } else {
-      if (!by_row) s = scale_of(group_max(abs_max(h, n), (int)a.group / 8));
+      if (!by_row) s = scale_of(group_max(abs_max<VEC>(h, n), (int)a.group / 8));
       if (n > 0) {
         save_codes<VEC>((uint8_t*)a.out + row * a.out_stride + c, n, h, s.to_unit);
-        if (!by_row && c % a.group == 0) a.scales[row * (cols / a.group) + c / a.group] = s.scale;
+        if (!by_row && (c & (a.group - 1)) == 0) a.scales[row * (cols >> shift) + (c >> shift)] = s.scale;
       }
     }
   }
@@ -297,7 +304,7 @@ template <int DT, bool CODES> static int launch_norm(const anna_mi_rms_norm_args
   const int64_t grid = blocks(vecs <= 8 ? 32 : vecs <= 16 ? 16 : vecs <= 32 ? 8 : vecs <= 64 ? 4 : 1);
   ANNA_CHECK(grid <= INT32_MAX / 256, "rms_norm: %lld rows of %lld columns are too many for a launch", (long long)a.rows, (long long)a.cols);
   // A vector a thread as far as a workgroup reaches, so that a row's loads all go out at once: 8192 rows of 4096 take
-  // 53 us with 256 threads a row and 147 with a wave that holds 8 vectors a thread.
+  // 55 us with 256 threads a row and 147 with a wave that holds 8 vectors a thread (both before other steps).
 #define ANNA_NORM(LANES, VECS)                                                                                          \
   (vec ? rms_norm_kernel<DT, LANES, VECS, CODES, true> : rms_norm_kernel<DT, LANES, VECS, CODES, false>)<<<blocks(256 / LANES), \
                                                                                                            256, 0, stream>>>(a)
