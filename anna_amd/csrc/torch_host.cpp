@@ -690,6 +690,15 @@ OptTensor causal_conv1d(const Tensor& x, const Tensor& weight, const OptTensor& 
   return out;
 }
 
+// Whether rows share no element: of other memory, or other columns of one matrix
+bool rows_apart(const Tensor& a, int64_t a_stride, const Tensor& b, int64_t b_stride, int64_t cols) {
+  const int64_t size = a.element_size(), between = reinterpret_cast<intptr_t>(ptr(b)) - reinterpret_cast<intptr_t>(ptr(a));
+  if (between >= ((a.numel() / cols - 1) * a_stride + cols) * size || -between >= ((b.numel() / cols - 1) * b_stride + cols) * size) return true;
+  if (a_stride != b_stride || between % size) return false;
+  const int64_t column = (between / size % a_stride + a_stride) % a_stride;
+  return column >= cols && column <= a_stride - cols;
+}
+
 // out, or with a group codes, and scales; undefined for calls that are left to the caller
 Tensor norm(const Tensor& x, const Tensor& weight, double eps, double weight_offset, const OptTensor& residual, const OptTensor& gate,
             int64_t group, Tensor* scales, int64_t device, uintptr_t stream) {
@@ -708,6 +717,10 @@ Tensor norm(const Tensor& x, const Tensor& weight, double eps, double weight_off
   anna_mi_rms_norm_args a{};
   if (!lies(x, a.x_stride) || (residual && !lies(*residual, a.residual_stride)) || (gate && !lies(*gate, a.gate_stride)) ||
       !given(weight, dev) || !is(weight, dev, dt) || weight.dim() != 1 || weight.size(0) != cols)
+    return none;
+  if (residual && ((!(ptr(*residual) == ptr(x) && a.residual_stride == a.x_stride) && !rows_apart(*residual, a.residual_stride, x, a.x_stride, cols)) ||
+                   (gate && !rows_apart(*residual, a.residual_stride, *gate, a.gate_stride, cols)) ||
+                   !rows_apart(*residual, a.residual_stride, weight, cols, cols)))
     return none;
   a.dtype = dtype_code(x), a.out_format = group > 0, a.rows = rows, a.cols = cols, a.group = group;
   a.x = ptr(x), a.weight = ptr(weight), a.residual = ptr(residual), a.gate = ptr(gate);

@@ -338,6 +338,16 @@ def _rows(what: str, t: torch.Tensor, x: torch.Tensor) -> tuple[torch.Tensor, in
     return t, (t.stride(0) if t.shape[0] > 1 else cols)
 
 
+def _rows_apart(a: torch.Tensor, a_stride: int, b: torch.Tensor, b_stride: int) -> bool:
+    """Whether rows of a and b share no element: of other memory, or other columns of one matrix."""
+    size, cols = a.element_size(), a.shape[-1]
+    a_bytes, b_bytes = (((t.numel() // cols - 1) * s + cols) * size for t, s in ((a, a_stride), (b, b_stride)))
+    between = b.data_ptr() - a.data_ptr()
+    if between >= a_bytes or -between >= b_bytes:
+        return True
+    return a_stride == b_stride and between % size == 0 and cols <= between // size % a_stride <= a_stride - cols
+
+
 def _norm(x, weight, eps, weight_offset, residual, gate, out, scales, group):
     if x.dim() < 1 or x.dtype not in _lib._DTYPE_CODES or x.shape[-1] < 1:
         raise ValueError(f"x must be [..., cols] in bfloat16, float16 or float32, got {x.dtype} {list(x.shape)}")
@@ -346,20 +356,26 @@ def _norm(x, weight, eps, weight_offset, residual, gate, out, scales, group):
         raise ValueError(f"weight must be {x.dtype} [{cols}], got {weight.dtype} {list(weight.shape)}")
     if not 0.0 <= eps < 1e30:
         raise ValueError(f"eps must be finite and not negative, got {eps}")
+    if x.numel() == 0:
+        _lib.require_device(x)
+        return _on(x.device, x=x, weight=weight, residual=residual, gate=gate, out=out)
+    rows, stride = _rows("x", x, x)
+    if residual is not None:
+        kept, residual_stride = _rows("residual", residual, x)
+        if kept.data_ptr() != residual.data_ptr():
+            raise ValueError("residual is written in place: its rows must lie at one stride, contiguous in the last dimension")
+        same = residual.data_ptr() == x.data_ptr() and residual_stride == stride  # x is then doubled
+        for name, t in (("x", None if same else rows), ("gate", gate), ("weight", weight)):
+            if t is not None and not _rows_apart(kept, residual_stride, *((t, cols) if t is weight else _rows(name, t, x))):
+                raise ValueError(f"residual must not overlap {name}")
     _lib.require_device(x)
     _on(x.device, x=x, weight=weight, residual=residual, gate=gate, out=out)
-    if x.numel() == 0:
-        return
-    rows, stride = _rows("x", x, x)
     args = _lib.RmsNormArgs(dtype=_lib.dtype_code(x.dtype), out_format=int(scales is not None), rows=rows.shape[0], cols=cols,
                             group=group, x=rows.data_ptr(), x_stride=stride, eps=eps, weight_offset=weight_offset)
     weight = weight.contiguous()
     args.weight = weight.data_ptr()
     if residual is not None:
-        kept, args.residual_stride = _rows("residual", residual, x)
-        if kept.data_ptr() != residual.data_ptr():
-            raise ValueError("residual is written in place: its rows must lie at one stride, contiguous in the last dimension")
-        args.residual = kept.data_ptr()
+        args.residual, args.residual_stride = kept.data_ptr(), residual_stride
     if gate is not None:
         gate, args.gate_stride = _rows("gate", gate, x)
         args.gate = gate.data_ptr()
@@ -374,7 +390,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, weight
     a gate is given; bf16, fp16 or fp32, sums in fp32.
 
     residual (same shape): x is added to it first, in place, and the sum, as the type holds it, is what is
-    normalised.  out (contiguous) may be x or gate themselves, and overlaps nothing else."""
+    normalised; it may be x itself, and overlaps nothing else.  out (contiguous) may be x or gate themselves, and overlaps nothing else."""
     if out is None:
         if x.is_cuda:
             device = _cuda_device()

@@ -154,6 +154,22 @@ def test_norm_refuses(kw, msg):
         la.rms_norm(**kw)
 
 
+def test_norm_refuses_a_residual_over_other_rows():
+    wide = torch.zeros(4, 64)
+    x, w = wide[:3, :16], torch.zeros(16)
+    for residual, kw, name in [(wide[1:, :16], {}, "x"), (wide[:3, 8:24], {}, "x"), (wide.view(-1)[4:52].view(3, 16), {}, "x"),
+                               (wide[:3, 16:32], dict(gate=wide[:3, 31:47]), "gate"), (wide[:3, 16:32], dict(gate=wide[:3, 16:32]), "gate")]:
+        with pytest.raises(ValueError, match=f"residual must not overlap {name}"):
+            la.rms_norm(x, w, residual=residual, **kw)
+        with pytest.raises(ValueError, match=f"residual must not overlap {name}"):
+            la.rms_norm_e4m3(x, w, residual=residual, **kw)
+    with pytest.raises(ValueError, match="residual must not overlap weight"):
+        la.rms_norm(x, wide[1, 24:40], residual=wide[:3, 16:32])
+    for residual in (x, wide[:3, 16:32], wide[:3, 48:], wide[3:, 16:64].view(3, 16)):
+        with pytest.raises(RuntimeError, match="ROCm"):  # nothing but the device
+            la.rms_norm(x, w, residual=residual)
+
+
 def test_norm_refuses_an_output_over_another_row():
     x = torch.zeros(64)
     with pytest.raises(ValueError, match="must not overlap x"):

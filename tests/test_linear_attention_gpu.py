@@ -517,6 +517,22 @@ def test_norm_of_many_short_rows(gpu):
     assert torch.equal(got[rows // 64 * 64:], got[:rows % 64])
 
 
+@pytest.mark.parametrize("cols", [64, 20000])
+def test_norm_of_slices_of_one_matrix(gpu, cols):
+    """x, residual and gate as columns of one matrix, and a residual that is x itself."""
+    wide, w = randn(1, 9, 3 * cols).to(BF).to(gpu), randn(2, cols).to(BF).to(gpu)
+    x, residual, gate = wide.split(cols, 1)
+    apart = [t.clone() for t in (x, residual, gate)]
+    want = la.rms_norm(apart[0], w, residual=apart[1], gate=apart[2])
+    assert torch.equal(la.rms_norm(x, w, residual=residual, gate=gate), want)
+    assert all(torch.equal(a, b) for a, b in zip((x, residual, gate), apart))
+    twice = 2 * x
+    want = la.rms_norm(twice, w)
+    assert torch.equal(la.rms_norm(x, w, residual=x), want) and torch.equal(x, twice)
+    with pytest.raises(ValueError, match="residual must not overlap x"):
+        la.rms_norm(wide[:-1, :cols], w, residual=wide[1:, :cols])
+
+
 def test_norm_layouts(gpu):
     """Rows of a wider tensor, an output in place, heads as leading dimensions."""
     x, w, z = randn(1, 6, 4, 64).to(BF), randn(2, 64).to(BF), randn(3, 6, 4, 64).to(BF)
