@@ -21,7 +21,7 @@
 // numbered so that the instruction's result, rows 4 g + r of a tile in lane (n, g), is at once the other operand of
 // the next product: row m of tile mt stands for index 32 (mt / 2) + 8 (m / 4) + 4 (mt % 2) + m % 4.
 //
-// What bounds it, 16 key and 32 value heads of 128, bf16.  One sequence of 16384 tokens: preparation 107 us, chain 415.
+// What bounds it, 16 key and 32 value heads of 128, bf16.  One sequence of 16384 tokens: preparation 105 us, chain 415.
 // The preparation writes 0.3 GB of workspace (58 us at a copy's rate); the rest is latency, about 36000 cycles a
 // workgroup of loads, products and the inverse's steps with three workgroups a compute unit to cover for each other (two: 121 us).
 // The chain is 256 chunks in a row at 1.6 us each on every compute unit: 82 matrix instructions of the state's
@@ -143,11 +143,14 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
   constexpr int LD = DK + 8;     // halves of a row of K in LDS
   constexpr int LF = CHUNK + 4;  // floats of a row of A, then T in its place, then P
   __shared__ _Float16 K[CHUNK][LD];
-  __shared__ float A[CHUNK][LF];
+  __shared__ __attribute__((aligned(16))) float a_rows[CHUNK * LF + 16 * 7];
   __shared__ Log2 sums[4][CHUNK];  // a / ln 2 of the next four value heads
   __shared__ float betas[4][CHUNK], kf[CHUNK], qf[CHUNK], tops[2][4];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+  // a wave writes rows 8 apart at the same time: every 8 rows 16 banks are left out (107 -> 105 us
+  // for 256 chunks of 16 key and 32 value heads)
+  auto A = [&](int i, int j) -> float& { return a_rows[i * LF + 16 * (i >> 3) + j]; };
   const uint32_t ratio = (uint32_t)a.value_heads / (uint32_t)a.key_heads, parts = (uint32_t)a.value_heads / (uint32_t)per;
   const uint32_t chunk = blockIdx.x / parts, hv0 = blockIdx.x % parts * per, hk = hv0 / ratio;
   const bool writes_k = hv0 % ratio == 0;
@@ -284,14 +287,14 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
           const int i = row_of(wave, 4 * g + r);
           const float t = (ai[r].hi - aj[ct].hi) + (ai[r].lo - aj[ct].lo), d = __builtin_amdgcn_exp2f(i >= j ? t : -INFINITY) * cj[ct];
           const float x = bi[r] * (ki[r] * kk[ct][r]) * d, y = qk[ct][r] * d;
-          A[i][j] = i > j ? x : 0.f;
+          A(i, j) = i > j ? x : 0.f;
           P[ct][r] = i >= j ? y : 0.f;
           p_top = fmaxf(p_top, fabsf(P[ct][r]) < INFINITY ? fabsf(P[ct][r]) : 0.f);  // a q that is not finite is its row's affair
         }
       } else {
         P[ct] = zero;
 #pragma unroll
-        for (int r = 0; r < 4; r++) A[row_of(wave, 4 * g + r)][j] = 0.f;
+        for (int r = 0; r < 4; r++) A(row_of(wave, 4 * g + r), j) = 0.f;
       }
     }
     __syncthreads();
@@ -305,31 +308,31 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
       for (int i = 0; i < 16; i++) {
         float s = i == n ? 1.f : 0.f;
 #pragma unroll
-        for (int k = 0; k < i; k++) s = fmaf(-A[16 * g + i][16 * g + k], x[k], s);
+        for (int k = 0; k < i; k++) s = fmaf(-A(16 * g + i, 16 * g + k), x[k], s);
         x[i] = s;
         t_top = fmaxf(t_top, fabsf(s * b));
       }
 #pragma unroll
-      for (int i = 0; i < 16; i++) A[16 * g + i][16 * g + n] = x[i];
+      for (int i = 0; i < 16; i++) A(16 * g + i, 16 * g + n) = x[i];
     }
     __syncthreads();
     // product of 16 x 16 blocks; the second form takes a result of the instruction as its right operand: its lane
     // (n, g) holds the rows 4 g + r
     auto block = [&](int lb, int lc, int rb, int rc, f32x4 c) {
 #pragma unroll
-      for (int k = 0; k < 4; k++) c = mfma4(A[16 * lb + n][16 * lc + 4 * g + k], A[16 * rb + 4 * g + k][16 * rc + n], c);
+      for (int k = 0; k < 4; k++) c = mfma4(A(16 * lb + n, 16 * lc + 4 * g + k), A(16 * rb + 4 * g + k, 16 * rc + n), c);
       return c;
     };
     auto times = [&](int lb, int lc, f32x4 x, f32x4 c) {
 #pragma unroll
-      for (int k = 0; k < 4; k++) c = mfma4(A[16 * lb + n][16 * lc + 4 * g + k], x[k], c);
+      for (int k = 0; k < 4; k++) c = mfma4(A(16 * lb + n, 16 * lc + 4 * g + k), x[k], c);
       return c;
     };
     auto put = [&](int rb, int cb, f32x4 y) {
       const float b = beta[16 * cb + n];
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        A[16 * rb + 4 * g + r][16 * cb + n] = -y[r];
+        A(16 * rb + 4 * g + r, 16 * cb + n) = -y[r];
         t_top = fmaxf(t_top, fabsf(y[r] * b));
       }
     };
@@ -368,7 +371,7 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
       const int i = row_of(mt, n), j = 32 * ks + 8 * g;
       float x[8];
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = A[i][j + e] * beta[j + e] * ts.down;
+      for (int e = 0; e < 8; e++) x[e] = A(i, j + e) * beta[j + e] * ts.down;
       f16x8 hi, lo;
       split(x, hi, lo);
       *(f16x8*)(t_to + (2 * f) * FRAG + 16 * lane) = hi;
@@ -391,7 +394,7 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
 #pragma unroll
     for (int ct = 0; ct < 4; ct++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) A[row_of(wave, 4 * g + r)][16 * ct + n] = P[ct][r];
+      for (int r = 0; r < 4; r++) A(row_of(wave, 4 * g + r), 16 * ct + n) = P[ct][r];
     __syncthreads();
     for (int f = wave; f < T_FRAGS; f += 4) {
       int mt, ks;
@@ -399,7 +402,7 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
       const int i = row_of(mt, n), j = 32 * ks + 8 * g;
       float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; e++) y[e] = A[i][j + e] * ps.down;
+      for (int e = 0; e < 8; e++) y[e] = A(i, j + e) * ps.down;
       f16x8 hi, lo;
       split(y, hi, lo);
       *(f16x8*)(p_to + ws.p_parts * f * FRAG + 16 * lane) = hi;
@@ -870,7 +873,7 @@ template <int DT, int DK>
 static int delta_chunks(const anna_mi_gated_delta_args& a, const anna_mi_state_span& s, hipStream_t stream) {
   const Places<DK> ws = places<DK>(a, s);
   // a key head's value heads in one workgroup share the products of K, where that still fills the chip: 256 chunks of
-  // 16 key heads take 107 us with both value heads and 143 with one; with the chains 32 chunks take 80 and 85, 16
+  // 16 key heads took 121 us with both value heads and 143 with one; with the chains 32 chunks take 80 and 85, 16
   // chunks 50 both ways
   const int64_t ratio = a.value_heads / a.key_heads;
   const int per = s.chunks * a.key_heads >= 512 ? (int)ratio : 1;
