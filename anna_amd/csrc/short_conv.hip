@@ -12,7 +12,10 @@
 //
 // Bound by the bytes of x and out.  12787 tokens of 8192 channels in 6 sequences, bf16, width 4 (0.42 GB): 85 us =
 // 4.9 TB/s; a copy of 1 GiB runs at 5.2.  8 channels a thread took 165 us (half the waves, so that loads wait for
-// stores), groups of four with branches in them 134.  One token of 64 sequences: 4.0 us, an empty launch takes 3.6.
+// stores), groups of four with branches in them 134; rows' addresses by addition and not by product took 284000 tokens of 96
+// channels from 29.5 to 27.4.  One token of 64 sequences: 4.0 us, an empty launch takes 3.6.
+#include <type_traits>
+
 #include "delta.hpp"
 
 namespace anna {
@@ -127,7 +130,10 @@ __global__ __launch_bounds__(256) void short_conv_kernel(const typename Elem<DT>
         save(to + (int64_t)j * channels, r);
       }
     }
-    auto outputs = [&](int k, int m) {  // of `m` tokens from k on; the next ones' rows are asked for in front of the stores
+    T* to = out + (int64_t)t * out_stride + c0;
+    const T* ahead = from + FOUR * x_stride;
+    // of `m` tokens from k on; the next ones' rows, which with `all` are all there, are asked for in front of the stores
+    auto outputs = [&](int k, int m, auto all) {
       Row rows[W - 1 + FOUR];
 #pragma unroll
       for (int j = 0; j < W - 1; j++) rows[j] = win[j];
@@ -135,9 +141,14 @@ __global__ __launch_bounds__(256) void short_conv_kernel(const typename Elem<DT>
       for (int i = 0; i < FOUR; i++) rows[W - 1 + i] = next[i];
 #pragma unroll
       for (int j = 0; j < W - 1; j++) win[j] = rows[FOUR + j];
-      if (m == FOUR)
+      if constexpr (all.value) {
+#pragma unroll
+        for (int i = 0; i < FOUR; i++) next[i] = load(ahead + i * x_stride);
+        ahead += FOUR * x_stride;
+      } else if (m == FOUR) {
 #pragma unroll
         for (int i = 0; i < FOUR; i++) next[i] = load(from + (int64_t)min(k + FOUR + i, run - 1) * x_stride);
+      }
       Row y[FOUR];
 #pragma unroll
       for (int i = 0; i < FOUR; i++)
@@ -150,11 +161,16 @@ __global__ __launch_bounds__(256) void short_conv_kernel(const typename Elem<DT>
         }
 #pragma unroll
       for (int i = 0; i < FOUR; i++)
-        if (i < m) save(out + (int64_t)(t + k + i) * out_stride + c0, y[i]);
+        if (i < m) save(to + i * out_stride, y[i]);
+      to += FOUR * out_stride;
     };
     int k = 0;
-    for (; k + FOUR <= run; k += FOUR) outputs(k, FOUR);
-    if (k < run) outputs(k, run - k);
+    for (; k + 2 * FOUR <= run; k += FOUR) outputs(k, FOUR, std::true_type());
+    if (k + FOUR <= run) {
+      outputs(k, FOUR, std::false_type());
+      k += FOUR;
+    }
+    if (k < run) outputs(k, run - k, std::false_type());
     t = stop;
   }
 }
