@@ -33,7 +33,7 @@
 // single buffers that the output's waves fill, took 430.
 #include <type_traits>
 
-#include "delta.hpp"
+#include "delta_step.hpp"
 
 namespace anna {
 
@@ -133,19 +133,45 @@ __device__ __forceinline__ double running_sum(double v, int row) {
   return v + (row > 2 ? t0 + t1 + t2 : row > 1 ? t0 + t1 : row > 0 ? t0 : 0.);
 }
 
-// A workgroup takes a chunk, a key head and `per` of its value heads.  A wave has the rows row_of(wave, 0..15) of K and Q,
+// Of the state's columns in a workgroup of the short sequences here: wide, as latency does not count beside the chunks
+// (24 sequences of 4 tokens and one of 2048: 95 us with 128 columns, 105 with 32)
+__host__ __device__ inline int step_cols(const anna_mi_gated_delta_args& a) { return a.value_dim % 128 == 0 ? 128 : 32; }
+
+// A workgroup takes a chunk, a key head and `per` of its value heads; those from `blocks` on take short sequences, which
+// then cost no launch of their own and run beside work that waits for latency (63 sequences of one token and one of 1024:
+// 106 us with a launch for each kind, 97.5 so; one of 1 token and four prompts of 268 to 1500 110 and 105).  A wave has the rows row_of(wave, 0..15) of K and Q,
 // which are at once their fragments and the left operands of K K^T and Q K^T.
 template <int DT, int DK>
 __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gated_delta_args a,
-                                                               const SpanChunk* __restrict__ chunks, const Places<DK> ws, int per) {
+                                                               const SpanChunk* __restrict__ chunks, const Places<DK> ws, int per,
+                                                               uint32_t blocks, const SpanSeq* __restrict__ steps) {
   typedef typename Elem<DT>::T T;
   constexpr int KS = DK / 32;
   constexpr int LD = DK + 8;     // halves of a row of K in LDS
   constexpr int LF = CHUNK + 4;  // floats of a row of A, then T in its place, then P
-  __shared__ _Float16 K[CHUNK][LD];
-  __shared__ __attribute__((aligned(16))) float a_rows[CHUNK * LF + 16 * 7];
-  __shared__ Log2 sums[4][CHUNK];  // a / ln 2 of the next four value heads
-  __shared__ float betas[4][CHUNK], kf[CHUNK], qf[CHUNK], tops[2][4];
+  struct Lds {
+    _Float16 K[CHUNK][LD];
+    float a_rows[CHUNK * LF + 16 * 7];
+    Log2 sums[4][CHUNK];  // a / ln 2 of the next four value heads
+    float betas[4][CHUNK], kf[CHUNK], qf[CHUNK], tops[2][4];
+  };
+  __shared__ __attribute__((aligned(16))) union {
+    Lds prepare;
+    StepLds<DK, 32> narrow;
+    StepLds<DK, 128> wide;
+  } lds;
+  if (blockIdx.x >= blocks) {  // the short sequences beside the chunks
+    const int slices = (int)a.value_dim / step_cols(a);
+    if (step_cols(a) == 32) delta_step_block<DT, DK, 32>(a, steps, slices, blockIdx.x - blocks, lds.narrow);
+    else delta_step_block<DT, DK, 128>(a, steps, slices, blockIdx.x - blocks, lds.wide);
+    return;
+  }
+  auto& K = lds.prepare.K;
+  auto& a_rows = lds.prepare.a_rows;
+  auto& sums = lds.prepare.sums;
+  auto& betas = lds.prepare.betas;
+  auto& tops = lds.prepare.tops;
+  auto &kf = lds.prepare.kf, &qf = lds.prepare.qf;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
   // a wave writes rows 8 apart at the same time: every 8 rows 16 banks are left out (107 -> 105 us
@@ -877,9 +903,9 @@ static int delta_chunks(const anna_mi_gated_delta_args& a, const anna_mi_state_s
   // chunks 50 both ways
   const int64_t ratio = a.value_heads / a.key_heads;
   const int per = s.chunks * a.key_heads >= 512 ? (int)ratio : 1;
-  const int64_t prepare = s.chunks * (a.value_heads / per), groups = s.chains * a.value_heads * (a.value_dim / 16);
-  ANNA_CHECK(prepare <= INT32_MAX / 256 && groups <= INT32_MAX / 128, "gated delta rule: too many tokens and heads for a launch");
-  delta_prepare_kernel<DT, DK><<<prepare, 256, 0, stream>>>(a, span_chunks(s), ws, per);
+  const int64_t steps = s.steps * a.value_heads * (a.value_dim / step_cols(a)), prepare = s.chunks * (a.value_heads / per), groups = s.chains * a.value_heads * (a.value_dim / 16);
+  ANNA_CHECK(prepare + steps <= INT32_MAX / 256 && groups <= INT32_MAX / 128, "gated delta rule: too many tokens and heads for a launch");
+  delta_prepare_kernel<DT, DK><<<prepare + steps, 256, 0, stream>>>(a, span_chunks(s), ws, per, (uint32_t)prepare, span_steps(s));
   ANNA_LAUNCH_CHECK("delta_prepare");
   const uint32_t units = (uint32_t)(s.chains * a.key_heads);
   hipError_t allowed = hipSuccess;
@@ -948,8 +974,7 @@ int anna_mi_gated_delta(const anna_mi_gated_delta_args* args, anna_mi_state_span
   ANNA_CHECK(span->chunks == 0 || (a.workspace && (uintptr_t)a.workspace % 256 == 0), "gated delta rule: no workspace, or not 256-byte aligned");
   span->least_slots = a.slots < span->least_slots ? a.slots : span->least_slots;
   hipStream_t st = anna::as_stream(stream);
-  if (const int rc = anna::delta_step(a, *span, st)) return rc;
-  if (span->chains == 0) return ANNA_MI_OK;
+  if (span->chains == 0) return anna::delta_step(a, *span, st);
   ANNA_DISPATCH_DTYPE(a.dtype, DT, {
     if constexpr (DT != ANNA_MI_F32)
       return a.key_dim == 64 ? anna::delta_chunks<DT, 64>(a, *span, st) : anna::delta_chunks<DT, 128>(a, *span, st);

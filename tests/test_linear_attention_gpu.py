@@ -300,6 +300,27 @@ def test_delta_rule_of_many_chunks(gpu, case):
     check_delta(c, counts, [False] * n, DK ** -0.5, out, state)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("DK,DV", [(64, 96), (128, 128), (64, 256), (128, 32)])
+def test_delta_rule_of_short_and_long_sequences(gpu, DK, DV, dtype):
+    """Sequences that are taken token by token beside those taken in chunks, of one call."""
+    counts = [1, 20, 12, 0, 13, 5, 130, 1, 7]
+    fresh = [False, True, True, False, False, False, False, True, False]
+    c = delta_case(DK + DV, counts, 2, 6, DK, DV, dtype, True)
+    out, state = run_delta(gpu, c, counts, fresh, DK ** -0.5)
+    check_delta(c, counts, fresh, DK ** -0.5, out, state)
+    for nobody in (0, 1):  # a short one, a long one
+        slots = list(c["slots"])
+        slots[nobody] = -1
+        part, after = run_delta(gpu, dict(c, slots=slots), counts, fresh, DK ** -0.5)
+        own = slice(0, 1) if nobody == 0 else slice(1, 21)
+        assert (part[own] == 0).all()
+        rest = torch.ones(len(part), dtype=torch.bool)
+        rest[own] = False
+        assert torch.equal(part[rest], out[rest])
+        assert torch.equal(after[c["slots"][nobody]], c["state"][c["slots"][nobody]].to(after))
+
+
 def test_delta_rule_in_pieces(gpu):
     """A sequence in one call, and in calls that continue each other through both forms."""
     counts = [150]
