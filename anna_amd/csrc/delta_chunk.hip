@@ -5,7 +5,7 @@
 //   out = e^a Q S + P u,    P_ij = e^{a_i - a_j} q_i . k_j  (j <= i)
 //   S'  = e^{a_63} S + (e^{a_63 - a} K)^T u
 // Everything that does not need S is computed for all chunks at once (delta_prepare_kernel, a workgroup a chunk and
-// value head); the chunks of a sequence then follow each other (delta_chain_kernel), where a wave owns 16 columns of
+// key head); the chunks of a sequence then follow each other (delta_chain_kernel), where a wave owns 16 columns of
 // one head's state and needs no other wave: columns of S, u and out depend on the same column of v only.
 //
 // Precision: the state stays fp32.  Products run on the fp16 matrix instructions with fp32 sums; an fp32

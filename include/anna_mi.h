@@ -835,7 +835,8 @@ int anna_mi_causal_conv1d(const void* x, int dtype, int64_t channels, int64_t x_
 /* y = h / sqrt(mean(h^2) + eps) * (weight + weight_offset) [* silu(gate)] of every row, with h = x, or
  * h = x + residual, rounded to the dtype and written back to residual.  out_format 0: out in dtype; 1: out e4m3
  * codes and scales fp32 [rows][cols / group]: scale = max|y| / 448 of the group's columns, code = e4m3(y / scale),
- * both 0 where max|y| < 2^-100.  group: 32, 64 or 128 (a divisor of cols, rows 16-byte aligned) or cols. */
+ * both 0 where max|y| < 2^-100.  group: 32, 64 or 128 (a divisor of cols) or cols.
+ * residual may be x itself with its stride; it and out overlap nothing else but out = x or gate. */
 typedef struct {
   int dtype, out_format;
   int64_t rows, cols, group;

@@ -554,6 +554,20 @@ def test_norm_of_slices_of_one_matrix(gpu, cols):
         la.rms_norm(wide[:-1, :cols], w, residual=wide[1:, :cols])
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("cols,group", [(96, 32), (128, None), (2048, 128), (20480, 64), (20480, None)])
+def test_norm_of_unaligned_rows(gpu, cols, group, dtype):
+    """Columns 3 and on of a wider matrix, to the bit as aligned ones."""
+    wide, w = randn(cols, 5, cols + 8).to(dtype).to(gpu), randn(2, cols).to(dtype).to(gpu)
+    x, residual = wide[:, 3:3 + cols], wide.flip(0)[:, 3:3 + cols]
+    kept = residual.contiguous()
+    for a, b in zip(la.rms_norm_e4m3(x, w, residual=residual, group_size=group),
+                    la.rms_norm_e4m3(x.contiguous(), w, residual=kept, group_size=group)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    assert torch.equal(residual, kept)
+    assert torch.equal(la.rms_norm(x, w), la.rms_norm(x.contiguous(), w))
+
+
 def test_norm_layouts(gpu):
     """Rows of a wider tensor, an output in place, heads as leading dimensions."""
     x, w, z = randn(1, 6, 4, 64).to(BF), randn(2, 64).to(BF), randn(3, 6, 4, 64).to(BF)
