@@ -251,7 +251,7 @@ class StateSpan(ctypes.Structure):
 
     _fields_ = [
         ("sequences", _I64), ("tokens", _I64), ("words", _I64), ("steps", _I64), ("chains", _I64), ("chunks", _I64),
-        ("max_slot", _I64), ("least_slots", _I64), ("buf", _P),
+        ("longest", _I64), ("max_slot", _I64), ("least_slots", _I64), ("buf", _P),
     ]
 
 

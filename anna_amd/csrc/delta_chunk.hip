@@ -31,6 +31,7 @@
 // busy, a third of the cycles with LDS, an eighth in its conflicts. Two column groups a wave, which halves what is
 // read, took 650: the vector unit of half the SIMDs is then too little. A wave more for every group's output, with operands in
 // single buffers that the output's waves fill, took 430.
+#include <algorithm>
 #include <type_traits>
 
 #include "delta_step.hpp"
@@ -919,12 +920,15 @@ static int delta_chunks(const anna_mi_gated_delta_args& a, const anna_mi_state_s
       kern<<<8 * ((units + 7) / 8) * (groups / units / CW), 64 * St::WAVES, St::BYTES, stream>>>(a, span_chains(s), ws, units); \
   }
   constexpr bool TWO = Stage<DT, DK, 2, true>::BYTES <= 160 * 1024;  // fp16 at 128 key dims: the second parts leave no room
-  // One workgroup fits a compute unit's LDS in each form.  Up to 256 column groups all have one to themselves: 415 us for
-  // 16384 tokens of 32 heads of 128, 461 with two groups in a workgroup, which in turn takes up to 512 groups in one go
-  // where one would need two.  From 1024 groups on four share the copies: 65 us for prompts of 1115 to 1500
-  // tokens, 77 with two; 350 for eight sequences in fp16, 714 with one.
-  if (a.value_dim % 64 == 0 && groups >= 1024) ANNA_CHAIN(4, false)
-  else if (TWO && groups > 256) ANNA_CHAIN((TWO ? 2 : 1), true)
+  // One workgroup fits a compute unit's LDS in each form.  Its time is the longest chain's or the work's share of 256 compute
+  // units, in chunks of 1.6 us with one column group (1.8 where the chip is full), 2.1 with two, 2.4 to 2.8 with four, which
+  // share the copies.  bf16, 32 heads of 128, the whole call, one against four: 4000 tokens 142 and 190 us, 4000 + 300
+  // 152 and 192, 3000 + 1000 + 200 153 and 154, 4000 + 2000 203 and 199, twice 2048 143 and 116, three times 208 and 129.
+  // Two are never better than four at 128 key dims (twice 2048: 119), and serve what four do not divide.
+  const int64_t work = s.chunks * a.value_heads * (a.value_dim / 16);
+  auto share = [&](int cw) { return std::max(256 * s.longest, work / cw); };
+  if (a.value_dim % 64 == 0 && 3 * share(1) > 4 * share(4)) ANNA_CHAIN(4, false)
+  else if (TWO && a.value_dim % 64 != 0 && 6 * share(1) > 7 * share(2)) ANNA_CHAIN((TWO ? 2 : 1), true)
   else ANNA_CHAIN(1, true)
 #undef ANNA_CHAIN
   if (allowed != hipSuccess) return fail_hip(allowed, "delta_chain");

@@ -14,7 +14,7 @@ static int lay_out(int64_t n, const int32_t* slots, const int64_t* counts, const
   ANNA_CHECK(s != nullptr, "state span: null span");
   ANNA_CHECK(n >= 0 && n <= INT32_MAX / 4, "state span: %lld sequences", (long long)n);
   ANNA_CHECK(n == 0 || (slots && counts), "state span: null slots or counts");
-  int64_t tokens = 0, steps = 0, chains = 0, chunks = 0, max_slot = -1;
+  int64_t tokens = 0, steps = 0, chains = 0, chunks = 0, longest = 0, max_slot = -1;
   for (int64_t i = 0; i < n; i++) {
     ANNA_CHECK(slots[i] >= -1, "state span: slot %d of sequence %lld", (int)slots[i], (long long)i);
     ANNA_CHECK(counts[i] >= 0 && counts[i] <= INT32_MAX, "state span: sequence %lld of %lld tokens", (long long)i, (long long)counts[i]);
@@ -23,7 +23,9 @@ static int lay_out(int64_t n, const int32_t* slots, const int64_t* counts, const
     max_slot = std::max<int64_t>(max_slot, slots[i]);
     if (counts[i] > STEP_TOKENS) {
       chains++;
-      chunks += (counts[i] + CHUNK - 1) / CHUNK;
+      const int64_t own = (counts[i] + CHUNK - 1) / CHUNK;
+      chunks += own;
+      longest = std::max(longest, own);
     } else if (counts[i] > 0) {
       steps++;
     }
@@ -39,7 +41,7 @@ static int lay_out(int64_t n, const int32_t* slots, const int64_t* counts, const
   }
   const int64_t total = 4 * n + 4 * steps + 8 * chains + 4 * chunks + tokens;
   if (words) {
-    ANNA_CHECK(s->sequences == n && s->tokens == tokens && s->steps == steps && s->chains == chains && s->chunks == chunks &&
+    ANNA_CHECK(s->sequences == n && s->tokens == tokens && s->steps == steps && s->chains == chains && s->chunks == chunks && s->longest == longest &&
                    s->words == std::max<int64_t>(1, total),
                "state span: filled with other counts than it was planned for");
     s->max_slot = max_slot;
@@ -79,6 +81,7 @@ static int lay_out(int64_t n, const int32_t* slots, const int64_t* counts, const
   s->steps = steps;
   s->chains = chains;
   s->chunks = chunks;
+  s->longest = longest;
   s->max_slot = max_slot;
   s->least_slots = INT64_MAX;
   return ANNA_MI_OK;

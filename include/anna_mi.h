@@ -777,6 +777,7 @@ typedef struct {
   int64_t sequences, tokens;
   int64_t words;                  /* int32 words of buf */
   int64_t steps, chains, chunks;  /* sequences taken token by token, in chunks of 64; chunks of all chains */
+  int64_t longest;                /* chunks of the longest chain */
   int64_t max_slot;               /* the largest slot, -1 without any */
   int64_t least_slots;            /* of the pools that calls took this span with: a captured call is replayed with slots
                                      below it (the kernels take others for a sequence of nobody) */

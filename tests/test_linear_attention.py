@@ -31,7 +31,7 @@ def test_struct_sizes():
 
 def test_layout():
     span, words = plan([5, -1, 0, 9, 2], [1, 12, 0, 13, 129], [0, 1, 0, 0, 7])
-    assert (span.sequences, span.tokens, span.steps, span.chains, span.chunks, span.max_slot) == (5, 155, 2, 2, 4, 9)
+    assert (span.sequences, span.tokens, span.steps, span.chains, span.chunks, span.longest, span.max_slot) == (5, 155, 2, 2, 4, 3, 9)
     assert words[:20] == [5, 0, 1, 0, -1, 1, 12, 1, 0, 13, 0, 0, 9, 13, 13, 0, 2, 26, 129, 1]
     assert words[20:28] == [5, 0, 1, 0, -1, 1, 12, 1]
     assert words[28:44] == [2, 26, 129, 1, 1, 0, 0, 0, 9, 13, 13, 0, 0, 0, 0, 0]
@@ -187,7 +187,7 @@ def test_e4m3_refuses_groups(cols, group):
 
 def test_c_entries_refuse():
     lib = _lib.load()
-    span = _lib.StateSpan(1, 1, 9, 1, 0, 0, 0, 1 << 40, None)
+    span = _lib.StateSpan(1, 1, 9, 1, 0, 0, 0, 0, 1 << 40, None)
     args = _lib.GatedDeltaArgs(dtype=_lib.F32)
     assert lib.anna_mi_gated_delta(None, ctypes.byref(span), None) == 1
     assert lib.anna_mi_gated_delta(ctypes.byref(args), ctypes.byref(span), None) == 1

@@ -102,8 +102,8 @@ def test_delta_rule(gpu, case):
     check_delta(c, counts, fresh, DK ** -0.5, out, state)
 
 
-# Workgroups of the chunks' form take 1, 2 or 4 groups of 16 columns, by sequences * value heads * columns / 16:
-# up to 256, to 1023, and more
+# Workgroups of the chunks' form take 1, 2 or 4 groups of 16 columns, by the work beside the longest sequence: chunks *
+# value heads * columns / 16 against 256 of its chunks.  The cases above take 1, these 4, or 2 where 64 does not divide value_dim.
 MANY = [
     (20, 2, 4, 128, 128, BF), (20, 4, 4, 64, 128, HF), (40, 2, 4, 128, 128, BF), (40, 1, 4, 128, 128, HF), (70, 2, 4, 64, 64, BF),
     (70, 1, 4, 64, 64, HF), (60, 2, 3 * 2, 128, 96, BF), (45, 2, 2, 128, 256, HF),
@@ -121,10 +121,21 @@ def test_delta_rule_of_many_sequences(gpu, case):
     check_delta(c, counts, fresh, DK ** -0.5, out, state)
 
 
-@pytest.mark.parametrize("n", [20, 40])
-def test_delta_rule_of_many_sequences_with_some_not_finite(gpu, n):
+@pytest.mark.parametrize("case", [(6, 16, 128, 128, BF), (6, 16, 128, 128, HF), (7, 24, 128, 96, BF), (6, 16, 64, 256, HF)],
+                         ids=lambda c: "x".join(map(str, c[:4])))
+def test_delta_rule_of_several_long_sequences(gpu, case):
+    n, HV, DK, DV, dtype = case
+    counts = [250 + 17 * i for i in range(n)]
+    fresh = [i % 2 == 0 for i in range(n)]
+    c = delta_case(n, counts, 2, HV, DK, DV, dtype, True)
+    out, state = run_delta(gpu, c, counts, fresh, DK ** -0.5)
+    check_delta(c, counts, fresh, DK ** -0.5, out, state)
+
+
+@pytest.mark.parametrize("n,DV", [(6, 128), (20, 128), (40, 96)])
+def test_delta_rule_of_many_sequences_with_some_not_finite(gpu, n, DV):
     counts = [70] * n
-    c = delta_case(n, counts, 2, 4, 128, 128, BF, False)
+    c = delta_case(n, counts, 2, 4, 128, DV, BF, False)
     c["v"][70 * 3 + 40, 2, 17] = float("nan")
     c["k"][70 * 5 + 66, 0, 3] = float("inf")
     out, state = run_delta(gpu, c, counts, [False] * n, 0.1)
@@ -135,7 +146,7 @@ def test_delta_rule_of_many_sequences_with_some_not_finite(gpu, n):
         assert torch.isfinite(part[:at]).all() and not torch.isfinite(part[at:, heads]).all(-1).any()
         rest = [h for h in range(4) if h not in heads]
         assert torch.isfinite(part[:, rest]).all() and torch.isfinite(state[c["slots"][i]][rest]).all()
-    assert torch.isfinite(state[c["slots"][3]][2][:, [j for j in range(128) if j != 17]]).all()
+    assert torch.isfinite(state[c["slots"][3]][2][:, [j for j in range(DV) if j != 17]]).all()
     # the tokens in front, and all other sequences
     c["v"][70 * 3 + 40:70 * 4] = 0
     c["k"][70 * 5 + 66:70 * 6] = 0
