@@ -54,18 +54,16 @@ struct Factors {
   float end, t_scale, p_scale, pad[253];
 };
 
-// The workspace: K and Q of every chunk and key head, T' (hi, lo), the factors and P (hi, and lo for fp16) of every
-// chunk and value head
+// The workspace: K and Q of every chunk and key head, T' (hi, lo), the factors and P (hi, lo) of every chunk and value head
 template <int DK> struct Places {
   static constexpr int64_t MAT = CHUNK * DK * 2;
   char* base;
   int64_t HK, HV, chunks;
-  int p_parts;
-  __host__ __device__ int64_t head_bytes() const { return T_FRAGS * FRAG * (2 + p_parts) + (int64_t)sizeof(Factors); }
-  __host__ __device__ int64_t bytes() const { return chunks * (HK * 2 * MAT + HV * head_bytes()); }
+  static constexpr int64_t HEAD = 4 * T_FRAGS * FRAG + (int64_t)sizeof(Factors);
+  __host__ __device__ int64_t bytes() const { return chunks * (HK * 2 * MAT + HV * HEAD); }
   __device__ char* k(int64_t chunk, int64_t hk) const { return base + (chunk * HK + hk) * 2 * MAT; }
   __device__ char* q(int64_t chunk, int64_t hk) const { return k(chunk, hk) + MAT; }
-  __device__ char* t(int64_t chunk, int64_t hv) const { return base + chunks * HK * 2 * MAT + (chunk * HV + hv) * head_bytes(); }
+  __device__ char* t(int64_t chunk, int64_t hv) const { return base + chunks * HK * 2 * MAT + (chunk * HV + hv) * HEAD; }
   __device__ Factors* factors(int64_t chunk, int64_t hv) const { return (Factors*)(t(chunk, hv) + 2 * T_FRAGS * FRAG); }
   __device__ char* p(int64_t chunk, int64_t hv) const { return (char*)(factors(chunk, hv) + 1); }
 };
@@ -432,8 +430,8 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
       for (int e = 0; e < 8; e++) y[e] = A(i, j + e) * ps.down;
       f16x8 hi, lo;
       split(y, hi, lo);
-      *(f16x8*)(p_to + ws.p_parts * f * FRAG + 16 * lane) = hi;
-      if (ws.p_parts == 2) *(f16x8*)(p_to + (2 * f + 1) * FRAG + 16 * lane) = lo;
+      *(f16x8*)(p_to + (2 * f) * FRAG + 16 * lane) = hi;
+      *(f16x8*)(p_to + (2 * f + 1) * FRAG + 16 * lane) = lo;
     }
   }
 }
@@ -519,26 +517,24 @@ __device__ __forceinline__ s16x4 read_column(const char* p) { return __builtin_a
 //     wave that copies operands from the workspace into LDS a chunk ahead.  For few sequences: the chain of states is
 //     all that counts, and what is not in it runs beside it.
 //   else: a wave for every column group, that takes the output too, and one for the copies.
-template <int DT, int DK, int CW, bool SPLIT> struct Stage {
-  static constexpr bool EXACT_OUT = DT == ANNA_MI_F16;  // an fp16 output shows the second parts of its operands
-  static constexpr int PARTS = EXACT_OUT ? 2 : 1, KS = DK / 32;
-  static constexpr int MAT = CHUNK * DK * 2, TS = 2 * T_FRAGS * FRAG, PS = PARTS * T_FRAGS * FRAG, FAC = (int)sizeof(Factors);
+template <int DK, int CW, bool SPLIT> struct Stage {
+  static constexpr int KS = DK / 32;
+  static constexpr int MAT = CHUNK * DK * 2, TS = 2 * T_FRAGS * FRAG, PS = TS, FAC = (int)sizeof(Factors);
   static constexpr int TILE = 16 * (CHUNK * 2 + 8);  // of v [64][16], and of the output's columns [16][64 + 4]
   static constexpr int STATE = MAT + TS + FAC + CW * TILE;  // K, T', factors, v
   static constexpr int OUT = MAT + (SPLIT ? FAC : 0) + PS;  // Q, factors, P
-  static constexpr int MAIL = SPLIT ? PARTS * (KS + 2) * FRAG + 256 + 64 : 0;  // S, u; their unit a lane; a flag
+  static constexpr int MAIL = SPLIT ? 2 * (KS + 2) * FRAG + 256 + 64 : 0;  // S, u; their unit a lane; a flag
   static constexpr int MAILS = 2 * STATE + 2 * OUT, TILES = MAILS + 2 * CW * MAIL, TOUCHED = TILES + (SPLIT ? CW * TILE : 0);
   static constexpr int COPIERS = SPLIT && CW == 1 ? 2 : 1, FIRST_COPIER = (SPLIT ? 2 : 1) * CW;
   static constexpr int WAVES = FIRST_COPIER + COPIERS, BYTES = TOUCHED + COPIERS * 256;
 };
 
 template <int DT, int DK, int CW, bool SPLIT>
-__global__ __launch_bounds__((64 * Stage<DT, DK, CW, SPLIT>::WAVES), 2) void delta_chain_kernel(
+__global__ __launch_bounds__((64 * Stage<DK, CW, SPLIT>::WAVES), 2) void delta_chain_kernel(
     const anna_mi_gated_delta_args a, const SpanChain* __restrict__ chains, const Places<DK> ws, uint32_t units) {
   typedef typename Elem<DT>::T T;
-  typedef Stage<DT, DK, CW, SPLIT> St;
+  typedef Stage<DK, CW, SPLIT> St;
   constexpr int NT = DK / 16, KS = DK / 32;
-  constexpr bool EXACT_OUT = St::EXACT_OUT;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t HV = a.value_heads, DV = a.value_dim;
@@ -645,31 +641,30 @@ __global__ __launch_bounds__((64 * Stage<DT, DK, CW, SPLIT>::WAVES), 2) void del
     for (int mt = 0; mt < 4; mt++) qs[mt] = zero;
 #pragma unroll
     for (int s = 0; s < KS; s++) {
-      if constexpr (EXACT_OUT)
 #pragma unroll
-        for (int mt = 0; mt < 4; mt++) qs[mt] = mfma16(Q[mt * KS + s], sl[s], qs[mt]);
+      for (int mt = 0; mt < 4; mt++) qs[mt] = mfma16(Q[mt * KS + s], sl[s], qs[mt]);
 #pragma unroll
       for (int mt = 0; mt < 4; mt++) qs[mt] = mfma16(Q[mt * KS + s], sh[s], qs[mt]);
     }
   };
-  auto load_p = [&](const char* at, const Factors* fac, f16x8 (&PF)[St::PARTS * T_FRAGS], f32x4 (&fd)[4], f32x4 (&fq)[4]) {
+  auto load_p = [&](const char* at, const Factors* fac, f16x8 (&PF)[2 * T_FRAGS], f32x4 (&fd)[4], f32x4 (&fq)[4]) {
 #pragma unroll
-    for (int f = 0; f < St::PARTS * T_FRAGS; f++) PF[f] = frag(at, f, lane);
+    for (int f = 0; f < 2 * T_FRAGS; f++) PF[f] = frag(at, f, lane);
 #pragma unroll
     for (int mt = 0; mt < 4; mt++) {
       fd[mt] = *(const f32x4*)&fac->decay[row_of(mt, 4 * g)];
       fq[mt] = *(const f32x4*)&fac->q[row_of(mt, 4 * g)];
     }
   };
-  auto finish = [&](int c, const f16x8 (&PF)[St::PARTS * T_FRAGS], const f32x4 (&fd)[4], const f32x4 (&fq)[4], const f16x8 (&uh)[2],
+  auto finish = [&](int c, const f16x8 (&PF)[2 * T_FRAGS], const f32x4 (&fd)[4], const f32x4 (&fq)[4], const f16x8 (&uh)[2],
                     const f16x8 (&ul)[2], const f32x4 (&qs)[4], float unit, float p_scale, char* tile) {
     f32x4 o[4] = {zero, zero, zero, zero};
 #pragma unroll
-    for (int part = EXACT_OUT ? 0 : 2; part < 3; part++)
+    for (int part = 0; part < 3; part++)
 #pragma unroll
       for (int f = 0; f < T_FRAGS; f++) {
         const int s = f >= 4, mt = s ? f - 2 : f;
-        o[mt] = mfma16(PF[St::PARTS * f + (part == 0)], part == 1 ? ul[s] : uh[s], o[mt]);
+        o[mt] = mfma16(PF[2 * f + (part == 0)], part == 1 ? ul[s] : uh[s], o[mt]);
       }
     // through LDS by columns, so that a lane takes a token's row of 32 bytes
 #pragma unroll
@@ -700,21 +695,21 @@ __global__ __launch_bounds__((64 * Stage<DT, DK, CW, SPLIT>::WAVES), 2) void del
         meet();
         const char *const st = lds + 2 * St::STATE + (c & 1) * St::OUT, *const mail = lds + St::MAILS + (2 * cg + (c & 1)) * St::MAIL;
         const Factors* const fac = (const Factors*)(st + St::MAT);
-        f16x8 sh[KS], sl[KS], uh[2], ul[2], Q[4 * KS], PF[St::PARTS * T_FRAGS];
+        f16x8 sh[KS], sl[KS], uh[2], ul[2], Q[4 * KS], PF[2 * T_FRAGS];
         f32x4 qs[4], fd[4], fq[4];
 #pragma unroll
         for (int s = 0; s < KS; s++) {
           sh[s] = frag(mail, s, lane);
-          if constexpr (EXACT_OUT) sl[s] = frag(mail, KS + 2 + s, lane);
+          sl[s] = frag(mail, KS + 2 + s, lane);
         }
         load_q(st, Q);
 #pragma unroll
         for (int s = 0; s < 2; s++) {
           uh[s] = frag(mail, KS + s, lane);
-          if constexpr (EXACT_OUT) ul[s] = frag(mail, 2 * KS + 2 + s, lane);
+          ul[s] = frag(mail, 2 * KS + 2 + s, lane);
         }
-        const float unit = *(const float*)(mail + St::PARTS * (KS + 2) * FRAG + 4 * lane);
-        const int taken = *(const int*)(mail + St::PARTS * (KS + 2) * FRAG + 256);
+        const float unit = *(const float*)(mail + 2 * (KS + 2) * FRAG + 4 * lane);
+        const int taken = *(const int*)(mail + 2 * (KS + 2) * FRAG + 256);
         load_p(st + St::MAT + St::FAC, fac, PF, fd, fq);
         const float p_scale = fac->p_scale;
         if (taken) continue;  // token by token, by the state's wave
@@ -797,7 +792,7 @@ __global__ __launch_bounds__((64 * Stage<DT, DK, CW, SPLIT>::WAVES), 2) void del
 #pragma unroll
       for (int s = 0; s < KS; s++) {
         *(f16x8*)(mail + s * FRAG + 16 * lane) = sh[s];
-        if constexpr (EXACT_OUT) *(f16x8*)(mail + (KS + 2 + s) * FRAG + 16 * lane) = sl[s];
+        *(f16x8*)(mail + (KS + 2 + s) * FRAG + 16 * lane) = sl[s];
       }
     }
     if constexpr (!SPLIT) {
@@ -860,10 +855,10 @@ __global__ __launch_bounds__((64 * Stage<DT, DK, CW, SPLIT>::WAVES), 2) void del
 #pragma unroll
       for (int s = 0; s < 2; s++) {
         *(f16x8*)(mail + (KS + s) * FRAG + 16 * lane) = uh[s];
-        if constexpr (EXACT_OUT) *(f16x8*)(mail + (2 * KS + 2 + s) * FRAG + 16 * lane) = ul[s];
+        *(f16x8*)(mail + (2 * KS + 2 + s) * FRAG + 16 * lane) = ul[s];
       }
-      *(float*)(mail + St::PARTS * (KS + 2) * FRAG + 4 * lane) = unit;
-      *(int*)(mail + St::PARTS * (KS + 2) * FRAG + 256) = taken;
+      *(float*)(mail + 2 * (KS + 2) * FRAG + 4 * lane) = unit;
+      *(int*)(mail + 2 * (KS + 2) * FRAG + 256) = taken;
     }
     if (taken) {
 #pragma unroll
@@ -876,7 +871,7 @@ __global__ __launch_bounds__((64 * Stage<DT, DK, CW, SPLIT>::WAVES), 2) void del
       for (int t = 0; t < NT; t++) S[t] = add[t];
       if constexpr (!SPLIT) {
         PHASE();
-        f16x8 PF[St::PARTS * T_FRAGS];
+        f16x8 PF[2 * T_FRAGS];
         f32x4 fd[4], fq[4];
         load_p(so + St::MAT, fac, PF, fd, fq);
         finish(c, PF, fd, fq, uh, ul, qs, unit, p_scale, tile);
@@ -893,7 +888,7 @@ __global__ __launch_bounds__((64 * Stage<DT, DK, CW, SPLIT>::WAVES), 2) void del
 // ---------------------------------------------------------------- host
 
 template <int DK> static Places<DK> places(const anna_mi_gated_delta_args& a, const anna_mi_state_span& s) {
-  return {(char*)a.workspace, a.key_heads, a.value_heads, s.chunks, a.dtype == ANNA_MI_F16 ? 2 : 1};
+  return {(char*)a.workspace, a.key_heads, a.value_heads, s.chunks};
 }
 
 template <int DT, int DK>
@@ -912,23 +907,24 @@ static int delta_chunks(const anna_mi_gated_delta_args& a, const anna_mi_state_s
   hipError_t allowed = hipSuccess;
 #define ANNA_CHAIN(CW, SPLIT)                                                                                             \
   {                                                                                                                       \
-    typedef Stage<DT, DK, CW, SPLIT> St;                                                                                  \
+    typedef Stage<DK, CW, SPLIT> St;                                                                                      \
     static_assert(St::BYTES <= 160 * 1024, "LDS");                                                                        \
     const auto kern = &delta_chain_kernel<DT, DK, CW, SPLIT>;                                                             \
     allowed = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, St::BYTES);              \
     if (allowed == hipSuccess)                                                                                            \
       kern<<<8 * ((units + 7) / 8) * (groups / units / CW), 64 * St::WAVES, St::BYTES, stream>>>(a, span_chains(s), ws, units); \
   }
-  constexpr bool TWO = Stage<DT, DK, 2, true>::BYTES <= 160 * 1024;  // fp16 at 128 key dims: the second parts leave no room
+  constexpr bool SPLIT_TWO = Stage<DK, 2, true>::BYTES <= 160 * 1024;  // at 128 key dims there is no room
   // One workgroup fits a compute unit's LDS in each form.  Its time is the longest chain's or the work's share of 256 compute
   // units, in chunks of 1.6 us with one column group (1.8 where the chip is full), 2.1 with two, 2.4 to 2.8 with four, which
   // share the copies.  bf16, 32 heads of 128, the whole call, one against four: 4000 tokens 142 and 190 us, 4000 + 300
   // 152 and 192, 3000 + 1000 + 200 153 and 154, 4000 + 2000 203 and 199, twice 2048 143 and 116, three times 208 and 129.
-  // Two are never better than four at 128 key dims (twice 2048: 119), and serve what four do not divide.
+  // Two are never better than four at 128 key dims (twice 2048: 119), and serve what four do not divide; there the
+  // output's wave of its own has no room in LDS (eight times 2048 at 96 columns: 351 us, 472 with one group).
   const int64_t work = s.chunks * a.value_heads * (a.value_dim / 16);
   auto share = [&](int cw) { return std::max(256 * s.longest, work / cw); };
   if (a.value_dim % 64 == 0 && 3 * share(1) > 4 * share(4)) ANNA_CHAIN(4, false)
-  else if (TWO && a.value_dim % 64 != 0 && 6 * share(1) > 7 * share(2)) ANNA_CHAIN((TWO ? 2 : 1), true)
+  else if (a.value_dim % 64 != 0 && 6 * share(1) > 7 * share(2)) ANNA_CHAIN(2, SPLIT_TWO)
   else ANNA_CHAIN(1, true)
 #undef ANNA_CHAIN
   if (allowed != hipSuccess) return fail_hip(allowed, "delta_chain");
