@@ -6,7 +6,7 @@
 // holds, as in a model that adds and normalises in two steps.  The output is rounded once, from fp32.
 //
 //   h = x + residual,   y = h / sqrt(mean(h^2) + eps) * (weight + offset) * silu(gate)
-//   e4m3: code = round(y 448 / m), scale = m / 448, m the largest |y| of a group
+//   e4m3: scale = m / 448, code = e4m3(y / scale), m the largest |y| of a group
 //
 // Bound by the rows' bytes.  8192 rows of 4096 with residual and e4m3 codes (0.24 GB): 49 us = 4.8 TB/s; a copy of
 // 1 GiB runs at 5.2 (55 us with a clamp of every code, which branches, and divisions by the group).  262144 rows of 128 with gate (0.2 GB): 41 us = 4.9 TB/s.  64 rows of 2048: 3.1 us, less
@@ -94,16 +94,31 @@ __device__ __forceinline__ uint32_t abs_max(const float (&y)[8], int n) {
     if (VEC || e < n) m = max(m, __float_as_uint(y[e]) & 0x7fffffffu);
   return m;
 }
-// Codes of eight values; `to_unit`: 448 / the group's largest, so that what two roundings add to a product is far from
-// 464, where e4m3 would end
+// What divides a group's values: its scale, the same or 0 where it is not finite, and 1 / scale.  With the reciprocal
+// rounded once, one step of Markstein's gives the quotient's own rounding: q = y r, q + (y - q scale) r.  A product with 448 / m
+// has two, and moves codes whose quotients are halfway between two.
+struct Scale {
+  float scale, finite, inverse;
+};
+__device__ __forceinline__ Scale scale_of(uint32_t largest) {
+  if (largest < TINY_BITS) return {0.f, 0.f, 0.f};
+  const float s = __uint_as_float(largest) / E4M3_MAX;
+  return {s, s < INFINITY ? s : 0.f, 1.f / s};
+}
+__device__ __forceinline__ float quotient(float y, const Scale& s) {
+  const float q = y * s.inverse;
+  return fmaf(fmaf(-q, s.finite, y), s.inverse, q);
+}
+
+// Codes of eight values; a quotient is at most 448 (1 + 2^-23), far from 464, where e4m3 would end
 template <bool VEC>
-__device__ __forceinline__ void save_codes(uint8_t* p, int n, const float (&y)[8], float to_unit) {
+__device__ __forceinline__ void save_codes(uint8_t* p, int n, const float (&y)[8], const Scale& s) {
   uint32_t w[2];
 #pragma unroll
   for (int h = 0; h < 2; h++) {
     float c[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) c[e] = y[4 * h + e] * to_unit;
+    for (int e = 0; e < 4; e++) c[e] = quotient(y[4 * h + e], s);
     int packed = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
     w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], packed, true);
   }
@@ -114,14 +129,6 @@ __device__ __forceinline__ void save_codes(uint8_t* p, int n, const float (&y)[8
     for (int e = 0; e < 8; e++)
       if (e < n) p[e] = (uint8_t)(w[e / 4] >> (8 * (e % 4)));
   }
-}
-struct Scale {
-  float scale, to_unit;
-};
-__device__ __forceinline__ Scale scale_of(uint32_t largest) {
-  if (largest < TINY_BITS) return {0.f, 0.f};
-  const float m = __uint_as_float(largest);
-  return {m / E4M3_MAX, E4M3_MAX / m};
 }
 
 // Group of `group` columns in lanes: of a row's LANES threads, group / 8 neighbours
@@ -203,7 +210,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(const anna_mi_rms_norm_ar
       } else {  // every group lies in neighbouring lanes of one vector row
         const Scale s = scale_of(group_max(m, (int)a.group / 8));
         if (live && n > 0) {
-          save_codes<VEC>((uint8_t*)a.out + row * a.out_stride + c, n, h[i], s.to_unit);
+          save_codes<VEC>((uint8_t*)a.out + row * a.out_stride + c, n, h[i], s);
           if ((c & (a.group - 1)) == 0) a.scales[row * (cols >> shift) + (c >> shift)] = s.scale;
         }
       }
@@ -217,7 +224,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(const anna_mi_rms_norm_ar
       for (int i = 0; i < VECS; i++) {
         const int64_t c = 8 * (int64_t)(lane + LANES * i);
         const int n = columns<VEC>(cols, c);
-        if (live && n > 0) save_codes<VEC>((uint8_t*)a.out + row * a.out_stride + c, n, h[i], s.to_unit);
+        if (live && n > 0) save_codes<VEC>((uint8_t*)a.out + row * a.out_stride + c, n, h[i], s);
       }
     }
   }
@@ -262,7 +269,7 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(const anna_mi_rms_no
   };
   const bool by_row = a.group == cols;
   const int shift = __builtin_ctz((uint32_t)a.group);  // of groups that are not whole rows
-  Scale s{0.f, 0.f};
+  Scale s{0.f, 0.f, 0.f};
   if constexpr (CODES) {
     if (by_row) {
       uint32_t top = 0;
@@ -286,7 +293,7 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(const anna_mi_rms_no
     } else {
       if (!by_row) s = scale_of(group_max(abs_max<VEC>(h, n), (int)a.group / 8));
       if (n > 0) {
-        save_codes<VEC>((uint8_t*)a.out + row * a.out_stride + c, n, h, s.to_unit);
+        save_codes<VEC>((uint8_t*)a.out + row * a.out_stride + c, n, h, s);
         if (!by_row && (c & (a.group - 1)) == 0) a.scales[row * (cols >> shift) + (c >> shift)] = s.scale;
       }
     }
