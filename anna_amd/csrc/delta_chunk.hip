@@ -730,7 +730,7 @@ __global__ __launch_bounds__((64 * Stage<DK, CW, SPLIT>::WAVES), 2) void delta_c
   // S, x and u of a column are held in its unit, a power of two, kept so that the largest of S and v is 2^3 to 2^11:
   // what is computed from them is then short of fp16's upper end, and 2^-25 below their roundings
   float unit = 1.f, per_unit = 1.f;
-  bool lost = false;  // the column is not finite any more
+  bool lost = false;  // the column's state is not finite any more
 
   for (int c = 0; c < count; c++) {
     meet();
@@ -865,7 +865,15 @@ __global__ __launch_bounds__((64 * Stage<DK, CW, SPLIT>::WAVES), 2) void delta_c
       for (int t = 0; t < NT; t++) S[t] *= unit;
       unit = per_unit = 1.f;
       delta_tokens<DT, DK>(a, seq.first + (int64_t)c * CHUNK, min(CHUNK, seq.tokens - c * CHUNK), hv, hk, col, g, S);
-      lost = lost || bad;
+      // 0, or a NaN where the state is not finite: products that overflow fp16 say nothing about it
+      float none = 0.f;
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) none = fmaf(S[t][r], 0.f, none);
+      none += lane_xor16(none);
+      none += lane_xor32(none);
+      lost = !(none == 0.f);
     } else {
 #pragma unroll
       for (int t = 0; t < NT; t++) S[t] = add[t];

@@ -53,3 +53,31 @@ def test_outputs_whose_terms_cancel(gpu, heads, DV, dtype):
     off = (out.double() - want).abs()
     assert (off <= tol).all(), float((off / tol).max())
     assert ((after.double() - S).norm(dim=1) <= 2.0 ** -18 * S.norm(dim=1)).all()
+
+
+def check(out, state, q, k, v, g, beta, S0, scaling, normalize=True):
+    """The bounds of tests/_linear.py for the chunks' form, without its allowance for outputs of fewer bits."""
+    want, S, sums, errors, E, c = plain.delta_rule(q, k, v, g.double(), beta.double(), S0, scaling, normalize, chunked=True)
+    size = 1.0 if normalize else float(q.double().norm(dim=-1).max())
+    tol = plain.delta_tolerance(want, sums, errors, c, out.dtype, scaling * size, False)
+    off = (out.double() - want).abs()
+    assert torch.isfinite(out).all() and (off <= tol).all(), float((off / tol).max())
+    off = (state.double() - S).norm(dim=1)
+    assert torch.isfinite(state).all() and (off <= E).all(), float((off / E).max())
+
+
+def sequence(seed, n, heads, DK, DV, dtype=BF):
+    q, k, v = randn(seed, n, heads, DK).to(dtype), randn(seed + 1, n, heads, DK).to(dtype), randn(seed + 2, n, heads, DV).to(dtype)
+    g, beta = -0.4 * torch.rand((n, heads), generator=torch.Generator().manual_seed(seed + 3)), torch.sigmoid(randn(seed + 4, n, heads))
+    return q, k, v, g, beta, 0.5 * randn(seed + 5, heads, DK, DV)
+
+
+# heads of 4 groups of columns a workgroup from 256 on, at 64 columns
+@pytest.mark.parametrize("heads", [2, 320])
+@pytest.mark.parametrize("power", [104, 110, 118])
+def test_values_that_no_unit_brings_into_fp16s_range(gpu, power, heads):
+    """Every chunk's products overflow; the state is finite all the time."""
+    q, k, v, g, beta, S = sequence(11, 260, heads, 64, 64)
+    v, S = (v.float() * 2.0 ** power).to(BF), S * 2.0 ** power
+    out, after = run(gpu, q, k, v, g, beta, S, 0.125)
+    check(out, after, q, k, v, g, beta, S, 0.125)
