@@ -48,11 +48,13 @@ __device__ __forceinline__ void t_frag(int f, int& mt, int& ks) {
 }
 
 // Factors of a chunk and value head: e^a and k's for K S; of (T' / its scale) x on its way to the state; e^a for Q S; q's
-// for the output (P and Q are without them, so rows of any size keep their bits); e^{a_63}, the scales of T' and P
+// for the output (P and Q are without them, so rows of any size keep their bits); e^{a_63}; of P times what `U_DOWN` leaves
+// of (T' / its scale) x, which is of x's size whatever beta is; the largest of that which P's product may take
 struct Factors {
   float decayed_k[CHUNK], to_end[CHUNK], decay[CHUNK], q[CHUNK];
-  float end, t_scale, p_scale, pad[253];
+  float end, p_scale, u_limit, pad[253];
 };
+constexpr float U_DOWN = 0x1p-15f;  // the largest of T' / its scale is 2^14 to 2^15
 
 // The workspace: K and Q of every chunk and key head, T' (hi, lo), the factors and P (hi, lo) of every chunk and value head
 template <int DK> struct Places {
@@ -411,8 +413,9 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
       to->to_end[tid] = exp2_of(at[CHUNK - 1], at[tid]) * kf[tid] * ts.up;
       if (tid == CHUNK - 1) to->end = e;
       if (tid == 0) {
-        to->t_scale = ts.up;
-        to->p_scale = ps.up;
+        const float scale = ps.up * (ts.up / U_DOWN);
+        to->p_scale = scale;
+        to->u_limit = scale < INFINITY ? 65504.f : -1.f;
       }
     }
     __syncthreads();
@@ -787,7 +790,7 @@ __global__ __launch_bounds__((64 * Stage<DK, CW, SPLIT>::WAVES), 2) void delta_c
     f32x4 fe[4];
 #pragma unroll
     for (int mt = 0; mt < 4; mt++) fe[mt] = *(const f32x4*)&fac->to_end[row_of(mt, 4 * g)];
-    const float t_scale = fac->t_scale, end = fac->end;
+    const float u_limit = fac->u_limit, end = fac->end;
     if constexpr (SPLIT) {
 #pragma unroll
       for (int s = 0; s < KS; s++) {
@@ -846,10 +849,12 @@ __global__ __launch_bounds__((64 * Stage<DK, CW, SPLIT>::WAVES), 2) void delta_c
       for (int t = 0; t < NT; t++) add[t] = mfma16(KT[2 * t + (j & 1)], j < 2 ? lo[j & 1] : hi[j & 1], add[t]);
     f16x8 uh[2], ul[2];
 #pragma unroll
-    for (int mt = 0; mt < 4; mt++) u[mt] *= t_scale;
+    for (int mt = 0; mt < 4; mt++) u[mt] *= U_DOWN;
     operand(u[0], u[1], uh[0], ul[0]);
     operand(u[2], u[3], uh[1], ul[1]);
-    const bool bad = !(fabsf(add[0][0]) < INFINITY) && !lost;
+    // u may overflow where the state's update does not
+    const float u_top = fmaxf(fmaxf(largest(u[0]), largest(u[1])), fmaxf(largest(u[2]), largest(u[3])));
+    const bool bad = !(fabsf(add[0][0]) < INFINITY && u_top <= u_limit) && !lost;
     const bool taken = __any(bad);
     if constexpr (SPLIT) {
 #pragma unroll

@@ -81,3 +81,24 @@ def test_values_that_no_unit_brings_into_fp16s_range(gpu, power, heads):
     v, S = (v.float() * 2.0 ** power).to(BF), S * 2.0 ** power
     out, after = run(gpu, q, k, v, g, beta, S, 0.125)
     check(out, after, q, k, v, g, beta, S, 0.125)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("heads", [2, 320])
+@pytest.mark.parametrize("length,beta", [(2.0 ** -5, 900.0), (2.0 ** -10, 2.0 ** 19)])
+def test_updates_beyond_fp16s_range(gpu, length, beta, heads, dtype):
+    """Short keys with a large beta, beta |k|^2 < 1: an update is of a thousand times the values' size, its part of the state is
+    not.  With k' = k / length, beta' = beta length^2 and v' = v / length the states are the same and keys are (nearly) unit ones,
+    so the bounds hold in these terms."""
+    q, k, v, g, _, S = sequence(31, 200, heads, 64, 64, dtype)
+    k = (k.float() / k.float().norm(dim=-1, keepdim=True) * length * 0.98).to(dtype)
+    q = (q.float() / 8).to(dtype)
+    beta = torch.full_like(g, beta)
+    out, after = run(gpu, q, k, v, g, beta, S, 1.0, normalize=False)
+    for h in range(0, heads, 16):  # the same rule in unit keys' terms
+        at = slice(h, h + 16)
+        want, end, sums, errors, E, c = plain.delta_rule(q[:, at], k[:, at].double() / length, v[:, at].double() / length,
+                                                         g[:, at].double(), beta[:, at].double() * length ** 2, S[at], 1.0, False, chunked=True)
+        tol = plain.delta_tolerance(want, sums, errors, c, dtype, float(q.double().norm(dim=-1).max()), False)
+        assert torch.isfinite(out[:, at]).all() and ((out[:, at].double() - want).abs() <= tol).all()
+        assert ((after[at].double() - end).norm(dim=1) <= E).all()
