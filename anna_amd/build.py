@@ -39,6 +39,10 @@ HIPCC_FLAGS = [
     "-packed-fp32-ops",
 ]
 
+# Of single sources.  Pairs of fp32 operations that end as a pair of fp16 values are made into vectors, which gfx950 then
+# takes apart, and not into the instructions that round on the way.
+FILE_FLAGS = {"delta_chunk.hip": ["-fno-slp-vectorize"]}
+
 
 def _hipcc() -> str:
     for cand in (os.environ.get("HIPCC"), "/opt/rocm/bin/hipcc", shutil.which("hipcc")):
@@ -81,7 +85,7 @@ def _compile(src: Path, stamp: str, force: bool = True) -> Path:
     obj = OBJ_DIR / (src.stem + ".o")
     if not force and src.name != "runtime.cpp" and _up_to_date(src, obj):
         return obj
-    cmd = [_hipcc(), *HIPCC_FLAGS, "-c", str(src), "-o", str(obj)]
+    cmd = [_hipcc(), *HIPCC_FLAGS, *FILE_FLAGS.get(src.name, []), "-c", str(src), "-o", str(obj)]
     if src.name == "runtime.cpp":
         cmd.insert(-4, f'-DANNA_MI_SOURCE_HASH="{stamp}"')
     proc = subprocess.run(cmd, capture_output=True, text=True)

@@ -9,28 +9,38 @@
 // one head's state and needs no other wave: columns of S, u and out depend on the same column of v only.
 //
 // Precision: the state stays fp32.  Products run on the fp16 matrix instructions with fp32 sums; an fp32
-// operand x enters as two fp16 values, hi = fp16(x / s) and lo = fp16(x / s - hi), 22 bits of it or 2^-25 where that is
-// more, with s a power of two of its column (of T': of the chunk).  q and k are exact in one fp16 value once a row's
-// power of two is taken out.
+// operand x enters as two fp16 values, hi = fp16(x / s) and lo = fp16(2^11 (x / s - hi)), 22 bits of it or 2^-36 where that
+// is more, with s a power of two of its column (of T' and P: of the chunk); what lo is a factor of is summed first, and
+// brought down by 2^11 in front of the other sums.  q and k are exact in one fp16 value once a row's power of two is
+// taken out.
+//
+// A column's unit s comes from the largest of its state and the chunk's values, which may be far above what a token sees
+// of them: an outlier that comes later, a state that a decay has made small.  What a token sees is
+//   n_i = max(e^{g_i} n_{i-1}, |k_i| beta_i |v_i|),   n_{-1} the state's largest,
+// and 2^-36 of the unit is below the roundings of fp32 sums of that size where n_i is at least 2^-14 units (times
+// |k| T' where that is above 1).  A chunk with a smaller n_i is taken token by token, from the state that the wave still has.
+// Most columns are fine at a glance: by the old state times the smallest e^a, or the smallest |v| times the smallest |k| beta.
+// The loop over n_i runs for the others: with ordinary values one chunk of some hundreds where decays are strong, for about
+// 1 us.  Without the factor 2^11 it would run in most chunks there.
 //
 // Zeros above the diagonals times what is not finite would reach the tokens in front of it.  It also reaches the whole
-// of its column's update, where a wave sees it and then takes the chunk token by token from the state that it still has.
+// of its column's update, where a wave sees it and also takes the chunk token by token.
 //
 // Operands are held in the order of the matrix instruction's registers: fragment (mt, ks) of an M x K operand
 // gives lane (n = lane % 16, g = lane / 16) the 8 values of row (mt, n) at k = 32 ks + 8 g + 0..7.  Rows of tile mt are
 // numbered so that the instruction's result, rows 4 g + r of a tile in lane (n, g), is at once the other operand of
 // the next product: row m of tile mt stands for index 32 (mt / 2) + 8 (m / 4) + 4 (mt % 2) + m % 4.
 //
-// What bounds it, 16 key and 32 value heads of 128, bf16.  One sequence of 16384 tokens: preparation 105 us, chain 415.
+// What bounds it, 16 key and 32 value heads of 128, bf16.  One sequence of 16384 tokens: preparation 111 us, chain 515.
 // The preparation writes 0.3 GB of workspace (58 us at a copy's rate); the rest is latency, about 36000 cycles a
 // workgroup of loads, products and the inverse's steps with three workgroups a compute unit to cover for each other (two: 121 us).
-// The chain is 256 chunks in a row at 1.6 us each on every compute unit: 82 matrix instructions of the state's
-// wave are a third of that, what makes their operands (splits, scales, LDS) another; the bytes alone would take 80 us.
-// Eight sequences of 25344 tokens together, fp16: preparation 160 us, chain 350. Four waves a compute unit there read all
-// operands from LDS, 2.7 to 2.9 us a chunk: without copies from memory it is as long, vector unit 41% and matrix cores 26%
-// busy, a third of the cycles with LDS, an eighth in its conflicts. Two column groups a wave, which halves what is
-// read, took 650: the vector unit of half the SIMDs is then too little. A wave more for every group's output, with operands in
-// single buffers that the output's waves fill, took 430.
+// The chain is 256 chunks in a row at 2.0 us each on every compute unit: 82 matrix instructions of the state's
+// wave are a quarter of that, some 400 vector instructions that make their operands (splits, scales) a third; the bytes alone
+// would take 80 us.  (1.6 us with outputs from one term and terms of one scale, 1.8 with both terms.)
+// Eight sequences of 25344 tokens together, fp16: preparation 168 us, chain 425 (350 with terms of one scale). Four waves a
+// compute unit there read all operands from LDS, 3.6 us a chunk: without copies from memory it is as long.
+// Two column groups a wave, which halves what is read, took 650 for 350: the vector unit of half the SIMDs is then too little.
+// A wave more for every group's output, with operands in single buffers that the output's waves fill, took 430 for 350.
 #include <algorithm>
 #include <type_traits>
 
@@ -47,14 +57,16 @@ __device__ __forceinline__ void t_frag(int f, int& mt, int& ks) {
   mt = ks ? f - 2 : f;
 }
 
-// Factors of a chunk and value head: e^a and k's for K S; of (T' / its scale) x on its way to the state; e^a for Q S; q's
-// for the output (P and Q are without them, so rows of any size keep their bits); e^{a_63}; of P times what `U_DOWN` leaves
-// of (T' / its scale) x, which is of x's size whatever beta is; the largest of that which P's product may take
+// Factors of a chunk and value head: e^a and k's for 2^11 K S; of (T' / its scale) x on its way to the state, times 2^11; e^a
+// for Q S; q's for the output (P and Q are without them, so rows of any size keep their bits); e^{a_63}; of P times
+// what `U_DOWN` leaves of (T' / its scale) x, which is of x's size whatever beta is.  For the n_i: e^g and |k| beta of
+// every token, the smallest of that and of e^a, and what no n_i may be below.
 struct Factors {
-  float decayed_k[CHUNK], to_end[CHUNK], decay[CHUNK], q[CHUNK];
-  float end, p_scale, u_limit, pad[253];
+  float decayed_k[CHUNK], to_end[CHUNK], decay[CHUNK], q[CHUNK], step[CHUNK], weight[CHUNK];
+  float end, p_scale, least_weight, least_decay, need, pad[123];
 };
 constexpr float U_DOWN = 0x1p-15f;  // the largest of T' / its scale is 2^14 to 2^15
+constexpr float LO_UP = 0x1p11f, LO_DOWN = 0x1p-11f;
 
 // The workspace: K and Q of every chunk and key head, T' (hi, lo), the factors and P (hi, lo) of every chunk and value head
 template <int DK> struct Places {
@@ -72,33 +84,37 @@ template <int DK> struct Places {
 
 // ---------------------------------------------------------------- powers of two
 
-// {2^(14 - e), 2^(e - 14)} for a largest value of exponent e, within fp32's normal range; of 0 the smallest
+// {2^(14 - e), 2^(e - 14)} for a largest value of exponent e, so that 2^11 of the first is in fp32's range; of 0 the smallest
 struct Pow2 {
   float down, up;
 };
 __device__ __forceinline__ Pow2 pow2_of(float largest) {
-  const uint32_t e = min(max((__float_as_uint(largest) >> 23) & 255u, 15u), 254u);
+  const uint32_t e = min(max((__float_as_uint(largest) >> 23) & 255u, 26u), 254u);
   return {__uint_as_float((268u - e) << 23), __uint_as_float((e - 14u) << 23)};
 }
 
 __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
-// hi and lo of eight values.  The pair of hi passes through a register of its own: a value that is a product may
-// be rounded in one step or two, and lo has to be what is left of the hi that the matrix instruction gets.  `one`
-// is 1, which the compiler does not know: x - hi is then one instruction with its rounding (v_fma_mix).
-__device__ __forceinline__ void split(const float (&x)[8], f16x8& hi, f16x8& lo) {
+// hi and lo of eight values x, with UP given as 2^11 x (what made them then has the factor).  The pair of hi
+// passes through a register of its own: a value that is a product may be rounded in one step or two, and lo has to be
+// what is left of the hi that the matrix instruction gets.  In the constants' registers, which the compiler does not look
+// into, a product or sum and its rounding to fp16 are one instruction (v_fma_mix).
+template <bool UP = false> __device__ __forceinline__ void split(const float (&x)[8], f16x8& hi, f16x8& lo) {
   typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-  float one = 1.f;
-  asm("" : "+s"(one));
+  float down = LO_DOWN, up = -LO_UP;
+  asm("" : "+s"(up));
+  if constexpr (UP) asm("" : "+s"(down));
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
-    f16x2 h = {(_Float16)x[e], (_Float16)x[e + 1]};
+    f16x2 h;
+    if constexpr (UP) h = {(_Float16)fmaf(x[e], down, 0.f), (_Float16)fmaf(x[e + 1], down, 0.f)};
+    else h = {(_Float16)x[e], (_Float16)x[e + 1]};
     asm("" : "+v"(h));
     hi[e] = h[0];
     hi[e + 1] = h[1];
-    lo[e] = (_Float16)fmaf(x[e], one, -(float)h[0]);
-    lo[e + 1] = (_Float16)fmaf(x[e + 1], one, -(float)h[1]);
+    lo[e] = (_Float16)fmaf((float)h[0], up, UP ? x[e] : x[e] * LO_UP);
+    lo[e + 1] = (_Float16)fmaf((float)h[1], up, UP ? x[e + 1] : x[e + 1] * LO_UP);
   }
 }
 
@@ -111,6 +127,15 @@ struct Log2 {
 };
 __device__ __forceinline__ float exp2_of(Log2 a, Log2 b) { return __builtin_amdgcn_exp2f((a.hi - b.hi) + (a.lo - b.lo)); }
 __device__ __forceinline__ float exp2_of(Log2 a) { return __builtin_amdgcn_exp2f(a.hi + a.lo); }
+
+__device__ __forceinline__ float wave_max_rows(float v) {
+  v = fmaxf(v, dpp_move<0xB1>(v));
+  v = fmaxf(v, dpp_move<0x4E>(v));
+  v = fmaxf(v, dpp_move<0x141>(v));
+  v = fmaxf(v, dpp_move<0x140>(v));
+  v = fmaxf(v, lane_xor16(v));
+  return fmaxf(v, lane_xor32(v));
+}
 
 // Sums up to and with every lane
 template <int SHIFT>
@@ -154,7 +179,7 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
     _Float16 K[CHUNK][LD];
     float a_rows[CHUNK * LF + 16 * 7];
     Log2 sums[4][CHUNK];  // a / ln 2 of the next four value heads
-    float betas[4][CHUNK], kf[CHUNK], qf[CHUNK], tops[2][4];
+    float betas[4][CHUNK], kf[CHUNK], qf[CHUNK], kn[CHUNK], tops[2][4];
   };
   __shared__ __attribute__((aligned(16))) union {
     Lds prepare;
@@ -172,7 +197,7 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
   auto& sums = lds.prepare.sums;
   auto& betas = lds.prepare.betas;
   auto& tops = lds.prepare.tops;
-  auto &kf = lds.prepare.kf, &qf = lds.prepare.qf;
+  auto &kf = lds.prepare.kf, &qf = lds.prepare.qf, &kn = lds.prepare.kn;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
   // a wave writes rows 8 apart at the same time: every 8 rows 16 banks are left out (107 -> 105 us
@@ -245,10 +270,21 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
     for (int s = 0; s < KS; s++)
 #pragma unroll
       for (int j = 0; j < 8; j++) (which ? qr : kr)[s][j] = (_Float16)ldexpf(x[s][j], e);
-    if (g == 0) {
-      const float f = ldexpf(a.normalize ? rsqrtf(ss + NORM_EPS) : 1.f, -e);
-      if (which) qf[mine] = f * a.scaling;
-      else kf[mine] = f;
+    const float f = ldexpf(a.normalize ? rsqrtf(ss + NORM_EPS) : 1.f, -e);
+    if (which) {
+      if (g == 0) qf[mine] = f * a.scaling;
+    } else {
+      float length = 0.f;  // |k|: of the row without its power of two, so of any size
+#pragma unroll
+      for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) length = fmaf((float)kr[s][j], (float)kr[s][j], length);
+      length += lane_xor16(length);
+      length += lane_xor32(length);
+      if (g == 0) {
+        kf[mine] = f;
+        kn[mine] = f * sqrtf(length);
+      }
     }
   }
 #pragma unroll
@@ -398,24 +434,30 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
       const int i = row_of(mt, n), j = 32 * ks + 8 * g;
       float x[8];
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = A(i, j + e) * beta[j + e] * ts.down;
+      for (int e = 0; e < 8; e++) x[e] = A(i, j + e) * beta[j + e] * (ts.down * LO_UP);
       f16x8 hi, lo;
-      split(x, hi, lo);
+      split<true>(x, hi, lo);
       *(f16x8*)(t_to + (2 * f) * FRAG + 16 * lane) = hi;
       *(f16x8*)(t_to + (2 * f + 1) * FRAG + 16 * lane) = lo;
     }
     if (tid < CHUNK) {
       Factors* to = ws.factors(chunk, hv);
-      const float e = exp2_of(at[tid]);
-      to->decayed_k[tid] = e * kf[tid];
+      const float e = exp2_of(at[tid]), weight = tid < tokens ? kn[tid] * fabsf(beta[tid]) : 0.f;
+      to->decayed_k[tid] = e * kf[tid] * LO_UP;
       to->decay[tid] = e;
       to->q[tid] = qf[tid];
-      to->to_end[tid] = exp2_of(at[CHUNK - 1], at[tid]) * kf[tid] * ts.up;
+      to->to_end[tid] = exp2_of(at[CHUNK - 1], at[tid]) * kf[tid] * ts.up * LO_UP;
+      to->step[tid] = tid > 0 ? exp2_of(at[tid], at[tid - 1]) : e;
+      to->weight[tid] = weight;
       if (tid == CHUNK - 1) to->end = e;
+      const float least_weight = -wave_max_rows(tid < tokens ? -weight : -INFINITY), least_decay = -wave_max_rows(-e);
+      const float longest = wave_max_rows(tid < tokens ? kn[tid] : 0.f);
       if (tid == 0) {
-        const float scale = ps.up * (ts.up / U_DOWN);
-        to->p_scale = scale;
-        to->u_limit = scale < INFINITY ? 65504.f : -1.f;
+        const float largest = ts.up / U_DOWN, scale = ps.up * largest;
+        to->p_scale = fminf(scale, 0x1p127f);
+        to->least_weight = least_weight;
+        to->least_decay = least_decay;
+        to->need = scale < 0x1p127f ? 0x1p-14f * fmaxf(1.f, longest * largest) : INFINITY;
       }
     }
     __syncthreads();
@@ -430,9 +472,9 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
       const int i = row_of(mt, n), j = 32 * ks + 8 * g;
       float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; e++) y[e] = A(i, j + e) * ps.down;
+      for (int e = 0; e < 8; e++) y[e] = A(i, j + e) * (ps.down * LO_UP);
       f16x8 hi, lo;
-      split(y, hi, lo);
+      split<true>(y, hi, lo);
       *(f16x8*)(p_to + (2 * f) * FRAG + 16 * lane) = hi;
       *(f16x8*)(p_to + (2 * f + 1) * FRAG + 16 * lane) = lo;
     }
@@ -453,17 +495,25 @@ template <int DT> __device__ __forceinline__ uint32_t pair_of(float x, float y) 
   else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
 }
 
-// Largest of a column, over the four lanes that hold it
+// Largest and smallest size, and the largest of a column over the four lanes that hold it.  A NaN is the answer of all three,
+// so that one instruction takes three values as they are.
+__device__ __forceinline__ float max_of(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ float min_of(float a, float b) { return __builtin_elementwise_minimum(a, b); }
 __device__ __forceinline__ float column_max(float v) {
-  v = fmaxf(v, lane_xor16(v));
-  return fmaxf(v, lane_xor32(v));
+  v = max_of(v, lane_xor16(v));
+  return max_of(v, lane_xor32(v));
 }
 // Tiles 2 s and 2 s + 1 of a product's result as the operand of the next
-__device__ __forceinline__ void operand(f32x4 x, f32x4 y, f16x8& hi, f16x8& lo) {
+template <bool UP> __device__ __forceinline__ void operand(f32x4 x, f32x4 y, f16x8& hi, f16x8& lo) {
   const float f[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-  split(f, hi, lo);
+  split<UP>(f, hi, lo);
 }
-__device__ __forceinline__ float largest(const f32x4& x) { return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))); }
+__device__ __forceinline__ float largest(float top, const f32x4& x) {
+  return max_of(max_of(max_of(top, fabsf(x[0])), fabsf(x[1])), max_of(fabsf(x[2]), fabsf(x[3])));
+}
+__device__ __forceinline__ float smallest(float least, const f32x4& x) {
+  return min_of(min_of(min_of(least, fabsf(x[0])), fabsf(x[1])), min_of(fabsf(x[2]), fabsf(x[3])));
+}
 
 // Tokens one after the other, on the chain's layout of the state: lane (n, g) holds rows row_of(t, 4 g + r) of column n
 template <int DT, int DK>
@@ -643,12 +693,15 @@ __global__ __launch_bounds__((64 * Stage<DK, CW, SPLIT>::WAVES), 2) void delta_c
 #pragma unroll
     for (int mt = 0; mt < 4; mt++) qs[mt] = zero;
 #pragma unroll
-    for (int s = 0; s < KS; s++) {
+    for (int s = 0; s < KS; s++)
 #pragma unroll
       for (int mt = 0; mt < 4; mt++) qs[mt] = mfma16(Q[mt * KS + s], sl[s], qs[mt]);
 #pragma unroll
+    for (int mt = 0; mt < 4; mt++) qs[mt] *= LO_DOWN;
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
       for (int mt = 0; mt < 4; mt++) qs[mt] = mfma16(Q[mt * KS + s], sh[s], qs[mt]);
-    }
   };
   auto load_p = [&](const char* at, const Factors* fac, f16x8 (&PF)[2 * T_FRAGS], f32x4 (&fd)[4], f32x4 (&fq)[4]) {
 #pragma unroll
@@ -659,16 +712,23 @@ __global__ __launch_bounds__((64 * Stage<DK, CW, SPLIT>::WAVES), 2) void delta_c
       fq[mt] = *(const f32x4*)&fac->q[row_of(mt, 4 * g)];
     }
   };
-  auto finish = [&](int c, const f16x8 (&PF)[2 * T_FRAGS], const f32x4 (&fd)[4], const f32x4 (&fq)[4], const f16x8 (&uh)[2],
-                    const f16x8 (&ul)[2], const f32x4 (&qs)[4], float unit, float p_scale, char* tile) {
+  auto finish = [&](int c, const f16x8 (&PF)[2 * T_FRAGS], const f32x4 (&fd)[4], const f32x4 (&fq)[4], const f32x4 (&u)[4],
+                    const f32x4 (&qs)[4], float unit, float p_scale, char* tile) {
+    f16x8 uh[2], ul[2];
+#pragma unroll
+    for (int s = 0; s < 2; s++) operand<true>(u[2 * s] * (U_DOWN * LO_UP), u[2 * s + 1] * (U_DOWN * LO_UP), uh[s], ul[s]);
     f32x4 o[4] = {zero, zero, zero, zero};
 #pragma unroll
-    for (int part = 0; part < 3; part++)
+    for (int part = 0; part < 3; part++) {
 #pragma unroll
       for (int f = 0; f < T_FRAGS; f++) {
         const int s = f >= 4, mt = s ? f - 2 : f;
         o[mt] = mfma16(PF[2 * f + (part == 0)], part == 1 ? ul[s] : uh[s], o[mt]);
       }
+      if (part == 1)
+#pragma unroll
+        for (int mt = 0; mt < 4; mt++) o[mt] *= LO_DOWN;
+    }
     // through LDS by columns, so that a lane takes a token's row of 32 bytes
 #pragma unroll
     for (int mt = 0; mt < 4; mt++) {
@@ -698,26 +758,23 @@ __global__ __launch_bounds__((64 * Stage<DK, CW, SPLIT>::WAVES), 2) void delta_c
         meet();
         const char *const st = lds + 2 * St::STATE + (c & 1) * St::OUT, *const mail = lds + St::MAILS + (2 * cg + (c & 1)) * St::MAIL;
         const Factors* const fac = (const Factors*)(st + St::MAT);
-        f16x8 sh[KS], sl[KS], uh[2], ul[2], Q[4 * KS], PF[2 * T_FRAGS];
-        f32x4 qs[4], fd[4], fq[4];
+        f16x8 sh[KS], sl[KS], Q[4 * KS], PF[2 * T_FRAGS];
+        f32x4 qs[4], u[4], fd[4], fq[4];
 #pragma unroll
         for (int s = 0; s < KS; s++) {
           sh[s] = frag(mail, s, lane);
-          sl[s] = frag(mail, KS + 2 + s, lane);
+          sl[s] = frag(mail, KS + s, lane);
         }
         load_q(st, Q);
 #pragma unroll
-        for (int s = 0; s < 2; s++) {
-          uh[s] = frag(mail, KS + s, lane);
-          ul[s] = frag(mail, 2 * KS + 2 + s, lane);
-        }
+        for (int mt = 0; mt < 4; mt++) u[mt] = *(const f32x4*)(mail + (2 * KS + mt) * FRAG + 16 * lane);
         const float unit = *(const float*)(mail + 2 * (KS + 2) * FRAG + 4 * lane);
         const int taken = *(const int*)(mail + 2 * (KS + 2) * FRAG + 256);
         load_p(st + St::MAT + St::FAC, fac, PF, fd, fq);
         const float p_scale = fac->p_scale;
         if (taken) continue;  // token by token, by the state's wave
         q_times(Q, sh, sl, qs);
-        finish(c, PF, fd, fq, uh, ul, qs, unit, p_scale, lds + St::TILES + cg * St::TILE);
+        finish(c, PF, fd, fq, u, qs, unit, p_scale, lds + St::TILES + cg * St::TILE);
       }
       return;
     }
@@ -730,8 +787,8 @@ __global__ __launch_bounds__((64 * Stage<DK, CW, SPLIT>::WAVES), 2) void delta_c
   for (int t = 0; t < NT; t++)
 #pragma unroll
     for (int r = 0; r < 4; r++) S[t][r] = seq.fresh ? 0.f : state[row_of(t, 4 * g + r) * DV];
-  // S, x and u of a column are held in its unit, a power of two, kept so that the largest of S and v is 2^3 to 2^11:
-  // what is computed from them is then short of fp16's upper end, and 2^-25 below their roundings
+  // S, x and u of a column are held in its unit, a power of two, kept so that the largest of S and v is 2^6 to 2^11:
+  // what is computed from them is then short of fp16's upper end
   float unit = 1.f, per_unit = 1.f;
   bool lost = false;  // the column's state is not finite any more
 
@@ -752,50 +809,65 @@ __global__ __launch_bounds__((64 * Stage<DK, CW, SPLIT>::WAVES), 2) void delta_c
 #pragma unroll
     for (int mt = 0; mt < 4; mt++) fk[mt] = *(const f32x4*)&fac->decayed_k[row_of(mt, 4 * g)];
     f32x4 x[4];
-    float top = 0.f, v_top = 0.f;
+    float s_top = 0.f, v_top = 0.f, v_least = INFINITY;
 #pragma unroll
-    for (int t = 0; t < NT; t++) top = fmaxf(top, largest(S[t]));
+    for (int t = 0; t < NT; t++) s_top = largest(s_top, S[t]);
 #pragma unroll
     for (int mt = 0; mt < 4; mt++) {
 #pragma unroll
       for (int r = 0; r < 4; r++) x[mt][r] = Elem<DT>::to_f32((T)v[mt][r]);
-      v_top = fmaxf(v_top, largest(x[mt]));
+      v_top = largest(v_top, x[mt]);
+      v_least = smallest(v_least, x[mt]);
     }
-    top = column_max(fmaxf(top, v_top * per_unit));
-    if (__any(top > 2048.f || (top < 8.f && top > 0.f))) {
+    const float top = column_max(max_of(s_top, v_top * per_unit));
+    bool taken = false;  // token by token
+    if (__any(top > 2048.f || (top < 64.f && top > 0.f))) {
       const uint32_t e = min(max((__float_as_uint(top) >> 23) & 255u, 10u), 250u);
-      const float up = __uint_as_float((e - 7u) << 23);  // the largest becomes 2^7
-      const bool change = (top > 2048.f || top < 8.f) && unit * up >= 0x1p-100f && unit * up <= 0x1p100f;
-      const float down = change ? __uint_as_float((261u - e) << 23) : 1.f;
+      const float up = __uint_as_float((e - 9u) << 23), down = __uint_as_float((263u - e) << 23);  // the largest becomes 2^9
+      const float s_col = column_max(s_top);
+      const bool far = s_col > 0.f && s_col * down < 0x1p-60f;  // the state would lose bits, which the tokens need
+      const bool change = ((top > 2048.f && top < INFINITY) || top < 64.f) && unit * up >= 0x1p-100f && unit * up <= 0x1p100f && !far;
+      taken = __any(far && !lost);
       unit *= change ? up : 1.f;
-      per_unit *= down;
+      per_unit *= change ? down : 1.f;
+      s_top *= change ? down : 1.f;
 #pragma unroll
-      for (int t = 0; t < NT; t++) S[t] *= down;
+      for (int t = 0; t < NT; t++) S[t] *= change ? down : 1.f;
     }
+    // whether every token sees something of the unit's order, at a glance: by the state or by all values
+    const uint64_t by_state = __ballot(lost || s_top * fac->least_decay >= fac->need);
+    const uint64_t by_values = __ballot(v_least * per_unit * fac->least_weight >= fac->need);
+    const uint64_t sure = by_state | by_state >> 16 | by_state >> 32 | by_state >> 48 | (by_values & by_values >> 16 & by_values >> 32 & by_values >> 48);
     // K S
     f16x8 sh[KS], sl[KS];
 #pragma unroll
-    for (int s = 0; s < KS; s++) operand(S[2 * s], S[2 * s + 1], sh[s], sl[s]);
+    for (int s = 0; s < KS; s++) operand<false>(S[2 * s], S[2 * s + 1], sh[s], sl[s]);
     f32x4 ks[4] = {zero, zero, zero, zero}, qs[4];
 #pragma unroll
-    for (int s = 0; s < KS; s++) {
+    for (int s = 0; s < KS; s++)
 #pragma unroll
       for (int mt = 0; mt < 4; mt++) ks[mt] = mfma16(K[mt * KS + s], sl[s], ks[mt]);
 #pragma unroll
+    for (int mt = 0; mt < 4; mt++) ks[mt] *= LO_DOWN;
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
       for (int mt = 0; mt < 4; mt++) ks[mt] = mfma16(K[mt * KS + s], sh[s], ks[mt]);
-    }
     f16x8 TF[2 * T_FRAGS];
-#pragma unroll
-    for (int f = 0; f < 2 * T_FRAGS; f++) TF[f] = frag(st + St::MAT, f, lane);
     f32x4 fe[4];
+    auto load_t = [&] {
 #pragma unroll
-    for (int mt = 0; mt < 4; mt++) fe[mt] = *(const f32x4*)&fac->to_end[row_of(mt, 4 * g)];
-    const float u_limit = fac->u_limit, end = fac->end;
+      for (int f = 0; f < 2 * T_FRAGS; f++) TF[f] = frag(st + St::MAT, f, lane);
+#pragma unroll
+      for (int mt = 0; mt < 4; mt++) fe[mt] = *(const f32x4*)&fac->to_end[row_of(mt, 4 * g)];
+    };
+    const float end = fac->end;
     if constexpr (SPLIT) {
+      load_t();
 #pragma unroll
       for (int s = 0; s < KS; s++) {
         *(f16x8*)(mail + s * FRAG + 16 * lane) = sh[s];
-        *(f16x8*)(mail + (KS + 2 + s) * FRAG + 16 * lane) = sl[s];
+        *(f16x8*)(mail + (KS + s) * FRAG + 16 * lane) = sl[s];
       }
     }
     if constexpr (!SPLIT) {
@@ -804,15 +876,16 @@ __global__ __launch_bounds__((64 * Stage<DK, CW, SPLIT>::WAVES), 2) void delta_c
       load_q(so, Q);
       q_times(Q, sh, sl, qs);
       PHASE();
+      load_t();
     }
-    // x = v - e^a K S
+    // x = v - e^a K S, 2^11 of it
 #pragma unroll
     for (int mt = 0; mt < 4; mt++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) x[mt][r] = fmaf(x[mt][r], per_unit, -(fk[mt][r] * ks[mt][r]));
+      for (int r = 0; r < 4; r++) x[mt][r] = fmaf(x[mt][r], per_unit * LO_UP, -(fk[mt][r] * ks[mt][r]));
     f16x8 hi[2], lo[2];
-    operand(x[0], x[1], hi[0], lo[0]);
-    operand(x[2], x[3], hi[1], lo[1]);
+    operand<true>(x[0], x[1], hi[0], lo[0]);
+    operand<true>(x[2], x[3], hi[1], lo[1]);
     // K^T: row (t, n) at tokens 32 j + 8 g + 0..7, as columns of K's fragments (2 j and 2 j + 1, t / 2)
     f16x8 KT[2 * NT];
 #pragma unroll
@@ -827,49 +900,77 @@ __global__ __launch_bounds__((64 * Stage<DK, CW, SPLIT>::WAVES), 2) void delta_c
     // u = T' x, the small parts first
     f32x4 u[4] = {zero, zero, zero, zero};
 #pragma unroll
-    for (int part = 0; part < 3; part++)
+    for (int part = 0; part < 3; part++) {
 #pragma unroll
       for (int f = 0; f < T_FRAGS; f++) {
         const int s = f >= 4, mt = s ? f - 2 : f;
         u[mt] = mfma16(TF[2 * f + (part == 0)], part == 1 ? lo[s] : hi[s], u[mt]);
       }
+      if (part == 1)
+#pragma unroll
+        for (int mt = 0; mt < 4; mt++) u[mt] *= LO_DOWN;
+    }
     f32x4 w[4];
 #pragma unroll
     for (int mt = 0; mt < 4; mt++) w[mt] = u[mt] * fe[mt];
-    operand(w[0], w[1], hi[0], lo[0]);
-    operand(w[2], w[3], hi[1], lo[1]);
+    operand<true>(w[0], w[1], hi[0], lo[0]);
+    operand<true>(w[2], w[3], hi[1], lo[1]);
     const float p_scale = fac->p_scale;
     // S' = e^{a_63} S + K^T (e^{a_63 - a} u)
     f32x4 add[NT];
 #pragma unroll
-    for (int t = 0; t < NT; t++) add[t] = S[t] * end;
+    for (int t = 0; t < NT; t++) add[t] = zero;
 #pragma unroll
-    for (int j = 0; j < 4; j++)
+    for (int j = 0; j < 4; j++) {
 #pragma unroll
       for (int t = 0; t < NT; t++) add[t] = mfma16(KT[2 * t + (j & 1)], j < 2 ? lo[j & 1] : hi[j & 1], add[t]);
-    f16x8 uh[2], ul[2];
+      if (j == 1)
 #pragma unroll
-    for (int mt = 0; mt < 4; mt++) u[mt] *= U_DOWN;
-    operand(u[0], u[1], uh[0], ul[0]);
-    operand(u[2], u[3], uh[1], ul[1]);
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) add[t][r] = fmaf(add[t][r], LO_DOWN, S[t][r] * end);
+    }
     // u may overflow where the state's update does not
-    const float u_top = fmaxf(fmaxf(largest(u[0]), largest(u[1])), fmaxf(largest(u[2]), largest(u[3])));
-    const bool bad = !(fabsf(add[0][0]) < INFINITY && u_top <= u_limit) && !lost;
-    const bool taken = __any(bad);
+    float u_top = 0.f;
+#pragma unroll
+    for (int mt = 0; mt < 4; mt++) u_top = largest(u_top, u[mt]);
+    taken = taken || __any(!(fabsf(add[0][0]) < INFINITY && u_top <= 65504.f / U_DOWN) && !lost);
+    if ((sure & 0xffff) != 0xffff) {
+      float seen = column_max(s_top), least = INFINITY;
+      const int tokens = min(CHUNK, seq.tokens - c * CHUNK);
+      int column = n;
+      asm volatile("" : "+v"(column));  // its address is made here, too
+      for (int t = 0; t < tokens; t++) {
+        seen = fmaxf(seen * fac->step[t], fac->weight[t] * (fabsf(Elem<DT>::load((const T*)tile, 16 * t + column)) * per_unit));
+        least = seen > 0.f ? fminf(least, seen) : least;
+      }
+      taken = taken || __any(least < fac->need && !lost);
+    }
     if constexpr (SPLIT) {
 #pragma unroll
-      for (int s = 0; s < 2; s++) {
-        *(f16x8*)(mail + (KS + s) * FRAG + 16 * lane) = uh[s];
-        *(f16x8*)(mail + (2 * KS + 2 + s) * FRAG + 16 * lane) = ul[s];
-      }
+      for (int mt = 0; mt < 4; mt++) *(f32x4*)(mail + (2 * KS + mt) * FRAG + 16 * lane) = u[mt];
       *(float*)(mail + 2 * (KS + 2) * FRAG + 4 * lane) = unit;
       *(int*)(mail + 2 * (KS + 2) * FRAG + 256) = taken;
     }
-    if (taken) {
+    if (!taken) {
+#pragma unroll
+      for (int t = 0; t < NT; t++) S[t] = add[t];
+      if constexpr (!SPLIT) {
+        PHASE();
+        f16x8 PF[2 * T_FRAGS];
+        f32x4 fd[4], fq[4];
+        load_p(so + St::MAT, fac, PF, fd, fq);
+        finish(c, PF, fd, fq, u, qs, unit, p_scale, tile);
+      }
+    } else {
 #pragma unroll
       for (int t = 0; t < NT; t++) S[t] *= unit;
       unit = per_unit = 1.f;
-      delta_tokens<DT, DK>(a, seq.first + (int64_t)c * CHUNK, min(CHUNK, seq.tokens - c * CHUNK), hv, hk, col, g, S);
+      // addresses made from these are made here, and not kept over the chunks
+      uint32_t here = col;
+      int rows = g;
+      asm volatile("" : "+v"(here), "+v"(rows));
+      delta_tokens<DT, DK>(a, seq.first + (int64_t)c * CHUNK, min(CHUNK, seq.tokens - c * CHUNK), hv, hk, here, rows, S);
       // 0, or a NaN where the state is not finite: products that overflow fp16 say nothing about it
       float none = 0.f;
 #pragma unroll
@@ -879,16 +980,6 @@ __global__ __launch_bounds__((64 * Stage<DK, CW, SPLIT>::WAVES), 2) void delta_c
       none += lane_xor16(none);
       none += lane_xor32(none);
       lost = !(none == 0.f);
-    } else {
-#pragma unroll
-      for (int t = 0; t < NT; t++) S[t] = add[t];
-      if constexpr (!SPLIT) {
-        PHASE();
-        f16x8 PF[2 * T_FRAGS];
-        f32x4 fd[4], fq[4];
-        load_p(so + St::MAT, fac, PF, fd, fq);
-        finish(c, PF, fd, fq, uh, ul, qs, unit, p_scale, tile);
-      }
     }
   }
   if constexpr (SPLIT) meet();
@@ -929,11 +1020,12 @@ static int delta_chunks(const anna_mi_gated_delta_args& a, const anna_mi_state_s
   }
   constexpr bool SPLIT_TWO = Stage<DK, 2, true>::BYTES <= 160 * 1024;  // at 128 key dims there is no room
   // One workgroup fits a compute unit's LDS in each form.  Its time is the longest chain's or the work's share of 256 compute
-  // units, in chunks of 1.6 us with one column group (1.8 where the chip is full), 2.1 with two, 2.4 to 2.8 with four, which
-  // share the copies.  bf16, 32 heads of 128, the whole call, one against four: 4000 tokens 142 and 190 us, 4000 + 300
-  // 152 and 192, 3000 + 1000 + 200 153 and 154, 4000 + 2000 203 and 199, twice 2048 143 and 116, three times 208 and 129.
-  // Two are never better than four at 128 key dims (twice 2048: 119), and serve what four do not divide; there the
-  // output's wave of its own has no room in LDS (eight times 2048 at 96 columns: 351 us, 472 with one group).
+  // units, in chunks of 2.0 us with one column group (2.2 where the chip is full), 2.9 with two, 3.1 to 3.6 with four, which
+  // share the copies.  bf16, 32 heads of 128, the whole call, one against four: 4000 tokens 161 and 223 us, 4000 + 300
+  // 177 and 227, 4000 + 1000 200 and 228, 3000 + 1000 + 200 178 and 180, 4000 + 2000 241 and 235, twice 2048 167 and
+  // 135, three times 247 and 147.  Two serve what four do not divide (three times 2048 at 64 key dims, fp16, 96 columns:
+  // 173, 201 with one; at 128 dims, bf16, 234 and 243, eight times 395 and 507); at 128 key dims, where the output's wave of
+  // its own has no room in LDS, the state's takes the outputs.
   const int64_t work = s.chunks * a.value_heads * (a.value_dim / 16);
   auto share = [&](int cw) { return std::max(256 * s.longest, work / cw); };
   if (a.value_dim % 64 == 0 && 3 * share(1) > 4 * share(4)) ANNA_CHAIN(4, false)

@@ -102,3 +102,110 @@ def test_updates_beyond_fp16s_range(gpu, length, beta, heads, dtype):
         tol = plain.delta_tolerance(want, sums, errors, c, dtype, float(q.double().norm(dim=-1).max()), False)
         assert torch.isfinite(out[:, at]).all() and ((out[:, at].double() - want).abs() <= tol).all()
         assert ((after[at].double() - end).norm(dim=1) <= E).all()
+
+
+# what: (powers of two, how the inputs get them)
+def outlier(c, p):  # a value that comes late: the tokens in front of it do not know it
+    c["S"][:] = 0
+    c["v"][50, :, 3] = 2.0 ** p
+    c["v"][90, :, 5] = -(2.0 ** p)
+
+
+def outlier_on_a_state(c, p):
+    c["v"][50, 0, 3] = 2.0 ** p
+    c["g"][:] = c["g"] * 20  # nothing of the state is left at the chunk's end
+
+
+def forgotten_state(c, p):
+    c["S"][:, :, 3] *= 2.0 ** p
+    c["g"][4] = -100.0
+
+
+def forgotten_value(c, p):
+    c["v"][20, :, 3] = 2.0 ** p
+    c["g"][25] = -70.0
+    c["g"][100] = float("-inf")
+
+
+def faint_state(c, p):
+    c["S"][:] *= 2.0 ** -p
+    c["v"][:40] = 0
+    c["v"][70:100] = 0
+
+
+def small_betas(c, p):
+    c["S"][:] = 0
+    c["beta"][:40] *= 2.0 ** -p
+    c["beta"][70:] *= 2.0 ** -p
+
+
+def small_columns(c, p):  # in front of, and beside others
+    c["S"][:, :, ::2] *= 2.0 ** -p
+    c["v"][:, :, ::2] *= 2.0 ** -p
+    c["v"][:, :, 1::2] *= 2.0 ** (p // 4)
+
+
+RANGES = [outlier, outlier_on_a_state, forgotten_state, forgotten_value, faint_state, small_betas, small_columns]
+
+
+@pytest.mark.parametrize("heads,DK,DV", [(2, 64, 64), (1, 128, 96), (160, 128, 64)])
+@pytest.mark.parametrize("power", [8, 14, 18, 22, 26, 34, 48, 90, 110])
+@pytest.mark.parametrize("what", RANGES, ids=lambda f: f.__name__)
+def test_sizes_far_apart_in_a_column(gpu, what, power, heads, DK, DV):
+    """A token's answer is as exact as what it sees allows, whatever else its chunk holds.  (160 heads go with four groups
+    of columns a workgroup.)"""
+    q, k, v, g, beta, S = sequence(100 + power, 150, heads, DK, DV)
+    c = dict(v=v.float(), g=g, beta=beta, S=S)
+    what(c, power)
+    v = c["v"].to(BF)
+    out, after = run(gpu, q, k, v, g, beta, S, 0.1)
+    check(out, after, q, k, v, g, beta, S, 0.1)
+
+
+@pytest.mark.parametrize("power", [6, 10, 13])
+def test_sizes_far_apart_in_fp16(gpu, power):
+    q, k, v, g, beta, S = sequence(200 + power, 150, 2, 128, 64, HF)
+    v[:] = (v.float() * 2.0 ** -12).to(HF)
+    S[:] = 0
+    v[50, :, 3] = 2.0 ** power
+    v[100, 1, ::2] = -(2.0 ** power)
+    g[::30] = -25
+    out, after = run(gpu, q, k, v, g, beta, S, 0.1)
+    check(out, after, q, k, v, g, beta, S, 0.1)
+
+
+@pytest.mark.parametrize("heads", [2, 320])
+@pytest.mark.parametrize("length,beta", [(3000.0, 0.5), (2.0 ** 40, 0.9), (2.0 ** -40, 0.5), (2.0 ** 12, 2.0 ** -30)])
+def test_keys_of_any_length(gpu, length, beta, heads):
+    """beta |k|^2 below 1, and each of them far from 1: the bounds hold in the terms of unit keys (v' = v / length)."""
+    q, k, v, g, _, S = sequence(41, 200, heads, 64, 64)
+    k = (k.float() / k.float().norm(dim=-1, keepdim=True) * length * 0.98).to(BF)
+    v, q = (v.float() * length ** 0.5).to(BF), (q.float() / 8).to(BF)
+    beta = torch.full_like(g, beta / length ** 2)
+    out, after = run(gpu, q, k, v, g, beta, S, 1.0, normalize=False)
+    want, end, sums, errors, E, c = plain.delta_rule(q, k.double() / length, v.double() / length, g.double(), beta.double() * length ** 2, S, 1.0, False,
+                                                     chunked=True)
+    tol = plain.delta_tolerance(want, sums, errors, c, BF, float(q.double().norm(dim=-1).max()), False)
+    assert torch.isfinite(out).all() and ((out.double() - want).abs() <= tol).all()
+    assert ((after.double() - end).norm(dim=1) <= E).all()
+
+
+@pytest.mark.parametrize("heads", [2, 320])
+def test_a_state_that_grows(gpu, heads):
+    """The same key again and again with beta 2.5: the state turns round and grows by 1.5 a token, 2^117 in all.  What a token
+    adds to the error, in the state's terms of then, is some 16 roundings of 2^-24 of the key's and beta's factors and those
+    of a product with the state, 2^-18 of the column's 2-norm at most; all of it grows on by 1.5 a token: after t tokens
+    t 2^-18 of 1.5^t of the first state's 2-norm."""
+    n = 200
+    q, k, v, g, _, S = sequence(51, n, heads, 64, 64)
+    k[:] = k[:1]
+    q[:] = k  # what grows
+    v[:], g[:] = 0, 0
+    beta = torch.full_like(g, 2.5)
+    out, after = run(gpu, q, k, v, g, beta, S, 1.0)
+    want, end, *_ = plain.delta_rule(q, k, v, g.double(), beta.double(), S, 1.0, chunked=True)
+    assert torch.isfinite(out).all() and torch.isfinite(after).all()
+    t = torch.arange(1, n + 1)[:, None, None].double()
+    grown = S.double().norm(dim=1) * 1.5 ** t
+    assert ((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + t * 2.0 ** -18 * grown).all()
+    assert ((after.double() - end).norm(dim=1) <= n * 2.0 ** -18 * grown[-1]).all()
