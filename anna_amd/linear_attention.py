@@ -401,9 +401,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, weight
     else:
         if out.dtype != x.dtype or out.shape != x.shape or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous {x.dtype} {list(x.shape)}")
-        same = [t for t in (x, gate) if t is not None and t.is_contiguous() and t.data_ptr() == out.data_ptr()]
-        _apart(out, **{n: t for n, t in dict(x=x, gate=gate, residual=residual, weight=weight).items()
-                       if not any(t is s for s in same)})
+        same = [n for n, t in (("x", x), ("gate", gate)) if t is not None and t.is_contiguous() and t.data_ptr() == out.data_ptr()]
+        _apart(out, **{n: t for n, t in dict(x=x, gate=gate, residual=residual, weight=weight).items() if n not in same})
     _norm(x, weight, float(eps), float(weight_offset), residual, gate, out, None, 0)
     return out
 
