@@ -28,6 +28,21 @@ inline const SpanChain* span_chains(const anna_mi_state_span& s) { return (const
 inline const SpanChunk* span_chunks(const anna_mi_state_span& s) { return (const SpanChunk*)(span_chains(s) + s.chains); }
 inline const int32_t* span_owners(const anna_mi_state_span& s) { return (const int32_t*)(span_chunks(s) + s.chunks); }
 
+// Rows of a tensor, in bytes; and whether those of two share none: of other memory, or other columns of one matrix
+struct Rows {
+  const void* p;
+  int64_t n, stride, bytes;
+};
+inline bool rows_apart(const Rows& a, const Rows& b) {
+  if (!a.p || !b.p || a.n < 1 || b.n < 1) return true;
+  const int64_t between = (intptr_t)b.p - (intptr_t)a.p;
+  if (between >= (a.n - 1) * a.stride + a.bytes || -between >= (b.n - 1) * b.stride + b.bytes) return true;
+  const int64_t stride = a.n > 1 ? a.stride : b.stride;  // a single row may lie between two of the other
+  if ((a.n == 1 && b.n == 1) || (b.n > 1 && b.stride != stride) || stride < 1) return false;
+  const int64_t column = (between % stride + stride) % stride;
+  return column >= a.bytes && column <= stride - b.bytes;
+}
+
 // x / (1 + e^-x), off by a few 2^-24 of itself (|x| 2^-24 where x is far below 0)
 __device__ __forceinline__ float silu_of(float x) {
   return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * x));

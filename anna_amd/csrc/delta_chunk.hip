@@ -1077,6 +1077,20 @@ int anna_mi_gated_delta(const anna_mi_gated_delta_args* args, anna_mi_state_span
   ANNA_CHECK((uintptr_t)a.state % 16 == 0 && a.state_stride_slot % 4 == 0, "gated delta rule: states must be 16-byte aligned");
   ANNA_CHECK(a.slots <= 1 || a.state_stride_slot >= a.value_heads * a.key_dim * a.value_dim, "gated delta rule: states overlap");
   ANNA_CHECK(span->chunks == 0 || (a.workspace && (uintptr_t)a.workspace % 256 == 0), "gated delta rule: no workspace, or not 256-byte aligned");
+  // a state is written while other workgroups still read the inputs
+  const int64_t gate = a.gates_dtype == ANNA_MI_F32 ? 4 : 2;
+  const anna::Rows states = {a.state, a.slots, a.state_stride_slot * 4, a.value_heads * a.key_dim * a.value_dim * 4};
+  const struct {
+    const char* name;
+    anna::Rows rows;
+  } inputs[] = {{"query", {a.query, span->tokens, a.query_stride_token * 2, ((a.key_heads - 1) * a.query_stride_head + a.key_dim) * 2}},
+                {"key", {a.key, span->tokens, a.key_stride_token * 2, ((a.key_heads - 1) * a.key_stride_head + a.key_dim) * 2}},
+                {"value", {a.value, span->tokens, a.value_stride_token * 2, ((a.value_heads - 1) * a.value_stride_head + a.value_dim) * 2}},
+                {"decay", {a.decay, span->tokens, a.decay_stride * gate, a.value_heads * gate}},
+                {"beta", {a.beta, span->tokens, a.beta_stride * gate, a.value_heads * gate}},
+                {"a_log", {a.a_log, 1, 0, a.value_heads * 4}},
+                {"dt_bias", {a.dt_bias, 1, 0, a.value_heads * 4}}};
+  for (const auto& i : inputs) ANNA_CHECK(anna::rows_apart(states, i.rows), "gated delta rule: the state overlaps %s", i.name);
   span->least_slots = a.slots < span->least_slots ? a.slots : span->least_slots;
   hipStream_t st = anna::as_stream(stream);
   if (span->chains == 0) return anna::delta_step(a, *span, st);

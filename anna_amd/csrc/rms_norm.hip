@@ -328,15 +328,6 @@ template <int DT, bool CODES> static int launch_norm(const anna_mi_rms_norm_args
   return ANNA_MI_OK;
 }
 
-// Whether rows of two tensors share no byte: of other memory, or other columns of one matrix
-static bool rows_apart(const void* a, int64_t a_stride, int64_t a_bytes, const void* b, int64_t b_stride, int64_t b_bytes, int64_t rows) {
-  const int64_t between = (intptr_t)b - (intptr_t)a;
-  if (between >= (rows - 1) * a_stride + a_bytes || -between >= (rows - 1) * b_stride + b_bytes) return true;
-  if (a_stride != b_stride || rows < 2) return false;
-  const int64_t column = (between % a_stride + a_stride) % a_stride;
-  return column >= a_bytes && column <= a_stride - b_bytes;
-}
-
 }  // namespace anna
 
 extern "C" int anna_mi_rms_norm(const anna_mi_rms_norm_args* args, void* stream) {
@@ -350,7 +341,7 @@ extern "C" int anna_mi_rms_norm(const anna_mi_rms_norm_args* args, void* stream)
   ANNA_CHECK(a.rows == 1 || (a.x_stride >= a.cols && a.out_stride >= a.cols && (!a.residual || a.residual_stride >= a.cols) &&
                              (!a.gate || a.gate_stride >= a.cols)), "rms_norm: rows overlap");
   const int64_t size = a.dtype == ANNA_MI_F32 ? 4 : 2, out_size = a.out_format == 1 ? 1 : size;
-  ANNA_CHECK(!a.residual || anna::rows_apart(a.residual, a.residual_stride * size, a.cols * size, a.out, a.out_stride * out_size, a.cols * out_size, a.rows),
+  ANNA_CHECK(anna::rows_apart({a.residual, a.rows, a.residual_stride * size, a.cols * size}, {a.out, a.rows, a.out_stride * out_size, a.cols * out_size}),
              "rms_norm: out overlaps the residual");
   if (a.out_format == 1) {
     ANNA_CHECK(a.group == a.cols || ((a.group == 32 || a.group == 64 || a.group == 128) && a.cols % a.group == 0),

@@ -221,6 +221,12 @@ extern "C" int anna_mi_causal_conv1d(const void* x, int dtype, int64_t channels,
   ANNA_CHECK(x_stride >= channels || span->tokens == 1, "causal_conv1d: rows of x overlap");
   ANNA_CHECK(out_stride >= channels || span->tokens == 1, "causal_conv1d: rows of out overlap");
   ANNA_CHECK(slots <= 1 || state_stride_slot >= (width - 1) * channels, "causal_conv1d: rows of the state overlap");
+  // a state is written while other workgroups still read x
+  const int64_t size = dtype == ANNA_MI_F32 ? 4 : 2;
+  const anna::Rows states = {state, slots, state_stride_slot * size, (width - 1) * channels * size};
+  ANNA_CHECK(anna::rows_apart(states, {x, span->tokens, x_stride * size, channels * size}), "causal_conv1d: the state overlaps x");
+  ANNA_CHECK(anna::rows_apart(states, {weight, 1, 0, channels * width * size}), "causal_conv1d: the state overlaps weight");
+  ANNA_CHECK(anna::rows_apart(states, {bias, 1, 0, channels * size}), "causal_conv1d: the state overlaps bias");
   span->least_slots = slots < span->least_slots ? slots : span->least_slots;
   ANNA_DISPATCH_DTYPE(dtype, DT, return anna::launch<DT>(x, channels, x_stride, weight, width, bias, state, slots, state_stride_slot,
                                                          activation, span, out, out_stride, anna::as_stream(stream)));

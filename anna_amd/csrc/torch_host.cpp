@@ -632,6 +632,25 @@ int64_t pool_stride(const Tensor& t, const at::Device& dev, at::ScalarType dt, a
   return t.size(0) > 1 ? (t.stride(0) >= size ? t.stride(0) : -1) : size;
 }
 
+// Bytes that a tensor's elements lie in, and whether those of two may meet
+std::pair<intptr_t, intptr_t> memory(const Tensor& t) {
+  const intptr_t start = reinterpret_cast<intptr_t>(ptr(t));
+  if (t.numel() == 0) return {start, start};
+  int64_t last = 0;
+  for (int64_t i = 0; i < t.dim(); i++) last += (t.size(i) - 1) * t.stride(i);
+  return {start, start + (last + 1) * (int64_t)t.element_size()};
+}
+bool may_meet(const Tensor& state, std::initializer_list<const Tensor*> inputs) {
+  const auto [low, high] = memory(state);
+  for (const Tensor* t : inputs) {
+    if (!t) continue;
+    const auto [first, end] = memory(*t);
+    if (first < high && low < end) return true;
+  }
+  return false;
+}
+const Tensor* of(const OptTensor& t) { return t ? &*t : nullptr; }
+
 OptTensor gated_delta(const Tensor& query, const Tensor& key, const Tensor& value, const Tensor& decay, const Tensor& beta,
                       const Tensor& state, const OptTensor& a_log, const OptTensor& dt_bias, uintptr_t span_address, int64_t device,
                       double scaling, bool normalize, uintptr_t stream) {
@@ -651,7 +670,9 @@ OptTensor gated_delta(const Tensor& query, const Tensor& key, const Tensor& valu
       (DK != 64 && DK != 128) || DV % 32 || DV < 32 || DV > 256 || HK < 1 || HV < 1 || HV % HK || !(scaling > -1e30 && scaling < 1e30))
     return std::nullopt;
   const int64_t stride = pool_stride(state, dev, at::kFloat, {HV, DK, DV});
-  if (stride < 0 || stride % 4 || reinterpret_cast<uintptr_t>(ptr(state)) % 16) return std::nullopt;
+  if (stride < 0 || stride % 4 || reinterpret_cast<uintptr_t>(ptr(state)) % 16 ||
+      may_meet(state, {&query, &key, &value, &decay, &beta, of(a_log), of(dt_bias)}))
+    return std::nullopt;
   Tensor out = at::empty({tokens, HV, DV}, value.options().requires_grad(false)), workspace;
   anna_mi_gated_delta_args a{};
   a.dtype = dtype_code(query), a.gates_dtype = dtype_code(decay), a.normalize = normalize, a.scaling = (float)scaling;
@@ -682,7 +703,7 @@ OptTensor causal_conv1d(const Tensor& x, const Tensor& weight, const OptTensor& 
       !given(bias, dev) || (bias && (!is(*bias, dev, dt) || bias->dim() != 1 || bias->size(0) != channels)))
     return std::nullopt;
   const int64_t width = weight.size(1), stride = pool_stride(state, dev, dt, {width - 1, channels});
-  if (stride < 0) return std::nullopt;
+  if (stride < 0 || may_meet(state, {&x, &weight, of(bias)})) return std::nullopt;
   Tensor out = at::empty({tokens, channels}, x.options().requires_grad(false));
   check(lib.causal_conv1d(ptr(x), dtype_code(x), channels, tokens > 1 ? x.stride(0) : channels, ptr(weight), width, ptr(bias), ptr(state),
                           state.size(0), stride, silu, span, ptr(out), channels, stream_ptr(stream)),

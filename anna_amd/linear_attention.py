@@ -159,6 +159,24 @@ def _apart(out: torch.Tensor, **tensors) -> None:
                 raise ValueError(f"out must not overlap {name}")
 
 
+def _state_apart(state: torch.Tensor, stride: int, **tensors) -> None:
+    """Refuses a pool of states over an input: a state is written while other workgroups still read it.  Inputs may lie
+    between the slots, as other columns of one matrix or in one row."""
+    low, high = _memory(state)
+    if low == high:
+        return
+    step, size = stride * state.element_size(), state[0].numel() * state.element_size()
+    for name, t in tensors.items():
+        if t is None or t.numel() == 0:
+            continue
+        a, b = _memory(t)
+        if a >= high or low >= b:
+            continue
+        column, single = (a - low) % step, _memory(t[0])
+        if column < size or not (column + b - a <= step or (t.stride(0) * t.element_size() == step and column + single[1] - a <= step)):
+            raise ValueError(f"state must not overlap {name}")
+
+
 def _heads(what: str, t: torch.Tensor, dtype: torch.dtype, tokens: int, heads: int, dim: int) -> torch.Tensor:
     """Rows [tokens, heads, dim] as the kernels read them, 16 bytes at a time; copied where they are not."""
     if t.dtype != dtype or tuple(t.shape) != (tokens, heads, dim):
@@ -211,7 +229,8 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | No
 
     with the rows of the sequence's state in front.  weight [channels, width], width 2 to 8; state [slots, width - 1,
     channels], the last inputs of every sequence, oldest first, updated in place; all of one type (bf16, fp16
-    or fp32; sums in fp32).  x may be strided by rows (a slice of a projection).  activation: "silu" or None.  out must not overlap x."""
+    or fp32; sums in fp32).  x may be strided by rows (a slice of a projection).  activation: "silu" or None.  out must not overlap
+    an input, and state neither."""
     if out is None and span is not None and x.is_cuda and _cuda_device() == span._index and (activation == "silu" or activation is None):
         got = _host().causal_conv1d(x, weight, bias, state, span._address, span._index, activation is not None, span._used())
         if got is not None:
@@ -229,6 +248,7 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | No
     if channels < 1:
         raise ValueError("x has no channels")
     stride = _pool("state", state, x.dtype, (width - 1, channels))
+    _state_apart(state, stride, x=x, weight=weight, bias=bias)
     _lib.require_device(x)
     _on(x.device, x=x, weight=weight, bias=bias, state=state, out=out)
     stream = _check_span("causal_conv1d", span, tokens, x.device)
@@ -258,7 +278,8 @@ def gated_delta_rule(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     with k and q divided by sqrt(|.|^2 + 1e-6) first (``normalize``).  query and key [tokens, key_heads, key_dim],
     value [tokens, value_heads, value_dim] in bf16 or fp16 -> out as value; value head h reads key head
     h // (value_heads // key_heads).  key_dim 64 or 128, value_dim a multiple of 32 up to 256.  Strided slices
-    of one projection are read where they lie.  state fp32 [slots, value_heads, key_dim, value_dim] is updated in place.
+    of one projection are read where they lie.  state fp32 [slots, value_heads, key_dim, value_dim] is updated in place;
+    it and out overlap no input.
 
     decay and beta [tokens, value_heads] (fp32 or 16 bits) are g, at most 0, and beta; with ``a_log`` and ``dt_bias``
     (fp32 [value_heads]) they are the projections that those are made from:
@@ -299,6 +320,7 @@ def gated_delta_rule(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     stride = _pool("state", state, torch.float32, (value_heads, key_dim, value_dim))
     if state.data_ptr() % 16 or stride % 4:
         raise ValueError("state must be 16-byte aligned in every slot")
+    _state_apart(state, stride, query=query, key=key, value=value, decay=decay, beta=beta, a_log=a_log, dt_bias=dt_bias)
     device = query.device
     _lib.require_device(query)
     _on(device, query=query, key=key, value=value, decay=decay, beta=beta, a_log=a_log, dt_bias=dt_bias, state=state, out=out)

@@ -801,7 +801,7 @@ int anna_mi_state_span_fill(int64_t n, const int32_t* slots, const int64_t* coun
  * else k and scaling * q), a value head's state S [key_dim][value_dim] takes a token by
  *   u = beta (v - e^g S^T k^),  S <- e^g S + k^ u^T,  out = S^T q^
  * key_dim 64 or 128; value_dim a multiple of 32 up to 256; value head h reads key head h / (value_heads /
- * key_heads).  Rows of query, key and value are 16-byte aligned. */
+ * key_heads).  Rows of query, key and value are 16-byte aligned; state and out overlap no input. */
 typedef struct {
   int dtype;       /* of query, key, value and out: bf16 or fp16 */
   int gates_dtype; /* of decay and beta: bf16, fp16 or fp32 */
@@ -828,7 +828,7 @@ int64_t anna_mi_sizeof_gated_delta_args(void);
 /* out[t][c] = act(bias[c] + sum_j weight[c][j] x[t - width + 1 + j][c]) over a sequence's tokens, with the rows
  * of its state [slots][width - 1][channels] (oldest first) in front of them; the state then holds the
  * last width - 1 inputs.  width 2 to 8; x, out, weight, bias and state of one dtype (bf16, fp16, fp32);
- * out must not overlap x.  activation: 0 none, 1 SiLU. */
+ * out and state must not overlap the other operands.  activation: 0 none, 1 SiLU. */
 int anna_mi_causal_conv1d(const void* x, int dtype, int64_t channels, int64_t x_stride, const void* weight,
                           int64_t width, const void* bias, void* state, int64_t slots, int64_t state_stride_slot,
                           int activation, anna_mi_state_span* span, void* out, int64_t out_stride, void* stream);
