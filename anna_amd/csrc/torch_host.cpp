@@ -617,8 +617,10 @@ OptTensor paged_attend(uintptr_t handle, int64_t layer, uintptr_t span, const Te
 
 // ---------------------------------------------------------------- linear attention
 
-// Without a gradient to lose
-bool given(const Tensor& t, const at::Device& dev) { return plain(t, dev) && !(t.requires_grad() && at::GradMode::is_enabled()); }
+// Without a gradient or a tangent to lose
+bool given(const Tensor& t, const at::Device& dev) {
+  return plain(t, dev) && !(t.requires_grad() && at::GradMode::is_enabled()) && !t._fw_grad(0).defined();
+}
 bool given(const OptTensor& t, const at::Device& dev) { return !t || given(*t, dev); }
 
 // A pool of states [slots][shape], contiguous in each slot; -> elements from one slot to the next, or -1
@@ -659,7 +661,8 @@ OptTensor gated_delta(const Tensor& query, const Tensor& key, const Tensor& valu
   const at::ScalarType dt = query.scalar_type();
   if (!query.is_cuda() || dev.index() != device || query.dim() != 3 || value.dim() != 3 || (dt != at::kBFloat16 && dt != at::kHalf) || span->tokens != query.size(0)) return std::nullopt;
   const int64_t tokens = query.size(0), HK = query.size(1), DK = query.size(2), HV = value.size(1), DV = value.size(2);
-  if (!paged_rows(query, dev, dt, tokens, HK, DK) || !paged_rows(key, dev, dt, tokens, HK, DK) || !paged_rows(value, dev, dt, tokens, HV, DV))
+  auto lies = [&](const Tensor& t, int64_t heads, int64_t dim) { return given(t, dev) && paged_rows(t, dev, dt, tokens, heads, dim); };
+  if (!lies(query, HK, DK) || !lies(key, HK, DK) || !lies(value, HV, DV))
     return std::nullopt;
   auto rows = [&](const Tensor& t) {
     return given(t, dev) && t.scalar_type() == decay.scalar_type() && dtype_code(t) >= 0 && t.dim() == 2 && t.size(0) == tokens &&

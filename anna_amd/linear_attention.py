@@ -14,7 +14,7 @@ rows ("slots") of pools; prompts, chunks of them, drafted and single tokens mix 
     out = rms_norm(out, norm_weight, gate=z)
     hidden = rms_norm(out_proj, next_weight, weight_offset=1.0, residual=stream)         # stream += out_proj
 
-The operators are for inference: tensors that require grad are refused outside ``torch.no_grad()``.  They run on
+The operators are for inference: tensors that require grad are refused outside ``torch.no_grad()``, dual tensors everywhere.  They run on
 the current stream of their tensors' device and can be captured in a graph, with a span made before; between replays
 ``StateSpan.refill`` names other slots.  Calls that share states must not overlap on the GPU.
 """
@@ -25,6 +25,7 @@ import ctypes
 import operator
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -131,6 +132,8 @@ def _on(device: torch.device, **tensors) -> None:
         if t.requires_grad and torch.is_grad_enabled():
             # an answer without a graph would lose its gradient without a word
             raise RuntimeError(f"{name} requires grad, but there is no backward pass: call it under torch.no_grad()")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has a tangent, but there is no forward derivative")
 
 
 def _call(device: torch.device, name: str, *args) -> None:

@@ -110,3 +110,14 @@ def test_the_c_entries_refuse_a_state_over_their_inputs():
         assert lib.anna_mi_gated_delta(ctypes.byref(args), ctypes.byref(span), None) == 1
         assert b"the state overlaps " + name.encode() in lib.anna_mi_last_error()
     assert span.least_slots == 1 << 40  # a refused call leaves no trace
+
+
+def test_dual_tensors_are_refused():
+    """Their tangents would be lost without a word, under no_grad too."""
+    x = torch.zeros(3, 16)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones(3, 16))
+        with torch.no_grad(), pytest.raises(RuntimeError, match="gate has a tangent"):
+            la._on(torch.device("cpu"), x=x, weight=None, gate=dual)
+        la._on(torch.device("cpu"), x=x)
+    la._on(torch.device("cpu"), x=x)
