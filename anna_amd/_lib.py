@@ -283,6 +283,7 @@ _STATE_SPAN = ctypes.POINTER(StateSpan)
 PROTOTYPES.update({
     "anna_mi_state_span_plan": [_I64, _P, _P, _P, _STATE_SPAN],
     "anna_mi_state_span_fill": [_I64, _P, _P, _P, _STATE_SPAN, _P],
+    "anna_mi_state_span_refill": [_STATE_SPAN, _STATE_SPAN],
     "anna_mi_gated_delta": [ctypes.POINTER(GatedDeltaArgs), _STATE_SPAN, _P],
     "anna_mi_causal_conv1d": [_P, _I, _I64, _I64, _P, _I64, _P, _P, _I64, _I64, _I, _STATE_SPAN, _P, _I64, _P],
     "anna_mi_rms_norm": [ctypes.POINTER(RmsNormArgs), _P],

@@ -28,6 +28,9 @@ inline const SpanChain* span_chains(const anna_mi_state_span& s) { return (const
 inline const SpanChunk* span_chunks(const anna_mi_state_span& s) { return (const SpanChunk*)(span_chains(s) + s.chains); }
 inline const int32_t* span_owners(const anna_mi_state_span& s) { return (const int32_t*)(span_chunks(s) + s.chunks); }
 
+// A call takes a span with a pool of so many slots
+int span_take(anna_mi_state_span* span, int64_t slots, const char* what);
+
 // Rows of a tensor, in bytes; and whether those of two share none: of other memory, or other columns of one matrix
 struct Rows {
   const void* p;

@@ -1091,7 +1091,7 @@ int anna_mi_gated_delta(const anna_mi_gated_delta_args* args, anna_mi_state_span
                 {"a_log", {a.a_log, 1, 0, a.value_heads * 4}},
                 {"dt_bias", {a.dt_bias, 1, 0, a.value_heads * 4}}};
   for (const auto& i : inputs) ANNA_CHECK(anna::rows_apart(states, i.rows), "gated delta rule: the state overlaps %s", i.name);
-  span->least_slots = a.slots < span->least_slots ? a.slots : span->least_slots;
+  if (const int rc = anna::span_take(span, a.slots, "gated delta rule")) return rc;
   hipStream_t st = anna::as_stream(stream);
   if (span->chains == 0) return anna::delta_step(a, *span, st);
   ANNA_DISPATCH_DTYPE(a.dtype, DT, {

@@ -227,7 +227,7 @@ extern "C" int anna_mi_causal_conv1d(const void* x, int dtype, int64_t channels,
   ANNA_CHECK(anna::rows_apart(states, {x, span->tokens, x_stride * size, channels * size}), "causal_conv1d: the state overlaps x");
   ANNA_CHECK(anna::rows_apart(states, {weight, 1, 0, channels * width * size}), "causal_conv1d: the state overlaps weight");
   ANNA_CHECK(anna::rows_apart(states, {bias, 1, 0, channels * size}), "causal_conv1d: the state overlaps bias");
-  span->least_slots = slots < span->least_slots ? slots : span->least_slots;
+  if (const int rc = anna::span_take(span, slots, "causal_conv1d")) return rc;
   ANNA_DISPATCH_DTYPE(dtype, DT, return anna::launch<DT>(x, channels, x_stride, weight, width, bias, state, slots, state_stride_slot,
                                                          activation, span, out, out_stride, anna::as_stream(stream)));
 }

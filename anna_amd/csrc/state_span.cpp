@@ -1,5 +1,6 @@
 // Layout of the packed tokens of sequences that continue states (anna_mi_state_span).
 #include <algorithm>
+#include <mutex>
 #include <new>
 #include <vector>
 
@@ -87,6 +88,17 @@ static int lay_out(int64_t n, const int32_t* slots, const int64_t* counts, const
   return ANNA_MI_OK;
 }
 
+// Calls of several threads may take one span, without a lock of theirs, while another names its next slots: what a span
+// promises a pool (slots below max_slot) and what pools it was taken with change together.
+static std::mutex span_lock;
+
+int span_take(anna_mi_state_span* s, int64_t slots, const char* what) {
+  const std::lock_guard<std::mutex> held(span_lock);
+  ANNA_CHECK(s->max_slot < slots, "%s: slot %lld of a state of %lld", what, (long long)s->max_slot, (long long)slots);
+  s->least_slots = std::min(s->least_slots, slots);
+  return ANNA_MI_OK;
+}
+
 }  // namespace anna
 
 extern "C" {
@@ -100,6 +112,18 @@ int anna_mi_state_span_fill(int64_t n, const int32_t* slots, const int64_t* coun
                             anna_mi_state_span* span, int32_t* words) {
   ANNA_CHECK(words != nullptr, "state span: null words");
   return anna::lay_out(n, slots, counts, fresh, span, words);
+}
+
+int anna_mi_state_span_refill(anna_mi_state_span* span, const anna_mi_state_span* plan) {
+  ANNA_CHECK(span != nullptr && plan != nullptr, "state span: null span or plan");
+  ANNA_CHECK(span->sequences == plan->sequences && span->words == plan->words && span->tokens == plan->tokens && span->steps == plan->steps &&
+                 span->chains == plan->chains && span->chunks == plan->chunks && span->longest == plan->longest,
+             "state span: filled with other counts than it was planned for");
+  const std::lock_guard<std::mutex> held(anna::span_lock);
+  ANNA_CHECK(plan->max_slot < span->least_slots, "slot %lld: the span was used with states of %lld slots", (long long)plan->max_slot,
+             (long long)span->least_slots);
+  span->max_slot = plan->max_slot;
+  return ANNA_MI_OK;
 }
 
 int64_t anna_mi_sizeof_state_span(void) { return (int64_t)sizeof(anna_mi_state_span); }

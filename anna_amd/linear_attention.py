@@ -78,14 +78,12 @@ class StateSpan:
             raise RuntimeError("a StateSpan cannot be made or filled while a graph is captured")
         plan = _lib.StateSpan()
         _lib.call("anna_mi_state_span_plan", n, slots, counts, fresh, ctypes.byref(plan))
-        if self._counts is not None:
-            plan.least_slots = self._c.least_slots
-            if plan.max_slot >= plan.least_slots:  # what a graph captured with this span would write to
-                raise RuntimeError(f"slot {plan.max_slot}: the span was used with states of {plan.least_slots} slots")
         words = torch.empty((plan.words,), dtype=torch.int32)
         _lib.call("anna_mi_state_span_fill", n, slots, counts, fresh, ctypes.byref(plan), words.data_ptr())
-        plan.buf = self._c.buf
-        ctypes.memmove(ctypes.addressof(self._c), ctypes.addressof(plan), ctypes.sizeof(plan))
+        if self._counts is None:
+            ctypes.memmove(ctypes.addressof(self._c), ctypes.addressof(plan), ctypes.sizeof(plan))
+        else:  # refuses what a graph captured with this span would write to; nothing else of the span changes
+            _lib.call("anna_mi_state_span_refill", self._ref, ctypes.byref(plan))
         self.slots, self._counts, self.fresh = list(slots), list(counts), [bool(f) for f in fresh]
         return words
 

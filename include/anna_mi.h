@@ -797,6 +797,11 @@ int anna_mi_state_span_plan(int64_t n, const int32_t* slots, const int64_t* coun
 int anna_mi_state_span_fill(int64_t n, const int32_t* slots, const int64_t* counts, const int32_t* fresh,
                             anna_mi_state_span* span, int32_t* words);
 
+/* The next slots of a span that calls were captured with, or are made with on other threads: takes over the slots' limit of
+ * `plan`, planned for the same counts, or refuses it where a pool that the span was taken with has fewer.  The caller then
+ * copies plan's words to span's buf. */
+int anna_mi_state_span_refill(anna_mi_state_span* span, const anna_mi_state_span* plan);
+
 /* The gated delta rule.  With k^ = k / sqrt(|k|^2 + 1e-6) and q^ = scaling * q / sqrt(|q|^2 + 1e-6) (normalize;
  * else k and scaling * q), a value head's state S [key_dim][value_dim] takes a token by
  *   u = beta (v - e^g S^T k^),  S <- e^g S + k^ u^T,  out = S^T q^

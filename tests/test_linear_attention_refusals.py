@@ -121,3 +121,57 @@ def test_dual_tensors_are_refused():
             la._on(torch.device("cpu"), x=x, weight=None, gate=dual)
         la._on(torch.device("cpu"), x=x)
     la._on(torch.device("cpu"), x=x)
+
+
+def refilled(monkeypatch, meanwhile):
+    """A span of two sequences whose layout is made again, with `meanwhile` run as a call of another thread would be."""
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: False)  # nothing here is captured
+    span = object.__new__(la.StateSpan)
+    span._counts, span._c = None, _lib.StateSpan()
+    span._ref = ctypes.byref(span._c)
+    span._lay_out([0, 1], [1, 1], None)
+    real = _lib.call
+
+    def call(name, *args):
+        real(name, *args)
+        if name == "anna_mi_state_span_fill":
+            meanwhile(span._c)
+
+    monkeypatch.setattr(_lib, "call", call)
+    return span
+
+
+def test_a_refill_keeps_what_a_call_beside_it_found_out(monkeypatch):
+    def small_pool(c):
+        c.least_slots = 4
+
+    span = refilled(monkeypatch, small_pool)
+    span._lay_out([3, 1], [1, 1], None)
+    assert span._c.least_slots == 4 and span._c.max_slot == 3
+    with pytest.raises(RuntimeError, match="slot 4: the span was used with states of 4 slots"):
+        span._lay_out([2, 4], [1, 1], None)
+    assert span._c.max_slot == 3 and span.slots == [3, 1]
+
+
+def test_a_refill_behind_the_pool_of_a_call_beside_it_is_refused(monkeypatch):
+    def small_pool(c):
+        c.least_slots = 4
+
+    span = refilled(monkeypatch, small_pool)
+    with pytest.raises(RuntimeError, match="slot 9: the span was used with states of 4 slots"):
+        span._lay_out([9, 1], [1, 1], None)
+    assert span._c.max_slot == 1 and span.slots == [0, 1]
+
+
+def test_the_c_refill_refuses():
+    lib = _lib.load()
+    span, plan = _lib.StateSpan(2, 2, 18, 2, 0, 0, 0, 1, 4, None), _lib.StateSpan(2, 2, 18, 2, 0, 0, 0, 4, 1 << 40, None)
+    assert lib.anna_mi_state_span_refill(ctypes.byref(span), ctypes.byref(plan)) == 1
+    assert b"slot 4: the span was used with states of 4 slots" in lib.anna_mi_last_error() and span.max_slot == 1
+    plan.max_slot = 3
+    assert lib.anna_mi_state_span_refill(ctypes.byref(span), ctypes.byref(plan)) == 0
+    assert (span.max_slot, span.least_slots) == (3, 4)
+    plan.tokens = 3
+    assert lib.anna_mi_state_span_refill(ctypes.byref(span), ctypes.byref(plan)) == 1
+    assert b"other counts" in lib.anna_mi_last_error()
+    assert lib.anna_mi_state_span_refill(None, ctypes.byref(plan)) == 1
