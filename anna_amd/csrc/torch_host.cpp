@@ -622,6 +622,10 @@ bool given(const Tensor& t, const at::Device& dev) {
   return plain(t, dev) && !(t.requires_grad() && at::GradMode::is_enabled()) && !t._fw_grad(0).defined();
 }
 bool given(const OptTensor& t, const at::Device& dev) { return !t || given(*t, dev); }
+// What a call has written, so that autograd sees it where it keeps the tensor; inference tensors have no version
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 
 // A pool of states [slots][shape], contiguous in each slot; -> elements from one slot to the next, or -1
 int64_t pool_stride(const Tensor& t, const at::Device& dev, at::ScalarType dt, at::IntArrayRef shape) {
@@ -691,6 +695,7 @@ OptTensor gated_delta(const Tensor& query, const Tensor& key, const Tensor& valu
     a.workspace = ptr(workspace);
   }
   check(lib.gated_delta(&a, span, stream_ptr(stream)), "anna_mi_gated_delta");
+  written(state);
   return out;
 }
 
@@ -711,6 +716,7 @@ OptTensor causal_conv1d(const Tensor& x, const Tensor& weight, const OptTensor& 
   check(lib.causal_conv1d(ptr(x), dtype_code(x), channels, tokens > 1 ? x.stride(0) : channels, ptr(weight), width, ptr(bias), ptr(state),
                           state.size(0), stride, silu, span, ptr(out), channels, stream_ptr(stream)),
         "anna_mi_causal_conv1d");
+  written(state);
   return out;
 }
 
@@ -759,6 +765,7 @@ Tensor norm(const Tensor& x, const Tensor& weight, double eps, double weight_off
     a.scales = (float*)ptr(*scales);
   }
   check(lib.rms_norm(&a, stream_ptr(stream)), "anna_mi_rms_norm");
+  if (residual) written(*residual);
   return out;
 }
 

@@ -142,6 +142,13 @@ def _call(device: torch.device, name: str, *args) -> None:
             _lib.call(name, *args)
 
 
+def _written(*tensors: torch.Tensor | None) -> None:
+    """Lets autograd see what a call has written, where it keeps the tensor; inference tensors have no version."""
+    for t in tensors:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def _memory(t: torch.Tensor) -> tuple[int, int]:
     """First byte and the one behind the last that a tensor's elements lie in."""
     start = t.data_ptr()
@@ -265,6 +272,7 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | No
     _call(x.device, "anna_mi_causal_conv1d", x.data_ptr(), _lib.dtype_code(x.dtype), channels, x.stride(0) if tokens > 1 else channels,
           weight.data_ptr(), width, _lib.ptr(bias), state.data_ptr(), state.shape[0], stride, int(activation == "silu"), span._ref,
           out.data_ptr(), channels, stream)
+    _written(state, out)
     return out
 
 
@@ -344,6 +352,7 @@ def gated_delta_rule(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         workspace = torch.empty((size,), dtype=torch.uint8, device=device)
         args.workspace = workspace.data_ptr()
     _call(device, "anna_mi_gated_delta", ctypes.byref(args), span._ref, stream)
+    _written(state, out)
     return out
 
 
@@ -404,6 +413,7 @@ def _norm(x, weight, eps, weight_offset, residual, gate, out, scales, group):
         args.gate = gate.data_ptr()
     args.out, args.out_stride, args.scales = out.data_ptr(), cols, _lib.ptr(scales)
     _call(x.device, "anna_mi_rms_norm", ctypes.byref(args), _lib.stream_of(x))
+    _written(residual, out)
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, weight_offset: float = 0.0,
