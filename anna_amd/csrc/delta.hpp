@@ -60,14 +60,23 @@ __device__ __forceinline__ float gate_value(const void* p, int dtype, int64_t i)
   const uint16_t h = ((const uint16_t*)p)[i];
   return dtype == ANNA_MI_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
 }
-__device__ __forceinline__ Gate gate_of(const anna_mi_gated_delta_args& a, Gate r, int64_t head) {
-  if (a.a_log) {
-    const float x = r.g + a.dt_bias[head];
-    r.g = -expf(a.a_log[head]) * (fmaxf(x, 0.f) + log1pf(expf(-fabsf(x))));  // softplus without overflow
+struct HeadGate {
+  bool made;  // from projections
+  float rate, bias;
+};
+__device__ __forceinline__ HeadGate head_gate(const anna_mi_gated_delta_args& a, int64_t head) {
+  if (!a.a_log) return {false, 0.f, 0.f};
+  return {true, expf(a.a_log[head]), a.dt_bias[head]};
+}
+__device__ __forceinline__ Gate gate_of(HeadGate h, Gate r) {
+  if (h.made) {
+    const float x = r.g + h.bias;
+    r.g = -h.rate * (fmaxf(x, 0.f) + log1pf(expf(-fabsf(x))));  // softplus without overflow
     r.beta = 1.f / (1.f + expf(-r.beta));
   }
   return r;
 }
+__device__ __forceinline__ Gate gate_of(const anna_mi_gated_delta_args& a, Gate r, int64_t head) { return gate_of(head_gate(a, head), r); }
 __device__ __forceinline__ Gate gate_of(const anna_mi_gated_delta_args& a, int64_t token, int64_t head) {
   return gate_of(a,
                  Gate{gate_value(a.decay, a.gates_dtype, token * a.decay_stride + head),

@@ -60,10 +60,10 @@ __device__ __forceinline__ void t_frag(int f, int& mt, int& ks) {
 // Factors of a chunk and value head: e^a and k's for 2^11 K S; of (T' / its scale) x on its way to the state, times 2^11; e^a
 // for Q S; q's for the output (P and Q are without them, so rows of any size keep their bits); e^{a_63}; of P times
 // what `U_DOWN` leaves of (T' / its scale) x, which is of x's size whatever beta is.  For the n_i: e^g and |k| beta of
-// every token, the smallest of that and of e^a, and what no n_i may be below.
+// every token, the smallest of that and of e^a, and what no n_i may be below.  For tokens one by one: K's and Q's factors.
 struct Factors {
-  float decayed_k[CHUNK], to_end[CHUNK], decay[CHUNK], q[CHUNK], step[CHUNK], weight[CHUNK];
-  float end, p_scale, least_weight, least_decay, need, pad[123];
+  float decayed_k[CHUNK], to_end[CHUNK], decay[CHUNK], q[CHUNK], step[CHUNK], weight[CHUNK], k[CHUNK];
+  float end, p_scale, least_weight, least_decay, need, pad[59];
 };
 constexpr float U_DOWN = 0x1p-15f;  // the largest of T' / its scale is 2^14 to 2^15
 constexpr float LO_UP = 0x1p11f, LO_DOWN = 0x1p-11f;
@@ -449,6 +449,7 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
       to->to_end[tid] = exp2_of(at[CHUNK - 1], at[tid]) * kf[tid] * ts.up * LO_UP;
       to->step[tid] = tid > 0 ? exp2_of(at[tid], at[tid - 1]) : e;
       to->weight[tid] = weight;
+      to->k[tid] = kf[tid];
       if (tid == CHUNK - 1) to->end = e;
       const float least_weight = -wave_max_rows(tid < tokens ? -weight : -INFINITY), least_decay = -wave_max_rows(-e);
       const float longest = wave_max_rows(tid < tokens ? kn[tid] : 0.f);
@@ -515,43 +516,64 @@ __device__ __forceinline__ float smallest(float least, const f32x4& x) {
   return min_of(min_of(min_of(least, fabsf(x[0])), fabsf(x[1])), min_of(fabsf(x[2]), fabsf(x[3])));
 }
 
-// Tokens one after the other, on the chain's layout of the state: lane (n, g) holds rows row_of(t, 4 g + r) of column n
+// A chunk's tokens one after the other, on the chain's layout of the state: lane (n, g) holds rows row_of(t, 4 g + r) of
+// column n, which are the 8 values that lane (m, g) has of token (mt, m) in K's and Q's fragments.  `keys`, `values` and the
+// factors are in LDS.  All of it is asked for a token ahead.  2048 tokens of 32 heads, one chunk of one group
+// of columns this way: 88 -> 136 us (169 with rows from memory when they are needed, and their norms made again).
 template <int DT, int DK>
-__device__ __forceinline__ void delta_tokens(const anna_mi_gated_delta_args& a, int64_t first, int tokens, int64_t hv, int64_t hk,
-                                          int64_t col, int g, f32x4 (&S)[DK / 16]) {
+__device__ __forceinline__ void delta_tokens(const anna_mi_gated_delta_args& a, const char* keys, const char* queries, const char* values,
+                                             const Factors& fac, int64_t first, int tokens, int64_t hv, int64_t col, int n, int g,
+                                             f32x4 (&S)[DK / 16]) {
   typedef typename Elem<DT>::T T;
+  constexpr int KS = DK / 32;
+  const bool wide = a.gates_dtype == ANNA_MI_F32;
+  struct Token {
+    f16x8 k[KS], q[KS];
+    uint32_t beta;  // as it is: what makes a value of it would wait for all of the loads
+    T v;
+    float step, kf, qf;
+  };
+  auto place = [&](int t, int s) {
+    const int mt = t / 32 * 2 + t / 4 % 2, m = t % 32 / 8 * 4 + t % 4;
+    return (mt * KS + s) * FRAG + 16 * (m + 16 * g);
+  };
+  auto ask = [&](int t) {
+    Token token;
+    const int64_t at = (first + t) * a.beta_stride + hv;
+    token.beta = wide ? ((const uint32_t*)a.beta)[at] : ((const uint16_t*)a.beta)[at];
+#pragma unroll
+    for (int s = 0; s < KS; s++) token.q[s] = *(const f16x8*)(queries + place(t, s));
+#pragma unroll
+    for (int s = 0; s < KS; s++) token.k[s] = *(const f16x8*)(keys + place(t, s));
+    token.v = ((const T*)values)[16 * t + n];
+    token.step = fac.step[t], token.kf = fac.k[t], token.qf = fac.q[t];
+    return token;
+  };
   auto total = [](float v) {
     v += lane_xor16(v);
     return v + lane_xor32(v);
   };
-  for (int64_t token = first; token < first + tokens; token++) {
-    const T* qp = (const T*)a.query + token * a.query_stride_token + hk * a.query_stride_head;
-    const T* kp = (const T*)a.key + token * a.key_stride_token + hk * a.key_stride_head;
-    const float v = Elem<DT>::load((const T*)a.value, token * a.value_stride_token + hv * a.value_stride_head + col);
-    const Gate gate = gate_of(a, token, hv);
-    float k[DK / 4], q[DK / 4], kk = 0.f, qq = 0.f, sk = 0.f, sq = 0.f, kq = 0.f;
+  const HeadGate head = head_gate(a, hv);
+  Token next = ask(0);
+  for (int t = 0; t < tokens; t++) {
+    const Token token = next;
+    next = ask(min(t + 1, tokens - 1));
+    const float v = Elem<DT>::to_f32(token.v), e = token.step, kf = token.kf, qf = token.qf;
+    const float bits = wide ? __uint_as_float(token.beta) : a.gates_dtype == ANNA_MI_BF16 ? bf16_bits_to_f32((uint16_t)token.beta) : f16_bits_to_f32((uint16_t)token.beta);
+    float k[DK / 4], sk[4] = {}, sq[4] = {};
 #pragma unroll
     for (int i = 0; i < DK / 4; i++) {
-      k[i] = Elem<DT>::load(kp, row_of(i / 4, 4 * g + i % 4));
-      q[i] = Elem<DT>::load(qp, row_of(i / 4, 4 * g + i % 4));
-      kk = fmaf(k[i], k[i], kk);
-      qq = fmaf(q[i], q[i], qq);
+      k[i] = fmaf((float)token.k[i / 8][i % 8], kf, 0.f);  // one instruction with its conversion
+      sk[i % 4] = fmaf(S[i / 4][i % 4], k[i], sk[i % 4]);
     }
-    const float ck = a.normalize ? rsqrtf(total(kk) + NORM_EPS) : 1.f;
-    const float cq = a.scaling * (a.normalize ? rsqrtf(total(qq) + NORM_EPS) : 1.f);
+    const float u = gate_of(head, Gate{0.f, bits}).beta * (v - e * total((sk[0] + sk[1]) + (sk[2] + sk[3])));
 #pragma unroll
     for (int i = 0; i < DK / 4; i++) {
-      k[i] *= ck;
-      q[i] *= cq;
-      sk = fmaf(S[i / 4][i % 4], k[i], sk);
-      sq = fmaf(S[i / 4][i % 4], q[i], sq);
-      kq = fmaf(k[i], q[i], kq);
+      S[i / 4][i % 4] = fmaf(k[i], u, e * S[i / 4][i % 4]);
+      sq[i % 4] = fmaf(S[i / 4][i % 4], fmaf((float)token.q[i / 8][i % 8], qf, 0.f), sq[i % 4]);
     }
-    const float e = expf(gate.g), u = gate.beta * (v - e * total(sk));
-    const float o = fmaf(total(kq), u, e * total(sq));
-#pragma unroll
-    for (int i = 0; i < DK / 4; i++) S[i / 4][i % 4] = fmaf(k[i], u, e * S[i / 4][i % 4]);
-    if (g == 0) ((T*)a.out)[(token * a.value_heads + hv) * a.value_dim + col] = Elem<DT>::cvt(o);
+    const float o = total((sq[0] + sq[1]) + (sq[2] + sq[3]));
+    if (g == 0) ((T*)a.out)[((first + t) * a.value_heads + hv) * a.value_dim + col] = Elem<DT>::cvt(o);
   }
 }
 
@@ -835,7 +857,7 @@ __global__ __launch_bounds__((64 * Stage<DK, CW, SPLIT>::WAVES), 2) void delta_c
       for (int t = 0; t < NT; t++) S[t] *= change ? down : 1.f;
     }
     // whether every token sees something of the unit's order, at a glance: by the state or by all values
-    const uint64_t by_state = __ballot(lost || s_top * fac->least_decay >= fac->need);
+    const uint64_t by_state = __ballot(lost || top == 0.f || s_top * fac->least_decay >= fac->need);
     const uint64_t by_values = __ballot(v_least * per_unit * fac->least_weight >= fac->need);
     const uint64_t sure = by_state | by_state >> 16 | by_state >> 32 | by_state >> 48 | (by_values & by_values >> 16 & by_values >> 32 & by_values >> 48);
     // K S
@@ -970,7 +992,8 @@ __global__ __launch_bounds__((64 * Stage<DK, CW, SPLIT>::WAVES), 2) void delta_c
       uint32_t here = col;
       int rows = g;
       asm volatile("" : "+v"(here), "+v"(rows));
-      delta_tokens<DT, DK>(a, seq.first + (int64_t)c * CHUNK, min(CHUNK, seq.tokens - c * CHUNK), hv, hk, here, rows, S);
+      delta_tokens<DT, DK>(a, st, ws.q(chunk0 + c, hk), tile, *fac, seq.first + (int64_t)c * CHUNK, min(CHUNK, seq.tokens - c * CHUNK), hv, here,
+                           (int)(here & 15), rows, S);
       // 0, or a NaN where the state is not finite: products that overflow fp16 say nothing about it
       float none = 0.f;
 #pragma unroll
