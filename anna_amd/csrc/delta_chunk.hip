@@ -18,10 +18,11 @@
 // of them: an outlier that comes later, a state that a decay has made small.  What a token sees is
 //   n_i = max(e^{g_i} n_{i-1}, |k_i| beta_i |v_i|),   n_{-1} the state's largest,
 // and 2^-36 of the unit is below the roundings of fp32 sums of that size where n_i is at least 2^-14 units (times
-// |k| T' where that is above 1).  A chunk with a smaller n_i is taken token by token, from the state that the wave still has.
+// |k| T', and again |k|, where these are above 1).  A chunk with a smaller n_i is taken token by token, from the state that the wave still has.
 // Most columns are fine at a glance: by the old state times the smallest e^a, or the smallest |v| times the smallest |k| beta.
-// The loop over n_i runs for the others: with ordinary values one chunk of some hundreds where decays are strong, for about
-// 1 us.  Without the factor 2^11 it would run in most chunks there.
+// The loop over n_i runs for the others, for about 1 us: with normal values behind a SiLU and decays of e^-0.06 to e^-2.3 a
+// token, in one chunk of a hundred at most, and no chunk goes token by token.  Without the factor 2^11 it would run in
+// nearly all of them from e^-0.26 on, and one in five would go token by token at the other end.
 //
 // Zeros above the diagonals times what is not finite would reach the tokens in front of it.  It also reaches the whole
 // of its column's update, where a wave sees it and also takes the chunk token by token.
@@ -31,14 +32,15 @@
 // numbered so that the instruction's result, rows 4 g + r of a tile in lane (n, g), is at once the other operand of
 // the next product: row m of tile mt stands for index 32 (mt / 2) + 8 (m / 4) + 4 (mt % 2) + m % 4.
 //
-// What bounds it, 16 key and 32 value heads of 128, bf16.  One sequence of 16384 tokens: preparation 111 us, chain 515.
+// What bounds it, 16 key and 32 value heads of 128, bf16.  One sequence of 16384 tokens: preparation 112 us, chain 500.
 // The preparation writes 0.3 GB of workspace (58 us at a copy's rate); the rest is latency, about 36000 cycles a
 // workgroup of loads, products and the inverse's steps with three workgroups a compute unit to cover for each other (two: 121 us).
 // The chain is 256 chunks in a row at 2.0 us each on every compute unit: 82 matrix instructions of the state's
 // wave are a quarter of that, some 400 vector instructions that make their operands (splits, scales) a third; the bytes alone
 // would take 80 us.  (1.6 us with outputs from one term and terms of one scale, 1.8 with both terms.)
-// Eight sequences of 25344 tokens together, fp16: preparation 168 us, chain 425 (350 with terms of one scale). Four waves a
-// compute unit there read all operands from LDS, 3.6 us a chunk: without copies from memory it is as long.
+// Eight sequences of 25344 tokens together, fp16: preparation 164 us, chain 390 (350 with terms of one scale). Four waves a
+// compute unit there read all operands from LDS, 3.3 to 3.6 us a chunk, vector unit 48% and matrix cores 27% busy, a tenth of
+// the cycles with LDS's conflicts.
 // Two column groups a wave, which halves what is read, took 650 for 350: the vector unit of half the SIMDs is then too little.
 // A wave more for every group's output, with operands in single buffers that the output's waves fill, took 430 for 350.
 #include <algorithm>
@@ -57,13 +59,14 @@ __device__ __forceinline__ void t_frag(int f, int& mt, int& ks) {
   mt = ks ? f - 2 : f;
 }
 
-// Factors of a chunk and value head: e^a and k's for 2^11 K S; of (T' / its scale) x on its way to the state, times 2^11; e^a
-// for Q S; q's for the output (P and Q are without them, so rows of any size keep their bits); e^{a_63}; of P times
+// Factors of a chunk and value head.  x is taken times 2^11, and down by a power of two where keys are longer than 1: e^a and
+// k's with that for K S, and it alone for v; of (T' / its scale) x on its way to the state, with 2^11 for its two terms; e^a for
+// Q S; q's for the output (P and Q are without them, so rows of any size keep their bits); e^{a_63}; of P times
 // what `U_DOWN` leaves of (T' / its scale) x, which is of x's size whatever beta is.  For the n_i: e^g and |k| beta of
 // every token, the smallest of that and of e^a, and what no n_i may be below.  For tokens one by one: K's and Q's factors.
 struct Factors {
   float decayed_k[CHUNK], to_end[CHUNK], decay[CHUNK], q[CHUNK], step[CHUNK], weight[CHUNK], k[CHUNK];
-  float end, p_scale, least_weight, least_decay, need, pad[59];
+  float end, x_down, p_scale, least_weight, least_decay, need, pad[58];
 };
 constexpr float U_DOWN = 0x1p-15f;  // the largest of T' / its scale is 2^14 to 2^15
 constexpr float LO_UP = 0x1p11f, LO_DOWN = 0x1p-11f;
@@ -160,7 +163,7 @@ __device__ __forceinline__ double running_sum(double v, int row) {
 }
 
 // Of the state's columns in a workgroup of the short sequences here: wide, as latency does not count beside the chunks
-// (24 sequences of 4 tokens and one of 2048: 95 us with 128 columns, 105 with 32)
+// (24 sequences of 4 tokens and one of 2048: 101 us with 128 columns, 107 with 32)
 __host__ __device__ inline int step_cols(const anna_mi_gated_delta_args& a) { return a.value_dim % 128 == 0 ? 128 : 32; }
 
 // A workgroup takes a chunk, a key head and `per` of its value heads; those from `blocks` on take short sequences, which
@@ -443,22 +446,26 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(const anna_mi_gat
     if (tid < CHUNK) {
       Factors* to = ws.factors(chunk, hv);
       const float e = exp2_of(at[tid]), weight = tid < tokens ? kn[tid] * fabsf(beta[tid]) : 0.f;
-      to->decayed_k[tid] = e * kf[tid] * LO_UP;
+      const float least_weight = -wave_max_rows(tid < tokens ? -weight : -INFINITY), least_decay = -wave_max_rows(-e);
+      const float longest = wave_max_rows(tid < tokens ? kn[tid] : 0.f);
+      // keys longer than 1 (and a third: unit vectors' lengths are rounded) make x larger than S and v
+      const uint32_t longer = min(max((__float_as_uint(0.75f * longest) >> 23) & 255u, 126u), 226u) - 126u;
+      const float x_down = __uint_as_float((127u - longer) << 23), x_up = __uint_as_float((127u + longer) << 23);
+      to->decayed_k[tid] = e * (kf[tid] * x_down) * LO_UP;
       to->decay[tid] = e;
       to->q[tid] = qf[tid];
-      to->to_end[tid] = exp2_of(at[CHUNK - 1], at[tid]) * kf[tid] * ts.up * LO_UP;
+      to->to_end[tid] = exp2_of(at[CHUNK - 1], at[tid]) * (kf[tid] * x_up) * ts.up * LO_UP;
       to->step[tid] = tid > 0 ? exp2_of(at[tid], at[tid - 1]) : e;
       to->weight[tid] = weight;
       to->k[tid] = kf[tid];
       if (tid == CHUNK - 1) to->end = e;
-      const float least_weight = -wave_max_rows(tid < tokens ? -weight : -INFINITY), least_decay = -wave_max_rows(-e);
-      const float longest = wave_max_rows(tid < tokens ? kn[tid] : 0.f);
       if (tid == 0) {
-        const float largest = ts.up / U_DOWN, scale = ps.up * largest;
+        const float largest = ts.up / U_DOWN, scale = ps.up * largest * x_up;
         to->p_scale = fminf(scale, 0x1p127f);
+        to->x_down = x_down;
         to->least_weight = least_weight;
         to->least_decay = least_decay;
-        to->need = scale < 0x1p127f ? 0x1p-14f * fmaxf(1.f, longest * largest) : INFINITY;
+        to->need = scale < 0x1p127f ? 0x1p-14f * fmaxf(1.f, longest * largest * x_up) : INFINITY;
       }
     }
     __syncthreads();
@@ -901,10 +908,11 @@ __global__ __launch_bounds__((64 * Stage<DK, CW, SPLIT>::WAVES), 2) void delta_c
       load_t();
     }
     // x = v - e^a K S, 2^11 of it
+    const float x_unit = per_unit * (fac->x_down * LO_UP);
 #pragma unroll
     for (int mt = 0; mt < 4; mt++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) x[mt][r] = fmaf(x[mt][r], per_unit * LO_UP, -(fk[mt][r] * ks[mt][r]));
+      for (int r = 0; r < 4; r++) x[mt][r] = fmaf(x[mt][r], x_unit, -(fk[mt][r] * ks[mt][r]));
     f16x8 hi[2], lo[2];
     operand<true>(x[0], x[1], hi[0], lo[0]);
     operand<true>(x[2], x[3], hi[1], lo[1]);
@@ -1021,9 +1029,8 @@ template <int DK> static Places<DK> places(const anna_mi_gated_delta_args& a, co
 template <int DT, int DK>
 static int delta_chunks(const anna_mi_gated_delta_args& a, const anna_mi_state_span& s, hipStream_t stream) {
   const Places<DK> ws = places<DK>(a, s);
-  // a key head's value heads in one workgroup share the products of K, where that still fills the chip: 256 chunks of
-  // 16 key heads took 121 us with both value heads and 143 with one; with the chains 32 chunks take 80 and 85, 16
-  // chunks 50 both ways
+  // a key head's value heads in one workgroup share the products of K, where that still fills the chip: the whole call at 16
+  // key heads takes 604 us with both value heads and 629 with one for 256 chunks, 86 and 90 for 32, 52 both ways for 16
   const int64_t ratio = a.value_heads / a.key_heads;
   const int per = s.chunks * a.key_heads >= 512 ? (int)ratio : 1;
   const int64_t steps = s.steps * a.value_heads * (a.value_dim / step_cols(a)), prepare = s.chunks * (a.value_heads / per), groups = s.chains * a.value_heads * (a.value_dim / 16);
