@@ -6,9 +6,10 @@
 namespace anna {
 
 constexpr int CHUNK = 64;        // tokens of a chunk
-// Sequences of at most so many tokens are taken token by token.  16 key and 32 value heads of 128, bf16: one sequence of
-// 12 tokens takes 15 us by steps and one of 13 takes 16 in chunks (16 by steps: 19); 8 sequences 21 and 29 (16 by
-// steps: 28), 64 sequences 83 and 136.
+// Sequences of at most so many tokens are taken token by token: about where one sequence is as fast both ways.  16 key and
+// 32 value heads of 128, bf16: one sequence of 12 tokens takes 13 us by steps and one of 13 takes 16 in chunks; 8
+// sequences 21 and 30, 64 sequences 77 and 144 (by steps 16 tokens of one sequence take 19, of eight 28).  More
+// sequences cross later; steps hold a sequence's tokens in LDS, which has room for so many.
 constexpr int STEP_TOKENS = 12;
 
 // The records of a span's buffer: a sequence, one taken in chunks, a chunk of it

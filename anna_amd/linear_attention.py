@@ -294,8 +294,11 @@ def gated_delta_rule(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     (fp32 [value_heads]) they are the projections that those are made from:
     g = -exp(a_log) softplus(decay + dt_bias), beta = sigmoid(beta).
 
-    Sequences of up to 12 tokens go token by token, longer ones in chunks of 64 tokens, with a
-    workspace of about 20 KB a chunk and value head.  Sums, products and the state are fp32 or as exact."""
+    Sequences of up to 12 tokens go token by token, longer ones in chunks of 64 tokens.  The state is fp32, and sums and
+    products are fp32 or as exact, at the size of what a token sees: values and states far larger that come later, or that
+    a decay has made small, take nothing from it.  (Chunks that hold both are taken token by token, which takes longer.)
+    Chunks need a workspace: each 256 * key_heads * key_dim + 26 KB * value_heads bytes, 1.4 MB at 16 and 32 heads of
+    128, for all of the call's chunks together (1.4 GB for 64 K tokens)."""
     if out is None and span is not None and query.is_cuda and _cuda_device() == span._index:
         got = _host().gated_delta(query, key, value, decay, beta, state, a_log, dt_bias, span._address, span._index, scaling, normalize, span._used())
         if got is not None:
