@@ -209,3 +209,42 @@ def test_a_state_that_grows(gpu, heads):
     grown = S.double().norm(dim=1) * 1.5 ** t
     assert ((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + t * 2.0 ** -18 * grown).all()
     assert ((after.double() - end).norm(dim=1) <= n * 2.0 ** -18 * grown[-1]).all()
+
+
+@pytest.mark.parametrize("DK,dtype,power", [(64, BF, 14), (64, BF, 22), (64, BF, 34), (128, BF, 14), (128, BF, 22), (128, BF, 34), (128, HF, 14)])
+@pytest.mark.parametrize("what", RANGES, ids=lambda f: f.__name__)
+def test_sizes_far_apart_with_two_groups_of_columns(gpu, what, DK, dtype, power):
+    """The forms that take columns that four groups do not divide."""
+    q, k, v, g, beta, S = sequence(300 + power, 140, 100, DK, 96, dtype)
+    c = dict(v=v.float(), g=g, beta=beta, S=S)
+    what(c, power)
+    v = c["v"].to(dtype)
+    out, after = run(gpu, q, k, v, g, beta, S, 0.1)
+    check(out, after, q, k, v, g, beta, S, 0.1)
+
+
+@pytest.mark.parametrize("DV", [32, 128])
+def test_a_chunk_by_tokens_between_others(gpu, DV):
+    """Chunks go token by token and in products in turn, of ragged sequences in one call, one of them of nobody: what is beside
+    them, and the next chunk, is as without."""
+    counts, DK, heads = [200, 13, 64, 65, 300], 128, 4
+    n = sum(counts)
+    q, k, v, g, beta, _ = sequence(61, n, heads, DK, DV)
+    S = 0.5 * randn(66, len(counts) + 1, heads, DK, DV)
+    first = [sum(counts[:i]) for i in range(len(counts))]
+    for at, p in ((first[0] + 70, 40), (first[2] + 5, 30), (first[3] + 64, 60), (first[4] + 130, 25)):
+        v[at, 1, 7] = 2.0 ** p
+        g[at + 1:at + 2, 1] = -80.0
+    slots = [3, 0, 5, -1, 2]
+    pool = S.to(gpu)
+    out = la.gated_delta_rule(*(t.to(gpu) for t in (q, k, v, g, beta)), pool, la.StateSpan(slots, counts, fresh=[False, True, False, False, True], device=gpu),
+                              scaling=0.1).cpu()
+    for slot, at, m, fresh in zip(slots, first, counts, [False, True, False, False, True]):
+        rows = slice(at, at + m)
+        if slot < 0:
+            assert (out[rows] == 0).all()
+            continue
+        start = torch.zeros_like(S[slot]) if fresh else S[slot]
+        check(out[rows], pool[slot].cpu(), q[rows], k[rows], v[rows], g[rows], beta[rows], start, 0.1)
+    for slot in (1, 4):
+        assert torch.equal(pool[slot].cpu(), S[slot])
